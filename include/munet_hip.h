@@ -76,8 +76,8 @@ int mh_init(int device);
 #define MH_POLICY_CPU_FALLBACK 1
 #define MH_POLICY_CONVERSION_FALLBACK 2
 int mh_query_support(int feature, int dtype, int *available, int *fallback_policy, int *accumulation_dtype);
-/* Poll and clear device-side error flags (embedding ids out of range);
- * synchronises the device.  Returns non-zero with a message if any was set. */
+/* Poll and clear device-side error flags (embedding ids out of range, pages
+ * and slots of the paged KV cache); synchronises the device.  Returns non-zero with a message if any was set. */
 int mh_check_device_errors(void);
 
 /* ---- BackendAllocationTransferCapability (src/core/backend.hpp:190-205) --- */
@@ -206,6 +206,101 @@ int mh_attention(int dt, const void *q, const void *k, const void *v, void *ctx,
  * "attention": "textbook". */
 int mh_attention_textbook(int dt, const void *q, const void *k, const void *v, void *ctx, int B, int H, int T,
                           int hd, int causal, void *stream);
+
+/* ---- paged 8-bit KV cache --------------------------------------------------
+ * No counterpart in the reference: keys and values of many requests in one
+ * pool of pages, read by ragged batches of queries (one token, a prompt, or a
+ * chunk of a prompt behind a cached prefix each).
+ *
+ * A page holds `page` tokens (16, 32, 64, 128 or 256) of every key/value head,
+ * in 8-bit floating point (e4m3: largest value 448, one NaN, no infinity) with
+ * one float scale per page and head for keys and one for values:
+ *   k_cache [n_pages][Hkv][page][hd], v_cache [n_pages][Hkv][hd][page] (a
+ *   page's values are stored transposed), k_scale, v_scale [n_pages][Hkv].
+ * An element stands for its e4m3 value times its scale.  Scales are positive;
+ * those that mh_kv_store_paged writes are powers of two.  A slot is
+ * page number * page + place.  A request's pages are its row of the block
+ * table [B][width]: token t lies in page table[t / page], place t % page.
+ * hd is a multiple of 16, at most 256; n_pages * page and width * page are
+ * below 2^31.  Caches are 16-byte aligned.
+ * Device-side data that cannot be checked on the host never leads outside the
+ * buffers: what is done instead is said below, and mh_check_device_errors
+ * reports it.  None of these calls allocates; all may be captured into graphs
+ * (after mh_init). */
+
+/* Where a step's new tokens go.  Request b has lens[b] tokens in the cache and
+ * gets new_lens[b] more (negative counts as 0).  The pages that it needs beyond the
+ * ceil(lens[b] / page) it holds are taken from free_pages [n_free] in order, request
+ * after request, and written into its row of `tables` (other entries stay).
+ * Outputs: total_lens [B] = lens + new_lens; cu [B + 1], the running sum of
+ * new_lens from 0; slots [n_slots], the slot of each new token, request after
+ * request, -1 behind the last; positions [n_slots] (may be NULL), its position,
+ * 0 behind the last; used [1], pages taken (above n_free: so many were
+ * needed).  A token whose page does not exist (the free pages or the table's
+ * width are exhausted, a held entry lies outside the pool) gets slot -1, a page
+ * that could not be had the entry -1, tokens past n_slots are left out (cu stops
+ * there), and the error flag is raised.  Outputs overlap no input but tables. */
+int mh_page_plan(const int32_t *lens, const int32_t *new_lens, const int32_t *free_pages, int32_t *tables,
+                 int32_t *total_lens, int32_t *cu, int32_t *slots, int32_t *positions, int32_t *used, int B, int n_free,
+                 int width, int page, int n_pages, int n_slots, void *stream);
+/* Keys and values of n tokens into their slots.  k, v: token rows of Hkv * hd
+ * values of `dt`, ldk / ldv values apart (multiples of 16 bytes, as are the
+ * pointers).  Tokens of one page follow each other, in the order of their
+ * places, as mh_page_plan lists them: two separate stretches of one page in one call
+ * leave that page's contents and scales unspecified.  Slots of -1 are skipped, slots
+ * outside the pool too, raising the error flag.
+ * For each page and head: e is the least power of two (from 2^-100) whose
+ * 448-fold holds the new values' largest magnitude; the scale becomes e where the
+ * page's first token is among them, else the larger of e and the scale held,
+ * and if it grows the page's earlier tokens are rounded to it; values are
+ * rounded to the nearest e4m3, ties to even.  Infinities and NaN become NaN and do not
+ * count towards the magnitude. */
+int mh_kv_store_paged(int dt, const void *k, const void *v, int64_t ldk, int64_t ldv, const int32_t *slots,
+                      void *k_cache, void *v_cache, float *k_scale, float *v_scale, int n, int Hkv, int hd, int page,
+                      int n_pages, void *stream);
+/* Attention of ragged queries over the cache.  Request b's queries are token
+ * rows cu[b] .. cu[b+1]-1 of q and out (Hq * hd values of `dt`, ldq / ldo values
+ * apart, multiples of 16 bytes, as are the pointers; cu does not decrease), the
+ * last of its lens[b] tokens: query i stands at position
+ * p = lens[b] - (cu[b+1] - cu[b]) + i.  Head h reads key/value head
+ * h / (Hq / Hkv).  It sees keys j < lens[b]; with `causal` only j <= p, with
+ * window > 0 only j > p - window.  out = softmax(scale q k) v over those, zeros
+ * for a query that sees none; scale 0 means 1 / sqrt(hd).  Rows of no request
+ * are left as they are.  Scores, softmax and sums are fp32, for fp16 and bf16
+ * probabilities enter the product with the values as fp16.
+ * max_q and max_len bound the requests' query and key counts; they size the
+ * launch (larger ones on the device are still served, more slowly).
+ * Table entries outside the pool hold no keys, and lengths past width * page
+ * are cut there, raising the error flag.
+ * workspace: mh_attention_paged_workspace bytes, 16-byte aligned, in use until the
+ * call's work on the stream has ended; calls that may overlap need one each.  out
+ * may not overlap another operand. */
+int mh_attention_paged_workspace(int dt, int B, int n_rows, int Hq, int Hkv, int hd, int max_q, int max_len, int window,
+                                 size_t *bytes);
+int mh_attention_paged(int dt, const void *q, int64_t ldq, const void *k_cache, const void *v_cache, const float *k_scale,
+                       const float *v_scale, const int32_t *tables, const int32_t *lens, const int32_t *cu, void *out,
+                       int64_t ldo, int B, int n_rows, int Hq, int Hkv, int hd, int page, int n_pages, int width, int max_q,
+                       int max_len, int causal, int window, float scale, void *workspace, size_t workspace_bytes,
+                       void *stream);
+
+/* ---- sampling ----------------------------------------------------------------
+ * No counterpart in the reference (its demos take np.argmax, mh_argmax here):
+ * one token per row of logits [rows][cols] (rows ld values apart), drawn with
+ * the given uniform numbers u [rows] in [0, 1).  Per row, from device arrays (NULL:
+ * off): temperature T (1; 0 and below, and NaN: the row's argmax), top_k (off
+ * at 0 and below), top_p (off at 1 and above), min_p (off at 0 and below).
+ * Tokens in the order of their logits, ties by index; w = e^((x - max) / T).  Kept
+ * are the first n: the least of top_k, of the fewest whose w reach top_p of the sum
+ * over the first top_k, and of the count with w >= min_p; one at least.  The draw is
+ * the first kept token, in index order, at which the running sum of kept w
+ * exceeds u times their sum.  Sums are whole 64-bit numbers: results do not vary
+ * from run to run.  NaN logits count as -inf; a row of nothing else gives -1.
+ * logprob [rows] (may be NULL): log of the drawn token's share of the kept w
+ * (-inf with -1).  workspace: mh_sample_workspace bytes, as in mh_attention_paged. */
+int mh_sample_workspace(int dt, int rows, int cols, size_t *bytes);
+int mh_sample(int dt, const void *logits, int64_t ld, int rows, int cols, const float *u, const float *temperature,
+              const int32_t *top_k, const float *top_p, const float *min_p, int32_t *out, float *logprob, void *workspace,
+              size_t workspace_bytes, void *stream);
 
 /* ---- BackendShapeCapability (src/core/backend.hpp:263-271) --------------- */
 /* :266-267 concat(inputs, out, dim, shapes): `count` contiguous inputs of rank

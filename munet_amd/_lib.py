@@ -65,6 +65,12 @@ _SIGS = {
     "mh_qkv_projection": [_i, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp],
     "mh_attention": [_i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp],
     "mh_attention_textbook": [_i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp],
+    "mh_page_plan": [_vp] * 9 + [_i] * 6 + [_vp],
+    "mh_kv_store_paged": [_i, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp],
+    "mh_attention_paged_workspace": [_i] * 9 + [ctypes.POINTER(_sz)],
+    "mh_attention_paged": [_i, _vp, _i64] + [_vp] * 8 + [_i64] + [_i] * 12 + [_f, _vp, _sz, _vp],
+    "mh_sample_workspace": [_i, _i, _i, ctypes.POINTER(_sz)],
+    "mh_sample": [_i, _vp, _i64, _i, _i] + [_vp] * 8 + [_sz, _vp],
     "mh_concat": [_i, ctypes.POINTER(_vp), _i, _vp, _i, _i, _ip, _vp],
     "mh_transpose2d": [_i, _vp, _vp, _i, _i, _i, _vp],
     "mh_conv2d": [_i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _i, _vp],

@@ -20,6 +20,7 @@
 #include "host_codec.hpp"
 #include "mh_kernels.hpp"
 #include "mh_runtime.hpp"
+#include "paged_index.hpp"
 
 namespace mh {
 
@@ -221,6 +222,43 @@ void matmul_call(int dt, const void *a, const void *b, void *out, int batch, int
 
 }  // namespace
 
+namespace {
+
+void aligned16(const void *p, const char *what) {
+  if (reinterpret_cast<uintptr_t>(p) % 16) throw Error(std::string(what) + " must be 16-byte aligned");
+}
+void check_page(const char *op, int page, int n_pages) {
+  if (page < kPageMin || page > kPageMax || (page & (page - 1)))
+    throw Error(std::string(op) + ": a page holds 16, 32, 64, 128 or 256 tokens");
+  if (n_pages < 1 || int64_t(n_pages) * page > 0x7fffffff) throw Error(std::string(op) + ": the pool must hold 1 to 2^31 - 1 tokens");
+}
+void check_pool(const char *op, const void *kc, const void *vc, const void *ks, const void *vs, int Hkv, int hd, int page,
+                int n_pages) {
+  check_page(op, page, n_pages);
+  if (Hkv < 1 || Hkv > 65535) throw Error(std::string(op) + ": bad key/value head count");
+  if (hd < 16 || hd > kPagedHeadMax || hd % 16) throw Error(std::string(op) + ": head_dim must be a multiple of 16, at most 256");
+  if (!kc || !vc || !ks || !vs) throw Error(std::string(op) + ": null cache");
+  aligned16(kc, "k_cache");
+  aligned16(vc, "v_cache");
+}
+void check_rows(const char *op, const char *what, int dt, const void *p, int64_t ld, int64_t cols) {
+  if (!p) throw Error(std::string(op) + ": null " + what);
+  aligned16(p, what);
+  if (ld < cols || ld * int64_t(dt_size(dt)) % 16)
+    throw Error(std::string(op) + ": rows of " + what + " must be whole, a multiple of 16 bytes apart");
+}
+// The cut of an attention_paged call, its sizes checked.
+PagedShape paged_call_shape(int dt, int B, int n_rows, int Hq, int Hkv, int hd, int max_q, int max_len, int window) {
+  check_dt(dt);
+  if (B < 0 || n_rows < 0 || max_q < 0 || max_len < 0 || window < 0) throw Error("attention_paged: negative size");
+  if (Hkv < 1 || Hq < 1 || Hq % Hkv) throw Error("attention_paged: query heads must be a multiple of key/value heads");
+  if (hd < 16 || hd > kPagedHeadMax || hd % 16) throw Error("attention_paged: head_dim must be a multiple of 16, at most 256");
+  if (int64_t(n_rows) * Hq > (1 << 30)) throw Error("attention_paged: more than 2^30 query rows");
+  return paged_shape(dt == F32, B, Hq, Hkv, hd, std::min(max_q, n_rows), max_len, window);
+}
+
+}  // namespace
+
 extern "C" {
 
 const char *mh_last_error(void) { return mh::g_last_error.c_str(); }
@@ -290,7 +328,9 @@ int mh_check_device_errors(void) {
     hip_check(hipMemcpy(&h, flag, sizeof(int), hipMemcpyDeviceToHost), "hipMemcpy(error flag)");
     if (h) {
       hip_check(hipMemset(flag, 0, sizeof(int)), "hipMemset(error flag)");
-      if (h & 1) throw Error("Embedding index out of range");
+      if (h & kErrEmbedding) throw Error("Embedding index out of range");
+      if (h & kErrPage) throw Error("paged KV cache: page, slot or length out of range");
+      if (h & kErrPlan) throw Error("page_plan: out of free pages, table width or slots");
       throw Error("device error flag set");
     }
   })
@@ -536,6 +576,144 @@ int mh_attention_textbook(int dt, const void *q, const void *k, const void *v, v
       throw Error("attention: sequence too long for the generic kernel");
     const float scale = host_round(dt, 1.0f / std::sqrt(float(hd)));
     hip_check(attention(dt, q, k, v, ctx, B, H, T, hd, causal, scale, 0, S_(stream), 1), "attention_textbook");
+  })
+}
+
+// ---- paged KV cache ----------------------------------------------------------
+int mh_page_plan(const int32_t *lens, const int32_t *new_lens, const int32_t *free_pages, int32_t *tables,
+                 int32_t *total_lens, int32_t *cu, int32_t *slots, int32_t *positions, int32_t *used, int B, int n_free,
+                 int width, int page, int n_pages, int n_slots, void *stream) {
+  MH_TRY({
+    check_page("page_plan", page, n_pages);
+    if (B < 0 || n_free < 0 || width < 0 || n_slots < 0) throw Error("page_plan: negative size");
+    if (int64_t(width) * page > 0x7fffffff) throw Error("page_plan: a table row must hold at most 2^31 - 1 tokens");
+    if (B == 0) return 0;
+    if (!lens || !new_lens || !total_lens || !cu || !used || (width && !tables) || (n_free && !free_pages) ||
+        (n_slots && !slots))
+      throw Error("page_plan: null argument");
+    PagePlan p;
+    p.lens = lens;
+    p.fresh = new_lens;
+    p.free_pages = free_pages;
+    p.tables = tables;
+    p.total = total_lens;
+    p.cu = cu;
+    p.slots = slots;
+    p.positions = positions;
+    p.used = used;
+    p.B = B;
+    p.n_free = n_free;
+    p.width = width;
+    p.page = page;
+    p.n_pages = n_pages;
+    p.cap = n_slots;
+    hip_check(page_plan(p, device_error_flag(), S_(stream)), "page_plan");
+  })
+}
+int mh_kv_store_paged(int dt, const void *k, const void *v, int64_t ldk, int64_t ldv, const int32_t *slots,
+                      void *k_cache, void *v_cache, float *k_scale, float *v_scale, int n, int Hkv, int hd, int page,
+                      int n_pages, void *stream) {
+  MH_TRY({
+    check_dt(dt);
+    check_pool("kv_store_paged", k_cache, v_cache, k_scale, v_scale, Hkv, hd, page, n_pages);
+    if (n < 0) throw Error("kv_store_paged: negative size");
+    if (n == 0) return 0;
+    if (!slots) throw Error("kv_store_paged: null slots");
+    check_rows("kv_store_paged", "k", dt, k, ldk, int64_t(Hkv) * hd);
+    check_rows("kv_store_paged", "v", dt, v, ldv, int64_t(Hkv) * hd);
+    hip_check(kv_store_paged(dt, k, v, long(ldk), long(ldv), slots, k_cache, v_cache, k_scale, v_scale, n, Hkv, hd, page, n_pages,
+                             device_error_flag(), S_(stream)),
+              "kv_store_paged");
+  })
+}
+int mh_attention_paged_workspace(int dt, int B, int n_rows, int Hq, int Hkv, int hd, int max_q, int max_len, int window,
+                                 size_t *bytes) {
+  MH_TRY({
+    if (!bytes) throw Error("attention_paged_workspace: null output");
+    const PagedShape s = paged_call_shape(dt, B, n_rows, Hq, Hkv, hd, max_q, max_len, window);
+    *bytes = B && n_rows ? paged_workspace_bytes(n_rows, Hq, hd, s.splits) : 0;
+  })
+}
+int mh_attention_paged(int dt, const void *q, int64_t ldq, const void *k_cache, const void *v_cache, const float *k_scale,
+                       const float *v_scale, const int32_t *tables, const int32_t *lens, const int32_t *cu, void *out,
+                       int64_t ldo, int B, int n_rows, int Hq, int Hkv, int hd, int page, int n_pages, int width, int max_q,
+                       int max_len, int causal, int window, float scale, void *workspace, size_t workspace_bytes,
+                       void *stream) {
+  MH_TRY({
+    const PagedShape s = paged_call_shape(dt, B, n_rows, Hq, Hkv, hd, max_q, max_len, window);
+    check_pool("attention_paged", k_cache, v_cache, k_scale, v_scale, Hkv, hd, page, n_pages);
+    if (width < 0 || int64_t(width) * page > 0x7fffffff)
+      throw Error("attention_paged: a table row must hold at most 2^31 - 1 tokens");
+    if (!(std::fabs(scale) <= 3.4e38f)) throw Error("attention_paged: the scale must be finite");
+    if (B == 0 || n_rows == 0) return 0;
+    if (!lens || !cu || (width && !tables)) throw Error("attention_paged: null argument");
+    check_rows("attention_paged", "q", dt, q, ldq, int64_t(Hq) * hd);
+    check_rows("attention_paged", "out", dt, out, ldo, int64_t(Hq) * hd);
+    const size_t need = paged_workspace_bytes(n_rows, Hq, hd, s.splits);
+    if (need > workspace_bytes || (need && !workspace))
+      throw Error("attention_paged: needs a workspace of " + std::to_string(need) + " bytes, got " + std::to_string(workspace_bytes));
+    if (need) aligned16(workspace, "workspace");
+    PagedAttention p;
+    p.q = q;
+    p.out = out;
+    p.k_cache = k_cache;
+    p.v_cache = v_cache;
+    p.k_scale = k_scale;
+    p.v_scale = v_scale;
+    p.tables = tables;
+    p.lens = lens;
+    p.cu = cu;
+    p.workspace = workspace;
+    p.err = device_error_flag();
+    p.ldq = long(ldq);
+    p.ldo = long(ldo);
+    p.B = B;
+    p.Hq = Hq;
+    p.Hkv = Hkv;
+    p.hd = hd;
+    p.page = page;
+    p.n_pages = n_pages;
+    p.n_rows = n_rows;
+    p.width = width;
+    p.causal = causal != 0;
+    p.window = window;
+    p.scale = scale == 0.f ? float(1.0 / std::sqrt(double(hd))) : scale;
+    hip_check(attention_paged(dt, p, s, S_(stream)), "attention_paged");
+  })
+}
+
+// ---- sampling ------------------------------------------------------------------
+int mh_sample_workspace(int dt, int rows, int cols, size_t *bytes) {
+  MH_TRY({
+    check_dt(dt);
+    if (!bytes) throw Error("sample_workspace: null output");
+    if (rows < 0 || cols < 1) throw Error("sample: bad row count or empty rows");
+    *bytes = 0;
+  })
+}
+int mh_sample(int dt, const void *logits, int64_t ld, int rows, int cols, const float *u, const float *temperature,
+              const int32_t *top_k, const float *top_p, const float *min_p, int32_t *out, float *logprob, void *workspace,
+              size_t workspace_bytes, void *stream) {
+  MH_TRY({
+    check_dt(dt);
+    if (rows < 0 || cols < 1) throw Error("sample: bad row count or empty rows");
+    if (rows == 0) return 0;
+    if (!logits || !u || !out) throw Error("sample: null argument");
+    if (ld < cols) throw Error("sample: rows overlap");
+    if (reinterpret_cast<uintptr_t>(logits) % dt_size(dt)) throw Error("sample: logits must be aligned to their type");
+    Sampling p;
+    p.logits = logits;
+    p.ld = long(ld);
+    p.rows = rows;
+    p.cols = cols;
+    p.u = u;
+    p.temperature = temperature;
+    p.top_k = top_k;
+    p.top_p = top_p;
+    p.min_p = min_p;
+    p.ids = out;
+    p.logprob = logprob;
+    hip_check(sample_rows(dt, p, S_(stream)), "sample");
   })
 }
 

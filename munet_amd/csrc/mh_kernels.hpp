@@ -243,6 +243,47 @@ hipError_t nchw_to_nhwc(int dt, const void *in, void *out, int B, int C, int HW,
 hipError_t nchw_to_nhwc_pad(int dt, const void *in, void *out, int B, int C, int HW, int Cp, hipStream_t st);
 hipError_t nhwc_to_nchw(int dt, const void *in, void *out, int B, int C, int HW, hipStream_t st);
 
+// Bits of the device error flag.
+constexpr int kErrEmbedding = 1, kErrPage = 2, kErrPlan = 4;
+
+// Attention over the paged 8-bit KV cache (attention_paged.hip); layouts and
+// the cut of a call in paged_index.hpp.
+struct PagedShape;
+struct PagedAttention {
+  const void *q = nullptr;
+  void *out = nullptr;
+  const void *k_cache = nullptr, *v_cache = nullptr;
+  const float *k_scale = nullptr, *v_scale = nullptr;
+  const int32_t *tables = nullptr, *lens = nullptr, *cu = nullptr;
+  void *workspace = nullptr;
+  int *err = nullptr;
+  long ldq = 0, ldo = 0;
+  int B = 0, Hq = 1, Hkv = 1, hd = 0, page = 0, n_pages = 0, n_rows = 0, width = 0, causal = 1, window = 0;
+  float scale = 1.f;
+};
+hipError_t attention_paged(int dt, const PagedAttention &p, const PagedShape &s, hipStream_t st);
+// n rows of keys and values (rows ld apart) into their slots (paged_cache.hip)
+hipError_t kv_store_paged(int dt, const void *k, const void *v, long ldk, long ldv, const int32_t *slots, void *k_cache,
+                          void *v_cache, float *k_scale, float *v_scale, int n, int Hkv, int hd, int page, int n_pages, int *err,
+                          hipStream_t st);
+struct PagePlan {
+  const int32_t *lens = nullptr, *fresh = nullptr, *free_pages = nullptr;
+  int32_t *tables = nullptr, *total = nullptr, *cu = nullptr, *slots = nullptr, *positions = nullptr, *used = nullptr;
+  int B = 0, n_free = 0, width = 0, page = 0, n_pages = 0, cap = 0;
+};
+hipError_t page_plan(const PagePlan &p, int *err, hipStream_t st);
+// The next tokens of rows of logits (sample.hip).
+struct Sampling {
+  const void *logits = nullptr;
+  long ld = 0;
+  int rows = 0, cols = 0;
+  const float *u = nullptr, *temperature = nullptr, *top_p = nullptr, *min_p = nullptr;
+  const int32_t *top_k = nullptr;
+  int32_t *ids = nullptr;
+  float *logprob = nullptr;
+};
+hipError_t sample_rows(int dt, const Sampling &p, hipStream_t st);
+
 inline size_t dt_size(int dt) { return (dt == 1 || dt == 2) ? 2 : 4; }
 
 }  // namespace mh

@@ -1,0 +1,319 @@
+// The paged 8-bit KV cache's bookkeeping and its writes (paged_index.hpp has the
+// layouts).
+#include "mh_common.hpp"
+#include "mh_kernels.hpp"
+#include "paged_index.hpp"
+
+namespace mh {
+namespace {
+
+// ---- page_plan ---------------------------------------------------------------
+
+// Exclusive sums over the requests before `b0` and the block's own 256: every
+// workgroup adds up the requests before its own instead of waiting for another
+// (8 bytes a request, from the caches; one launch).
+struct Need {
+  int64_t tokens, pages;
+};
+__device__ __forceinline__ int64_t wave_sum64(int64_t v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+
+__device__ __forceinline__ Need need_of(const PagePlan &p, int b) {
+  const PlanNeed n = plan_need(p.lens[b], p.fresh[b], p.page, p.width);
+  return Need{n.fresh, n.need - n.have};
+}
+
+// One workgroup per kPlanRequests requests, and the slots behind the last token
+// by whoever comes to them.
+__global__ void __launch_bounds__(256) page_plan_kernel(PagePlan p, int *err) {
+  __shared__ int64_t part[2][4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int b0 = blockIdx.x * kPlanRequests, b1 = min(b0 + kPlanRequests, p.B);
+  Need before{0, 0};
+  for (int b = tid; b < b0; b += 256) {
+    const Need n = need_of(p, b);
+    before.tokens += n.tokens;
+    before.pages += n.pages;
+  }
+  const int64_t t = wave_sum64(before.tokens), g = wave_sum64(before.pages);
+  if (lane == 0) {
+    part[0][wave] = t;
+    part[1][wave] = g;
+  }
+  __syncthreads();
+  int64_t tok = part[0][0] + part[0][1] + part[0][2] + part[0][3], pg = part[1][0] + part[1][1] + part[1][2] + part[1][3];
+  if (blockIdx.x == 0 && tid == 0) p.cu[0] = 0;
+  int bad = 0;
+  for (int b = b0; b < b1; ++b) {
+    const PlanNeed n = plan_need(p.lens[b], p.fresh[b], p.page, p.width);
+    int32_t *table = p.tables + int64_t(b) * p.width;
+    const int64_t first = pg;
+    // a page of this request's list: held before, or the next free one
+    auto page_at = [&](int i) -> int {
+      int page = -1;
+      if (i < n.have) page = i < p.width ? table[i] : -1;
+      else if (i < n.need) page = first + i - n.have < p.n_free ? p.free_pages[first + i - n.have] : -1;
+      return page_in_pool(page, p.n_pages) ? page : -1;
+    };
+    for (int i = n.have + tid; i < n.need; i += 256) table[i] = page_at(i);
+    if (n.fresh > 0) {
+      for (int64_t i = tid; i < n.fresh; i += 256) {
+        const int64_t at = tok + i, pos = int64_t(n.len) + i;
+        if (at >= p.cap) {
+          bad = 1;
+          break;
+        }
+        const int page = pos / p.page < p.width ? page_at(int(pos / p.page)) : -1;
+        if (page < 0) bad = 1;
+        p.slots[at] = page < 0 ? -1 : page * p.page + int(pos % p.page);
+        if (p.positions) p.positions[at] = int(pos);
+      }
+    }
+    tok += n.fresh;
+    pg += n.need - n.have;
+    if (tid == 0) {
+      p.total[b] = int(int64_t(n.len) + n.fresh);
+      p.cu[b + 1] = int(tok < p.cap ? tok : p.cap);
+      if (b + 1 == p.B) p.used[0] = int(pg);
+    }
+  }
+  if (bad) atomicOr(err, kErrPlan);
+  // the slots behind the last token (a batch padded to a captured graph's size)
+  if (b1 == p.B)
+    for (int64_t i = tok + tid; i < p.cap; i += 256) {
+      p.slots[i] = -1;
+      if (p.positions) p.positions[i] = 0;
+    }
+}
+
+// ---- kv_store_paged -----------------------------------------------------------
+
+// The least power of two whose 448-fold holds amax (e4m3's largest value is
+// 1.75 * 2^8), between 2^-100 and 2^120.  A power of two costs no precision (the
+// values are floating point) and moves a page to a larger scale without a
+// second rounding but of the smallest values.
+__device__ __forceinline__ float e4m3_scale(float amax) {
+  const uint32_t b = __float_as_uint(amax);
+  const int e = int(b >> 23) - 127 - ((b & 0x7fffffu) > 0x600000u ? 7 : 8);
+  return __uint_as_float(uint32_t(min(max(e, -100), 120) + 127) << 23);
+}
+
+// four values to e4m3, to nearest even; what is not finite becomes NaN
+__device__ __forceinline__ uint32_t e4m3x4(const float v[4]) {
+  float w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = __builtin_fabsf(v[i]) < __builtin_inff() ? v[i] : __builtin_nanf("");
+  int r = __builtin_amdgcn_cvt_pk_fp8_f32(w[0], w[1], 0, false);
+  return uint32_t(__builtin_amdgcn_cvt_pk_fp8_f32(w[2], w[3], r, true));
+}
+__device__ __forceinline__ void e4m3x4_dec(uint32_t w, float v[4]) {
+  typedef float f2 __attribute__((ext_vector_type(2)));
+  const f2 a = __builtin_amdgcn_cvt_pk_f32_fp8(int(w), false), b = __builtin_amdgcn_cvt_pk_f32_fp8(int(w), true);
+  v[0] = a[0]; v[1] = a[1]; v[2] = b[0]; v[3] = b[1];
+}
+__device__ __forceinline__ uint32_t rescale4(uint32_t w, float ratio) {
+  float v[4];
+  e4m3x4_dec(w, v);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] *= ratio;
+  return e4m3x4(v);
+}
+
+// eight consecutive values
+template <int DT> __device__ __forceinline__ void ld8(const typename Store<DT>::T *p, float v[8]) {
+  if constexpr (DT == F32) {
+    ld4<F32>(p, v);
+    ld4<F32>(p + 4, v + 4);
+  } else {
+    dec8<DT>(*reinterpret_cast<const uint4 *>(p), v);
+  }
+}
+__device__ __forceinline__ float amax8(const float v[8], float big) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float m = __builtin_fabsf(v[e]);
+    big = m < __builtin_inff() ? fmaxf(big, m) : big;
+  }
+  return big;
+}
+
+struct StoreArgs {
+  const void *k, *v;
+  const int32_t *slots;
+  uint8_t *kc, *vc;
+  float *ks, *vs;
+  int *err;
+  long ldk, ldv;
+  int n, Hkv, hd, page, n_pages, per;
+};
+
+// A run is a stretch of tokens with consecutive slots inside one page.  The
+// workgroup that holds a run's first token writes all of it for one head, and
+// so owns the page's two scales.  Tokens at `per` consecutive places per
+// workgroup.
+template <int DT>
+__global__ void __launch_bounds__(256) kv_store_paged_kernel(StoreArgs a) {
+  typedef typename Store<DT>::T T;
+  constexpr int VT = 64;  // tokens of a value tile
+  __shared__ float red[2][4];
+  __shared__ __align__(16) uint8_t vt[kPagedHeadMax][VT + 4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, head = blockIdx.y;
+  const int t0 = blockIdx.x * a.per, hd = a.hd, P = a.page, h8 = hd / 8;
+  const int64_t limit = int64_t(a.n_pages) * P;
+  // the run starts among this workgroup's tokens (every wave finds the same)
+  uint64_t starts;
+  {
+    const int t = t0 + lane;
+    bool first = false;
+    if (lane < a.per && t < a.n) {
+      const int s = a.slots[t];
+      if (s >= limit && head == 0 && wave == 0) atomicOr(a.err, kErrPage);
+      first = s >= 0 && s < limit && (s % P == 0 || t == 0 || a.slots[t - 1] != s - 1);
+    }
+    starts = __ballot(first);
+  }
+  while (starts) {
+    const int t = t0 + __builtin_ctzll(starts);
+    starts &= starts - 1;
+    const int slot = a.slots[t], page = slot / P, place = slot - page * P;
+    int n = 0;  // tokens of the run
+    for (;;) {
+      const int i = n + lane;
+      const bool in = place + i < P && t + i < a.n && a.slots[min(t + i, a.n - 1)] == slot + i;
+      const uint64_t out = ~__ballot(in);
+      if (out) {
+        n += __builtin_ctzll(out);
+        break;
+      }
+      n += 64;
+    }
+    const T *kp = static_cast<const T *>(a.k) + int64_t(t) * a.ldk + int64_t(head) * hd;
+    const T *vp = static_cast<const T *>(a.v) + int64_t(t) * a.ldv + int64_t(head) * hd;
+    uint8_t *kd = a.kc + page_base(page, a.Hkv, head, P, hd), *vd = a.vc + page_base(page, a.Hkv, head, P, hd);
+
+    float big[2] = {0.f, 0.f};
+    for (int c = tid; c < n * h8; c += 256) {
+      const int i = c / h8, d = 8 * (c - i * h8);
+      float v[8];
+      ld8<DT>(kp + int64_t(i) * a.ldk + d, v);
+      big[0] = amax8(v, big[0]);
+      ld8<DT>(vp + int64_t(i) * a.ldv + d, v);
+      big[1] = amax8(v, big[1]);
+    }
+    const int64_t sc = int64_t(page) * a.Hkv + head;
+    float now[2], inv[2], ratio[2];
+    const float held[2] = {a.ks[sc], a.vs[sc]};
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const float m = wave_max(big[x]);
+      if (lane == 0) red[x][wave] = m;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const float want = e4m3_scale(fmaxf(fmaxf(red[x][0], red[x][1]), fmaxf(red[x][2], red[x][3])));
+      const bool keep = place > 0 && held[x] > want && held[x] < __builtin_inff();
+      now[x] = keep ? held[x] : want;
+      inv[x] = 1.0f / now[x];
+      ratio[x] = place > 0 && held[x] > 0.f && held[x] < now[x] ? held[x] * inv[x] : 1.f;
+    }
+    // the page's earlier tokens in the larger scale
+    if (ratio[0] != 1.f)
+      for (int c = tid; c < place * hd / 16; c += 256) {
+        uint4 *p = reinterpret_cast<uint4 *>(kd) + c;
+        const uint4 w = *p;
+        *p = make_uint4(rescale4(w.x, ratio[0]), rescale4(w.y, ratio[0]), rescale4(w.z, ratio[0]), rescale4(w.w, ratio[0]));
+      }
+    if (ratio[1] != 1.f) {
+      // (whole 16-byte pieces of a row: what lies behind the earlier tokens is
+      // kept, or written by the run below)
+      const int pieces = (place + 15) / 16;
+      for (int c = tid; c < hd * pieces; c += 256) {
+        const int d = c / pieces, i = c - d * pieces;
+        uint4 *p = reinterpret_cast<uint4 *>(vd + int64_t(d) * P + 16 * i);
+        const uint4 w = *p;
+        const uint32_t o[4] = {w.x, w.y, w.z, w.w};
+        uint32_t r[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int left = place - 16 * i - 4 * q;  // earlier tokens from this word on
+          const uint32_t m = left >= 4 ? 0xffffffffu : left <= 0 ? 0u : (1u << (8 * left)) - 1u;
+          r[q] = (rescale4(o[q], ratio[1]) & m) | (o[q] & ~m);
+        }
+        *p = make_uint4(r[0], r[1], r[2], r[3]);
+      }
+    }
+    __syncthreads();
+
+    // keys, in their rows
+    for (int c = tid; c < n * h8; c += 256) {
+      const int i = c / h8, d = 8 * (c - i * h8);
+      float v[8];
+      ld8<DT>(kp + int64_t(i) * a.ldk + d, v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] *= inv[0];
+      *reinterpret_cast<uint2 *>(kd + int64_t(place + i) * hd + d) = make_uint2(e4m3x4(v), e4m3x4(v + 4));
+    }
+    // values, transposed through LDS in tiles of VT places
+    for (int c0 = place & ~(VT - 1); c0 < place + n; c0 += VT) {
+      const int lo = max(c0, place), hi = min(c0 + VT, place + n);
+      for (int c = tid; c < (hi - lo) * h8; c += 256) {
+        const int i = c / h8, d = 8 * (c - i * h8);
+        float v[8];
+        ld8<DT>(vp + int64_t(lo - place + i) * a.ldv + d, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] *= inv[1];
+        const uint32_t w[2] = {e4m3x4(v), e4m3x4(v + 4)};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) vt[d + e][lo - c0 + i] = uint8_t(w[e >> 2] >> (8 * (e & 3)));
+      }
+      __syncthreads();
+      const int first = lo & ~15, pieces = ((hi + 15) / 16) - lo / 16;
+      for (int c = tid; c < hd * pieces; c += 256) {
+        const int d = c / pieces, at = first + 16 * (c - d * pieces);
+        const uint32_t *src = reinterpret_cast<const uint32_t *>(&vt[d][at - c0]);
+        uint8_t *dst = vd + int64_t(d) * P + at;
+        if (at >= lo && at + 16 <= hi) {
+          *reinterpret_cast<uint4 *>(dst) = make_uint4(src[0], src[1], src[2], src[3]);
+        } else {
+          for (int e = max(lo - at, 0); e < min(hi - at, 16); ++e) dst[e] = vt[d][at - c0 + e];
+        }
+      }
+      __syncthreads();
+    }
+    if (tid == 0) {
+      a.ks[sc] = now[0];
+      a.vs[sc] = now[1];
+    }
+  }
+}
+
+}  // namespace
+
+hipError_t page_plan(const PagePlan &p, int *err, hipStream_t st) {
+  if (p.B < 1) return hipErrorInvalidValue;
+  const int blocks = (p.B + kPlanRequests - 1) / kPlanRequests;
+  hipLaunchKernelGGL(page_plan_kernel, dim3(unsigned(blocks)), dim3(256), 0, st, p, err);
+  return hipGetLastError();
+}
+
+hipError_t kv_store_paged(int dt, const void *k, const void *v, long ldk, long ldv, const int32_t *slots, void *k_cache,
+                          void *v_cache, float *k_scale, float *v_scale, int n, int Hkv, int hd, int page, int n_pages, int *err,
+                          hipStream_t st) {
+  if (n < 1 || Hkv < 1 || Hkv > 65535) return hipErrorInvalidValue;
+  StoreArgs a{k, v, slots, static_cast<uint8_t *>(k_cache), static_cast<uint8_t *>(v_cache), k_scale, v_scale, err, ldk, ldv,
+              n, Hkv, hd, page, n_pages, store_tokens(n, Hkv)};
+  const dim3 grid(unsigned((n + a.per - 1) / a.per), unsigned(Hkv));
+  switch (dt) {
+  case F32: hipLaunchKernelGGL(kv_store_paged_kernel<F32>, grid, dim3(256), 0, st, a); break;
+  case F16: hipLaunchKernelGGL(kv_store_paged_kernel<F16>, grid, dim3(256), 0, st, a); break;
+  case BF16: hipLaunchKernelGGL(kv_store_paged_kernel<BF16>, grid, dim3(256), 0, st, a); break;
+  default: return hipErrorInvalidValue;
+  }
+  return hipGetLastError();
+}
+
+}  // namespace mh

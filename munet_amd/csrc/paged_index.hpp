@@ -1,0 +1,117 @@
+// Index rules of the paged 8-bit KV cache, shared by its kernels and, free of
+// device code, run by the host up to sizes that no test can allocate
+// (tests/cxx/paged_index_check.cpp).
+//
+// A page holds P tokens of every key/value head.  Keys lie [page][head][P][hd],
+// values [page][head][hd][P]: a page's values are stored transposed, so that
+// both products of attention read their operand in 16-byte runs along the
+// contracted dimension.  A slot is page * P + place.
+#pragma once
+
+#include <stddef.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+namespace mh {
+
+constexpr int kPageMin = 16, kPageMax = 256;  // tokens per page, powers of two
+constexpr int kPagedHeadMax = 256;            // head size, a multiple of 16
+constexpr int kKeyBlock = 64;                 // keys that a wave takes at once
+
+__host__ __device__ __forceinline__ bool page_in_pool(int page, int n_pages) { return page >= 0 && page < n_pages; }
+
+// Byte of a page's first key or value of a head.  64 bits: a pool passes 2^32
+// bytes at a million pages of 16 tokens and a few heads.
+__host__ __device__ __forceinline__ int64_t page_base(int page, int heads, int head, int tokens, int hd) {
+  return (int64_t(page) * heads + head) * (int64_t(tokens) * hd);
+}
+
+// Keys [lo, hi) that queries i0..i1 (inclusive) of a sequence with n queries and
+// len keys can see: query i stands at position len - n + i.
+struct KeyRange {
+  int lo, hi;
+};
+__host__ __device__ __forceinline__ KeyRange seen_keys(int len, int n, int i0, int i1, bool causal, int window) {
+  KeyRange r;
+  const int64_t p0 = int64_t(len) - n + i0, p1 = int64_t(len) - n + i1;
+  const int64_t hi = causal ? (p1 + 1 < len ? p1 + 1 : len) : len;
+  const int64_t lo = window > 0 ? p0 - window + 1 : 0;
+  r.lo = int(lo < 0 ? 0 : lo);
+  r.hi = int(hi < 0 ? 0 : hi);
+  if (r.hi < r.lo) r.hi = r.lo;
+  return r;
+}
+
+// Share s of `splits` of a key range: `chunk` keys (a multiple of kKeyBlock) from
+// the range's start rounded down to a block; the last share takes what is left,
+// so that the shares cover the range whatever length the chunk was chosen for.
+__host__ __device__ __forceinline__ KeyRange key_share(KeyRange all, int s, int splits, int chunk) {
+  const int first = all.lo & ~(kKeyBlock - 1);
+  const int64_t a = int64_t(first) + int64_t(s) * chunk, b = s + 1 < splits ? a + chunk : int64_t(all.hi);
+  KeyRange r;
+  r.lo = int(a < all.hi ? a : all.hi);
+  r.hi = int(b < all.hi ? b : all.hi);
+  if (r.hi < r.lo) r.hi = r.lo;
+  return r;
+}
+
+// What a request of `len` cached and `fresh` new tokens holds and needs, in
+// pages, with room for `width` pages in its row of the block table.
+struct PlanNeed {
+  int len, fresh, have, need;
+};
+__host__ __device__ __forceinline__ PlanNeed plan_need(int len, int fresh, int page, int width) {
+  PlanNeed n;
+  n.len = len > 0 ? len : 0;
+  n.fresh = fresh > 0 ? fresh : 0;
+  if (n.fresh > 0x7fffffff - n.len) n.fresh = 0x7fffffff - n.len;
+  const int have = n.len / page + (n.len % page != 0), all = n.len + n.fresh, need = all / page + (all % page != 0);
+  n.have = have;
+  n.need = need < width ? need : width;
+  if (n.need < n.have) n.need = n.have;
+  return n;
+}
+// Requests per workgroup of the plan: each adds up the ones before its own.
+constexpr int kPlanRequests = 1;
+
+// Tokens per workgroup of the store: one while that leaves at most 16384
+// workgroups (a decode step: every token starts a run), up to 64 for prompts,
+// where one token in a page does.
+inline int store_tokens(int n, int heads) { return int(std::min<int64_t>(64, std::max<int64_t>(1, int64_t(n) * heads / 16384))); }
+
+// How a call is cut: rows of one (sequence, key/value head) in tiles, and each
+// tile's keys in `splits` shares of `chunk`.
+struct PagedShape {
+  int wide, tiles, splits, chunk;
+};
+// Rows that a workgroup of the wide form takes: four waves of one or two MFMA
+// tiles (one for fp32, whose operands are in two parts, and for heads above 128).
+inline int paged_wide_rows(bool f32, int hd) { return f32 || hd > 128 ? 64 : 128; }
+inline PagedShape paged_shape(bool f32, int B, int Hq, int Hkv, int hd, int max_q, int max_len, int window) {
+  PagedShape s;
+  const int64_t rows = int64_t(max_q) * (Hq / Hkv);
+  s.wide = rows > 16;
+  const int per = s.wide ? paged_wide_rows(f32, hd) : 16;
+  s.tiles = int(std::max<int64_t>(1, (rows + per - 1) / per));
+  // Shares so that about 1024 workgroups are in flight (four per CU), none
+  // shorter than one block per wave.
+  const int64_t whole = std::max<int64_t>(1, int64_t(B) * Hkv * s.tiles);
+  const int64_t keys = window > 0 ? std::min<int64_t>(max_len, int64_t(window) + max_q + kKeyBlock) : max_len;
+  const int64_t least = 4 * kKeyBlock;
+  int64_t n = std::min<int64_t>((keys + least - 1) / least, (1024 + whole - 1) / whole);
+  n = std::max<int64_t>(1, std::min<int64_t>(n, 256));
+  s.chunk = int(std::min<int64_t>(((keys + n - 1) / n + least - 1) / least * least, 1 << 30));
+  if (s.chunk == 0) s.chunk = int(least);
+  s.splits = int(std::max<int64_t>(1, (keys + s.chunk - 1) / s.chunk));
+  return s;
+}
+// Workspace: the shares' outputs, then their (maximum, sum) pairs.
+inline size_t paged_part_bytes(int n_rows, int Hq, int hd, int splits) {
+  return splits > 1 ? size_t(n_rows) * Hq * splits * hd * 4 : 0;
+}
+inline size_t paged_workspace_bytes(int n_rows, int Hq, int hd, int splits) {
+  return splits > 1 ? paged_part_bytes(n_rows, Hq, hd, splits) + size_t(n_rows) * Hq * splits * 8 : 0;
+}
+
+}  // namespace mh
