@@ -173,7 +173,7 @@ def load():
 
 
 def call(name, *args):
-    lib = load()
+    lib = _lib or load()
     rc = getattr(lib, name)(*args)
     if rc != 0:
         msg = lib.mh_last_error()

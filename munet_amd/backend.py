@@ -78,90 +78,90 @@ def _dt(x):
     return dtype_code(x.dtype)
 
 
-def _float_dt(op, x):
+def _operand(op, d, name, x, dtype, shape):
+    """Address of a contiguous operand of the given type and shape on GPU d."""
+    if x.get_device() != d or x.dtype is not dtype or x.shape != shape or not x.is_contiguous():
+        _refuse(op, d, name, x, (dtype,), shape, True)
+    return x.data_ptr()
+
+
+def _optional(op, d, name, x, dtype, shape):
+    return None if x is None else _operand(op, d, name, x, dtype, shape)
+
+
+def _token_rows(op, d, name, x, dtype, shape):
+    """(address, values between rows) of [rows, heads, hd] on GPU d whose heads are contiguous."""
+    if x.get_device() != d or x.dtype is not dtype or x.shape != shape:
+        _refuse(op, d, name, x, (dtype,), shape, False)
+    n, h, e = x.stride()
+    if (e != 1 and shape[2] > 1) or (h != shape[2] and shape[1] > 1):
+        raise ValueError(f"{op}: the heads of {name} must be contiguous")
+    return x.data_ptr(), n if shape[0] > 1 else shape[1] * shape[2]
+
+
+def _pool(op, d, k_cache, v_cache, k_scale, v_scale):
+    """Addresses and (pages, Hkv, page, hd) of the paged cache's four tensors."""
+    if k_cache.dim() != 4:
+        _refuse(op, d, "k_cache", k_cache, (k_cache.dtype,), (None,) * 4, True)
+    n_pages, Hkv, page, hd = size = k_cache.shape
     t = _torch()
-    if x.dtype not in (t.float32, t.float16, t.bfloat16):
-        raise ValueError(f"{op}: float32, float16 or bfloat16, not {x.dtype}")
-    return dtype_code(x.dtype)
+    dt = k_cache.dtype
+    if dt is not t.uint8 and dt is not t.float8_e4m3fn:
+        _refuse(op, d, "k_cache", k_cache, (t.uint8, t.float8_e4m3fn), size, True)
+    return (_operand(op, d, "k_cache", k_cache, dt, size), _operand(op, d, "v_cache", v_cache, dt, (n_pages, Hkv, hd, page)),
+            _operand(op, d, "k_scale", k_scale, t.float32, (n_pages, Hkv)),
+            _operand(op, d, "v_scale", v_scale, t.float32, (n_pages, Hkv)), n_pages, Hkv, page, hd)
 
 
-def _size(op, name, x, dim):
-    if x.dim() <= dim:
-        raise ValueError(f"{op}: {name} has no dimension {dim}")
-    return x.shape[dim]
+def _refuse(op, d, name, x, dtypes, shape, contiguous):
+    """Say what is wrong with an operand."""
+    if d < 0 or x.get_device() != d:
+        raise ValueError(f"{op}: all tensors must be on one GPU; {name} is on {x.device}")
+    if x.dtype not in dtypes:
+        raise ValueError(f"{op}: {name} must be {' or '.join(str(t)[6:] for t in dtypes)}, not {str(x.dtype)[6:]}")
+    if x.dim() != len(shape) or any(w is not None and w != n for w, n in zip(shape, x.shape)):
+        raise ValueError(f"{op}: {name} must be of shape [" + ", ".join("*" if w is None else str(w) for w in shape)
+                         + f"], not {list(x.shape)}")
+    raise ValueError(f"{op}: {name} must be contiguous")
 
 
-def _nbytes(x):
-    return 0 if x is None else x.numel() * x.element_size()
+def _rank(op, d, name, x, rank):
+    if d < 0 or x.dim() != rank:
+        _refuse(op, d, name, x, (x.dtype,), (None,) * rank, False)
+    return x.shape
 
 
-class _Call:
-    """The checks of a call whose sizes come from its tensors, and its stream:
-    all tensors on one GPU, which is the current device while the call runs, on
-    torch's current stream of that device."""
+def _float_dt(op, name, x):
+    t = _torch()
+    dt = x.dtype
+    if dt is t.bfloat16:
+        return BF16
+    if dt is t.float16:
+        return F16
+    if dt is not t.float32:
+        _refuse(op, x.get_device(), name, x, (t.float32, t.float16, t.bfloat16), x.shape, False)
+    return F32
 
-    def __init__(self, op, **tensors):
-        self.op = op
-        self.t = {k: v for k, v in tensors.items() if v is not None}
-        devices = {v.device for v in self.t.values()}
-        if len(devices) != 1 or next(iter(devices)).type != "cuda":
-            raise ValueError(f"{op}: all tensors must be on one GPU, got {sorted(map(str, devices))}")
-        self.guard = _torch().cuda.device(next(iter(devices)))
 
-    def __enter__(self):
-        self.guard.__enter__()
-        self.stream = _stream()
-        return self
+def _workspace(op, d, ws, need):
+    """(workspace, its address, its bytes): the caller's, or one of ``need()`` bytes."""
+    t = _torch()
+    if ws is None:
+        n = need()
+        ws = t.empty(n, dtype=t.uint8, device=d) if n else None
+        return ws, None if ws is None else ws.data_ptr(), n
+    n = ws.numel()
+    return ws, _operand(op, d, "workspace", ws, t.uint8, (n,)), n
 
-    def __exit__(self, *exc):
-        return self.guard.__exit__(*exc)
 
-    def _each(self, names, ok, what):
-        for n in names:
-            if n in self.t and not ok(self.t[n]):
-                raise ValueError(f"{self.op}: {n} must be {what}")
-        return self
-
-    def int32(self, *names):
-        return self._each(names, lambda x: x.dtype == _torch().int32, "int32")
-
-    def float32(self, *names):
-        return self._each(names, lambda x: x.dtype == _torch().float32, "float32")
-
-    def contiguous(self, *names):
-        return self._each(names, lambda x: x.is_contiguous(), "contiguous")
-
-    def shape(self, name, want):
-        def ok(x):
-            return x.dim() == len(want) and all(w is None or w == d for w, d in zip(want, x.shape))
-        return self._each((name,), ok, "of shape [" + ", ".join("*" if w is None else str(w) for w in want) + "]")
-
-    def pool(self):
-        """(pages, Hkv, page, hd) of the cache operands, their shapes and types checked."""
-        t = _torch()
-        k = self.t["k_cache"]
-        self.shape("k_cache", (None, None, None, None))
-        n_pages, Hkv, page, hd = k.shape
-        self.shape("v_cache", (n_pages, Hkv, hd, page)).shape("k_scale", (n_pages, Hkv)).shape("v_scale", (n_pages, Hkv))
-        self._each(("k_cache", "v_cache"), lambda x: x.dtype in (t.uint8, t.float8_e4m3fn), "uint8 or float8_e4m3fn")
-        self.float32("k_scale", "v_scale").contiguous("k_cache", "v_cache", "k_scale", "v_scale")
-        return n_pages, Hkv, page, hd
-
-    def row_stride(self, name):
-        """Values between the rows of [rows, heads, hd] whose heads are contiguous."""
-        x = self.t[name]
-        rows, heads, hd = x.shape
-        if (hd > 1 and x.stride(2) != 1) or (heads > 1 and x.stride(1) != hd):
-            raise ValueError(f"{self.op}: the heads of {name} must be contiguous")
-        return x.stride(0) if rows > 1 else heads * hd
-
-    def workspace(self, ws, need):
-        t = _torch()
-        if ws is None:
-            return t.empty(need, dtype=t.uint8, device=self.guard.idx) if need else None
-        if ws.dtype != t.uint8:
-            raise ValueError(f"{self.op}: the workspace must be uint8")
-        return ws
+def _launch(name, d, *args):
+    """The call with GPU d as the current device, on torch's current stream of it."""
+    cuda = _torch().cuda
+    if cuda.current_device() == d:
+        call(name, *args, cuda.current_stream().cuda_stream)
+    else:
+        with cuda.device(d):
+            call(name, *args, cuda.current_stream().cuda_stream)
 
 
 def compute_broadcast(a_shape, a_strides, b_shape, b_strides):
@@ -384,94 +384,91 @@ class HipBackend:
         call("mh_attention_textbook", _dt(q), _p(q), _p(k), _p(v), _p(ctx), B, H, T, hd, int(causal), _stream())
 
     # ---- paged 8-bit KV cache (no MuNet counterpart) --------------------------
+    # These calls take their sizes from their tensors and check them; all of a
+    # call's tensors lie on one GPU, and it runs on torch's current stream there.
     def page_plan(self, lens, new_lens, free_pages, tables, total_lens, cu, slots, positions, used, page, n_pages):
         """Pages and slots of a step's new tokens (mh_page_plan): ``new_lens``
-        [B] more tokens behind ``lens`` [B]; ``tables`` [B, width] gets the pages taken
-        from ``free_pages``; ``total_lens`` [B], ``cu`` [B + 1], ``slots``, ``positions`` (or
-        None) and ``used`` [1] are written."""
-        B = _size("page_plan", "lens", lens, 0)
-        with _Call("page_plan", lens=lens, new_lens=new_lens, free_pages=free_pages, tables=tables, total_lens=total_lens, cu=cu,
-                   slots=slots, positions=positions, used=used) as c:
-            c.int32("lens", "new_lens", "free_pages", "tables", "total_lens", "cu", "slots", "positions", "used")
-            c.contiguous("lens", "new_lens", "free_pages", "tables", "total_lens", "cu", "slots", "positions", "used")
-            c.shape("new_lens", (B,)).shape("total_lens", (B,)).shape("cu", (B + 1,)).shape("used", (1,))
-            c.shape("tables", (B, None)).shape("free_pages", (None,)).shape("slots", (None,))
-            c.shape("positions", tuple(slots.shape))
-            call("mh_page_plan", _p(lens), _p(new_lens), _p(free_pages), _p(tables), _p(total_lens), _p(cu), _p(slots),
-                 _p(positions), _p(used), B, free_pages.shape[0], tables.shape[1], page, n_pages, slots.shape[0], c.stream)
+        [B] more tokens behind ``lens`` [B]; ``tables`` [B, width] gets the pages
+        taken from ``free_pages``; ``total_lens`` [B], ``cu`` [B + 1], ``slots``,
+        ``positions`` (or None) and ``used`` [1] are written.  All int32."""
+        op, d, i32 = "page_plan", lens.get_device(), _torch().int32
+        (B,), (_, width) = _rank(op, d, "lens", lens, 1), _rank(op, d, "tables", tables, 2)
+        (n_free,), (n,) = _rank(op, d, "free_pages", free_pages, 1), _rank(op, d, "slots", slots, 1)
+        _launch("mh_page_plan", d, _operand(op, d, "lens", lens, i32, (B,)), _operand(op, d, "new_lens", new_lens, i32, (B,)),
+                _operand(op, d, "free_pages", free_pages, i32, (n_free,)), _operand(op, d, "tables", tables, i32, (B, width)),
+                _operand(op, d, "total_lens", total_lens, i32, (B,)), _operand(op, d, "cu", cu, i32, (B + 1,)),
+                _operand(op, d, "slots", slots, i32, (n,)), _optional(op, d, "positions", positions, i32, (n,)),
+                _operand(op, d, "used", used, i32, (1,)), B, n_free, width, page, n_pages, n)
 
     def kv_store_paged(self, k, v, slots, k_cache, v_cache, k_scale, v_scale):
-        """Keys and values [n, Hkv, hd] (heads contiguous, any row stride of whole
-        16 bytes) into their slots (mh_kv_store_paged): ``k_cache`` [pages, Hkv,
-        page, hd] and ``v_cache`` [pages, Hkv, hd, page] of 8-bit elements,
-        scales [pages, Hkv] float32."""
-        with _Call("kv_store_paged", k=k, v=v, slots=slots, k_cache=k_cache, v_cache=v_cache, k_scale=k_scale, v_scale=v_scale) as c:
-            n_pages, Hkv, page, hd = c.pool()
-            n = _size("kv_store_paged", "k", k, 0)
-            c.shape("k", (n, Hkv, hd)).shape("v", (n, Hkv, hd)).shape("slots", (n,)).int32("slots").contiguous("slots")
-            if v.dtype != k.dtype:
-                raise ValueError("kv_store_paged: k and v must have one type")
-            call("mh_kv_store_paged", _float_dt("kv_store_paged", k), _p(k), _p(v), c.row_stride("k"), c.row_stride("v"), _p(slots),
-                 _p(k_cache), _p(v_cache), _p(k_scale), _p(v_scale), n, Hkv, hd, page, n_pages, c.stream)
+        """Keys and values [n, Hkv, hd] (heads contiguous, rows any multiple of 16
+        bytes apart) into their slots (mh_kv_store_paged): ``k_cache`` [pages,
+        Hkv, page, hd] and ``v_cache`` [pages, Hkv, hd, page] of 8-bit
+        elements, scales [pages, Hkv] float32."""
+        op, d = "kv_store_paged", k.get_device()
+        kc, vc, ks, vs, n_pages, Hkv, page, hd = _pool(op, d, k_cache, v_cache, k_scale, v_scale)
+        shape = (_rank(op, d, "k", k, 3)[0], Hkv, hd)
+        dt = _float_dt(op, "k", k)
+        (kp, ldk), (vp, ldv) = _token_rows(op, d, "k", k, k.dtype, shape), _token_rows(op, d, "v", v, k.dtype, shape)
+        _launch("mh_kv_store_paged", d, dt, kp, vp, ldk, ldv, _operand(op, d, "slots", slots, _torch().int32, shape[:1]), kc, vc, ks,
+                vs, shape[0], Hkv, hd, page, n_pages)
 
     def attention_paged_workspace(self, q, k_cache, lens, max_q, max_len, window=0) -> int:
         """Bytes of workspace that ``attention_paged`` needs for these sizes."""
         n = ctypes.c_size_t()
-        call("mh_attention_paged_workspace", _float_dt("attention_paged", q), lens.shape[0], q.shape[0], q.shape[1],
-             k_cache.shape[1], q.shape[2], max_q, max_len, window, ctypes.byref(n))
+        rows, Hq, hd = q.shape
+        call("mh_attention_paged_workspace", _float_dt("attention_paged", "q", q), lens.shape[0], rows, Hq, k_cache.shape[1], hd,
+             max_q, max_len, window, ctypes.byref(n))
         return n.value
 
     def attention_paged(self, q, k_cache, v_cache, k_scale, v_scale, tables, lens, cu, out, max_q, max_len, causal=True,
                         window=0, scale=None, workspace=None):
         """Attention of ragged queries over the paged cache (mh_attention_paged):
-        request b's queries are rows cu[b]..cu[b+1]-1 of ``q`` and ``out`` [rows, Hq,
-        hd], the last of its lens[b] tokens; ``tables`` [B, width].  ``scale`` None:
-        1 / sqrt(hd).  ``workspace``: a uint8 tensor of
+        request b's queries are rows cu[b]..cu[b+1]-1 of ``q`` and ``out`` [rows,
+        Hq, hd], the last of its lens[b] tokens; ``tables`` [B, width].
+        ``scale`` None: 1 / sqrt(hd).  ``workspace``: a uint8 tensor of
         ``attention_paged_workspace`` bytes, else one is allocated."""
-        B = _size("attention_paged", "lens", lens, 0)
-        with _Call("attention_paged", q=q, k_cache=k_cache, v_cache=v_cache, k_scale=k_scale, v_scale=v_scale, tables=tables,
-                   lens=lens, cu=cu, out=out, workspace=workspace) as c:
-            n_pages, Hkv, page, hd = c.pool()
-            c.shape("q", (None, None, hd)).shape("out", tuple(q.shape)).shape("tables", (B, None)).shape("cu", (B + 1,))
-            c.int32("tables", "lens", "cu").contiguous("tables", "lens", "cu", "workspace")
-            if out.dtype != q.dtype:
-                raise ValueError("attention_paged: q and out must have one type")
-            if scale is not None and not float(scale):
-                raise ValueError("attention_paged: scale 0 (None is 1 / sqrt(hd))")
-            need = self.attention_paged_workspace(q, k_cache, lens, max_q, max_len, window)
-            workspace = c.workspace(workspace, need)
-            call("mh_attention_paged", _float_dt("attention_paged", q), _p(q), c.row_stride("q"), _p(k_cache), _p(v_cache), _p(k_scale),
-                 _p(v_scale), _p(tables), _p(lens), _p(cu), _p(out), c.row_stride("out"), B, q.shape[0], q.shape[1], Hkv, hd,
-                 page, n_pages, tables.shape[1], max_q, max_len, int(causal), window, 0.0 if scale is None else float(scale),
-                 _p(workspace), _nbytes(workspace), c.stream)
+        op, d, i32 = "attention_paged", q.get_device(), _torch().int32
+        kc, vc, ks, vs, n_pages, Hkv, page, hd = _pool(op, d, k_cache, v_cache, k_scale, v_scale)
+        shape = (rows, Hq, _) = _rank(op, d, "q", q, 3)
+        (B,), (_, width) = _rank(op, d, "lens", lens, 1), _rank(op, d, "tables", tables, 2)
+        dt = _float_dt(op, "q", q)
+        (qp, ldq), (po, ldo) = _token_rows(op, d, "q", q, q.dtype, (rows, Hq, hd)), _token_rows(op, d, "out", out, q.dtype, shape)
+        if scale is None:
+            scale = 0.0
+        elif not scale:
+            raise ValueError("attention_paged: scale 0 (None is 1 / sqrt(hd))")
+        workspace, wp, wn = _workspace(op, d, workspace,
+                                       lambda: self.attention_paged_workspace(q, k_cache, lens, max_q, max_len, window))
+        _launch("mh_attention_paged", d, dt, qp, ldq, kc, vc, ks, vs, _operand(op, d, "tables", tables, i32, (B, width)),
+                _operand(op, d, "lens", lens, i32, (B,)), _operand(op, d, "cu", cu, i32, (B + 1,)), po, ldo, B, rows, Hq, Hkv, hd, page,
+                n_pages, width, max_q, max_len, causal, window, scale, wp, wn)
 
     # ---- sampling (no MuNet counterpart) ---------------------------------------
     def sample_workspace(self, logits) -> int:
         """Bytes of workspace that ``sample`` needs for these logits."""
         n = ctypes.c_size_t()
-        call("mh_sample_workspace", _float_dt("sample", logits), logits.shape[0], logits.shape[1], ctypes.byref(n))
+        rows, cols = logits.shape
+        call("mh_sample_workspace", _float_dt("sample", "logits", logits), rows, cols, ctypes.byref(n))
         return n.value
 
     def sample(self, logits, u, out, temperature=None, top_k=None, top_p=None, min_p=None, logprob=None, workspace=None):
         """One token per row of ``logits`` [rows, cols], drawn with the uniform
-        numbers ``u`` [rows] (mh_sample): ``out`` [rows] int32; ``temperature``, ``top_p``,
-        ``min_p`` float32 and ``top_k`` int32 [rows], or None; ``logprob`` [rows] float32
-        optional.  ``workspace``: a uint8 tensor of ``sample_workspace`` bytes,
-        else one is allocated."""
-        rows = _size("sample", "logits", logits, 0)
-        with _Call("sample", logits=logits, u=u, out=out, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p,
-                   logprob=logprob, workspace=workspace) as c:
-            c.shape("logits", (rows, None))
-            for name in ("u", "out", "temperature", "top_k", "top_p", "min_p", "logprob"):
-                c.shape(name, (rows,))
-            c.contiguous("u", "out", "temperature", "top_k", "top_p", "min_p", "logprob", "workspace")
-            c.int32("out", "top_k").float32("u", "temperature", "top_p", "min_p", "logprob")
-            if logits.shape[1] > 1 and logits.stride(1) != 1:
-                raise ValueError("sample: logits must be contiguous along a row")
-            ld = logits.stride(0) if rows > 1 else logits.shape[1]
-            workspace = c.workspace(workspace, self.sample_workspace(logits))
-            call("mh_sample", _float_dt("sample", logits), _p(logits), ld, rows, logits.shape[1], _p(u), _p(temperature),
-                 _p(top_k), _p(top_p), _p(min_p), _p(out), _p(logprob), _p(workspace), _nbytes(workspace), c.stream)
+        numbers ``u`` [rows] (mh_sample): ``out`` [rows] int32; ``temperature``,
+        ``top_p``, ``min_p`` float32 and ``top_k`` int32 [rows], or None;
+        ``logprob`` [rows] float32 optional.  ``workspace``: a uint8 tensor of
+        ``sample_workspace`` bytes, else one is allocated."""
+        op, d, t = "sample", logits.get_device(), _torch()
+        rows, cols = _rank(op, d, "logits", logits, 2)
+        dt, f32, each = _float_dt(op, "logits", logits), t.float32, (rows,)
+        ld, e = logits.stride()
+        if e != 1 and cols > 1:
+            raise ValueError("sample: logits must be contiguous along a row")
+        workspace, wp, wn = _workspace(op, d, workspace, lambda: self.sample_workspace(logits))
+        _launch("mh_sample", d, dt, logits.data_ptr(), ld if rows > 1 else cols, rows, cols, _operand(op, d, "u", u, f32, each),
+                _optional(op, d, "temperature", temperature, f32, each), _optional(op, d, "top_k", top_k, t.int32, each),
+                _optional(op, d, "top_p", top_p, f32, each), _optional(op, d, "min_p", min_p, f32, each),
+                _operand(op, d, "out", out, t.int32, each), _optional(op, d, "logprob", logprob, f32, each), wp, wn)
 
     # ---- shape (backend.hpp:263-271) ---------------------------------------
     def concat(self, inputs, out, dim, shapes):

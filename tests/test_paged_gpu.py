@@ -592,14 +592,14 @@ def test_wrapper_refusals(torch, hip):
     out = torch.empty_like(q)
     base = dict(q=q, k_cache=c.kc, v_cache=c.vc, k_scale=c.ks, v_scale=c.vs, tables=c.d_tables, lens=c.d_lens, cu=c.d_cu, out=out,
                 max_q=1, max_len=40)
-    for change, match in ((dict(v_cache=c.kc), "v_cache must be of shape"), (dict(q=q.double()), "float32, float16|one type"),
-                          (dict(out=out.float()), "one type"), (dict(tables=c.d_tables.long()), "int32"),
+    for change, match in ((dict(v_cache=c.kc), "v_cache must be of shape"), (dict(q=q.double()), "float32 or float16"),
+                          (dict(out=out.float()), "out must be bfloat16"), (dict(tables=c.d_tables.long()), "int32"),
                           (dict(k_scale=c.ks.half()), "float32"), (dict(cu=c.d_cu[:1]), "shape"), (dict(lens=c.d_lens.cpu()), "one GPU"),
                           (dict(q=q.transpose(1, 2)), "shape"), (dict(k_cache=c.kc.float()), "uint8"), (dict(scale=0.0), "scale 0"),
                           (dict(q=torch.empty((1, 64, 4), dtype=q.dtype, device="cuda").transpose(1, 2)), "contiguous")):
         with pytest.raises(ValueError, match=match):
             hip.attention_paged(**{**base, **change})
-    with pytest.raises(ValueError, match="one type"):
+    with pytest.raises(ValueError, match="v must be bfloat16"):
         hip.kv_store_paged(q[:, :2], q[:, :2].float(), c.d_lens, c.kc, c.vc, c.ks, c.vs)
     with pytest.raises(ValueError, match="slots must be of shape"):
         hip.kv_store_paged(q[:, :2], q[:, :2], c.d_cu, c.kc, c.vc, c.ks, c.vs)

@@ -220,7 +220,7 @@ def test_agrees_with_argmax(torch, hip):
 
 def test_wrapper_refusals(torch, hip):
     x, u, out = torch.zeros((2, 8), device="cuda"), torch.zeros(2, device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda")
-    for args, kw, match in (((x.double(), u, out), {}, "float32, float16"), ((x, u[:1], out), {}, "u must be of shape"),
+    for args, kw, match in (((x.double(), u, out), {}, "float32 or float16"), ((x, u[:1], out), {}, "u must be of shape"),
                             ((x, u, out.long()), {}, "int32"), ((x, u.double(), out), {}, "float32"),
                             ((x, u, out), dict(top_k=u), "int32"), ((x, u, out), dict(top_p=out), "float32"),
                             ((x.t().contiguous().t(), u, out), {}, "contiguous along a row"), ((x, u.cpu(), out), {}, "one GPU"),
