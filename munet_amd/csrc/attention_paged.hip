@@ -79,65 +79,41 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
   return (x >> 7) & 0x01010101u;
 }
 
-// NQ 16-row tiles of one (sequence, key/value head).  WIDE: the four waves take
-// different rows and the same keys (many rows); else the same rows, and every
-// fourth block of the keys each (few rows).
-template <int DT, int HDP, int NQ, bool WIDE>
-__global__ void __launch_bounds__(256) attn_paged_kernel(PagedArgs a) {
-  typedef Store<DT> S;
-  typedef typename S::T T;
-  constexpr int NP = DT == F32 ? 2 : 1;  // fp16 parts of q and of the probabilities
-  constexpr int J = HDP / 64, MT = HDP / 16;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
-  int id = blockIdx.x;
-  const int tile0 = id % a.tiles;
-  id /= a.tiles;
-  const int split = id % a.splits;
-  id /= a.splits;
-  const int kvh = id % a.Hkv, b = id / a.Hkv;
+// The query rows of a wave: NQ tiles of 16 (column n of tile x is row r_first + 16 x
+// + n of the packed rows; past the last row, that row again, not stored), their
+// running softmax and their outputs O^T.
+template <int DT, int HDP, int NQ> struct RowTiles {
+  typedef typename Store<DT>::T T;
+  static constexpr int NP = DT == F32 ? 2 : 1;  // fp16 parts of q and of the probabilities
+  static constexpr int KS = HDP / 32, MT = HDP / 16, RW = 16 * NQ;
+  f16x8 qf[NP][NQ][KS];
+  f16x8 pf[NP][NQ][2];
+  f32x4 acc[MT][NQ];
+  float c_row[NQ], mx[NQ], l[NQ];
+  float lref[NQ];  // log2 of the largest value scale that the row has seen
+  int lo_row[NQ], hi_row[NQ];
+  uint32_t ok[NQ];  // bit e: the row sees key 16 g + e of the block
+  int every_lo, every_hi;  // keys that every row sees
+  int some_lo, some_hi;    // keys that some row sees
 
-  const int P = 1 << a.plog;
-  // (lengths past the block table's pages, and rows past the buffer, are cut)
-  const int most = a.width << a.plog, len = min(max(a.lens[b], 0), most);
-  const int row0 = a.cu[b], nq = min(a.cu[b + 1], a.n_rows) - row0;
-  if (row0 < 0 || nq <= 0) return;
-  if (a.lens[b] > most && tid == 0) atomicOr(a.err, kErrPage);
-  const int rows = nq * a.G;
-  const int32_t *table = a.tables + long(b) * a.width;
-  constexpr int RW = 16 * NQ;               // rows per wave
-  constexpr int RB = WIDE ? 4 * RW : RW;    // rows per workgroup
-
-  // The merge of the four waves' shares (narrow form): 128 head values at a time.
-  constexpr int MW = HDP < 128 ? HDP : 128, LD = MW + 4;
-  __shared__ __align__(16) float wo[WIDE ? 1 : 4][WIDE ? 1 : RW][WIDE ? 4 : LD];
-  __shared__ float2 wml[WIDE ? 1 : 4][WIDE ? 1 : RW];
-
-  // (more tiles than the launch was sized for are walked)
-  for (int tile = tile0; long(tile) * RB < rows; tile += a.tiles) {
-    const int r_first = tile * RB + (WIDE ? wave * RW : 0);
-    if (WIDE && r_first >= rows) break;  // (no barrier in this form)
+  // head values d_of(s) .. + 7 are the operand of step s
+  template <class D>
+  __device__ __forceinline__ void start(const PagedArgs &a, int row0, int nq, int len, int rows, int r_first, int kvh, int n,
+                                        KeyRange mine, D d_of) {
     const int i0 = r_first / a.G, i1 = (min(r_first + RW, rows) - 1) / a.G;
     const KeyRange all = seen_keys(len, nq, i0, i1, a.causal, a.window);
-    const KeyRange mine = key_share(all, split, a.splits, a.chunk);
-    // keys that every row of the wave sees: [every_lo, every_hi)
-    const int every_lo = seen_keys(len, nq, i1, i1, a.causal, a.window).lo;
-    const int every_hi = seen_keys(len, nq, i0, i0, a.causal, a.window).hi;
-
-    // the wave's queries: column n of tile x is row r_first + 16 x + n (past the
-    // end: the last row again, not stored)
-    f16x8 qf[NP][NQ][2 * J];
-    float c_row[NQ], mx[NQ], l[NQ];
-    float lref[NQ];  // log2 of the largest value scale that the row has seen
-    int hi_row[NQ], lo_row[NQ];
-    f32x4 acc[MT][NQ];
+    every_lo = max(seen_keys(len, nq, i1, i1, a.causal, a.window).lo, mine.lo);
+    every_hi = min(seen_keys(len, nq, i0, i0, a.causal, a.window).hi, mine.hi);
+    some_lo = max(all.lo, mine.lo);
+    some_hi = min(all.hi, mine.hi);
 #pragma unroll
     for (int x = 0; x < NQ; ++x) {
       const int r = min(r_first + 16 * x + n, rows - 1), i = r / a.G, h = kvh * a.G + r - i * a.G;
       const T *qp = static_cast<const T *>(a.q) + long(row0 + i) * a.ldq + long(h) * a.hd;
-      float v[2 * J][8], big = 0.f;
+      float v[KS][8], big = 0.f;
 #pragma unroll
-      for (int s = 0; s < 2 * J; ++s) {
-        const int d = 64 * (s >> 1) + 16 * g + 8 * (s & 1);
+      for (int s = 0; s < KS; ++s) {
+        const int d = d_of(s);
         if (d < a.hd) {
           if constexpr (DT == F32) {
             ld4<F32>(qp + d, v[s]);
@@ -162,7 +138,7 @@ __global__ void __launch_bounds__(256) attn_paged_kernel(PagedArgs a) {
       const float up = __uint_as_float(uint32_t(k + 127) << 23);
       c_row[x] = a.c * __uint_as_float(uint32_t(127 - k) << 23);
 #pragma unroll
-      for (int s = 0; s < 2 * J; ++s) {
+      for (int s = 0; s < KS; ++s) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const float w = v[s][e] * up;
@@ -180,9 +156,196 @@ __global__ void __launch_bounds__(256) attn_paged_kernel(PagedArgs a) {
 #pragma unroll
       for (int i = 0; i < MT; ++i) acc[i][x] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
+  }
 
-    const int step = WIDE ? kKeyBlock : 4 * kKeyBlock;
-    for (int base = (mine.lo & ~(kKeyBlock - 1)) + (WIDE ? 0 : wave * kKeyBlock); base < mine.hi; base += step) {
+  // Raw scores of a block (this lane group's keys tv .. tv + 15, with their
+  // page's key scale and log2 of its value scale) to probabilities pf; the sums
+  // and outputs so far scaled to the new maximum.  MASKED: some row does not
+  // see some key.
+  template <bool MASKED>
+  __device__ __forceinline__ void probabilities(f32x4 (&s)[4][NQ], float ksc, float lv, bool page_ok, int tv) {
+    const float lv_block = MASKED ? 0.f : xor32_max(xor16_max(lv));
+#pragma unroll
+    for (int x = 0; x < NQ; ++x) {
+      ok[x] = 0xffffu;
+      if constexpr (MASKED) {
+        const int lo = min(max(lo_row[x] - tv, 0), 16), hi = min(max(hi_row[x] - tv, 0), 16);
+        ok[x] = page_ok ? ((1u << hi) - 1u) & ~((1u << lo) - 1u) : 0u;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s[t][x][r] = (ok[x] >> (4 * t + r)) & 1u ? s[t][x][r] : -__builtin_inff();
+      }
+      // the value scales: this lane group's over the largest that the row has seen
+      const float lnew = fmaxf(MASKED ? xor32_max(xor16_max(ok[x] ? lv : -126.f)) : lv_block, lref[x]);
+      const float lf = !MASKED || ok[x] ? lv - lnew : 0.f;
+      const float rescale = lnew == lref[x] ? 1.f : __builtin_amdgcn_exp2f(lref[x] - lnew);
+      const float unscale = __builtin_amdgcn_exp2f(-lf), scale14 = __builtin_amdgcn_exp2f(lf + 14.f);
+      lref[x] = lnew;
+      // (a page's scale is positive: the largest raw score is the largest score)
+      float f = ksc * c_row[x];
+      float top = s[0][x][0];
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) top = fmaxf(top, s[t][x][r]);
+      top = top > -__builtin_inff() ? top * f : -__builtin_inff();
+      top = fmaxf(xor32_max(xor16_max(top)), mx[x]);
+      float ref = top > -__builtin_inff() ? top : 0.f;
+      const float down = mx[x] == top ? 1.f : __builtin_amdgcn_exp2f(mx[x] - ref);
+      mx[x] = top;
+      if (__any(down * rescale != 1.f)) {
+        l[x] *= down;
+#pragma unroll
+        for (int i = 0; i < MT; ++i) acc[i][x] *= down * rescale;
+      }
+      // The product below is not rounded before the maximum, which is, goes off it.
+      // Where that could leave much (scores past 2^16), both are rounded.
+      const bool far = __builtin_fabsf(ref) > 65536.f;
+      if (__any(far)) {
+#pragma clang fp contract(off)
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s[t][x][r] = far ? s[t][x][r] * f - ref : s[t][x][r];
+        f = far ? 1.f : f;
+        ref = far ? 0.f : ref;
+      }
+      float sum = 0.f;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+          float p[2];
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            const float raw = s[2 * u + (e >> 2)][x][(e & 3) + y];
+            // fp32: the difference from the maximum is rounded once, and the
+            // power of two applied to the result
+            float t = NP == 2 ? fmaf(raw, f, -ref) : fmaf(raw, f, lf + 14.f - ref);
+            if (MASKED) t = raw == -__builtin_inff() ? raw : t;
+            p[y] = __builtin_amdgcn_exp2f(t);
+            if constexpr (NP == 2) p[y] *= scale14;
+            sum += p[y];
+          }
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            const _Float16 h0 = _Float16(p[y]);
+            pf[0][x][u][e + y] = h0;
+            if constexpr (NP == 2) pf[1][x][u][e + y] = _Float16(p[y] - float(h0));
+          }
+        }
+      l[x] = fmaf(sum, unscale, l[x]);  // (2^14 w)
+    }
+  }
+
+  // O^T += V^T P^T for head rows 16 i .. 16 i + 15
+  __device__ __forceinline__ void values(int i, f16x8 v0, f16x8 v1) {
+#pragma unroll
+    for (int x = 0; x < NQ; ++x)
+#pragma unroll
+      for (int p = NP - 1; p >= 0; --p) {
+        acc[i][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pf[p][x][0], acc[i][x], 0, 0, 0);
+        acc[i][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pf[p][x][1], acc[i][x], 0, 0, 0);
+      }
+  }
+
+  // A NaN value that only some rows see must reach these alone, which a zero
+  // probability does not give: outputs of rows that see a marked value (m0, m1:
+  // 1 at a NaN value, 0 else) become NaN.
+  __device__ __forceinline__ void mark_nans(int i, f16x8 m0, f16x8 m1) {
+#pragma unroll
+    for (int x = 0; x < NQ; ++x) {
+      f16x8 s0, s1;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        s0[e] = (ok[x] >> e) & 1u ? _Float16(1.f) : _Float16(0.f);
+        s1[e] = (ok[x] >> (8 + e)) & 1u ? _Float16(1.f) : _Float16(0.f);
+      }
+      f32x4 hit = f32x4{0.f, 0.f, 0.f, 0.f};
+      hit = __builtin_amdgcn_mfma_f32_16x16x32_f16(m0, s0, hit, 0, 0, 0);
+      hit = __builtin_amdgcn_mfma_f32_16x16x32_f16(m1, s1, hit, 0, 0, 0);
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (hit[r] > 0.f) acc[i][x][r] = __builtin_nanf("");
+    }
+  }
+
+  // the sums over the lane groups, the outputs in the values' scale
+  __device__ __forceinline__ void finish() {
+#pragma unroll
+    for (int x = 0; x < NQ; ++x) {
+      l[x] = xor32_add(xor16_add(l[x]));
+#pragma unroll
+      for (int i = 0; i < MT; ++i) acc[i][x] *= __builtin_amdgcn_exp2f(lref[x]);
+    }
+  }
+};
+
+// Four head values d .. d + 3 of packed row r out: o / sum, or this share's (o,
+// maximum, sum) for the join.
+template <int DT>
+__device__ __forceinline__ void put(const PagedArgs &a, int row0, int kvh, int split, int r, int d, f32x4 o, float m, float sum) {
+  typedef typename Store<DT>::T T;
+  const int i = r / a.G, h = kvh * a.G + r - i * a.G;
+  if (a.splits == 1) {
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;  // (a row that sees no key is zero)
+    const float v[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
+    st4<DT>(static_cast<T *>(a.out) + long(row0 + i) * a.ldo + long(h) * a.hd + d, v);
+  } else {
+    const long at = ((long(row0) + i) * a.Hq + h) * a.splits + split;
+    if (!(sum == 0.f)) *reinterpret_cast<f32x4 *>(a.part_o + at * a.hd + d) = o;  // (the join skips empty shares)
+    if (d == 0) a.part_ml[at] = make_float2(m, sum);
+  }
+}
+
+// The part of a call that a workgroup is: request, its rows and keys (cut to the
+// table and the buffer).
+struct Part {
+  int split, kvh, b, len, row0, nq, rows;
+};
+__device__ __forceinline__ bool part_of(const PagedArgs &a, int id, Part &w) {
+  w.split = id % a.splits;
+  id /= a.splits;
+  w.kvh = id % a.Hkv;
+  w.b = id / a.Hkv;
+  const int most = a.width << a.plog, len = a.lens[w.b];
+  w.len = min(max(len, 0), most);
+  w.row0 = a.cu[w.b];
+  w.nq = min(a.cu[w.b + 1], a.n_rows) - w.row0;
+  if (w.row0 < 0 || w.nq <= 0) return false;
+  if (len > most && threadIdx.x == 0) atomicOr(a.err, kErrPage);
+  w.rows = w.nq * a.G;
+  return true;
+}
+
+// Few rows (a decode step): the four waves take the same 16 rows and every fourth
+// block of the keys each.  Keys and values go from memory straight into the
+// MFMA operands.
+template <int DT, int HDP>
+__global__ void __launch_bounds__(256) attn_paged_kernel(PagedArgs a) {
+  constexpr int J = HDP / 64, MT = HDP / 16, RW = 16;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
+  Part w;
+  if (!part_of(a, int(blockIdx.x) / a.tiles, w)) return;
+  const int P = 1 << a.plog;
+  const int32_t *table = a.tables + long(w.b) * a.width;
+  // The merge of the four waves' shares: 128 head values at a time.
+  constexpr int MW = HDP < 128 ? HDP : 128, LD = MW + 4;
+  __shared__ __align__(16) float wo[4][RW][LD];
+  __shared__ float2 wml[4][RW];
+
+  // (more tiles than the launch was sized for are walked)
+  for (int tile = int(blockIdx.x) % a.tiles; long(tile) * RW < w.rows; tile += a.tiles) {
+    const int r_first = tile * RW;
+    const int i0 = r_first / a.G, i1 = (min(r_first + RW, w.rows) - 1) / a.G;
+    const KeyRange mine = key_share(seen_keys(w.len, w.nq, i0, i1, a.causal, a.window), w.split, a.splits, a.chunk);
+    RowTiles<DT, HDP, 1> q;
+    // (the order of the head values in a step is that of the 16-byte runs in which
+    // a lane loads its keys)
+    q.start(a, w.row0, w.nq, w.len, w.rows, r_first, w.kvh, n, mine, [&](int s) { return 64 * (s >> 1) + 16 * g + 8 * (s & 1); });
+
+    for (int base = (mine.lo & ~(kKeyBlock - 1)) + wave * kKeyBlock; base < mine.hi; base += 4 * kKeyBlock) {
       // the pages of this lane's key rows (group n >> 2) and of its scores and
       // values (group g); a page outside the pool holds no keys (page 0 is read
       // in its place and masked)
@@ -193,8 +356,8 @@ __global__ void __launch_bounds__(256) attn_paged_kernel(PagedArgs a) {
       if (!page_ok && tv < mine.hi && n == 0) atomicOr(a.err, kErrPage);
       pk = page_in_pool(pk, a.n_pages) ? pk : 0;
       pv = page_ok ? pv : 0;
-      const uint8_t *kp = a.kc + page_base(pk, a.Hkv, kvh, P, a.hd) + long(tk & (P - 1)) * a.hd;
-      const uint8_t *vp = a.vc + page_base(pv, a.Hkv, kvh, P, a.hd) + (tv & (P - 1));
+      const uint8_t *kp = a.kc + page_base(pk, a.Hkv, w.kvh, P, a.hd) + long(tk & (P - 1)) * a.hd;
+      const uint8_t *vp = a.vc + page_base(pv, a.Hkv, w.kvh, P, a.hd) + (tv & (P - 1));
       uint4 kr[4][J], vr[MT];
 #pragma unroll
       for (int t = 0; t < 4; ++t)
@@ -206,115 +369,32 @@ __global__ void __launch_bounds__(256) attn_paged_kernel(PagedArgs a) {
 #pragma unroll
       for (int i = 0; i < MT; ++i)
         vr[i] = 16 * i < a.hd ? *reinterpret_cast<const uint4 *>(vp + (16 * i + n) * P) : make_uint4(0, 0, 0, 0);
-      const float ksc = a.ks[long(pv) * a.Hkv + kvh], vsc = a.vs[long(pv) * a.Hkv + kvh];
+      const float ksc = a.ks[long(pv) * a.Hkv + w.kvh], vsc = a.vs[long(pv) * a.Hkv + w.kvh];
 
-      // scores
-      f32x4 s[4][NQ];
+      f32x4 s[4][1];
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-#pragma unroll
-        for (int x = 0; x < NQ; ++x) s[t][x] = f32x4{0.f, 0.f, 0.f, 0.f};
+        s[t][0] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int j = 0; j < J; ++j) {
           const f16x8 k0 = cvt8(kr[t][j].x, kr[t][j].y), k1 = cvt8(kr[t][j].z, kr[t][j].w);
 #pragma unroll
-          for (int x = 0; x < NQ; ++x) {
-#pragma unroll
-            for (int p = NP - 1; p >= 0; --p) {
-              s[t][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, qf[p][x][2 * j], s[t][x], 0, 0, 0);
-              s[t][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, qf[p][x][2 * j + 1], s[t][x], 0, 0, 0);
-            }
+          for (int p = q.NP - 1; p >= 0; --p) {
+            s[t][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, q.qf[p][0][2 * j], s[t][0], 0, 0, 0);
+            s[t][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, q.qf[p][0][2 * j + 1], s[t][0], 0, 0, 0);
           }
         }
       }
-
       const float lv = page_ok ? fmaxf(__builtin_amdgcn_logf(vsc), -126.f) : -126.f;
+      const bool masked = base < q.every_lo || base + kKeyBlock > q.every_hi || __any(!page_ok);
+      if (masked) q.template probabilities<true>(s, ksc, lv, page_ok, tv);
+      else q.template probabilities<false>(s, ksc, lv, page_ok, tv);
 
-      // some row does not see every key of the block
-      const bool masked = base < max(every_lo, mine.lo) || base + kKeyBlock > min(every_hi, mine.hi) || __any(!page_ok);
-      f16x8 pf[NP][NQ][2];
-      uint32_t ok[NQ];
-#pragma unroll
-      for (int x = 0; x < NQ; ++x) {
-        ok[x] = 0xffffu;
-        if (masked) {
-          // keys tv + e, lo <= tv + e < hi
-          const int lo = min(max(lo_row[x] - tv, 0), 16), hi = min(max(hi_row[x] - tv, 0), 16);
-          ok[x] = page_ok ? ((1u << hi) - 1u) & ~((1u << lo) - 1u) : 0u;
-#pragma unroll
-          for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) s[t][x][r] = (ok[x] >> (4 * t + r)) & 1u ? s[t][x][r] : -__builtin_inff();
-        }
-        // the value scales: this lane group's over the largest that the row has seen
-        const float lnew = fmaxf(xor32_max(xor16_max(ok[x] ? lv : -126.f)), lref[x]), lf = ok[x] ? lv - lnew : 0.f;
-        const float rescale = lnew == lref[x] ? 1.f : __builtin_amdgcn_exp2f(lref[x] - lnew);
-        const float unscale = __builtin_amdgcn_exp2f(-lf), scale14 = __builtin_amdgcn_exp2f(lf + 14.f);
-        lref[x] = lnew;
-        // (a page's scale is positive: the largest raw score is the largest score)
-        float f = ksc * c_row[x];
-        float top = s[0][x][0];
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) top = fmaxf(top, s[t][x][r]);
-        top = top > -__builtin_inff() ? top * f : -__builtin_inff();
-        top = fmaxf(xor32_max(xor16_max(top)), mx[x]);
-        float ref = top > -__builtin_inff() ? top : 0.f;
-        const float down = mx[x] == top ? 1.f : __builtin_amdgcn_exp2f(mx[x] - ref);
-        mx[x] = top;
-        if (__any(down * rescale != 1.f)) {
-          l[x] *= down;
-#pragma unroll
-          for (int i = 0; i < MT; ++i) acc[i][x] *= down * rescale;
-        }
-        // The product below is not rounded before the maximum, which is, goes off it.
-        // Where that could leave much (scores past 2^16), both are rounded.
-        const bool far = __builtin_fabsf(ref) > 65536.f;
-        if (__any(far)) {
-#pragma clang fp contract(off)
-#pragma unroll
-          for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) s[t][x][r] = far ? s[t][x][r] * f - ref : s[t][x][r];
-          f = far ? 1.f : f;
-          ref = far ? 0.f : ref;
-        }
-        float sum = 0.f;
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int e = 0; e < 8; e += 2) {
-            float p[2];
-#pragma unroll
-            for (int y = 0; y < 2; ++y) {
-              const float raw = s[2 * u + (e >> 2)][x][(e & 3) + y];
-              // fp32: the difference from the maximum is rounded once, and the
-              // power of two applied to the result
-              float t = NP == 2 ? fmaf(raw, f, -ref) : fmaf(raw, f, lf + 14.f - ref);
-              if (masked) t = raw == -__builtin_inff() ? raw : t;
-              p[y] = __builtin_amdgcn_exp2f(t);
-              if constexpr (NP == 2) p[y] *= scale14;
-              sum += p[y];
-            }
-#pragma unroll
-            for (int y = 0; y < 2; ++y) {
-              const _Float16 h0 = _Float16(p[y]);
-              pf[0][x][u][e + y] = h0;
-              if constexpr (NP == 2) pf[1][x][u][e + y] = _Float16(p[y] - float(h0));
-            }
-          }
-        l[x] = fmaf(sum, unscale, l[x]);  // (2^14 w)
-      }
-
-      // values.  Keys that no row sees may hold anything, NaN among it: their
-      // bytes are cleared.  A NaN value that only some rows see must reach
-      // these alone, which a zero probability does not give: such a block (one
-      // at the edge of the mask with a NaN byte) clears the NaN bytes and marks
-      // the outputs of the rows that see them.
+      // Keys that no row sees may hold anything, NaN among it: their bytes are
+      // cleared.
       bool nans = false;
       if (masked) {
-        const int lo = min(max(max(all.lo, mine.lo) - tv, 0), 16), hi = page_ok ? min(max(min(all.hi, mine.hi) - tv, 0), 16) : 0;
+        const int lo = min(max(q.some_lo - tv, 0), 16), hi = page_ok ? min(max(q.some_hi - tv, 0), 16) : 0;
         uint32_t any = 0;
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
@@ -326,113 +406,241 @@ __global__ void __launch_bounds__(256) attn_paged_kernel(PagedArgs a) {
       if (nans) {
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
-          uint32_t w[4] = {vr[i].x, vr[i].y, vr[i].z, vr[i].w}, mark[4];
+          uint32_t b[4] = {vr[i].x, vr[i].y, vr[i].z, vr[i].w}, mark[4];
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            const uint32_t nb = nan_bytes(w[c]);
-            w[c] &= ~(nb * 0xffu);
+            const uint32_t nb = nan_bytes(b[c]);
+            b[c] &= ~(nb * 0xffu);
             mark[c] = nb * 0x38u;  // e4m3 1.0
           }
-          vr[i] = make_uint4(w[0], w[1], w[2], w[3]);
-          const f16x8 m0 = cvt8(mark[0], mark[1]), m1 = cvt8(mark[2], mark[3]);
-#pragma unroll
-          for (int x = 0; x < NQ; ++x) {
-            f16x8 s0, s1;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              s0[e] = (ok[x] >> e) & 1u ? _Float16(1.f) : _Float16(0.f);
-              s1[e] = (ok[x] >> (8 + e)) & 1u ? _Float16(1.f) : _Float16(0.f);
-            }
-            f32x4 hit = f32x4{0.f, 0.f, 0.f, 0.f};
-            hit = __builtin_amdgcn_mfma_f32_16x16x32_f16(m0, s0, hit, 0, 0, 0);
-            hit = __builtin_amdgcn_mfma_f32_16x16x32_f16(m1, s1, hit, 0, 0, 0);
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (hit[r] > 0.f) acc[i][x][r] = __builtin_nanf("");
-          }
+          vr[i] = make_uint4(b[0], b[1], b[2], b[3]);
+          q.mark_nans(i, cvt8(mark[0], mark[1]), cvt8(mark[2], mark[3]));
         }
       }
 #pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        const f16x8 v0 = cvt8(vr[i].x, vr[i].y), v1 = cvt8(vr[i].z, vr[i].w);
+      for (int i = 0; i < MT; ++i) q.values(i, cvt8(vr[i].x, vr[i].y), cvt8(vr[i].z, vr[i].w));
+    }
+    q.finish();
+
+    // the four waves' shares of the keys, in wave order
+    if (g == 0) wml[wave][n] = make_float2(q.mx[0], q.l[0]);
 #pragma unroll
-        for (int x = 0; x < NQ; ++x)
+    for (int part = 0; part < HDP / MW; ++part) {
 #pragma unroll
-          for (int p = NP - 1; p >= 0; --p) {
-            acc[i][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pf[p][x][0], acc[i][x], 0, 0, 0);
-            acc[i][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pf[p][x][1], acc[i][x], 0, 0, 0);
+      for (int i = 0; i < MW / 16; ++i) *reinterpret_cast<f32x4 *>(&wo[wave][n][16 * i + 4 * g]) = q.acc[part * (MW / 16) + i][0];
+      __syncthreads();
+      for (int e = tid; e < RW * (MW / 4); e += 256) {
+        const int rr = e / (MW / 4), d = 4 * (e % (MW / 4)), r = r_first + rr;
+        if (r < w.rows && part * MW + d < a.hd) {
+          float top = wml[0][rr].x;
+#pragma unroll
+          for (int v = 1; v < 4; ++v) top = fmaxf(top, wml[v][rr].x);
+          float sum = 0.f;
+          f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            const float2 ml = wml[v][rr];
+            if (ml.y == 0.f) continue;  // (this wave saw no key)
+            const float f = ml.x == top ? 1.f : __builtin_amdgcn_exp2f(ml.x - top);
+            sum = fmaf(ml.y, f, sum);
+            const f32x4 y = *reinterpret_cast<const f32x4 *>(&wo[v][rr][d]);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) o[c] = fmaf(y[c], f, o[c]);
           }
+          put<DT>(a, w.row0, w.kvh, w.split, r, part * MW + d, o, top, sum);
+        }
       }
+      __syncthreads();
     }
+  }
+}
 
-    // the values' scale, and the rows' sums over the lane groups
+// Many rows (prompts): eight waves of NQ tiles each share every block of keys.
+// The workgroup converts a block to fp16 once, into LDS (two buffers: the next
+// block's bytes are on their way while this one is multiplied), from where each
+// wave reads its operands.
+// LDS rows are swizzled in 16-byte chunks so that the 16 rows that a lane group
+// reads at a time lie in different banks: keys as tile rows 16 t + m (m the
+// operand's row), chunk c at c ^ (row & 15) (rows of 128 bytes: c ^ (row >> 1 & 7),
+// as for the values, rows of a head value's 64 keys).
+template <int DT, int HDP, int NQ>
+__global__ void __launch_bounds__(512, 2) attn_paged_wide_kernel(PagedArgs a) {
+  constexpr int MT = HDP / 16, RW = 16 * NQ, RB = 8 * RW;
+  constexpr int XK = HDP / 16;                  // 16-byte pieces of a key in the cache
+  constexpr int NK = 64 * XK, CH = 2 * NK / 512;  // pieces of a block's keys; pieces (keys and values) per thread
+  constexpr int KROW = HDP * 2, KB = 64 * KROW, VB = HDP * 128;
+  __shared__ __align__(16) uint8_t lds[2][KB + VB];
+  __shared__ float4 info[2][4];     // per lane group: key scale, log2 of the value scale, page in the pool
+  __shared__ uint32_t dirty[2][8];  // a NaN byte among the values
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
+  Part w;
+  if (!part_of(a, int(blockIdx.x) / a.tiles, w)) return;
+  const int P = 1 << a.plog;
+  const int32_t *table = a.tables + long(w.b) * a.width;
+  auto k_at = [](int row, int c) { return row * KROW + 16 * (KROW == 128 ? c ^ ((row >> 1) & 7) : c ^ (row & 15)); };
+  auto v_at = [](int row, int c) { return KB + row * 128 + 16 * (c ^ ((row >> 1) & 7)); };
+
+  // this thread's pieces: of the keys (row, 16 head values) or the values (head
+  // value, 16 keys; neighbours within a page follow each other)
+  const int ql = min(a.plog - 4, 2);  // log2 of the lane groups per page and block
+  struct Piece {
+    bool key, live;
+    int grp, off, l0, l1;  // lane group of the keys, byte within the page's keys or values, LDS bytes
+  } pc[CH];
 #pragma unroll
-    for (int x = 0; x < NQ; ++x) {
-      l[x] = xor32_add(xor16_add(l[x]));
-#pragma unroll
-      for (int i = 0; i < MT; ++i) acc[i][x] *= __builtin_amdgcn_exp2f(lref[x]);
+  for (int i = 0; i < CH; ++i) {
+    const int e = tid + 512 * i;
+    pc[i].key = e < NK;
+    if (e < NK) {
+      const int row = e / XK, x = e % XK, R = 16 * ((row >> 2) & 3) + 4 * (row >> 4) + (row & 3);
+      pc[i].grp = row >> 4;
+      pc[i].live = 16 * x < a.hd;
+      pc[i].off = (row & 15) * a.hd + 16 * x;
+      pc[i].l0 = k_at(R, 2 * x);
+      pc[i].l1 = k_at(R, 2 * x + 1);
+    } else {
+      const int f = e - NK, lo = f & ((1 << ql) - 1), row = (f >> ql) % HDP, grp = ((f >> ql) / HDP << ql) + lo;
+      pc[i].grp = grp;
+      pc[i].live = row < a.hd;
+      pc[i].off = row * P;
+      pc[i].l0 = v_at(row, 2 * grp);
+      pc[i].l1 = v_at(row, 2 * grp + 1);
     }
+  }
 
-    // rows out: o = acc / l, or this share's (acc, maximum, l)
-    auto put = [&](int r, int d, f32x4 o, float m, float sum) {
-      const int i = r / a.G, h = kvh * a.G + r - i * a.G;
-      if (a.splits == 1) {
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;  // (a row that sees no key is zero)
-        const float v[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
-        st4<DT>(static_cast<T *>(a.out) + long(row0 + i) * a.ldo + long(h) * a.hd + d, v);
-      } else {
-        const long at = ((long(row0) + i) * a.Hq + h) * a.splits + split;
-        if (!(sum == 0.f)) *reinterpret_cast<f32x4 *>(a.part_o + at * a.hd + d) = o;  // (the join skips empty shares)
-        if (d == 0) a.part_ml[at] = make_float2(m, sum);
+  for (int tile = a.tiles - 1 - int(blockIdx.x) % a.tiles; long(tile) * RB < w.rows; tile += a.tiles) {
+    const int R0 = tile * RB, r_first = R0 + wave * RW;
+    const int i0 = R0 / a.G, i1 = (min(R0 + RB, w.rows) - 1) / a.G;
+    const KeyRange all = seen_keys(w.len, w.nq, i0, i1, a.causal, a.window);
+    const KeyRange mine = key_share(all, w.split, a.splits, a.chunk);
+    const int some_lo = max(all.lo, mine.lo), all_hi = min(seen_keys(w.len, w.nq, i0, i0, a.causal, a.window).hi, mine.hi),
+              all_lo = max(seen_keys(w.len, w.nq, i1, i1, a.causal, a.window).lo, mine.lo);
+    const bool on = r_first < w.rows;
+    RowTiles<DT, HDP, NQ> q;
+    if (on) q.start(a, w.row0, w.nq, w.len, w.rows, r_first, w.kvh, n, mine, [&](int s) { return 32 * s + 8 * g; });
+
+    const int first = mine.lo & ~(kKeyBlock - 1);
+    auto page_of = [&](int base, int grp) {  // -1: no such page, or no key in range
+      const int t = base + 16 * grp;
+      const int p = t < mine.hi && (t >> a.plog) < a.width ? table[t >> a.plog] : -1;
+      return page_in_pool(p, a.n_pages) ? p : -1;
+    };
+    int page[CH], ipage = -1;
+    uint4 raw[CH];
+    float isc = 0.f, ivs = 0.f;
+    auto ask = [&](int base) {  // pages of the block
+#pragma unroll
+      for (int i = 0; i < CH; ++i) page[i] = page_of(base, pc[i].grp);
+      if (tid < 4) ipage = page_of(base, tid);
+    };
+    auto fetch = [&](int base) {  // its bytes and scales
+#pragma unroll
+      for (int i = 0; i < CH; ++i) {
+        raw[i] = make_uint4(0, 0, 0, 0);
+        const int at = (base + 16 * pc[i].grp) & (P - 1);
+        if (page[i] >= 0 && pc[i].live)
+          raw[i] = *reinterpret_cast<const uint4 *>((pc[i].key ? a.kc + at * a.hd : a.vc + at) +
+                                                    page_base(page[i], a.Hkv, w.kvh, P, a.hd) + pc[i].off);
+      }
+      if (tid < 4) {
+        isc = ipage >= 0 ? a.ks[long(ipage) * a.Hkv + w.kvh] : 1.f;
+        ivs = ipage >= 0 ? a.vs[long(ipage) * a.Hkv + w.kvh] : 1.f;
       }
     };
-    if constexpr (WIDE) {
+    auto place = [&](int base, int ip, int buf) {  // into LDS as fp16
+      uint32_t any = 0;
+      const bool edge = base < all_lo || base + kKeyBlock > all_hi;
+#pragma unroll
+      for (int i = 0; i < CH; ++i) {
+        uint4 r = raw[i];
+        if (edge && !pc[i].key) {
+          const int t = base + 16 * pc[i].grp;
+          r = keep_bytes(r, min(max(some_lo - t, 0), 16), min(max(mine.hi - t, 0), 16));
+          any |= nan_bytes(r.x) | nan_bytes(r.y) | nan_bytes(r.z) | nan_bytes(r.w);
+        }
+        *reinterpret_cast<f16x8 *>(&lds[buf][pc[i].l0]) = cvt8(r.x, r.y);
+        *reinterpret_cast<f16x8 *>(&lds[buf][pc[i].l1]) = cvt8(r.z, r.w);
+      }
+      any = __any(any != 0);
+      if (lane == 0) dirty[buf][wave] = any;
+      if (tid < 4) {
+        if (ip < 0 && base + 16 * tid < mine.hi) atomicOr(a.err, kErrPage);
+        info[buf][tid] = make_float4(isc, ip >= 0 ? fmaxf(__builtin_amdgcn_logf(ivs), -126.f) : -126.f, ip >= 0 ? 1.f : 0.f, 0.f);
+      }
+    };
+
+    if (mine.lo < mine.hi) {
+      ask(first);
+      fetch(first);
+      int ip = ipage;
+      ask(first + kKeyBlock);
+      place(first, ip, 0);
+      __syncthreads();
+      int buf = 0;
+      for (int base = first; base < mine.hi; base += kKeyBlock, buf ^= 1) {
+        const bool more = base + kKeyBlock < mine.hi;
+        ip = ipage;
+        if (more) {
+          fetch(base + kKeyBlock);
+          ask(base + 2 * kKeyBlock);
+        }
+        if (on && base < q.some_hi && base + kKeyBlock > q.some_lo) {
+          const float4 in = info[buf][g];
+          const bool page_ok = in.z != 0.f;
+          const uint8_t *L = lds[buf];
+          f32x4 s[4][NQ];
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+#pragma unroll
+            for (int x = 0; x < NQ; ++x) s[t][x] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < HDP / 32; ++c) {
+              const f16x8 k = *reinterpret_cast<const f16x8 *>(L + k_at(16 * t + n, 4 * c + g));
+#pragma unroll
+              for (int x = 0; x < NQ; ++x)
+#pragma unroll
+                for (int p = q.NP - 1; p >= 0; --p)
+                  s[t][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q.qf[p][x][c], s[t][x], 0, 0, 0);
+            }
+          }
+          const bool masked = base < q.every_lo || base + kKeyBlock > q.every_hi || __any(!page_ok);
+          if (masked) q.template probabilities<true>(s, in.x, in.y, page_ok, base + 16 * g);
+          else q.template probabilities<false>(s, in.x, in.y, page_ok, base + 16 * g);
+          bool nans = false;
+          if (masked) nans = (dirty[buf][0] | dirty[buf][1] | dirty[buf][2] | dirty[buf][3] | dirty[buf][4] | dirty[buf][5] | dirty[buf][6] |
+                              dirty[buf][7]) != 0;
+#pragma unroll
+          for (int i = 0; i < MT; ++i) {
+            f16x8 v0 = *reinterpret_cast<const f16x8 *>(L + v_at(16 * i + n, 2 * g)),
+                  v1 = *reinterpret_cast<const f16x8 *>(L + v_at(16 * i + n, 2 * g + 1));
+            if (nans) {
+              f16x8 m0, m1;
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                m0[e] = v0[e] == v0[e] ? _Float16(0.f) : _Float16(1.f);
+                m1[e] = v1[e] == v1[e] ? _Float16(0.f) : _Float16(1.f);
+                v0[e] = v0[e] == v0[e] ? v0[e] : _Float16(0.f);
+                v1[e] = v1[e] == v1[e] ? v1[e] : _Float16(0.f);
+              }
+              q.mark_nans(i, m0, m1);
+            }
+            q.values(i, v0, v1);
+          }
+        }
+        if (more) place(base + kKeyBlock, ip, buf ^ 1);
+        __syncthreads();
+      }
+    }
+    if (on) {
+      q.finish();
 #pragma unroll
       for (int x = 0; x < NQ; ++x) {
         const int r = r_first + 16 * x + n;
-        if (r < rows) {
+        if (r < w.rows) {
 #pragma unroll
           for (int i = 0; i < MT; ++i)
-            if (16 * i < a.hd) put(r, 16 * i + 4 * g, acc[i][x], mx[x], l[x]);
+            if (16 * i < a.hd) put<DT>(a, w.row0, w.kvh, w.split, r, 16 * i + 4 * g, q.acc[i][x], q.mx[x], q.l[x]);
         }
-      }
-    } else {
-      // the four waves' shares of the keys, in wave order
-      if (g == 0) {
-#pragma unroll
-        for (int x = 0; x < NQ; ++x) wml[wave][16 * x + n] = make_float2(mx[x], l[x]);
-      }
-#pragma unroll
-      for (int part = 0; part < HDP / MW; ++part) {
-#pragma unroll
-        for (int x = 0; x < NQ; ++x)
-#pragma unroll
-          for (int i = 0; i < MW / 16; ++i)
-            *reinterpret_cast<f32x4 *>(&wo[wave][16 * x + n][16 * i + 4 * g]) = acc[part * (MW / 16) + i][x];
-        __syncthreads();
-        for (int e = tid; e < RW * (MW / 4); e += 256) {
-          const int rr = e / (MW / 4), d = 4 * (e % (MW / 4));
-          const int r = r_first + rr;
-          if (r < rows && part * MW + d < a.hd) {
-            float top = wml[0][rr].x;
-#pragma unroll
-            for (int w = 1; w < 4; ++w) top = fmaxf(top, wml[w][rr].x);
-            float sum = 0.f;
-            f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-              const float2 ml = wml[w][rr];
-              if (ml.y == 0.f) continue;  // (this wave saw no key)
-              const float f = ml.x == top ? 1.f : __builtin_amdgcn_exp2f(ml.x - top);
-              sum = fmaf(ml.y, f, sum);
-              const f32x4 v = *reinterpret_cast<const f32x4 *>(&wo[w][rr][d]);
-#pragma unroll
-              for (int c = 0; c < 4; ++c) o[c] = fmaf(v[c], f, o[c]);
-            }
-            put(r, part * MW + d, o, top, sum);
-          }
-        }
-        __syncthreads();
       }
     }
   }
@@ -476,13 +684,13 @@ paged_join_kernel(const float *__restrict__ part_o, const float2 *__restrict__ p
 template <int DT, int HDP>
 hipError_t launch(const PagedArgs &a, const PagedShape &s, hipStream_t st) {
   const long blocks = long(s.tiles) * s.splits * a.Hkv * a.B;
-  if (blocks * 256 > 0xffffffffL) return hipErrorInvalidValue;
+  if (blocks * 512 > 0xffffffffL) return hipErrorInvalidValue;
   const dim3 grid{unsigned(blocks)};
   constexpr int NQ = DT == F32 || HDP > 128 ? 1 : 2;
   if (s.wide)
-    hipLaunchKernelGGL((attn_paged_kernel<DT, HDP, NQ, true>), grid, dim3(256), 0, st, a);
+    hipLaunchKernelGGL((attn_paged_wide_kernel<DT, HDP, NQ>), grid, dim3(512), 0, st, a);
   else
-    hipLaunchKernelGGL((attn_paged_kernel<DT, HDP, 1, false>), grid, dim3(256), 0, st, a);
+    hipLaunchKernelGGL((attn_paged_kernel<DT, HDP>), grid, dim3(256), 0, st, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || s.splits == 1) return e;
   const int rpb = 256 / (a.hd / 4);
