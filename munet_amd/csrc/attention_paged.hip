@@ -282,22 +282,35 @@ template <int DT, int HDP, int NQ> struct RowTiles {
   }
 };
 
-// Four head values d .. d + 3 of packed row r out: o / sum, or this share's (o,
-// maximum, sum) for the join.
-template <int DT>
-__device__ __forceinline__ void put(const PagedArgs &a, int row0, int kvh, int split, int r, int d, f32x4 o, float m, float sum) {
+// Where a packed row's output goes: o / sum, or this share's (o, maximum, sum)
+// for the join.
+template <int DT> struct RowOut {
   typedef typename Store<DT>::T T;
-  const int i = r / a.G, h = kvh * a.G + r - i * a.G;
-  if (a.splits == 1) {
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;  // (a row that sees no key is zero)
-    const float v[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
-    st4<DT>(static_cast<T *>(a.out) + long(row0 + i) * a.ldo + long(h) * a.hd + d, v);
-  } else {
-    const long at = ((long(row0) + i) * a.Hq + h) * a.splits + split;
-    if (!(sum == 0.f)) *reinterpret_cast<f32x4 *>(a.part_o + at * a.hd + d) = o;  // (the join skips empty shares)
-    if (d == 0) a.part_ml[at] = make_float2(m, sum);
+  T *out;
+  float *part;
+  float inv;
+  __device__ __forceinline__ RowOut(const PagedArgs &a, int row0, int kvh, int split, int r, float m, float sum, bool first) {
+    const int i = r / a.G, h = kvh * a.G + r - i * a.G;
+    out = nullptr;
+    part = nullptr;
+    inv = sum == 0.f ? 0.f : 1.f / sum;  // (a row that sees no key is zero)
+    if (a.splits == 1) {
+      out = static_cast<T *>(a.out) + long(row0 + i) * a.ldo + long(h) * a.hd;
+    } else {
+      const long at = ((long(row0) + i) * a.Hq + h) * a.splits + split;
+      if (first) a.part_ml[at] = make_float2(m, sum);
+      if (!(sum == 0.f)) part = a.part_o + at * a.hd;  // (the join skips empty shares)
+    }
   }
-}
+  __device__ __forceinline__ void put(int d, f32x4 o) const {
+    if (out) {
+      const float v[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
+      st4<DT>(out + d, v);
+    } else if (part) {
+      *reinterpret_cast<f32x4 *>(part + d) = o;
+    }
+  }
+};
 
 // The part of a call that a workgroup is: request, its rows and keys (cut to the
 // table and the buffer).
@@ -447,7 +460,8 @@ __global__ void __launch_bounds__(256) attn_paged_kernel(PagedArgs a) {
 #pragma unroll
             for (int c = 0; c < 4; ++c) o[c] = fmaf(y[c], f, o[c]);
           }
-          put<DT>(a, w.row0, w.kvh, w.split, r, part * MW + d, o, top, sum);
+          const int at = part * MW + d;
+          RowOut<DT>(a, w.row0, w.kvh, w.split, r, top, sum, at == 0).put(at, o);
         }
       }
       __syncthreads();
@@ -471,7 +485,10 @@ __global__ void __launch_bounds__(512, 2) attn_paged_wide_kernel(PagedArgs a) {
   constexpr int KROW = HDP * 2, KB = 64 * KROW, VB = HDP * 128;
   __shared__ __align__(16) uint8_t lds[2][KB + VB];
   __shared__ float4 info[2][4];     // per lane group: key scale, log2 of the value scale, page in the pool
-  __shared__ uint32_t dirty[2][8];  // a NaN byte among the values
+  // NaN values of a block at the edge of some row's mask (they are zeros in
+  // LDS): bit k of nan_at, key k of the block
+  __shared__ uint64_t nan_at[2][HDP];
+  __shared__ uint32_t dirty[2][8];  // whether there are any
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
   Part w;
   if (!part_of(a, int(blockIdx.x) / a.tiles, w)) return;
@@ -485,7 +502,7 @@ __global__ void __launch_bounds__(512, 2) attn_paged_wide_kernel(PagedArgs a) {
   const int ql = min(a.plog - 4, 2);  // log2 of the lane groups per page and block
   struct Piece {
     bool key, live;
-    int grp, off, l0, l1;  // lane group of the keys, byte within the page's keys or values, LDS bytes
+    int grp, off, l0, l1, vrow;  // lane group of the keys, byte within the page's keys or values, LDS bytes
   } pc[CH];
 #pragma unroll
   for (int i = 0; i < CH; ++i) {
@@ -503,6 +520,7 @@ __global__ void __launch_bounds__(512, 2) attn_paged_wide_kernel(PagedArgs a) {
       pc[i].grp = grp;
       pc[i].live = row < a.hd;
       pc[i].off = row * P;
+      pc[i].vrow = row;
       pc[i].l0 = v_at(row, 2 * grp);
       pc[i].l1 = v_at(row, 2 * grp + 1);
     }
@@ -525,6 +543,8 @@ __global__ void __launch_bounds__(512, 2) attn_paged_wide_kernel(PagedArgs a) {
       const int p = t < mine.hi && (t >> a.plog) < a.width ? table[t >> a.plog] : -1;
       return page_in_pool(p, a.n_pages) ? p : -1;
     };
+    const uint8_t *kc = a.kc + page_base(0, a.Hkv, w.kvh, P, a.hd), *vc = a.vc + page_base(0, a.Hkv, w.kvh, P, a.hd);
+    const int64_t stride = page_base(1, a.Hkv, 0, P, a.hd);
     int page[CH], ipage = -1;
     uint4 raw[CH];
     float isc = 0.f, ivs = 0.f;
@@ -539,8 +559,7 @@ __global__ void __launch_bounds__(512, 2) attn_paged_wide_kernel(PagedArgs a) {
         raw[i] = make_uint4(0, 0, 0, 0);
         const int at = (base + 16 * pc[i].grp) & (P - 1);
         if (page[i] >= 0 && pc[i].live)
-          raw[i] = *reinterpret_cast<const uint4 *>((pc[i].key ? a.kc + at * a.hd : a.vc + at) +
-                                                    page_base(page[i], a.Hkv, w.kvh, P, a.hd) + pc[i].off);
+          raw[i] = *reinterpret_cast<const uint4 *>((pc[i].key ? kc + at * a.hd : vc + at) + page[i] * stride + pc[i].off);
       }
       if (tid < 4) {
         isc = ipage >= 0 ? a.ks[long(ipage) * a.Hkv + w.kvh] : 1.f;
@@ -556,7 +575,16 @@ __global__ void __launch_bounds__(512, 2) attn_paged_wide_kernel(PagedArgs a) {
         if (edge && !pc[i].key) {
           const int t = base + 16 * pc[i].grp;
           r = keep_bytes(r, min(max(some_lo - t, 0), 16), min(max(mine.hi - t, 0), 16));
-          any |= nan_bytes(r.x) | nan_bytes(r.y) | nan_bytes(r.z) | nan_bytes(r.w);
+          uint32_t b[4] = {r.x, r.y, r.z, r.w}, bits = 0;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const uint32_t nb = nan_bytes(b[c]);
+            b[c] &= ~(nb * 0xffu);
+            bits |= ((nb & 1u) | (nb >> 7 & 2u) | (nb >> 14 & 4u) | (nb >> 21 & 8u)) << (4 * c);
+          }
+          r = make_uint4(b[0], b[1], b[2], b[3]);
+          any |= bits;
+          reinterpret_cast<uint16_t *>(nan_at[buf])[pc[i].vrow * 4 + pc[i].grp] = uint16_t(bits);
         }
         *reinterpret_cast<f16x8 *>(&lds[buf][pc[i].l0]) = cvt8(r.x, r.y);
         *reinterpret_cast<f16x8 *>(&lds[buf][pc[i].l1]) = cvt8(r.z, r.w);
@@ -606,25 +634,30 @@ __global__ void __launch_bounds__(512, 2) attn_paged_wide_kernel(PagedArgs a) {
           const bool masked = base < q.every_lo || base + kKeyBlock > q.every_hi || __any(!page_ok);
           if (masked) q.template probabilities<true>(s, in.x, in.y, page_ok, base + 16 * g);
           else q.template probabilities<false>(s, in.x, in.y, page_ok, base + 16 * g);
-          bool nans = false;
-          if (masked) nans = (dirty[buf][0] | dirty[buf][1] | dirty[buf][2] | dirty[buf][3] | dirty[buf][4] | dirty[buf][5] | dirty[buf][6] |
-                              dirty[buf][7]) != 0;
 #pragma unroll
-          for (int i = 0; i < MT; ++i) {
-            f16x8 v0 = *reinterpret_cast<const f16x8 *>(L + v_at(16 * i + n, 2 * g)),
-                  v1 = *reinterpret_cast<const f16x8 *>(L + v_at(16 * i + n, 2 * g + 1));
-            if (nans) {
-              f16x8 m0, m1;
+          for (int i = 0; i < MT; ++i)
+            q.values(i, *reinterpret_cast<const f16x8 *>(L + v_at(16 * i + n, 2 * g)),
+                     *reinterpret_cast<const f16x8 *>(L + v_at(16 * i + n, 2 * g + 1)));
+          if (masked && (dirty[buf][0] | dirty[buf][1] | dirty[buf][2] | dirty[buf][3] | dirty[buf][4] | dirty[buf][5] | dirty[buf][6] |
+                         dirty[buf][7])) {
+            // outputs of rows that see a NaN value (a zero probability alone would
+            // not keep it from the others)
+            uint64_t seen[NQ];
 #pragma unroll
-              for (int e = 0; e < 8; ++e) {
-                m0[e] = v0[e] == v0[e] ? _Float16(0.f) : _Float16(1.f);
-                m1[e] = v1[e] == v1[e] ? _Float16(0.f) : _Float16(1.f);
-                v0[e] = v0[e] == v0[e] ? v0[e] : _Float16(0.f);
-                v1[e] = v1[e] == v1[e] ? v1[e] : _Float16(0.f);
-              }
-              q.mark_nans(i, m0, m1);
+            for (int x = 0; x < NQ; ++x) {
+              seen[x] = 0;
+#pragma unroll
+              for (int c = 0; c < 4; ++c) seen[x] |= uint64_t(uint32_t(__shfl(int(q.ok[x]), 16 * c + n, 64))) << (16 * c);
             }
-            q.values(i, v0, v1);
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                const uint64_t at = nan_at[buf][16 * i + 4 * g + r];
+#pragma unroll
+                for (int x = 0; x < NQ; ++x)
+                  if (at & seen[x]) q.acc[i][x][r] = __builtin_nanf("");
+              }
           }
         }
         if (more) place(base + kKeyBlock, ip, buf ^ 1);
@@ -637,9 +670,10 @@ __global__ void __launch_bounds__(512, 2) attn_paged_wide_kernel(PagedArgs a) {
       for (int x = 0; x < NQ; ++x) {
         const int r = r_first + 16 * x + n;
         if (r < w.rows) {
+          const RowOut<DT> to(a, w.row0, w.kvh, w.split, r, q.mx[x], q.l[x], g == 0);
 #pragma unroll
           for (int i = 0; i < MT; ++i)
-            if (16 * i < a.hd) put<DT>(a, w.row0, w.kvh, w.split, r, 16 * i + 4 * g, q.acc[i][x], q.mx[x], q.l[x]);
+            if (16 * i < a.hd) to.put(16 * i + 4 * g, q.acc[i][x]);
         }
       }
     }
