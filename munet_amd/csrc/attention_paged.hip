@@ -225,8 +225,10 @@ template <int DT, int HDP, int NQ> struct RowTiles {
             float t = NP == 2 ? fmaf(raw, f, -ref) : fmaf(raw, f, lf + 14.f - ref);
             if (MASKED) t = raw == -__builtin_inff() ? raw : t;
             p[y] = __builtin_amdgcn_exp2f(t);
-            if constexpr (NP == 2) p[y] *= scale14;
-            sum += p[y];
+            if constexpr (NP == 2) {
+              p[y] *= scale14;
+              sum += p[y];
+            }
           }
 #pragma unroll
           for (int y = 0; y < 2; ++y) {
@@ -234,6 +236,8 @@ template <int DT, int HDP, int NQ> struct RowTiles {
             pf[0][x][u][e + y] = h0;
             if constexpr (NP == 2) pf[1][x][u][e + y] = _Float16(p[y] - float(h0));
           }
+          // (16-bit types: the sum takes the rounded values, two in an instruction)
+          if constexpr (NP == 1) sum = __builtin_amdgcn_fdot2(f16x2{pf[0][x][u][e], pf[0][x][u][e + 1]}, f16x2{_Float16(1.f), _Float16(1.f)}, sum, false);
         }
       l[x] = fmaf(sum, unscale, l[x]);  // (2^14 w)
     }
@@ -477,18 +481,19 @@ __global__ void __launch_bounds__(256) attn_paged_kernel(PagedArgs a) {
 // reads at a time lie in different banks: keys as tile rows 16 t + m (m the
 // operand's row), chunk c at c ^ (row & 15) (rows of 128 bytes: c ^ (row >> 1 & 7),
 // as for the values, rows of a head value's 64 keys).
-template <int DT, int HDP, int NQ>
-__global__ void __launch_bounds__(512, 2) attn_paged_wide_kernel(PagedArgs a) {
-  constexpr int MT = HDP / 16, RW = 16 * NQ, RB = 8 * RW;
+template <int DT, int HDP, int NQ, int NW>
+__global__ void __launch_bounds__(64 * NW, 2) attn_paged_wide_kernel(PagedArgs a) {
+  constexpr int NT = 64 * NW;
+  constexpr int MT = HDP / 16, RW = 16 * NQ, RB = NW * RW;
   constexpr int XK = HDP / 16;                  // 16-byte pieces of a key in the cache
-  constexpr int NK = 64 * XK, CH = 2 * NK / 512;  // pieces of a block's keys; pieces (keys and values) per thread
+  constexpr int NK = 64 * XK, CH = 2 * NK / NT;  // pieces of a block's keys; pieces (keys and values) per thread
   constexpr int KROW = HDP * 2, KB = 64 * KROW, VB = HDP * 128;
   __shared__ __align__(16) uint8_t lds[2][KB + VB];
   __shared__ float4 info[2][4];     // per lane group: key scale, log2 of the value scale, page in the pool
   // NaN values of a block at the edge of some row's mask (they are zeros in
   // LDS): bit k of nan_at, key k of the block
   __shared__ uint64_t nan_at[2][HDP];
-  __shared__ uint32_t dirty[2][8];  // whether there are any
+  __shared__ uint32_t dirty[2][NW];  // whether there are any
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
   Part w;
   if (!part_of(a, int(blockIdx.x) / a.tiles, w)) return;
@@ -506,7 +511,7 @@ __global__ void __launch_bounds__(512, 2) attn_paged_wide_kernel(PagedArgs a) {
   } pc[CH];
 #pragma unroll
   for (int i = 0; i < CH; ++i) {
-    const int e = tid + 512 * i;
+    const int e = tid + NT * i;
     pc[i].key = e < NK;
     if (e < NK) {
       const int row = e / XK, x = e % XK, R = 16 * ((row >> 2) & 3) + 4 * (row >> 4) + (row & 3);
@@ -638,8 +643,11 @@ __global__ void __launch_bounds__(512, 2) attn_paged_wide_kernel(PagedArgs a) {
           for (int i = 0; i < MT; ++i)
             q.values(i, *reinterpret_cast<const f16x8 *>(L + v_at(16 * i + n, 2 * g)),
                      *reinterpret_cast<const f16x8 *>(L + v_at(16 * i + n, 2 * g + 1)));
-          if (masked && (dirty[buf][0] | dirty[buf][1] | dirty[buf][2] | dirty[buf][3] | dirty[buf][4] | dirty[buf][5] | dirty[buf][6] |
-                         dirty[buf][7])) {
+          uint32_t nans = 0;
+          if (masked)
+#pragma unroll
+            for (int v = 0; v < NW; ++v) nans |= dirty[buf][v];
+          if (nans) {
             // outputs of rows that see a NaN value (a zero probability alone would
             // not keep it from the others)
             uint64_t seen[NQ];
@@ -720,9 +728,9 @@ hipError_t launch(const PagedArgs &a, const PagedShape &s, hipStream_t st) {
   const long blocks = long(s.tiles) * s.splits * a.Hkv * a.B;
   if (blocks * 512 > 0xffffffffL) return hipErrorInvalidValue;
   const dim3 grid{unsigned(blocks)};
-  constexpr int NQ = DT == F32 || HDP > 128 ? 1 : 2;
+  constexpr int NQ = DT == F32 || HDP > 128 ? 1 : 2, NW = HDP > 128 ? 8 : 4;
   if (s.wide)
-    hipLaunchKernelGGL((attn_paged_wide_kernel<DT, HDP, NQ>), grid, dim3(512), 0, st, a);
+    hipLaunchKernelGGL((attn_paged_wide_kernel<DT, HDP, NQ, NW>), grid, dim3(64 * NW), 0, st, a);
   else
     hipLaunchKernelGGL((attn_paged_kernel<DT, HDP>), grid, dim3(256), 0, st, a);
   hipError_t e = hipGetLastError();

@@ -87,7 +87,7 @@ struct PagedShape {
 };
 // Rows that a workgroup of the wide form takes: eight waves of one or two MFMA
 // tiles (one for fp32, whose operands are in two parts, and for heads above 128).
-inline int paged_wide_rows(bool f32, int hd) { return f32 || hd > 128 ? 128 : 256; }
+inline int paged_wide_rows(bool f32, int hd) { return f32 && hd <= 128 ? 64 : 128; }
 inline PagedShape paged_shape(bool f32, int B, int Hq, int Hkv, int hd, int max_q, int max_len, int window) {
   PagedShape s;
   const int64_t rows = int64_t(max_q) * (Hq / Hkv);
