@@ -225,10 +225,10 @@ template <int DT, int HDP, int NQ> struct RowTiles {
             float t = NP == 2 ? fmaf(raw, f, -ref) : fmaf(raw, f, lf + 14.f - ref);
             if (MASKED) t = raw == -__builtin_inff() ? raw : t;
             p[y] = __builtin_amdgcn_exp2f(t);
-            if constexpr (NP == 2) {
-              p[y] *= scale14;
-              sum += p[y];
-            }
+            if constexpr (NP == 2) p[y] *= scale14;
+            // (not of the rounded values: those of a page whose value scale is far
+            // below the largest are zero)
+            sum += p[y];
           }
 #pragma unroll
           for (int y = 0; y < 2; ++y) {
@@ -236,8 +236,6 @@ template <int DT, int HDP, int NQ> struct RowTiles {
             pf[0][x][u][e + y] = h0;
             if constexpr (NP == 2) pf[1][x][u][e + y] = _Float16(p[y] - float(h0));
           }
-          // (16-bit types: the sum takes the rounded values, two in an instruction)
-          if constexpr (NP == 1) sum = __builtin_amdgcn_fdot2(f16x2{pf[0][x][u][e], pf[0][x][u][e + 1]}, f16x2{_Float16(1.f), _Float16(1.f)}, sum, false);
         }
       l[x] = fmaf(sum, unscale, l[x]);  // (2^14 w)
     }
@@ -347,6 +345,8 @@ __global__ void __launch_bounds__(256) attn_paged_kernel(PagedArgs a) {
   if (!part_of(a, int(blockIdx.x) / a.tiles, w)) return;
   const int P = 1 << a.plog;
   const int32_t *table = a.tables + long(w.b) * a.width;
+  const uint8_t *kc = a.kc + page_base(0, a.Hkv, w.kvh, P, a.hd), *vc = a.vc + page_base(0, a.Hkv, w.kvh, P, a.hd);
+  const int64_t stride = page_base(1, a.Hkv, 0, P, a.hd);
   // The merge of the four waves' shares: 128 head values at a time.
   constexpr int MW = HDP < 128 ? HDP : 128, LD = MW + 4;
   __shared__ __align__(16) float wo[4][RW][LD];
@@ -364,28 +364,27 @@ __global__ void __launch_bounds__(256) attn_paged_kernel(PagedArgs a) {
 
     for (int base = (mine.lo & ~(kKeyBlock - 1)) + wave * kKeyBlock; base < mine.hi; base += 4 * kKeyBlock) {
       // the pages of this lane's key rows (group n >> 2) and of its scores and
-      // values (group g); a page outside the pool holds no keys (page 0 is read
-      // in its place and masked)
+      // values (group g).  Every load is made, at an address that exists, and
+      // what should not count is masked: a load under a condition makes the
+      // compiler wait for it before the next.  Keys past the range take its
+      // last page; a page outside the pool holds no keys (page 0 is read); head
+      // values past hd repeat earlier ones (their queries are zero, their outputs
+      // not stored).
       const int tk = base + 16 * (n >> 2), tv = base + 16 * g;
-      int pk = tk < mine.hi && (tk >> a.plog) < a.width ? table[tk >> a.plog] : -1;
-      int pv = tv < mine.hi && (tv >> a.plog) < a.width ? table[tv >> a.plog] : -1;
+      int pk = table[min(tk, mine.hi - 1) >> a.plog], pv = table[min(tv, mine.hi - 1) >> a.plog];
       const bool page_ok = page_in_pool(pv, a.n_pages);
       if (!page_ok && tv < mine.hi && n == 0) atomicOr(a.err, kErrPage);
       pk = page_in_pool(pk, a.n_pages) ? pk : 0;
       pv = page_ok ? pv : 0;
-      const uint8_t *kp = a.kc + page_base(pk, a.Hkv, w.kvh, P, a.hd) + long(tk & (P - 1)) * a.hd;
-      const uint8_t *vp = a.vc + page_base(pv, a.Hkv, w.kvh, P, a.hd) + (tv & (P - 1));
+      const uint8_t *kp = kc + pk * stride + (tk & (P - 1)) * a.hd, *vp = vc + pv * stride + (tv & (P - 1)) + n * P;
       uint4 kr[4][J], vr[MT];
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int j = 0; j < J; ++j) {
-          const int d = 64 * j + 16 * g;
-          kr[t][j] = d < a.hd ? *reinterpret_cast<const uint4 *>(kp + (4 * t + (n & 3)) * a.hd + d) : make_uint4(0, 0, 0, 0);
-        }
+        for (int j = 0; j < J; ++j)
+          kr[t][j] = *reinterpret_cast<const uint4 *>(kp + (4 * t + (n & 3)) * a.hd + min(64 * j + 16 * g, a.hd - 16));
 #pragma unroll
-      for (int i = 0; i < MT; ++i)
-        vr[i] = 16 * i < a.hd ? *reinterpret_cast<const uint4 *>(vp + (16 * i + n) * P) : make_uint4(0, 0, 0, 0);
+      for (int i = 0; i < MT; ++i) vr[i] = *reinterpret_cast<const uint4 *>(vp + min(16 * i, a.hd - 16) * P);
       const float ksc = a.ks[long(pv) * a.Hkv + w.kvh], vsc = a.vs[long(pv) * a.Hkv + w.kvh];
 
       f32x4 s[4][1];
@@ -506,7 +505,7 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_paged_wide_kernel(PagedArgs a
   // value, 16 keys; neighbours within a page follow each other)
   const int ql = min(a.plog - 4, 2);  // log2 of the lane groups per page and block
   struct Piece {
-    bool key, live;
+    bool key, holed;
     int grp, off, l0, l1, vrow;  // lane group of the keys, byte within the page's keys or values, LDS bytes
   } pc[CH];
 #pragma unroll
@@ -516,15 +515,13 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_paged_wide_kernel(PagedArgs a
     if (e < NK) {
       const int row = e / XK, x = e % XK, R = 16 * ((row >> 2) & 3) + 4 * (row >> 4) + (row & 3);
       pc[i].grp = row >> 4;
-      pc[i].live = 16 * x < a.hd;
-      pc[i].off = (row & 15) * a.hd + 16 * x;
+      pc[i].off = (row & 15) * a.hd + min(16 * x, a.hd - 16);
       pc[i].l0 = k_at(R, 2 * x);
       pc[i].l1 = k_at(R, 2 * x + 1);
     } else {
       const int f = e - NK, lo = f & ((1 << ql) - 1), row = (f >> ql) % HDP, grp = ((f >> ql) / HDP << ql) + lo;
       pc[i].grp = grp;
-      pc[i].live = row < a.hd;
-      pc[i].off = row * P;
+      pc[i].off = min(row, a.hd - 1) * P;
       pc[i].vrow = row;
       pc[i].l0 = v_at(row, 2 * grp);
       pc[i].l1 = v_at(row, 2 * grp + 1);
@@ -543,43 +540,44 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_paged_wide_kernel(PagedArgs a
     if (on) q.start(a, w.row0, w.nq, w.len, w.rows, r_first, w.kvh, n, mine, [&](int s) { return 32 * s + 8 * g; });
 
     const int first = mine.lo & ~(kKeyBlock - 1);
-    auto page_of = [&](int base, int grp) {  // -1: no such page, or no key in range
-      const int t = base + 16 * grp;
-      const int p = t < mine.hi && (t >> a.plog) < a.width ? table[t >> a.plog] : -1;
+    // (as above: every load is made)
+    auto page_of = [&](int base, int grp) {
+      const int p = table[min(base + 16 * grp, mine.hi - 1) >> a.plog];
       return page_in_pool(p, a.n_pages) ? p : -1;
     };
     const uint8_t *kc = a.kc + page_base(0, a.Hkv, w.kvh, P, a.hd), *vc = a.vc + page_base(0, a.Hkv, w.kvh, P, a.hd);
     const int64_t stride = page_base(1, a.Hkv, 0, P, a.hd);
     int page[CH], ipage = -1;
+    bool hole = false;  // a page of the fetched block is outside the pool
     uint4 raw[CH];
     float isc = 0.f, ivs = 0.f;
     auto ask = [&](int base) {  // pages of the block
 #pragma unroll
       for (int i = 0; i < CH; ++i) page[i] = page_of(base, pc[i].grp);
-      if (tid < 4) ipage = page_of(base, tid);
+      ipage = page_of(base, tid & 3);
     };
     auto fetch = [&](int base) {  // its bytes and scales
+      hole = false;
 #pragma unroll
       for (int i = 0; i < CH; ++i) {
-        raw[i] = make_uint4(0, 0, 0, 0);
         const int at = (base + 16 * pc[i].grp) & (P - 1);
-        if (page[i] >= 0 && pc[i].live)
-          raw[i] = *reinterpret_cast<const uint4 *>((pc[i].key ? kc + at * a.hd : vc + at) + page[i] * stride + pc[i].off);
+        raw[i] = *reinterpret_cast<const uint4 *>((pc[i].key ? kc + at * a.hd : vc + at) + max(page[i], 0) * stride + pc[i].off);
+        pc[i].holed = page[i] < 0;
+        hole |= pc[i].holed;
       }
-      if (tid < 4) {
-        isc = ipage >= 0 ? a.ks[long(ipage) * a.Hkv + w.kvh] : 1.f;
-        ivs = ipage >= 0 ? a.vs[long(ipage) * a.Hkv + w.kvh] : 1.f;
-      }
+      hole = __any(hole);
+      isc = a.ks[long(max(ipage, 0)) * a.Hkv + w.kvh];
+      ivs = a.vs[long(max(ipage, 0)) * a.Hkv + w.kvh];
     };
     auto place = [&](int base, int ip, int buf) {  // into LDS as fp16
       uint32_t any = 0;
-      const bool edge = base < all_lo || base + kKeyBlock > all_hi;
+      const bool edge = base < all_lo || base + kKeyBlock > all_hi || hole;
 #pragma unroll
       for (int i = 0; i < CH; ++i) {
         uint4 r = raw[i];
         if (edge && !pc[i].key) {
           const int t = base + 16 * pc[i].grp;
-          r = keep_bytes(r, min(max(some_lo - t, 0), 16), min(max(mine.hi - t, 0), 16));
+          r = keep_bytes(r, min(max(some_lo - t, 0), 16), pc[i].holed ? 0 : min(max(mine.hi - t, 0), 16));
           uint32_t b[4] = {r.x, r.y, r.z, r.w}, bits = 0;
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
