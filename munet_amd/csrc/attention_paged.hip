@@ -24,10 +24,10 @@
 // two to below 2^14 and is then exact in fp16 for bf16 and fp16 inputs (down to
 // 2^-38 of the row's largest value); fp32 inputs are the sum of two fp16 parts
 // (22 bits and a sign).  Scores, the running maximum, the sum and the outputs are
-// fp32.  A probability enters the second product as 2^14 w times its page's
-// value scale over the largest one that the row has seen, rounded to fp16 (half a unit of 11
-// bits down to 2^-28 of the largest; outputs of 16 bits are rounded as much
-// once more), or as two such parts for fp32 inputs.
+// fp32.  A probability enters the second product as 2^9 w times its page's value
+// scale over the largest one that the row has seen, rounded to fp16 (half a unit
+// of 11 bits down to 2^-23 of the reference; outputs of 16 bits are rounded as
+// much once more), or as two such parts for fp32 inputs.
 #include "mh_common.hpp"
 #include "mh_kernels.hpp"
 #include "paged_index.hpp"
@@ -36,6 +36,10 @@ namespace mh {
 namespace {
 
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+
+// Probabilities are taken times 2^kLift, against a reference that the row's
+// largest score passes by at most kRaise (log2): below 2^15 in fp16.
+constexpr float kLift = 9.f, kRaise = 5.f;
 
 struct PagedArgs {
   const void *q;
@@ -92,7 +96,6 @@ template <int DT, int HDP, int NQ> struct RowTiles {
   float c_row[NQ], mx[NQ], l[NQ];
   float lref[NQ];  // log2 of the largest value scale that the row has seen
   int lo_row[NQ], hi_row[NQ];
-  uint32_t ok[NQ];  // bit e: the row sees key 16 g + e of the block
   int every_lo, every_hi;  // keys that every row sees
   int some_lo, some_hi;    // keys that some row sees
 
@@ -159,38 +162,50 @@ template <int DT, int HDP, int NQ> struct RowTiles {
   }
 
   // Raw scores of a block (this lane group's keys tv .. tv + 15, with their
-  // page's key scale and log2 of its value scale) to probabilities pf; the sums
-  // and outputs so far scaled to the new maximum.  MASKED: some row does not
-  // see some key.
-  template <bool MASKED>
-  __device__ __forceinline__ void probabilities(f32x4 (&s)[4][NQ], float ksc, float lv, bool page_ok, int tv) {
-    const float lv_block = MASKED ? 0.f : xor32_max(xor16_max(lv));
+  // page's key scale and log2 of its value scale, and the block's largest) to
+  // probabilities pf; the sums and outputs so far scaled to the new reference.
+  // masked: some row does not see some key.
+  __device__ __forceinline__ void probabilities(f32x4 (&s)[4][NQ], float ksc, float lv, float lv_block, bool page_ok, int tv,
+                                                bool masked) {
+    float lvs[NQ], tops[NQ];
 #pragma unroll
     for (int x = 0; x < NQ; ++x) {
-      ok[x] = 0xffffu;
-      if constexpr (MASKED) {
-        const int lo = min(max(lo_row[x] - tv, 0), 16), hi = min(max(hi_row[x] - tv, 0), 16);
-        ok[x] = page_ok ? ((1u << hi) - 1u) & ~((1u << lo) - 1u) : 0u;
+      lvs[x] = lv;
+      tops[x] = lv_block;
+    }
+    if (masked) {
+#pragma unroll
+      for (int x = 0; x < NQ; ++x) {
+        const uint32_t ok = seen(x, tv, page_ok);
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) s[t][x][r] = (ok[x] >> (4 * t + r)) & 1u ? s[t][x][r] : -__builtin_inff();
+          for (int r = 0; r < 4; ++r) s[t][x][r] = (ok >> (4 * t + r)) & 1u ? s[t][x][r] : -__builtin_inff();
+        // a page of which the row sees nothing does not count for its values' scale
+        tops[x] = xor32_max(xor16_max(ok ? lv : -126.f));
+        lvs[x] = ok ? lv : fmaxf(tops[x], lref[x]);
       }
+    }
+#pragma unroll
+    for (int x = 0; x < NQ; ++x) {
       // the value scales: this lane group's over the largest that the row has seen
-      const float lnew = fmaxf(MASKED ? xor32_max(xor16_max(ok[x] ? lv : -126.f)) : lv_block, lref[x]);
-      const float lf = !MASKED || ok[x] ? lv - lnew : 0.f;
+      const float lnew = fmaxf(tops[x], lref[x]), lf = lvs[x] - lnew;
       const float rescale = lnew == lref[x] ? 1.f : __builtin_amdgcn_exp2f(lref[x] - lnew);
-      const float unscale = __builtin_amdgcn_exp2f(-lf), scale14 = __builtin_amdgcn_exp2f(lf + 14.f);
+      const float unscale = __builtin_amdgcn_exp2f(-lf), lift = __builtin_amdgcn_exp2f(lf + kLift);
       lref[x] = lnew;
       // (a page's scale is positive: the largest raw score is the largest score)
       float f = ksc * c_row[x];
+      f = f == 0.f ? 1e-37f : f;  // (so that a masked score stays -inf)
       float top = s[0][x][0];
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r) top = fmaxf(top, s[t][x][r]);
       top = top > -__builtin_inff() ? top * f : -__builtin_inff();
-      top = fmaxf(xor32_max(xor16_max(top)), mx[x]);
+      top = xor32_max(xor16_max(top));
+      // the reference moves only when a score passes it by 2^kRaise: sums and
+      // outputs are seldom scaled
+      top = top > mx[x] + kRaise ? top : mx[x];
       float ref = top > -__builtin_inff() ? top : 0.f;
       const float down = mx[x] == top ? 1.f : __builtin_amdgcn_exp2f(mx[x] - ref);
       mx[x] = top;
@@ -222,10 +237,8 @@ template <int DT, int HDP, int NQ> struct RowTiles {
             const float raw = s[2 * u + (e >> 2)][x][(e & 3) + y];
             // fp32: the difference from the maximum is rounded once, and the
             // power of two applied to the result
-            float t = NP == 2 ? fmaf(raw, f, -ref) : fmaf(raw, f, lf + 14.f - ref);
-            if (MASKED) t = raw == -__builtin_inff() ? raw : t;
-            p[y] = __builtin_amdgcn_exp2f(t);
-            if constexpr (NP == 2) p[y] *= scale14;
+            p[y] = __builtin_amdgcn_exp2f(NP == 2 ? fmaf(raw, f, -ref) : fmaf(raw, f, lf + kLift - ref));
+            if constexpr (NP == 2) p[y] *= lift;
             // (not of the rounded values: those of a page whose value scale is far
             // below the largest are zero)
             sum += p[y];
@@ -237,8 +250,14 @@ template <int DT, int HDP, int NQ> struct RowTiles {
             if constexpr (NP == 2) pf[1][x][u][e + y] = _Float16(p[y] - float(h0));
           }
         }
-      l[x] = fmaf(sum, unscale, l[x]);  // (2^14 w)
+      l[x] = fmaf(sum, unscale, l[x]);  // (2^kLift w)
     }
+  }
+
+  // bit e: row x sees key tv + e
+  __device__ __forceinline__ uint32_t seen(int x, int tv, bool page_ok) const {
+    const int lo = min(max(lo_row[x] - tv, 0), 16), hi = min(max(hi_row[x] - tv, 0), 16);
+    return page_ok ? ((1u << hi) - 1u) & ~((1u << lo) - 1u) : 0u;
   }
 
   // O^T += V^T P^T for head rows 16 i .. 16 i + 15
@@ -255,14 +274,15 @@ template <int DT, int HDP, int NQ> struct RowTiles {
   // A NaN value that only some rows see must reach these alone, which a zero
   // probability does not give: outputs of rows that see a marked value (m0, m1:
   // 1 at a NaN value, 0 else) become NaN.
-  __device__ __forceinline__ void mark_nans(int i, f16x8 m0, f16x8 m1) {
+  __device__ __forceinline__ void mark_nans(int i, f16x8 m0, f16x8 m1, int tv, bool page_ok) {
 #pragma unroll
     for (int x = 0; x < NQ; ++x) {
       f16x8 s0, s1;
+      const uint32_t ok = seen(x, tv, page_ok);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        s0[e] = (ok[x] >> e) & 1u ? _Float16(1.f) : _Float16(0.f);
-        s1[e] = (ok[x] >> (8 + e)) & 1u ? _Float16(1.f) : _Float16(0.f);
+        s0[e] = (ok >> e) & 1u ? _Float16(1.f) : _Float16(0.f);
+        s1[e] = (ok >> (8 + e)) & 1u ? _Float16(1.f) : _Float16(0.f);
       }
       f32x4 hit = f32x4{0.f, 0.f, 0.f, 0.f};
       hit = __builtin_amdgcn_mfma_f32_16x16x32_f16(m0, s0, hit, 0, 0, 0);
@@ -340,7 +360,8 @@ __device__ __forceinline__ bool part_of(const PagedArgs &a, int id, Part &w) {
 template <int DT, int HDP>
 __global__ void __launch_bounds__(256) attn_paged_kernel(PagedArgs a) {
   constexpr int J = HDP / 64, MT = HDP / 16, RW = 16;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
+  // (the wave's number as a scalar: what follows from it are scalar tests)
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, g = lane >> 4;
   Part w;
   if (!part_of(a, int(blockIdx.x) / a.tiles, w)) return;
   const int P = 1 << a.plog;
@@ -403,8 +424,7 @@ __global__ void __launch_bounds__(256) attn_paged_kernel(PagedArgs a) {
       }
       const float lv = page_ok ? fmaxf(__builtin_amdgcn_logf(vsc), -126.f) : -126.f;
       const bool masked = base < q.every_lo || base + kKeyBlock > q.every_hi || __any(!page_ok);
-      if (masked) q.template probabilities<true>(s, ksc, lv, page_ok, tv);
-      else q.template probabilities<false>(s, ksc, lv, page_ok, tv);
+      q.probabilities(s, ksc, lv, xor32_max(xor16_max(lv)), page_ok, tv, masked);
 
       // Keys that no row sees may hold anything, NaN among it: their bytes are
       // cleared.
@@ -430,7 +450,7 @@ __global__ void __launch_bounds__(256) attn_paged_kernel(PagedArgs a) {
             mark[c] = nb * 0x38u;  // e4m3 1.0
           }
           vr[i] = make_uint4(b[0], b[1], b[2], b[3]);
-          q.mark_nans(i, cvt8(mark[0], mark[1]), cvt8(mark[2], mark[3]));
+          q.mark_nans(i, cvt8(mark[0], mark[1]), cvt8(mark[2], mark[3]), tv, page_ok);
         }
       }
 #pragma unroll
@@ -488,12 +508,14 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_paged_wide_kernel(PagedArgs a
   constexpr int NK = 64 * XK, CH = 2 * NK / NT;  // pieces of a block's keys; pieces (keys and values) per thread
   constexpr int KROW = HDP * 2, KB = 64 * KROW, VB = HDP * 128;
   __shared__ __align__(16) uint8_t lds[2][KB + VB];
-  __shared__ float4 info[2][4];     // per lane group: key scale, log2 of the value scale, page in the pool
+  // per lane group: key scale, log2 of the value scale, page in the pool, the block's largest log2
+  __shared__ float4 info[2][4];
   // NaN values of a block at the edge of some row's mask (they are zeros in
   // LDS): bit k of nan_at, key k of the block
   __shared__ uint64_t nan_at[2][HDP];
   __shared__ uint32_t dirty[2][NW];  // whether there are any
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
+  // (the wave's number as a scalar: what follows from it are scalar tests)
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, g = lane >> 4;
   Part w;
   if (!part_of(a, int(blockIdx.x) / a.tiles, w)) return;
   const int P = 1 << a.plog;
@@ -501,32 +523,38 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_paged_wide_kernel(PagedArgs a
   auto k_at = [](int row, int c) { return row * KROW + 16 * (KROW == 128 ? c ^ ((row >> 1) & 7) : c ^ (row & 15)); };
   auto v_at = [](int row, int c) { return KB + row * 128 + 16 * (c ^ ((row >> 1) & 7)); };
 
-  // this thread's pieces: of the keys (row, 16 head values) or the values (head
-  // value, 16 keys; neighbours within a page follow each other)
+  // This thread's pieces: of the keys (row, 16 head values) or the values (head
+  // value, 16 keys; neighbours within a page follow each other).  The pieces of a wave
+  // lie in one page, whatever the page holds: its number and the page's address
+  // are scalars, and a thread adds a constant.
   const int ql = min(a.plog - 4, 2);  // log2 of the lane groups per page and block
-  struct Piece {
-    bool key, holed;
-    int grp, off, l0, l1, vrow;  // lane group of the keys, byte within the page's keys or values, LDS bytes
-  } pc[CH];
+  uint32_t off[CH];                   // byte within the page's keys or values, less the scalar part
+  int l0[CH];                         // LDS byte of its first chunk; the second one's is l0 ^ 16
+  int grp0[CH];                       // first lane group of the wave's piece (scalar)
+  auto value_piece = [&](int i, int &row, int &grp) {
+    const int f = tid + NT * i - NK, lo = f & ((1 << ql) - 1);
+    row = (f >> ql) % HDP;
+    grp = ((f >> ql) / HDP << ql) + lo;
+    return lo;
+  };
 #pragma unroll
   for (int i = 0; i < CH; ++i) {
     const int e = tid + NT * i;
-    pc[i].key = e < NK;
     if (e < NK) {
       const int row = e / XK, x = e % XK, R = 16 * ((row >> 2) & 3) + 4 * (row >> 4) + (row & 3);
-      pc[i].grp = row >> 4;
-      pc[i].off = (row & 15) * a.hd + min(16 * x, a.hd - 16);
-      pc[i].l0 = k_at(R, 2 * x);
-      pc[i].l1 = k_at(R, 2 * x + 1);
+      off[i] = uint32_t((row & 15) * a.hd + min(16 * x, a.hd - 16));
+      l0[i] = k_at(R, 2 * x);
+      grp0[i] = __builtin_amdgcn_readfirstlane(row >> 4);
     } else {
-      const int f = e - NK, lo = f & ((1 << ql) - 1), row = (f >> ql) % HDP, grp = ((f >> ql) / HDP << ql) + lo;
-      pc[i].grp = grp;
-      pc[i].off = min(row, a.hd - 1) * P;
-      pc[i].vrow = row;
-      pc[i].l0 = v_at(row, 2 * grp);
-      pc[i].l1 = v_at(row, 2 * grp + 1);
+      int row, grp;
+      const int lo = value_piece(i, row, grp);
+      off[i] = uint32_t(min(row, a.hd - 1) * P + 16 * lo);
+      l0[i] = v_at(row, 2 * grp);
+      grp0[i] = __builtin_amdgcn_readfirstlane(grp - lo);
     }
   }
+  // (pieces of keys come first; a wave's i-th pieces are all of one kind)
+  auto of_keys = [&](int i) { return wave * 64 + NT * i < NK; };
 
   for (int tile = a.tiles - 1 - int(blockIdx.x) % a.tiles; long(tile) * RB < w.rows; tile += a.tiles) {
     const int R0 = tile * RB, r_first = R0 + wave * RW;
@@ -547,56 +575,66 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_paged_wide_kernel(PagedArgs a
     };
     const uint8_t *kc = a.kc + page_base(0, a.Hkv, w.kvh, P, a.hd), *vc = a.vc + page_base(0, a.Hkv, w.kvh, P, a.hd);
     const int64_t stride = page_base(1, a.Hkv, 0, P, a.hd);
-    int page[CH], ipage = -1;
-    bool hole = false;  // a page of the fetched block is outside the pool
+    int page[CH], ipage = -1, holes = 0;  // holes: pieces of the fetched block whose page is outside the pool
     uint4 raw[CH];
     float isc = 0.f, ivs = 0.f;
     auto ask = [&](int base) {  // pages of the block
 #pragma unroll
-      for (int i = 0; i < CH; ++i) page[i] = page_of(base, pc[i].grp);
-      ipage = page_of(base, tid & 3);
+      for (int i = 0; i < CH; ++i) page[i] = page_of(base, grp0[i]);
+      if (wave == 0) ipage = page_of(base, tid & 3);
     };
     auto fetch = [&](int base) {  // its bytes and scales
-      hole = false;
+      holes = 0;
 #pragma unroll
       for (int i = 0; i < CH; ++i) {
-        const int at = (base + 16 * pc[i].grp) & (P - 1);
-        raw[i] = *reinterpret_cast<const uint4 *>((pc[i].key ? kc + at * a.hd : vc + at) + max(page[i], 0) * stride + pc[i].off);
-        pc[i].holed = page[i] < 0;
-        hole |= pc[i].holed;
+        const int p = __builtin_amdgcn_readfirstlane(page[i]), at = (base + 16 * grp0[i]) & (P - 1);
+        if (p < 0) holes |= 1 << i;
+        const uint8_t *from = (of_keys(i) ? kc + at * a.hd : vc + at) + max(p, 0) * stride;
+        raw[i] = *reinterpret_cast<const uint4 *>(from + off[i]);
       }
-      hole = __any(hole);
-      isc = a.ks[long(max(ipage, 0)) * a.Hkv + w.kvh];
-      ivs = a.vs[long(max(ipage, 0)) * a.Hkv + w.kvh];
+      if (wave == 0) {
+        isc = a.ks[long(max(ipage, 0)) * a.Hkv + w.kvh];
+        ivs = a.vs[long(max(ipage, 0)) * a.Hkv + w.kvh];
+      }
     };
     auto place = [&](int base, int ip, int buf) {  // into LDS as fp16
       uint32_t any = 0;
-      const bool edge = base < all_lo || base + kKeyBlock > all_hi || hole;
+      if (base < all_lo || base + kKeyBlock > all_hi || holes) {
 #pragma unroll
-      for (int i = 0; i < CH; ++i) {
-        uint4 r = raw[i];
-        if (edge && !pc[i].key) {
-          const int t = base + 16 * pc[i].grp;
-          r = keep_bytes(r, min(max(some_lo - t, 0), 16), pc[i].holed ? 0 : min(max(mine.hi - t, 0), 16));
-          uint32_t b[4] = {r.x, r.y, r.z, r.w}, bits = 0;
+        for (int i = 0; i < CH; ++i) {
+          if (of_keys(i)) continue;
+          int row, grp;
+          (void)value_piece(i, row, grp);
+          const int t = base + 16 * grp;
+          raw[i] = keep_bytes(raw[i], min(max(some_lo - t, 0), 16), holes >> i & 1 ? 0 : min(max(mine.hi - t, 0), 16));
+          uint32_t b[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w}, bits = 0;
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             const uint32_t nb = nan_bytes(b[c]);
             b[c] &= ~(nb * 0xffu);
             bits |= ((nb & 1u) | (nb >> 7 & 2u) | (nb >> 14 & 4u) | (nb >> 21 & 8u)) << (4 * c);
           }
-          r = make_uint4(b[0], b[1], b[2], b[3]);
+          raw[i] = make_uint4(b[0], b[1], b[2], b[3]);
           any |= bits;
-          reinterpret_cast<uint16_t *>(nan_at[buf])[pc[i].vrow * 4 + pc[i].grp] = uint16_t(bits);
+          reinterpret_cast<uint16_t *>(nan_at[buf])[row * 4 + grp] = uint16_t(bits);
         }
-        *reinterpret_cast<f16x8 *>(&lds[buf][pc[i].l0]) = cvt8(r.x, r.y);
-        *reinterpret_cast<f16x8 *>(&lds[buf][pc[i].l1]) = cvt8(r.z, r.w);
+        any = __any(any != 0);
       }
-      any = __any(any != 0);
+#pragma unroll
+      for (int i = 0; i < CH; ++i) {
+        *reinterpret_cast<f16x8 *>(&lds[buf][l0[i]]) = cvt8(raw[i].x, raw[i].y);
+        *reinterpret_cast<f16x8 *>(&lds[buf][l0[i] ^ 16]) = cvt8(raw[i].z, raw[i].w);
+      }
       if (lane == 0) dirty[buf][wave] = any;
-      if (tid < 4) {
-        if (ip < 0 && base + 16 * tid < mine.hi) atomicOr(a.err, kErrPage);
-        info[buf][tid] = make_float4(isc, ip >= 0 ? fmaxf(__builtin_amdgcn_logf(ivs), -126.f) : -126.f, ip >= 0 ? 1.f : 0.f, 0.f);
+      if (wave == 0) {
+        const float lv = ip >= 0 ? fmaxf(__builtin_amdgcn_logf(ivs), -126.f) : -126.f;
+        float m = lv;
+        m = fmaxf(m, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(m), 0xb1, 0xf, 0xf, false)));  // quad [1,0,3,2]
+        m = fmaxf(m, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(m), 0x4e, 0xf, 0xf, false)));  // quad [2,3,0,1]
+        if (tid < 4) {
+          if (ip < 0 && base + 16 * tid < mine.hi) atomicOr(a.err, kErrPage);
+          info[buf][tid] = make_float4(isc, lv, ip >= 0 ? 1.f : 0.f, m);
+        }
       }
     };
 
@@ -635,8 +673,7 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_paged_wide_kernel(PagedArgs a
             }
           }
           const bool masked = base < q.every_lo || base + kKeyBlock > q.every_hi || __any(!page_ok);
-          if (masked) q.template probabilities<true>(s, in.x, in.y, page_ok, base + 16 * g);
-          else q.template probabilities<false>(s, in.x, in.y, page_ok, base + 16 * g);
+          q.probabilities(s, in.x, in.y, in.w, page_ok, base + 16 * g, masked);
 #pragma unroll
           for (int i = 0; i < MT; ++i)
             q.values(i, *reinterpret_cast<const f16x8 *>(L + v_at(16 * i + n, 2 * g)),
@@ -645,7 +682,7 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_paged_wide_kernel(PagedArgs a
           if (masked)
 #pragma unroll
             for (int v = 0; v < NW; ++v) nans |= dirty[buf][v];
-          if (nans) {
+          if (__builtin_amdgcn_readfirstlane(nans)) {
             // outputs of rows that see a NaN value (a zero probability alone would
             // not keep it from the others)
             uint64_t seen[NQ];
@@ -653,7 +690,8 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_paged_wide_kernel(PagedArgs a
             for (int x = 0; x < NQ; ++x) {
               seen[x] = 0;
 #pragma unroll
-              for (int c = 0; c < 4; ++c) seen[x] |= uint64_t(uint32_t(__shfl(int(q.ok[x]), 16 * c + n, 64))) << (16 * c);
+              for (int c = 0; c < 4; ++c)
+                seen[x] |= uint64_t(uint32_t(__shfl(int(q.seen(x, base + 16 * g, page_ok)), 16 * c + n, 64))) << (16 * c);
             }
 #pragma unroll
             for (int i = 0; i < MT; ++i)
