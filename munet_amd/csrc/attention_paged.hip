@@ -83,6 +83,21 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
   return (x >> 7) & 0x01010101u;
 }
 
+__device__ __forceinline__ float finite_max8(const float v[8], float big) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float m = __builtin_fabsf(v[e]);
+    big = m < __builtin_inff() ? fmaxf(big, m) : big;
+  }
+  return big;
+}
+// 2^k: 2^k times a row of this largest magnitude lies below 2^14
+__device__ __forceinline__ float row_lift(float big) {
+  const int ex = int(__float_as_uint(big) >> 23);  // biased exponent, 0 for zero and subnormal rows
+  const int k = ex == 0 ? 0 : min(13 - (ex - 127), 120);
+  return __uint_as_float(uint32_t(k + 127) << 23);
+}
+
 // The query rows of a wave: NQ tiles of 16 (column n of tile x is row r_first + 16 x
 // + n of the packed rows; past the last row, that row again, not stored), their
 // running softmax and their outputs O^T.
@@ -128,18 +143,10 @@ template <int DT, int HDP, int NQ> struct RowTiles {
 #pragma unroll
           for (int e = 0; e < 8; ++e) v[s][e] = 0.f;
         }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float m = __builtin_fabsf(v[s][e]);
-          big = m < __builtin_inff() ? fmaxf(big, m) : big;
-        }
+        big = finite_max8(v[s], big);
       }
-      big = xor32_max(xor16_max(big));
-      // 2^k times the row lies below 2^14
-      const int ex = int(__float_as_uint(big) >> 23);  // biased exponent, 0 for zero and subnormal rows
-      const int k = ex == 0 ? 0 : min(13 - (ex - 127), 120);
-      const float up = __uint_as_float(uint32_t(k + 127) << 23);
-      c_row[x] = a.c * __uint_as_float(uint32_t(127 - k) << 23);
+      const float up = row_lift(xor32_max(xor16_max(big)));
+      c_row[x] = a.c / up;  // (a power of two)
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
 #pragma unroll
@@ -340,8 +347,6 @@ struct Part {
   int split, kvh, b, len, row0, nq, rows;
 };
 __device__ __forceinline__ bool part_of(const PagedArgs &a, int id, Part &w) {
-  w.split = id % a.splits;
-  id /= a.splits;
   w.kvh = id % a.Hkv;
   w.b = id / a.Hkv;
   const int most = a.width << a.plog, len = a.lens[w.b];
@@ -363,7 +368,8 @@ __global__ void __launch_bounds__(256) attn_paged_kernel(PagedArgs a) {
   // (the wave's number as a scalar: what follows from it are scalar tests)
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, g = lane >> 4;
   Part w;
-  if (!part_of(a, int(blockIdx.x) / a.tiles, w)) return;
+  w.split = int(blockIdx.x) / a.tiles % a.splits;
+  if (!part_of(a, int(blockIdx.x) / a.tiles / a.splits, w)) return;
   const int P = 1 << a.plog;
   const int32_t *table = a.tables + long(w.b) * a.width;
   const uint8_t *kc = a.kc + page_base(0, a.Hkv, w.kvh, P, a.hd), *vc = a.vc + page_base(0, a.Hkv, w.kvh, P, a.hd);
@@ -492,34 +498,45 @@ __global__ void __launch_bounds__(256) attn_paged_kernel(PagedArgs a) {
   }
 }
 
-// Many rows (prompts): eight waves of NQ tiles each share every block of keys.
-// The workgroup converts a block to fp16 once, into LDS (two buffers: the next
-// block's bytes are on their way while this one is multiplied), from where each
-// wave reads its operands.
-// LDS rows are swizzled in 16-byte chunks so that the 16 rows that a lane group
-// reads at a time lie in different banks: keys as tile rows 16 t + m (m the
-// operand's row), chunk c at c ^ (row & 15) (rows of 128 bytes: c ^ (row >> 1 & 7),
-// as for the values, rows of a head value's 64 keys).
-template <int DT, int HDP, int NQ, int NW>
-__global__ void __launch_bounds__(64 * NW, 2) attn_paged_wide_kernel(PagedArgs a) {
-  constexpr int NT = 64 * NW;
-  constexpr int MT = HDP / 16, RW = 16 * NQ, RB = NW * RW;
-  constexpr int XK = HDP / 16;                  // 16-byte pieces of a key in the cache
+// Many rows (prompts): 32 to a wave, on 32 x 32 MFMA tiles, four waves to a
+// workgroup, which share every block of 64 keys.  The workgroup converts a block to
+// fp16 once, into LDS (two buffers: the next block's bytes are on their way while
+// this one is multiplied), from where each wave reads its operands.
+// As above, the scores' tiles S^T = K Q^T end in the operand order of O^T = V^T P^T:
+// key 16 h + i of a tile of 32 is its row 8 (i / 4) + 4 h + i % 4, so that lane half
+// h holds the scores of the 16 consecutive keys 16 h .. 16 h + 15 of its column.
+// LDS rows are swizzled in 16-byte chunks so that 16 lanes that read the same chunk
+// of 16 rows find them in different banks: chunk c of a row of 256 bytes or more
+// lies at c ^ (row & 15), of 128 bytes (values: a head value's 64 keys) at c ^
+// (row / 2 & 7).
+// Registers bound the waves: 64 outputs, 32 of q and 32 scores a lane at hd 128
+// leave two waves to a SIMD; fp32 and heads above 128 take all registers for one.
+template <int DT, int HDP>
+__global__ void __launch_bounds__(256, DT == F32 || HDP > 128 ? 1 : 2) attn_paged_wide_kernel(PagedArgs a) {
+  typedef typename Store<DT>::T T;
+  constexpr int NT = 256, NW = 4, RW = 32, RB = NW * RW;
+  constexpr int NP = DT == F32 ? 2 : 1;          // fp16 parts of q and of the probabilities
+  constexpr int KS = HDP / 16, MT = HDP / 32;
+  constexpr int XK = HDP / 16;                   // 16-byte pieces of a key in the cache
   constexpr int NK = 64 * XK, CH = 2 * NK / NT;  // pieces of a block's keys; pieces (keys and values) per thread
   constexpr int KROW = HDP * 2, KB = 64 * KROW, VB = HDP * 128;
   __shared__ __align__(16) uint8_t lds[2][KB + VB];
-  // per lane group: key scale, log2 of the value scale, page in the pool, the block's largest log2
+  // per 16 keys: key scale, log2 of the value scale, page in the pool, the block's largest log2
   __shared__ float4 info[2][4];
   // NaN values of a block at the edge of some row's mask (they are zeros in
   // LDS): bit k of nan_at, key k of the block
   __shared__ uint64_t nan_at[2][HDP];
   __shared__ uint32_t dirty[2][NW];  // whether there are any
   // (the wave's number as a scalar: what follows from it are scalar tests)
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, g = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 31, h = lane >> 5;
   Part w;
-  if (!part_of(a, int(blockIdx.x) / a.tiles, w)) return;
+  const PairItem it = pair_item(blockIdx.x, a.B * a.Hkv, a.tiles * a.splits);
+  w.split = it.item % a.splits;
+  if (!part_of(a, it.pair, w)) return;
   const int P = 1 << a.plog;
   const int32_t *table = a.tables + long(w.b) * a.width;
+  const uint8_t *kc = a.kc + page_base(0, a.Hkv, w.kvh, P, a.hd), *vc = a.vc + page_base(0, a.Hkv, w.kvh, P, a.hd);
+  const int64_t stride = page_base(1, a.Hkv, 0, P, a.hd);
   auto k_at = [](int row, int c) { return row * KROW + 16 * (KROW == 128 ? c ^ ((row >> 1) & 7) : c ^ (row & 15)); };
   auto v_at = [](int row, int c) { return KB + row * 128 + 16 * (c ^ ((row >> 1) & 7)); };
 
@@ -527,10 +544,10 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_paged_wide_kernel(PagedArgs a
   // value, 16 keys; neighbours within a page follow each other).  The pieces of a wave
   // lie in one page, whatever the page holds: its number and the page's address
   // are scalars, and a thread adds a constant.
-  const int ql = min(a.plog - 4, 2);  // log2 of the lane groups per page and block
+  const int ql = min(a.plog - 4, 2);  // log2 of the runs of 16 keys per page and block
   uint32_t off[CH];                   // byte within the page's keys or values, less the scalar part
   int l0[CH];                         // LDS byte of its first chunk; the second one's is l0 ^ 16
-  int grp0[CH];                       // first lane group of the wave's piece (scalar)
+  int grp0[CH];                       // first run of the wave's piece (scalar)
   auto value_piece = [&](int i, int &row, int &grp) {
     const int f = tid + NT * i - NK, lo = f & ((1 << ql) - 1);
     row = (f >> ql) % HDP;
@@ -541,8 +558,8 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_paged_wide_kernel(PagedArgs a
   for (int i = 0; i < CH; ++i) {
     const int e = tid + NT * i;
     if (e < NK) {
-      const int row = e / XK, x = e % XK, R = 16 * ((row >> 2) & 3) + 4 * (row >> 4) + (row & 3);
-      off[i] = uint32_t((row & 15) * a.hd + min(16 * x, a.hd - 16));
+      const int row = e / XK, x = e % XK, k = row & 15, R = (row & 32) + 8 * (k >> 2) + 4 * ((row >> 4) & 1) + (k & 3);
+      off[i] = uint32_t(k * a.hd + min(16 * x, a.hd - 16));
       l0[i] = k_at(R, 2 * x);
       grp0[i] = __builtin_amdgcn_readfirstlane(row >> 4);
     } else {
@@ -556,25 +573,66 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_paged_wide_kernel(PagedArgs a
   // (pieces of keys come first; a wave's i-th pieces are all of one kind)
   auto of_keys = [&](int i) { return wave * 64 + NT * i < NK; };
 
-  for (int tile = a.tiles - 1 - int(blockIdx.x) % a.tiles; long(tile) * RB < w.rows; tile += a.tiles) {
+  // (the last rows first: with causal masks they have the most keys)
+  for (int tile = a.tiles - 1 - it.item / a.splits; long(tile) * RB < w.rows; tile += a.tiles) {
     const int R0 = tile * RB, r_first = R0 + wave * RW;
-    const int i0 = R0 / a.G, i1 = (min(R0 + RB, w.rows) - 1) / a.G;
-    const KeyRange all = seen_keys(w.len, w.nq, i0, i1, a.causal, a.window);
+    const KeyRange all = seen_keys(w.len, w.nq, R0 / a.G, (min(R0 + RB, w.rows) - 1) / a.G, a.causal, a.window);
     const KeyRange mine = key_share(all, w.split, a.splits, a.chunk);
-    const int some_lo = max(all.lo, mine.lo), all_hi = min(seen_keys(w.len, w.nq, i0, i0, a.causal, a.window).hi, mine.hi),
-              all_lo = max(seen_keys(w.len, w.nq, i1, i1, a.causal, a.window).lo, mine.lo);
+    // keys that every row of the workgroup sees, and the first that some row does
+    const int all_lo = max(seen_keys(w.len, w.nq, (min(R0 + RB, w.rows) - 1) / a.G, 0, a.causal, a.window).lo, mine.lo),
+              all_hi = min(seen_keys(w.len, w.nq, 0, R0 / a.G, a.causal, a.window).hi, mine.hi), any_lo = max(all.lo, mine.lo);
     const bool on = r_first < w.rows;
-    RowTiles<DT, HDP, NQ> q;
-    if (on) q.start(a, w.row0, w.nq, w.len, w.rows, r_first, w.kvh, n, mine, [&](int s) { return 32 * s + 8 * g; });
 
-    const int first = mine.lo & ~(kKeyBlock - 1);
-    // (as above: every load is made)
+    // ---- this wave's rows: column n is row r_first + n (past the last, that row
+    // again, not stored)
+    const int row = min(r_first + n, w.rows - 1), qi = row / a.G;
+    const int i0 = min(r_first, w.rows - 1) / a.G, i1 = (min(r_first + RW, w.rows) - 1) / a.G;
+    const KeyRange kr = seen_keys(w.len, w.nq, qi, qi, a.causal, a.window);
+    const int row_lo = max(kr.lo, mine.lo), row_hi = min(kr.hi, mine.hi);
+    const KeyRange some = seen_keys(w.len, w.nq, i0, i1, a.causal, a.window);
+    const int every_lo = max(seen_keys(w.len, w.nq, i1, i1, a.causal, a.window).lo, mine.lo);
+    const int every_hi = min(seen_keys(w.len, w.nq, i0, i0, a.causal, a.window).hi, mine.hi);
+    f16x8 qf[NP][KS];
+    float c_row, mx = -__builtin_inff(), l = 0.f, lref = -126.f;  // lref: log2 of the largest value scale seen
+    f32x16 acc[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) acc[i][j] = 0.f;
+    {
+      const T *qp = static_cast<const T *>(a.q) + long(w.row0 + qi) * a.ldq + long(w.kvh * a.G + row - qi * a.G) * a.hd;
+      float v[KS][8], big = 0.f;
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const int d = 16 * s + 8 * h, e = min(d, a.hd - 8);
+        if constexpr (DT == F32) {
+          ld4<F32>(qp + e, v[s]);
+          ld4<F32>(qp + e + 4, v[s] + 4);
+        } else {
+          dec8<DT>(*reinterpret_cast<const uint4 *>(qp + e), v[s]);
+        }
+#pragma unroll
+        for (int e8 = 0; e8 < 8; ++e8) v[s][e8] = d < a.hd ? v[s][e8] : 0.f;
+        big = finite_max8(v[s], big);
+      }
+      const float up = row_lift(xor32_max(big));
+      c_row = a.c / up;  // (a power of two)
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float x = v[s][e] * up;
+          const _Float16 h0 = _Float16(x);
+          qf[0][s][e] = h0;
+          if constexpr (NP == 2) qf[1][s][e] = _Float16(x - float(h0));
+        }
+    }
+
+    // ---- the loader.  Every load is made, at an address that exists (see above).
     auto page_of = [&](int base, int grp) {
       const int p = table[min(base + 16 * grp, mine.hi - 1) >> a.plog];
       return page_in_pool(p, a.n_pages) ? p : -1;
     };
-    const uint8_t *kc = a.kc + page_base(0, a.Hkv, w.kvh, P, a.hd), *vc = a.vc + page_base(0, a.Hkv, w.kvh, P, a.hd);
-    const int64_t stride = page_base(1, a.Hkv, 0, P, a.hd);
     int page[CH], ipage = -1, holes = 0;  // holes: pieces of the fetched block whose page is outside the pool
     uint4 raw[CH];
     float isc = 0.f, ivs = 0.f;
@@ -603,10 +661,10 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_paged_wide_kernel(PagedArgs a
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
           if (of_keys(i)) continue;
-          int row, grp;
-          (void)value_piece(i, row, grp);
+          int vrow, grp;
+          (void)value_piece(i, vrow, grp);
           const int t = base + 16 * grp;
-          raw[i] = keep_bytes(raw[i], min(max(some_lo - t, 0), 16), holes >> i & 1 ? 0 : min(max(mine.hi - t, 0), 16));
+          raw[i] = keep_bytes(raw[i], min(max(any_lo - t, 0), 16), holes >> i & 1 ? 0 : min(max(mine.hi - t, 0), 16));
           uint32_t b[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w}, bits = 0;
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
@@ -616,7 +674,7 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_paged_wide_kernel(PagedArgs a
           }
           raw[i] = make_uint4(b[0], b[1], b[2], b[3]);
           any |= bits;
-          reinterpret_cast<uint16_t *>(nan_at[buf])[row * 4 + grp] = uint16_t(bits);
+          reinterpret_cast<uint16_t *>(nan_at[buf])[vrow * 4 + grp] = uint16_t(bits);
         }
         any = __any(any != 0);
       }
@@ -639,6 +697,7 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_paged_wide_kernel(PagedArgs a
     };
 
     if (mine.lo < mine.hi) {
+      const int first = mine.lo & ~(kKeyBlock - 1);
       ask(first);
       fetch(first);
       int ip = ipage;
@@ -653,31 +712,104 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_paged_wide_kernel(PagedArgs a
           fetch(base + kKeyBlock);
           ask(base + 2 * kKeyBlock);
         }
-        if (on && base < q.some_hi && base + kKeyBlock > q.some_lo) {
-          const float4 in = info[buf][g];
-          const bool page_ok = in.z != 0.f;
+        if (on && base < some.hi && base + kKeyBlock > some.lo) {
           const uint8_t *L = lds[buf];
-          f32x4 s[4][NQ];
+          // this lane half's two runs of keys: 16 h of either tile
+          const float4 in[2] = {info[buf][h], info[buf][2 + h]};
+          f32x16 s[2];
 #pragma unroll
-          for (int t = 0; t < 4; ++t) {
+          for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int x = 0; x < NQ; ++x) s[t][x] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int j = 0; j < 16; ++j) s[t][j] = 0.f;
 #pragma unroll
-            for (int c = 0; c < HDP / 32; ++c) {
-              const f16x8 k = *reinterpret_cast<const f16x8 *>(L + k_at(16 * t + n, 4 * c + g));
+          for (int c = 0; c < KS; ++c)
 #pragma unroll
-              for (int x = 0; x < NQ; ++x)
+            for (int t = 0; t < 2; ++t) {
+              const f16x8 k = *reinterpret_cast<const f16x8 *>(L + k_at(32 * t + n, 2 * c + h));
 #pragma unroll
-                for (int p = q.NP - 1; p >= 0; --p)
-                  s[t][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q.qf[p][x][c], s[t][x], 0, 0, 0);
+              for (int p = NP - 1; p >= 0; --p) s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qf[p][c], s[t], 0, 0, 0);
             }
-          }
-          const bool masked = base < q.every_lo || base + kKeyBlock > q.every_hi || __any(!page_ok);
-          q.probabilities(s, in.x, in.y, in.w, page_ok, base + 16 * g, masked);
+          float lv[2] = {in[0].y, in[1].y}, lv_top = in[0].w;
+          const bool ok0 = in[0].z != 0.f, ok1 = in[1].z != 0.f;
+          auto seen = [&](int t) -> uint32_t {  // bit i: this row sees key 32 t + 16 h + i
+            const int k0 = base + 32 * t + 16 * h, lo = min(max(row_lo - k0, 0), 16), hi = min(max(row_hi - k0, 0), 16);
+            return (t ? ok1 : ok0) ? ((1u << hi) - 1u) & ~((1u << lo) - 1u) : 0u;
+          };
+          const bool masked = base < every_lo || base + kKeyBlock > every_hi || __any(!ok0 || !ok1);
+          if (masked) {
+            const uint32_t ok[2] = {seen(0), seen(1)};
 #pragma unroll
-          for (int i = 0; i < MT; ++i)
-            q.values(i, *reinterpret_cast<const f16x8 *>(L + v_at(16 * i + n, 2 * g)),
-                     *reinterpret_cast<const f16x8 *>(L + v_at(16 * i + n, 2 * g + 1)));
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+              for (int j = 0; j < 16; ++j) s[t][j] = (ok[t] >> j) & 1u ? s[t][j] : -__builtin_inff();
+            // a page of which the row sees nothing does not count for its values' scale
+            lv_top = xor32_max(fmaxf(ok[0] ? lv[0] : -126.f, ok[1] ? lv[1] : -126.f));
+#pragma unroll
+            for (int t = 0; t < 2; ++t) lv[t] = ok[t] ? lv[t] : fmaxf(lv_top, lref);
+          }
+          const float lnew = fmaxf(lv_top, lref);
+          const float rescale = lnew == lref ? 1.f : __builtin_amdgcn_exp2f(lref - lnew);
+          lref = lnew;
+          // (a page's scale is positive: the largest raw score is its largest score)
+          float f[2] = {in[0].x * c_row, in[1].x * c_row}, top = -__builtin_inff();
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            f[t] = f[t] == 0.f ? 1e-37f : f[t];  // (so that a masked score stays -inf)
+            float m = s[t][0];
+#pragma unroll
+            for (int j = 1; j < 16; ++j) m = fmaxf(m, s[t][j]);
+            top = fmaxf(top, m > -__builtin_inff() ? m * f[t] : m);
+          }
+          top = xor32_max(top);
+          top = top > mx + kRaise ? top : mx;
+          float ref = top > -__builtin_inff() ? top : 0.f;
+          const float down = mx == top ? 1.f : __builtin_amdgcn_exp2f(mx - ref);
+          mx = top;
+          if (__any(down * rescale != 1.f)) {
+            l *= down;
+#pragma unroll
+            for (int i = 0; i < MT; ++i) acc[i] *= down * rescale;
+          }
+          const bool far = __builtin_fabsf(ref) > 65536.f;
+          if (__any(far)) {
+#pragma clang fp contract(off)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+#pragma unroll
+              for (int j = 0; j < 16; ++j) s[t][j] = far ? s[t][j] * f[t] - ref : s[t][j];
+              f[t] = far ? 1.f : f[t];
+            }
+            ref = far ? 0.f : ref;
+          }
+          // probabilities of 32 keys, and their values
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            const float lf = lv[t] - lnew, unscale = __builtin_amdgcn_exp2f(-lf), lift = __builtin_amdgcn_exp2f(lf + kLift),
+                        shift = lf + kLift - ref;
+            float sum = 0.f;
+            f16x8 pf[NP][2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                const float raw_s = s[t][8 * u + e];
+                float p = __builtin_amdgcn_exp2f(NP == 2 ? fmaf(raw_s, f[t], -ref) : fmaf(raw_s, f[t], shift));
+                if constexpr (NP == 2) p *= lift;
+                sum += p;  // (not of the rounded values: see above)
+                const _Float16 h0 = _Float16(p);
+                pf[0][u][e] = h0;
+                if constexpr (NP == 2) pf[1][u][e] = _Float16(p - float(h0));
+              }
+            l = fmaf(sum, unscale, l);
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+              for (int u = 0; u < 2; ++u) {
+                const f16x8 v = *reinterpret_cast<const f16x8 *>(L + v_at(32 * i + n, 4 * t + 2 * h + u));
+#pragma unroll
+                for (int p = NP - 1; p >= 0; --p) acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pf[p][u], acc[i], 0, 0, 0);
+              }
+          }
           uint32_t nans = 0;
           if (masked)
 #pragma unroll
@@ -685,41 +817,31 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_paged_wide_kernel(PagedArgs a
           if (__builtin_amdgcn_readfirstlane(nans)) {
             // outputs of rows that see a NaN value (a zero probability alone would
             // not keep it from the others)
-            uint64_t seen[NQ];
-#pragma unroll
-            for (int x = 0; x < NQ; ++x) {
-              seen[x] = 0;
-#pragma unroll
-              for (int c = 0; c < 4; ++c)
-                seen[x] |= uint64_t(uint32_t(__shfl(int(q.seen(x, base + 16 * g, page_ok)), 16 * c + n, 64))) << (16 * c);
-            }
+            uint64_t sees = uint64_t(seen(0)) << (16 * h) | uint64_t(seen(1)) << (32 + 16 * h);
+            sees |= uint64_t(uint32_t(__shfl_xor(int(uint32_t(sees)), 32, 64))) |
+                    uint64_t(uint32_t(__shfl_xor(int(uint32_t(sees >> 32)), 32, 64))) << 32;
 #pragma unroll
             for (int i = 0; i < MT; ++i)
 #pragma unroll
-              for (int r = 0; r < 4; ++r) {
-                const uint64_t at = nan_at[buf][16 * i + 4 * g + r];
-#pragma unroll
-                for (int x = 0; x < NQ; ++x)
-                  if (at & seen[x]) q.acc[i][x][r] = __builtin_nanf("");
-              }
+              for (int j = 0; j < 16; ++j)
+                if (nan_at[buf][32 * i + 8 * (j >> 2) + 4 * h + (j & 3)] & sees) acc[i][j] = __builtin_nanf("");
           }
         }
         if (more) place(base + kKeyBlock, ip, buf ^ 1);
         __syncthreads();
       }
     }
-    if (on) {
-      q.finish();
+    l = xor32_add(l);
+    if (r_first + n < w.rows) {
+      const RowOut<DT> to(a, w.row0, w.kvh, w.split, row, mx, l, h == 0);
+      const float vref = __builtin_amdgcn_exp2f(lref);
 #pragma unroll
-      for (int x = 0; x < NQ; ++x) {
-        const int r = r_first + 16 * x + n;
-        if (r < w.rows) {
-          const RowOut<DT> to(a, w.row0, w.kvh, w.split, r, q.mx[x], q.l[x], g == 0);
+      for (int i = 0; i < MT; ++i)
 #pragma unroll
-          for (int i = 0; i < MT; ++i)
-            if (16 * i < a.hd) to.put(16 * i + 4 * g, q.acc[i][x]);
+        for (int j = 0; j < 4; ++j) {
+          const int d = 32 * i + 8 * j + 4 * h;
+          if (d < a.hd) to.put(d, f32x4{acc[i][4 * j], acc[i][4 * j + 1], acc[i][4 * j + 2], acc[i][4 * j + 3]} * vref);
         }
-      }
     }
   }
 }
@@ -764,9 +886,8 @@ hipError_t launch(const PagedArgs &a, const PagedShape &s, hipStream_t st) {
   const long blocks = long(s.tiles) * s.splits * a.Hkv * a.B;
   if (blocks * 512 > 0xffffffffL) return hipErrorInvalidValue;
   const dim3 grid{unsigned(blocks)};
-  constexpr int NQ = DT == F32 || HDP > 128 ? 1 : 2, NW = HDP > 128 ? 8 : 4;
   if (s.wide)
-    hipLaunchKernelGGL((attn_paged_wide_kernel<DT, HDP, NQ, NW>), grid, dim3(64 * NW), 0, st, a);
+    hipLaunchKernelGGL((attn_paged_wide_kernel<DT, HDP>), grid, dim3(256), 0, st, a);
   else
     hipLaunchKernelGGL((attn_paged_kernel<DT, HDP>), grid, dim3(256), 0, st, a);
   hipError_t e = hipGetLastError();

@@ -254,7 +254,7 @@ PagedShape paged_call_shape(int dt, int B, int n_rows, int Hq, int Hkv, int hd, 
   if (Hkv < 1 || Hq < 1 || Hq % Hkv) throw Error("attention_paged: query heads must be a multiple of key/value heads");
   if (hd < 16 || hd > kPagedHeadMax || hd % 16) throw Error("attention_paged: head_dim must be a multiple of 16, at most 256");
   if (int64_t(n_rows) * Hq > (1 << 30)) throw Error("attention_paged: more than 2^30 query rows");
-  return paged_shape(dt == F32, B, Hq, Hkv, hd, std::min(max_q, n_rows), max_len, window);
+  return paged_shape(B, Hq, Hkv, std::min(max_q, n_rows), max_len, window);
 }
 
 }  // namespace

@@ -80,19 +80,42 @@ constexpr int kPlanRequests = 1;
 // where one token in a page does.
 inline int store_tokens(int n, int heads) { return int(std::min<int64_t>(64, std::max<int64_t>(1, int64_t(n) * heads / 16384))); }
 
+// Workgroup i of a launch over `pairs` (sequence, key/value head) pairs of `per`
+// items each.  Workgroups go round the eight XCDs, each with an L2 of its own:
+// eight pairs at a time, one to an XCD, so that the items that read the same
+// keys find them there (6 requests of 8000 tokens, 8 heads: 1029 us with a pair's
+// items in any XCD and items of all pairs at once, 820 with one pair's items
+// after another over all XCDs).  The pairs left over go round all of them.
+constexpr int kXcds = 8;
+struct PairItem {
+  int pair, item;
+};
+__host__ __device__ __forceinline__ PairItem pair_item(uint32_t i, int pairs, int per) {
+  PairItem r;
+  const uint32_t whole = uint32_t(pairs / kXcds) * kXcds * uint32_t(per);
+  if (i < whole) {
+    const uint32_t j = i / kXcds;
+    r.pair = int(i % kXcds + kXcds * (j / uint32_t(per)));
+    r.item = int(j % uint32_t(per));
+  } else {
+    r.pair = pairs / kXcds * kXcds + int((i - whole) / uint32_t(per));
+    r.item = int((i - whole) % uint32_t(per));
+  }
+  return r;
+}
+
 // How a call is cut: rows of one (sequence, key/value head) in tiles, and each
 // tile's keys in `splits` shares of `chunk`.
 struct PagedShape {
   int wide, tiles, splits, chunk;
 };
-// Rows that a workgroup of the wide form takes: eight waves of one or two MFMA
-// tiles (one for fp32, whose operands are in two parts, and for heads above 128).
-inline int paged_wide_rows(bool f32, int hd) { return f32 && hd <= 128 ? 64 : 128; }
-inline PagedShape paged_shape(bool f32, int B, int Hq, int Hkv, int hd, int max_q, int max_len, int window) {
+// Rows that a workgroup of the wide form takes: 32 to each of four waves.
+constexpr int kPagedWideRows = 128;
+inline PagedShape paged_shape(int B, int Hq, int Hkv, int max_q, int max_len, int window) {
   PagedShape s;
   const int64_t rows = int64_t(max_q) * (Hq / Hkv);
   s.wide = rows > 16;
-  const int per = s.wide ? paged_wide_rows(f32, hd) : 16;
+  const int per = s.wide ? kPagedWideRows : 16;
   s.tiles = int(std::max<int64_t>(1, (rows + per - 1) / per));
   // Shares so that about 1024 workgroups are in flight (four per CU), none
   // shorter than one block per wave.

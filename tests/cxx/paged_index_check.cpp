@@ -86,15 +86,25 @@ int main() {
       const int per = store_tokens(n, heads);
       need(per >= 1 && per <= 64, "tokens per workgroup of the store");
     }
+  for (int t = 0; t < 300; ++t) {  // every item of every pair once
+    const int pairs = 1 + upto(40), per = 1 + upto(30);
+    std::vector<int> hits(size_t(pairs * per), 0);
+    for (int i = 0; i < pairs * per; ++i) {
+      const PairItem r = pair_item(uint32_t(i), pairs, per);
+      need(r.pair >= 0 && r.pair < pairs && r.item >= 0 && r.item < per, "pair and item");
+      ++hits[size_t(r.pair * per + r.item)];
+    }
+    for (int h : hits) need(h == 1, "every item once");
+  }
   for (int t = 0; t < 50000; ++t) {
     const int kv = 1 + upto(16), g = 1 + upto(16), hd = 16 * (1 + upto(16)), B = 1 + upto(t % 4 ? 300 : 100000);
     const int max_q = 1 + upto(t % 2 ? 4 : 5000), max_len = upto(t % 3 ? 0x7fffffff : 5000), window = t % 5 ? 0 : 1 + upto(5000);
-    const PagedShape s = paged_shape(t & 1, B, kv * g, kv, hd, max_q, max_len, window);
+    const PagedShape s = paged_shape(B, kv * g, kv, max_q, max_len, window);
     need(s.tiles >= 1 && s.splits >= 1 && s.splits <= 256 && s.chunk % kKeyBlock == 0, "cut of a call");
     const long keys = window ? std::min<long>(max_len, long(window) + max_q + kKeyBlock) : max_len;
     need(long(s.splits) * s.chunk >= keys, "the shares hold the longest request");
     need((s.splits > 1) == (paged_workspace_bytes(max_q, kv * g, hd, s.splits) > 0), "workspace where shares are joined");
   }
-  need(paged_shape(false, 0, 8, 8, 64, 0, 0, 0).splits == 1, "empty call");
+  need(paged_shape(0, 8, 8, 0, 0, 0).splits == 1, "empty call");
   std::puts("ok");
 }
