@@ -55,6 +55,11 @@ struct PagedArgs {
   float c;  // scale * log2(e)
 };
 
+// A table that the launch does not change, for loads into scalar registers at
+// scalar indexes.
+typedef const __attribute__((address_space(4))) int32_t *ScalarTable;
+__device__ __forceinline__ ScalarTable scalar_ptr(const int32_t *p) { return (ScalarTable)(uintptr_t)p; }
+
 // 8 e4m3 bytes -> 8 fp16 values, exact
 __device__ __forceinline__ f16x8 cvt8(uint32_t lo, uint32_t hi) {
   const f16x2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, false);
@@ -346,9 +351,9 @@ template <int DT> struct RowOut {
 struct Part {
   int split, kvh, b, len, row0, nq, rows;
 };
-__device__ __forceinline__ bool part_of(const PagedArgs &a, int id, Part &w) {
-  w.kvh = id % a.Hkv;
-  w.b = id / a.Hkv;
+__device__ __forceinline__ bool part_of(const PagedArgs &a, int b, int kvh, Part &w) {
+  w.kvh = kvh;
+  w.b = b;
   const int most = a.width << a.plog, len = a.lens[w.b];
   w.len = min(max(len, 0), most);
   w.row0 = a.cu[w.b];
@@ -369,7 +374,8 @@ __global__ void __launch_bounds__(256) attn_paged_kernel(PagedArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, g = lane >> 4;
   Part w;
   w.split = int(blockIdx.x) / a.tiles % a.splits;
-  if (!part_of(a, int(blockIdx.x) / a.tiles / a.splits, w)) return;
+  const int pair = int(blockIdx.x) / a.tiles / a.splits;
+  if (!part_of(a, pair / a.Hkv, pair % a.Hkv, w)) return;
   const int P = 1 << a.plog;
   const int32_t *table = a.tables + long(w.b) * a.width;
   const uint8_t *kc = a.kc + page_base(0, a.Hkv, w.kvh, P, a.hd), *vc = a.vc + page_base(0, a.Hkv, w.kvh, P, a.hd);
@@ -532,7 +538,22 @@ __global__ void __launch_bounds__(256, DT == F32 || HDP > 128 ? 1 : 2) attn_page
   Part w;
   const PairItem it = pair_item(blockIdx.x, a.B * a.Hkv, a.tiles * a.splits);
   w.split = it.item % a.splits;
-  if (!part_of(a, it.pair, w)) return;
+  int b = it.pair / a.Hkv;
+  if (a.B <= NT && a.B > 1) {
+    // Requests from the longest to the shortest, so that none of the long ones is left
+    // for the end (6 requests of 1200 to 8000 keys: the last workgroup ends 3 %
+    // past the mean instead of 6 to 33 %)
+    __shared__ int lens[NT], found;
+    const int mine = tid < a.B ? a.lens[tid] : 0;
+    lens[tid] = mine;
+    __syncthreads();
+    int rank = 0;
+    for (int v = 0; v < a.B; ++v) rank += lens[v] > mine || (lens[v] == mine && v < tid);
+    if (tid < a.B && rank == b) found = tid;
+    __syncthreads();
+    b = __builtin_amdgcn_readfirstlane(found);
+  }
+  if (!part_of(a, b, it.pair % a.Hkv, w)) return;
   const int P = 1 << a.plog;
   const int32_t *table = a.tables + long(w.b) * a.width;
   const uint8_t *kc = a.kc + page_base(0, a.Hkv, w.kvh, P, a.hd), *vc = a.vc + page_base(0, a.Hkv, w.kvh, P, a.hd);
@@ -634,20 +655,23 @@ __global__ void __launch_bounds__(256, DT == F32 || HDP > 128 ? 1 : 2) attn_page
       return page_in_pool(p, a.n_pages) ? p : -1;
     };
     int page[CH], ipage = -1, holes = 0;  // holes: pieces of the fetched block whose page is outside the pool
+    const int last = __builtin_amdgcn_readfirstlane(mine.hi) - 1;
+    const auto table_s = scalar_ptr(table);
     uint4 raw[CH];
     float isc = 0.f, ivs = 0.f;
     auto ask = [&](int base) {  // pages of the block
 #pragma unroll
-      for (int i = 0; i < CH; ++i) page[i] = page_of(base, grp0[i]);
+      for (int i = 0; i < CH; ++i) page[i] = table_s[min(base + 16 * grp0[i], last) >> a.plog];
       if (wave == 0) ipage = page_of(base, tid & 3);
     };
     auto fetch = [&](int base) {  // its bytes and scales
       holes = 0;
 #pragma unroll
       for (int i = 0; i < CH; ++i) {
-        const int p = __builtin_amdgcn_readfirstlane(page[i]), at = (base + 16 * grp0[i]) & (P - 1);
-        if (p < 0) holes |= 1 << i;
-        const uint8_t *from = (of_keys(i) ? kc + at * a.hd : vc + at) + max(p, 0) * stride;
+        const bool in = page_in_pool(page[i], a.n_pages);
+        const int p = in ? page[i] : 0, at = (base + 16 * grp0[i]) & (P - 1);
+        if (!in) holes |= 1 << i;
+        const uint8_t *from = (of_keys(i) ? kc + at * a.hd : vc + at) + p * stride;
         raw[i] = *reinterpret_cast<const uint4 *>(from + off[i]);
       }
       if (wave == 0) {
@@ -708,12 +732,16 @@ __global__ void __launch_bounds__(256, DT == F32 || HDP > 128 ? 1 : 2) attn_page
       for (int base = first; base < mine.hi; base += kKeyBlock, buf ^= 1) {
         const bool more = base + kKeyBlock < mine.hi;
         ip = ipage;
-        if (more) {
+        const bool busy = on && base < some.hi && base + kKeyBlock > some.lo;
+        if (more && !busy) {
           fetch(base + kKeyBlock);
           ask(base + 2 * kKeyBlock);
         }
-        if (on && base < some.hi && base + kKeyBlock > some.lo) {
-          const uint8_t *L = lds[buf];
+        if (busy) {
+          // LDS bytes of this lane's first operands; the chunks of a row differ in an
+          // exclusive or (hidden from the compiler, which would keep every sum)
+          uint32_t at_k = uint32_t(buf) * (KB + VB) + k_at(n, h), at_v = uint32_t(buf) * (KB + VB) + v_at(n, 2 * h);
+          asm volatile("" : "+v"(at_k), "+v"(at_v));
           // this lane half's two runs of keys: 16 h of either tile
           const float4 in[2] = {info[buf][h], info[buf][2 + h]};
           f32x16 s[2];
@@ -721,14 +749,36 @@ __global__ void __launch_bounds__(256, DT == F32 || HDP > 128 ? 1 : 2) attn_page
           for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int j = 0; j < 16; ++j) s[t][j] = 0.f;
+          // Operands are read two steps ahead of their products (left alone, the
+          // compiler reads one, waits, multiplies: 1.2 of 3 us a block).
+          f16x8 kf[2][2][2];
+          auto read_keys = [&](int b) {
 #pragma unroll
-          for (int c = 0; c < KS; ++c)
+            for (int c = 0; c < 2; ++c)
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-              const f16x8 k = *reinterpret_cast<const f16x8 *>(L + k_at(32 * t + n, 2 * c + h));
+              for (int t = 0; t < 2; ++t)
+                kf[b & 1][c][t] = *reinterpret_cast<const f16x8 *>(lds[0] + (at_k ^ (32 * (2 * b + c))) + 32 * t * KROW);
+          };
+          read_keys(0);
 #pragma unroll
-              for (int p = NP - 1; p >= 0; --p) s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qf[p][c], s[t], 0, 0, 0);
-            }
+          for (int b = 0; b < KS / 2; ++b) {
+            if (b + 1 < KS / 2) read_keys(b + 1);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+              for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int p = NP - 1; p >= 0; --p)
+                  s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[b & 1][c][t], qf[p][2 * b + c], s[t], 0, 0, 0);
+          }
+          // (here, where the operands of the scores have left their registers; and
+          // scalar loads where no LDS read is on its way: the two share a counter and
+          // come back in any order)
+          if (more) {
+            fetch(base + kKeyBlock);
+            ask(base + 2 * kKeyBlock);
+          }
           float lv[2] = {in[0].y, in[1].y}, lv_top = in[0].w;
           const bool ok0 = in[0].z != 0.f, ok1 = in[1].z != 0.f;
           auto seen = [&](int t) -> uint32_t {  // bit i: this row sees key 32 t + 16 h + i
@@ -781,7 +831,21 @@ __global__ void __launch_bounds__(256, DT == F32 || HDP > 128 ? 1 : 2) attn_page
             }
             ref = far ? 0.f : ref;
           }
-          // probabilities of 32 keys, and their values
+          // probabilities of 32 keys, and their values; the next values on their way
+          // (heads up to 128: above, the registers do not hold two tiles' values)
+          constexpr bool AHEAD = HDP <= 128;
+          f16x8 vf[2][AHEAD ? MT : 1];
+          auto value_at = [&](int k, int i) {  // step k: keys 8 (k & 1) .. + 7 of tile k / 2's runs
+            return *reinterpret_cast<const f16x8 *>(lds[0] + (at_v ^ (16 * (4 * (k >> 1) + (k & 1)))) + 32 * i * 128);
+          };
+          auto read_values = [&](int k) {
+            if constexpr (AHEAD) {
+#pragma unroll
+              for (int i = 0; i < MT; ++i) vf[k & 1][i] = value_at(k, i);
+              __builtin_amdgcn_sched_barrier(0);
+            }
+          };
+          read_values(0);
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
             const float lf = lv[t] - lnew, unscale = __builtin_amdgcn_exp2f(-lf), lift = __builtin_amdgcn_exp2f(lf + kLift),
@@ -802,13 +866,17 @@ __global__ void __launch_bounds__(256, DT == F32 || HDP > 128 ? 1 : 2) attn_page
               }
             l = fmaf(sum, unscale, l);
 #pragma unroll
-            for (int i = 0; i < MT; ++i)
+            for (int u = 0; u < 2; ++u) {
+              if (2 * t + u < 3) read_values(2 * t + u + 1);
 #pragma unroll
-              for (int u = 0; u < 2; ++u) {
-                const f16x8 v = *reinterpret_cast<const f16x8 *>(L + v_at(32 * i + n, 4 * t + 2 * h + u));
+              for (int i = 0; i < MT; ++i) {
+                f16x8 v;
+                if constexpr (AHEAD) v = vf[u][i];
+                else v = value_at(2 * t + u, i);
 #pragma unroll
                 for (int p = NP - 1; p >= 0; --p) acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pf[p][u], acc[i], 0, 0, 0);
               }
+            }
           }
           uint32_t nans = 0;
           if (masked)
