@@ -55,6 +55,15 @@ struct PagedArgs {
   float c;  // scale * log2(e)
 };
 
+// Barrier that waits for this wave's LDS operations and not for its loads from
+// memory.
+__device__ __forceinline__ void lds_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
 // A table that the launch does not change, for loads into scalar registers at
 // scalar indexes.
 typedef const __attribute__((address_space(4))) int32_t *ScalarTable;
@@ -395,31 +404,53 @@ __global__ void __launch_bounds__(256) attn_paged_kernel(PagedArgs a) {
     // a lane loads its keys)
     q.start(a, w.row0, w.nq, w.len, w.rows, r_first, w.kvh, n, mine, [&](int s) { return 64 * (s >> 1) + 16 * g + 8 * (s & 1); });
 
-    for (int base = (mine.lo & ~(kKeyBlock - 1)) + wave * kKeyBlock; base < mine.hi; base += 4 * kKeyBlock) {
-      // the pages of this lane's key rows (group n >> 2) and of its scores and
-      // values (group g).  Every load is made, at an address that exists, and
-      // what should not count is masked: a load under a condition makes the
-      // compiler wait for it before the next.  Keys past the range take its
-      // last page; a page outside the pool holds no keys (page 0 is read); head
-      // values past hd repeat earlier ones (their queries are zero, their outputs
-      // not stored).
+    // A block's keys are on their way while the probabilities and values of the block
+    // before are worked on, its values during its scores: they take the registers
+    // that those have left.  Every load is made, at an address that exists, and
+    // what should not count is masked: a load under a condition makes the compiler
+    // wait for it before the next.  Keys past the range take its last page; a page
+    // outside the pool holds no keys (page 0 is read); head values past hd repeat
+    // earlier ones (their queries are zero, their outputs not stored).
+    int pk = 0, pv = 0;                 // pages of this lane's key rows (group n >> 2), of its scores and values (group g)
+    bool next_ok = false;
+    uint4 kr[4][J], vr[MT];
+    float ksc = 0.f, vsc = 0.f;
+    auto pages = [&](int base) {
+      pk = table[min(base + 16 * (n >> 2), mine.hi - 1) >> a.plog];
+      pv = table[min(base + 16 * g, mine.hi - 1) >> a.plog];
+    };
+    auto load_keys = [&](int base) {
       const int tk = base + 16 * (n >> 2), tv = base + 16 * g;
-      int pk = table[min(tk, mine.hi - 1) >> a.plog], pv = table[min(tv, mine.hi - 1) >> a.plog];
-      const bool page_ok = page_in_pool(pv, a.n_pages);
-      if (!page_ok && tv < mine.hi && n == 0) atomicOr(a.err, kErrPage);
+      next_ok = page_in_pool(pv, a.n_pages);
+      if (!next_ok && tv < mine.hi && n == 0) atomicOr(a.err, kErrPage);
       pk = page_in_pool(pk, a.n_pages) ? pk : 0;
-      pv = page_ok ? pv : 0;
-      const uint8_t *kp = kc + pk * stride + (tk & (P - 1)) * a.hd, *vp = vc + pv * stride + (tv & (P - 1)) + n * P;
-      uint4 kr[4][J], vr[MT];
+      pv = next_ok ? pv : 0;
+      const uint8_t *kp = kc + pk * stride + (tk & (P - 1)) * a.hd;
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int j = 0; j < J; ++j)
           kr[t][j] = *reinterpret_cast<const uint4 *>(kp + (4 * t + (n & 3)) * a.hd + min(64 * j + 16 * g, a.hd - 16));
+      ksc = a.ks[long(pv) * a.Hkv + w.kvh];
+      vsc = a.vs[long(pv) * a.Hkv + w.kvh];
+    };
+    auto load_values = [&](int base) {
+      const uint8_t *vp = vc + pv * stride + ((base + 16 * g) & (P - 1)) + n * P;
 #pragma unroll
       for (int i = 0; i < MT; ++i) vr[i] = *reinterpret_cast<const uint4 *>(vp + min(16 * i, a.hd - 16) * P);
-      const float ksc = a.ks[long(pv) * a.Hkv + w.kvh], vsc = a.vs[long(pv) * a.Hkv + w.kvh];
-
+    };
+    int base = (mine.lo & ~(kKeyBlock - 1)) + wave * kKeyBlock;
+    if (base < mine.hi) {
+      pages(base);
+      load_keys(base);
+      load_values(base);
+    }
+    while (base < mine.hi) {
+      // (the last block's successor is itself: its bytes are in the caches)
+      const int next = base + 4 * kKeyBlock, then = next < mine.hi ? next : base, tv = base + 16 * g;
+      const bool page_ok = next_ok;
+      const float lv = page_ok ? fmaxf(__builtin_amdgcn_logf(vsc), -126.f) : -126.f, kscale = ksc;
+      pages(then);
       f32x4 s[4][1];
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
@@ -434,9 +465,10 @@ __global__ void __launch_bounds__(256) attn_paged_kernel(PagedArgs a) {
           }
         }
       }
-      const float lv = page_ok ? fmaxf(__builtin_amdgcn_logf(vsc), -126.f) : -126.f;
+      load_keys(then);
+      __builtin_amdgcn_sched_barrier(0);
       const bool masked = base < q.every_lo || base + kKeyBlock > q.every_hi || __any(!page_ok);
-      q.probabilities(s, ksc, lv, xor32_max(xor16_max(lv)), page_ok, tv, masked);
+      q.probabilities(s, kscale, lv, xor32_max(xor16_max(lv)), page_ok, tv, masked);
 
       // Keys that no row sees may hold anything, NaN among it: their bytes are
       // cleared.
@@ -467,6 +499,8 @@ __global__ void __launch_bounds__(256) attn_paged_kernel(PagedArgs a) {
       }
 #pragma unroll
       for (int i = 0; i < MT; ++i) q.values(i, cvt8(vr[i].x, vr[i].y), cvt8(vr[i].z, vr[i].w));
+      base = next;
+      if (base < mine.hi) load_values(base);
     }
     q.finish();
 
@@ -476,7 +510,7 @@ __global__ void __launch_bounds__(256) attn_paged_kernel(PagedArgs a) {
     for (int part = 0; part < HDP / MW; ++part) {
 #pragma unroll
       for (int i = 0; i < MW / 16; ++i) *reinterpret_cast<f32x4 *>(&wo[wave][n][16 * i + 4 * g]) = q.acc[part * (MW / 16) + i][0];
-      __syncthreads();
+      lds_barrier();  // (not for the loads of the block after the last)
       for (int e = tid; e < RW * (MW / 4); e += 256) {
         const int rr = e / (MW / 4), d = 4 * (e % (MW / 4)), r = r_first + rr;
         if (r < w.rows && part * MW + d < a.hd) {
@@ -499,7 +533,7 @@ __global__ void __launch_bounds__(256) attn_paged_kernel(PagedArgs a) {
           RowOut<DT>(a, w.row0, w.kvh, w.split, r, top, sum, at == 0).put(at, o);
         }
       }
-      __syncthreads();
+      lds_barrier();
     }
   }
 }
@@ -915,38 +949,52 @@ __global__ void __launch_bounds__(256, DT == F32 || HDP > 128 ? 1 : 2) attn_page
 }
 
 // The shares of a row joined: M the largest maximum, o = sum_s o_s 2^(m_s - M) /
-// sum_s l_s 2^(m_s - M), in share order.  hd / 4 threads per row.
+// sum_s l_s 2^(m_s - M).  hd / 4 threads take a share's values; `groups` of them a row,
+// each every groups-th share, added in group order (with one, a row of 64 shares
+// took 31 us for 128 rows).
 template <int DT>
 __global__ void __launch_bounds__(256)
 paged_join_kernel(const float *__restrict__ part_o, const float2 *__restrict__ part_ml, const int32_t *__restrict__ cu, void *out,
-                  long ldo, int B, int Hq, int hd, int splits, int n_rows) {
+                  long ldo, int B, int Hq, int hd, int splits, int groups, int n_rows) {
   typedef typename Store<DT>::T T;
-  const int per = hd / 4, rpb = 256 / per, rr = threadIdx.x / per;
-  const long row = long(blockIdx.x) * rpb + rr;
-  if (rr >= rpb) return;
-  const int d = 4 * (threadIdx.x - rr * per);
-  const long t = row / Hq;
-  if (t < cu[0] || t >= min(cu[B], n_rows)) return;  // rows of no sequence are left as they are
-  const int h = int(row - t * Hq);
-  const float2 *ml = part_ml + row * splits;
-  const float *po = part_o + row * splits * hd + d;
-  float top = -__builtin_inff();
-  for (int s = 0; s < splits; ++s) top = fmaxf(top, ml[s].x);
-  float sum = 0.f;
+  __shared__ f32x4 so[256];
+  __shared__ float2 sm[256];
+  const int tid = threadIdx.x, per = hd / 4, rpb = 256 / (per * groups), unit = tid / per;  // unit: (row, group)
+  const int rr = unit / groups, grp = unit - rr * groups, d = 4 * (tid - unit * per);
+  const long row = long(blockIdx.x) * rpb + rr, t = row / Hq;
+  const bool live = rr < rpb && t >= cu[0] && t < min(cu[B], n_rows);  // rows of no request are left as they are
+  float top = -__builtin_inff(), sum = 0.f;
   f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (int s = 0; s < splits; ++s) {
-    const float2 m = ml[s];
-    if (m.y == 0.f) continue;  // (no key in this share)
-    const float f = m.x == top ? 1.f : __builtin_amdgcn_exp2f(m.x - top);
-    sum = fmaf(m.y, f, sum);
-    const f32x4 v = *reinterpret_cast<const f32x4 *>(po + long(s) * hd);
+  auto add = [&](float m, float l, f32x4 v) {  // one more share
+    if (l == 0.f) return;                      // (of no key)
+    const float up = fmaxf(top, m), f0 = top == up ? 1.f : __builtin_amdgcn_exp2f(top - up), f1 = m == up ? 1.f : __builtin_amdgcn_exp2f(m - up);
+    top = up;
+    sum = fmaf(l, f1, sum * f0);
 #pragma unroll
-    for (int c = 0; c < 4; ++c) o[c] = fmaf(v[c], f, o[c]);
+    for (int c = 0; c < 4; ++c) o[c] = fmaf(v[c], f1, o[c] * f0);
+  };
+  if (live) {
+    const float2 *ml = part_ml + row * splits;
+    const float *po = part_o + row * splits * hd + d;
+#pragma unroll 4
+    for (int s = grp; s < splits; s += groups) {
+      const float2 m = ml[s];
+      // (nothing was written where there was no key)
+      const f32x4 v = *reinterpret_cast<const f32x4 *>(po + long(s) * hd);
+      add(m.x, m.y, v);
+    }
   }
+  if (groups > 1) {
+    so[tid] = o;
+    sm[tid] = make_float2(top, sum);
+    __syncthreads();
+    if (grp != 0) return;
+    for (int k = 1; k < groups; ++k) add(sm[tid + k * per].x, sm[tid + k * per].y, so[tid + k * per]);
+  }
+  if (!live) return;
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   const float v[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
-  st4<DT>(static_cast<T *>(out) + t * ldo + long(h) * hd + d, v);
+  st4<DT>(static_cast<T *>(out) + t * ldo + long(row - t * Hq) * hd + d, v);
 }
 
 template <int DT, int HDP>
@@ -960,11 +1008,11 @@ hipError_t launch(const PagedArgs &a, const PagedShape &s, hipStream_t st) {
     hipLaunchKernelGGL((attn_paged_kernel<DT, HDP>), grid, dim3(256), 0, st, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || s.splits == 1) return e;
-  const int rpb = 256 / (a.hd / 4);
+  const int per = a.hd / 4, groups = std::max(1, std::min((s.splits + 3) / 4, 256 / per)), rpb = 256 / (per * groups);
   const long rows = long(a.n_rows) * a.Hq, jb = (rows + rpb - 1) / rpb;
   if (jb * 256 > 0xffffffffL) return hipErrorInvalidValue;
   hipLaunchKernelGGL(paged_join_kernel<DT>, dim3(unsigned(jb)), dim3(256), 0, st, a.part_o, a.part_ml, a.cu, a.out, a.ldo, a.B, a.Hq,
-                     a.hd, a.splits, a.n_rows);
+                     a.hd, a.splits, groups, a.n_rows);
   return hipGetLastError();
 }
 
