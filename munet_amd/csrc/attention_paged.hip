@@ -363,10 +363,11 @@ struct Part {
 __device__ __forceinline__ bool part_of(const PagedArgs &a, int b, int kvh, Part &w) {
   w.kvh = kvh;
   w.b = b;
-  const int most = a.width << a.plog, len = a.lens[w.b];
+  const auto lens = scalar_ptr(a.lens), cu = scalar_ptr(a.cu);
+  const int most = a.width << a.plog, len = lens[w.b];
   w.len = min(max(len, 0), most);
-  w.row0 = a.cu[w.b];
-  w.nq = min(a.cu[w.b + 1], a.n_rows) - w.row0;
+  w.row0 = cu[w.b];
+  w.nq = min(cu[w.b + 1], a.n_rows) - w.row0;
   if (w.row0 < 0 || w.nq <= 0) return false;
   if (len > most && threadIdx.x == 0) atomicOr(a.err, kErrPage);
   w.rows = w.nq * a.G;
@@ -382,9 +383,11 @@ __global__ void __launch_bounds__(256) attn_paged_kernel(PagedArgs a) {
   // (the wave's number as a scalar: what follows from it are scalar tests)
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, g = lane >> 4;
   Part w;
-  w.split = int(blockIdx.x) / a.tiles % a.splits;
-  const int pair = int(blockIdx.x) / a.tiles / a.splits;
-  if (!part_of(a, pair / a.Hkv, pair % a.Hkv, w)) return;
+  // The heads of a page lie together: the workgroups that read them follow each
+  // other on an XCD.
+  const PairItem it = pair_item(blockIdx.x, a.B * a.splits * a.tiles, a.Hkv);
+  w.split = it.pair / a.tiles % a.splits;
+  if (!part_of(a, it.pair / a.tiles / a.splits, it.item, w)) return;
   const int P = 1 << a.plog;
   const int32_t *table = a.tables + long(w.b) * a.width;
   const uint8_t *kc = a.kc + page_base(0, a.Hkv, w.kvh, P, a.hd), *vc = a.vc + page_base(0, a.Hkv, w.kvh, P, a.hd);
@@ -395,15 +398,10 @@ __global__ void __launch_bounds__(256) attn_paged_kernel(PagedArgs a) {
   __shared__ float2 wml[4][RW];
 
   // (more tiles than the launch was sized for are walked)
-  for (int tile = int(blockIdx.x) % a.tiles; long(tile) * RW < w.rows; tile += a.tiles) {
+  for (int tile = it.pair % a.tiles; long(tile) * RW < w.rows; tile += a.tiles) {
     const int r_first = tile * RW;
     const int i0 = r_first / a.G, i1 = (min(r_first + RW, w.rows) - 1) / a.G;
     const KeyRange mine = key_share(seen_keys(w.len, w.nq, i0, i1, a.causal, a.window), w.split, a.splits, a.chunk);
-    RowTiles<DT, HDP, 1> q;
-    // (the order of the head values in a step is that of the 16-byte runs in which
-    // a lane loads its keys)
-    q.start(a, w.row0, w.nq, w.len, w.rows, r_first, w.kvh, n, mine, [&](int s) { return 64 * (s >> 1) + 16 * g + 8 * (s & 1); });
-
     // A block's keys are on their way while the probabilities and values of the block
     // before are worked on, its values during its scores: they take the registers
     // that those have left.  Every load is made, at an address that exists, and
@@ -411,16 +409,29 @@ __global__ void __launch_bounds__(256) attn_paged_kernel(PagedArgs a) {
     // wait for it before the next.  Keys past the range take its last page; a page
     // outside the pool holds no keys (page 0 is read); head values past hd repeat
     // earlier ones (their queries are zero, their outputs not stored).
-    int pk = 0, pv = 0;                 // pages of this lane's key rows (group n >> 2), of its scores and values (group g)
+    // The pages come by scalar loads, a block ahead: a vector load's result is waited
+    // for together with all loads before it, here the block's bytes.
+    const auto table_s = scalar_ptr(table);
+    const int last = __builtin_amdgcn_readfirstlane(mine.hi) - 1;
+    int page0 = 0, page1 = 0, page2 = 0, page3 = 0;  // of the block's runs of 16 keys
+    int pv = 0;                                      // of this lane's scores and values (run g)
     bool next_ok = false;
     uint4 kr[4][J], vr[MT];
     float ksc = 0.f, vsc = 0.f;
     auto pages = [&](int base) {
-      pk = table[min(base + 16 * (n >> 2), mine.hi - 1) >> a.plog];
-      pv = table[min(base + 16 * g, mine.hi - 1) >> a.plog];
+      page0 = table_s[min(base, last) >> a.plog];
+      page1 = table_s[min(base + 16, last) >> a.plog];
+      page2 = table_s[min(base + 32, last) >> a.plog];
+      page3 = table_s[min(base + 48, last) >> a.plog];
+    };
+    auto of_run = [&](int c) {
+      const int lo = c & 1 ? page1 : page0, hi = c & 1 ? page3 : page2;
+      return c & 2 ? hi : lo;
     };
     auto load_keys = [&](int base) {
       const int tk = base + 16 * (n >> 2), tv = base + 16 * g;
+      int pk = of_run(n >> 2);  // of this lane's key rows
+      pv = of_run(g);
       next_ok = page_in_pool(pv, a.n_pages);
       if (!next_ok && tv < mine.hi && n == 0) atomicOr(a.err, kErrPage);
       pk = page_in_pool(pk, a.n_pages) ? pk : 0;
@@ -440,17 +451,23 @@ __global__ void __launch_bounds__(256) attn_paged_kernel(PagedArgs a) {
       for (int i = 0; i < MT; ++i) vr[i] = *reinterpret_cast<const uint4 *>(vp + min(16 * i, a.hd - 16) * P);
     };
     int base = (mine.lo & ~(kKeyBlock - 1)) + wave * kKeyBlock;
+    // (the last block's successor is itself: its bytes are in the caches)
+    auto after = [&](int b) { return b + 4 * kKeyBlock < mine.hi ? b + 4 * kKeyBlock : b; };
     if (base < mine.hi) {
       pages(base);
       load_keys(base);
       load_values(base);
+      pages(after(base));
     }
+    // (the queries' loads after the first block's: all of them are waited for at once)
+    RowTiles<DT, HDP, 1> q;
+    // (the order of the head values in a step is that of the 16-byte runs in which
+    // a lane loads its keys)
+    q.start(a, w.row0, w.nq, w.len, w.rows, r_first, w.kvh, n, mine, [&](int s) { return 64 * (s >> 1) + 16 * g + 8 * (s & 1); });
     while (base < mine.hi) {
-      // (the last block's successor is itself: its bytes are in the caches)
-      const int next = base + 4 * kKeyBlock, then = next < mine.hi ? next : base, tv = base + 16 * g;
+      const int next = base + 4 * kKeyBlock, then = after(base), tv = base + 16 * g;
       const bool page_ok = next_ok;
       const float lv = page_ok ? fmaxf(__builtin_amdgcn_logf(vsc), -126.f) : -126.f, kscale = ksc;
-      pages(then);
       f32x4 s[4][1];
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
@@ -466,6 +483,7 @@ __global__ void __launch_bounds__(256) attn_paged_kernel(PagedArgs a) {
         }
       }
       load_keys(then);
+      pages(after(then));
       __builtin_amdgcn_sched_barrier(0);
       const bool masked = base < q.every_lo || base + kKeyBlock > q.every_hi || __any(!page_ok);
       q.probabilities(s, kscale, lv, xor32_max(xor16_max(lv)), page_ok, tv, masked);

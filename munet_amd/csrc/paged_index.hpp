@@ -117,12 +117,14 @@ inline PagedShape paged_shape(int B, int Hq, int Hkv, int max_q, int max_len, in
   s.wide = rows > 16;
   const int per = s.wide ? kPagedWideRows : 16;
   s.tiles = int(std::max<int64_t>(1, (rows + per - 1) / per));
-  // Shares so that about 1024 workgroups are in flight (four per CU), none
-  // shorter than one block per wave.
+  // Shares so that the workgroups, two to a CU, are all there at once or nearly
+  // (64 requests of up to 8192 keys, 8 heads of 128: one share 121 us, two 133 +
+  // join 5, four 145 + 6; 2 requests of which one has 131072: 32 shares 85 + 6,
+  // 64 74 + 7, 128 83 + 12), none shorter than one block per wave.
   const int64_t whole = std::max<int64_t>(1, int64_t(B) * Hkv * s.tiles);
   const int64_t keys = window > 0 ? std::min<int64_t>(max_len, int64_t(window) + max_q + kKeyBlock) : max_len;
   const int64_t least = 4 * kKeyBlock;
-  int64_t n = std::min<int64_t>((keys + least - 1) / least, (1024 + whole - 1) / whole);
+  int64_t n = std::min<int64_t>((keys + least - 1) / least, 1025 / (whole + 1));
   n = std::max<int64_t>(1, std::min<int64_t>(n, 256));
   s.chunk = int(std::min<int64_t>(((keys + n - 1) / n + least - 1) / least * least, 1 << 30));
   if (s.chunk == 0) s.chunk = int(least);
