@@ -88,16 +88,16 @@ template <int DT> __device__ __forceinline__ float logit(typename Store<DT>::T v
   return x == x ? x : -__builtin_inff();
 }
 
-// f(logit) over a row, in any order: whole 16-byte chunks where the row's start
+// f(logit, index) over a row, in any order: whole 16-byte chunks where the row's start
 // allows it, single values before and after.
 template <int DT, int NT, class F> __device__ __forceinline__ void each_value(const typename Store<DT>::T *row, int cols, F f) {
   typedef typename Store<DT>::T T;
   constexpr int E = 16 / sizeof(T);
   const int tid = threadIdx.x;
   const int head = min(int((16 - (uintptr_t(row) & 15)) & 15) / int(sizeof(T)), cols), chunks = (cols - head) / E;
-  if (tid < head) f(logit<DT>(row[tid]));
+  if (tid < head) f(logit<DT>(row[tid]), tid);
   const uint4 *c = reinterpret_cast<const uint4 *>(row + head);
-#pragma unroll 2
+#pragma unroll 4
   for (int i = tid; i < chunks; i += NT) {
     const uint4 w = c[i];
     float v[E];
@@ -107,10 +107,10 @@ template <int DT, int NT, class F> __device__ __forceinline__ void each_value(co
       dec8<DT>(w, v);
     }
 #pragma unroll
-    for (int e = 0; e < E; ++e) f(v[e] == v[e] ? v[e] : -__builtin_inff());
+    for (int e = 0; e < E; ++e) f(v[e] == v[e] ? v[e] : -__builtin_inff(), head + i * E + e);
   }
   const int tail = head + chunks * E + tid;
-  if (tail < cols) f(logit<DT>(row[tail]));
+  if (tail < cols) f(logit<DT>(row[tail]), tail);
 }
 
 // A prefix of the order: values above K, and the first `ties` equal to it.
@@ -119,13 +119,31 @@ struct Cut {
   uint32_t ties;
 };
 
+// One workgroup per row.
+//  1. The largest logit, and the largest of each thread's own.
+//  2. Top-k: the k-th of the threads' largest bounds the k-th logit from below: what
+//     passes it, the top k and little more, goes into a list in LDS.  No weights
+//     but those of the list.  Min-p alone: what passes its least weight.
+//     Top-p of all tokens: a histogram of their weights; the tokens of the bin in
+//     which the prefix ends go into the list.
+//  3. The threshold by histograms over the list.
+//  4. The draw: from the list by histograms of weight over its indexes, or, where more
+//     is kept than the list, by the weights of groups of consecutive tokens (top-p:
+//     added up while the list is gathered).
+// Where a list does not hold what it should (thousands of equal logits), its histograms
+// run over the row in memory instead.
 template <int DT, int NT>
 __global__ void __launch_bounds__(NT) sample_kernel(Sampling p, int S) {
   typedef typename Store<DT>::T T;
-  constexpr int NW = NT / 64;
+  constexpr int NW = NT / 64, kList = 4096;
   __shared__ unsigned long long mass[kBins];
   __shared__ unsigned int count[kBins];
+  __shared__ unsigned long long group_mass[kMaxGroups];
   __shared__ unsigned int red[2][NW];
+  __shared__ unsigned long long red64[NW];
+  __shared__ uint32_t list_key[kList];
+  __shared__ int list_at[kList];
+  __shared__ int listed;
   __shared__ struct {
     uint32_t bin;
     uint32_t count;  // tokens above the bin
@@ -134,12 +152,37 @@ __global__ void __launch_bounds__(NT) sample_kernel(Sampling p, int S) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int r = blockIdx.x, V = p.cols;
   const T *row = static_cast<const T *>(p.logits) + long(r) * p.ld;
+  const float T_ = p.temperature ? p.temperature[r] : 1.f;
+  const bool greedy = !(T_ > 0.f);
+  const int k = p.top_k ? p.top_k[r] : 0;
+  const float tp = p.top_p ? p.top_p[r] : 1.f, mp = p.min_p ? p.min_p[r] : 0.f;
+  const bool by_k = k > 0 && k < V, by_p = tp < 1.f, by_m = mp > 0.f;
 
-  // ---- the largest value
-  uint32_t top = 0;
-  each_value<DT, NT>(row, V, [&](float x) {
-    top = max(top, value_key(x));
-  });
+  // ---- the largest value; with temperature 0 its first index too
+  uint32_t own = 0;
+  unsigned long long first = 0;  // (key, ~index)
+  if (greedy) {
+    each_value<DT, NT>(row, V, [&](float x, int i) {
+      const unsigned long long c = (static_cast<unsigned long long>(value_key(x)) << 32) | (0xffffffffu - uint32_t(i));
+      first = c > first ? c : first;
+    });
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+      const unsigned long long c = __shfl_xor(first, o, 64);
+      first = c > first ? c : first;
+    }
+    if (lane == 0) red64[wave] = first;
+    __syncthreads();
+    for (int w = 0; w < NW; ++w) first = red64[w] > first ? red64[w] : first;
+    if (tid == 0) {
+      const bool none = uint32_t(first >> 32) <= value_key(-__builtin_inff());
+      p.ids[r] = none ? -1 : int(0xffffffffu - uint32_t(first));
+      if (p.logprob) p.logprob[r] = none ? -__builtin_inff() : 0.f;
+    }
+    return;
+  }
+  each_value<DT, NT>(row, V, [&](float x, int) { own = max(own, value_key(x)); });
+  uint32_t top = own;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) top = max(top, uint32_t(__shfl_xor(top, o, 64)));
   if (lane == 0) red[0][wave] = top;
@@ -154,260 +197,360 @@ __global__ void __launch_bounds__(NT) sample_kernel(Sampling p, int S) {
     }
     return;
   }
-  const float T_ = p.temperature ? p.temperature[r] : 1.f;
-  const bool greedy = !(T_ > 0.f);
-  const int k = p.top_k ? p.top_k[r] : 0;
-  const float tp = p.top_p ? p.top_p[r] : 1.f, mp = p.min_p ? p.min_p[r] : 0.f;
   Weigh w;
   w.max = double(xmax);
-  w.per = greedy ? 0.0 : 1.4426950408889634074 / double(T_);
+  w.per = 1.4426950408889634074 / double(T_);
   w.S = S;
-
-  // ---- the prefix
-  Cut cut{0u, 0xffffffffu};
-  if (greedy) {
-    cut = Cut{top, 1u};
-  } else if ((k > 0 && k < V) || tp < 1.f) {
-    // bins of equal width in z over the S bits that weigh anything
-    const float per_bin = float(kBins) / float(S + 1), slope = fminf(float(w.per) * per_bin, 1e30f);
-    auto bin_of = [&](float x) -> uint32_t {
-      return x == xmax ? 0u : uint32_t(fminf((xmax - x) * slope, float(kBins - 1)));
-    };
-    // bins of the tokens that `in` takes, and where a prefix of `n` tokens or of
-    // weight `goal` ends: the bin, and what lies above it
-    auto fill = [&](auto in, auto where) {
-      for (int i = tid; i < kBins; i += NT) {
-        mass[i] = 0;
-        count[i] = 0;
-      }
-      __syncthreads();
-      each_value<DT, NT>(row, V, [&](float x) {
-        if (in(x)) {
-          const uint32_t b = where(x);
-          atomicAdd(&count[b], 1u);
-          const uint64_t m = w(x);
-          if (m) atomicAdd(&mass[b], (unsigned long long)m);
-        }
-      });
-      __syncthreads();
-    };
-    auto find = [&](bool by_mass, uint64_t goal) {
-      if (wave == 0) {
-        constexpr int per = kBins / 64;
-        uint64_t m = 0;
-        uint32_t c = 0;
-        for (int i = 0; i < per; ++i) {
-          m += mass[lane * per + i];
-          c += count[lane * per + i];
-        }
-        const uint64_t ms = wave_scan((unsigned long long)m, lane);
-        const uint32_t cs = wave_scan(c, lane);
-        const bool hit = (by_mass ? ms : uint64_t(cs)) >= goal;
-        const uint64_t hits = __ballot(hit);
-        const int l = hits ? __builtin_ctzll(hits) : 63;
-        if (lane == l) {
-          uint64_t am = ms - m;
-          uint32_t ac = cs - c;
-          int b = lane * per;
-          for (int i = 0; i + 1 < per; ++i) {
-            if ((by_mass ? am + mass[b] : uint64_t(ac) + count[b]) >= goal) break;
-            am += mass[b];
-            ac += count[b];
-            ++b;
-          }
-          at.bin = b;
-          at.count = ac;
-          at.mass = am;
-        }
-      }
-      __syncthreads();
-    };
-    // the exact end of a prefix of `goal` tokens or weight
-    auto end_of = [&](bool by_mass, uint64_t goal, uint64_t &above_mass) -> Cut {
-      find(by_mass, goal);
-      const uint32_t b0 = at.bin;
-      uint64_t am = at.mass;
-      uint64_t ac = at.count;
-      // the keys of that bin
-      uint32_t lo = 0xffffffffu, hi = 0;
-      each_value<DT, NT>(row, V, [&](float x) {
-        if (bin_of(x) == b0) {
-          const uint32_t kk = value_key(x);
-          lo = min(lo, kk);
-          hi = max(hi, kk);
-        }
-      });
-#pragma unroll
-      for (int o = 32; o > 0; o >>= 1) {
-        lo = min(lo, uint32_t(__shfl_xor(lo, o, 64)));
-        hi = max(hi, uint32_t(__shfl_xor(hi, o, 64)));
-      }
-      if (lane == 0) {
-        red[0][wave] = lo;
-        red[1][wave] = hi;
-      }
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < NW; ++i) {
-        lo = min(lo, red[0][i]);
-        hi = max(hi, red[1][i]);
-      }
-      __syncthreads();
-      for (;;) {
-        int sh = 0;
-        while (((hi - lo) >> sh) >= uint32_t(kBins)) ++sh;
-        fill([&](float x) { const uint32_t kk = value_key(x); return bin_of(x) == b0 && kk >= lo && kk <= hi; },
-             [&](float x) { return (hi - value_key(x)) >> sh; });
-        find(by_mass, by_mass ? goal - am : goal - ac);
-        const uint32_t sb = at.bin;
-        am += at.mass;
-        ac += at.count;
-        __syncthreads();
-        if (sh == 0) {
-          const uint32_t K = hi - sb;
-          above_mass = am;
-          uint64_t ties = goal - ac;
-          if (by_mass) {
-            const uint64_t one = w(key_value(K));
-            ties = one ? (goal - am + one - 1) / one : 1;
-          }
-          return Cut{K, uint32_t(ties > 0xffffffffu ? 0xffffffffu : ties)};
-        }
-        hi -= sb << sh;
-        const uint32_t span = (1u << sh) - 1u;
-        lo = hi - lo > span ? hi - span : lo;
-      }
-    };
-    fill([&](float) { return true; }, bin_of);
-    uint64_t total = 0;  // the weight that top-k leaves
-    if (k > 0 && k < V) {
-      uint64_t above = 0;
-      cut = end_of(false, uint64_t(k), above);
-      total = above + uint64_t(cut.ties) * w(key_value(cut.K));
-      if (tp < 1.f) fill([&](float) { return true; }, bin_of);
-    } else {
-      if (wave == 0) {
-        uint64_t m = 0;
-        for (int i = lane; i < kBins; i += 64) m += mass[i];
-        m = wave_sum_u64(m);
-        if (lane == 0) at.mass = m;
-      }
-      __syncthreads();
-      total = at.mass;
-      __syncthreads();
-    }
-    if (tp < 1.f) {
-      const double g = __builtin_ceil(double(fmaxf(tp, 0.f)) * double(total));
-      const uint64_t goal = g < 1.0 ? 1 : min(uint64_t(g), total);
-      uint64_t above = 0;
-      const Cut c = end_of(true, goal, above);
-      if (c.K > cut.K || (c.K == cut.K && c.ties < cut.ties)) cut = c;
-    }
-  }
   // min-p: a weight below this (times 2^S) is dropped
-  const double least = mp > 0.f && !greedy ? double(fminf(mp, 1.f)) * __builtin_ldexp(1.0, S) : 0.0;
+  const double least = by_m ? double(fminf(mp, 1.f)) * __builtin_ldexp(1.0, S) : 0.0;
+  // bins of equal width in z over the S bits that weigh anything
+  const float per_bin = float(kBins) / float(S + 1), slope = fminf(float(w.per) * per_bin, 1e30f);
+  auto bin_of = [&](float x) -> uint32_t { return x == xmax ? 0u : uint32_t(fminf((xmax - x) * slope, float(kBins - 1))); };
 
-  // ---- kept weight and ties of each group of consecutive tokens
-  __syncthreads();
+  auto clear = [&] {
+    for (int i = tid; i < kBins; i += NT) {
+      mass[i] = 0;
+      count[i] = 0;
+    }
+    __syncthreads();
+  };
+  // where a prefix of `goal` tokens or weight of the bins ends, and what lies above
+  auto find = [&](bool by_mass, uint64_t goal) {
+    __syncthreads();
+    if (wave == 0) {
+      constexpr int per = kBins / 64;
+      uint64_t m = 0;
+      uint32_t c = 0;
+#pragma unroll 8
+      for (int i = 0; i < per; ++i) {
+        m += mass[lane * per + i];
+        c += count[lane * per + i];
+      }
+      const uint64_t ms = wave_scan((unsigned long long)m, lane);
+      const uint32_t cs = wave_scan(c, lane);
+      const uint64_t hits = __ballot((by_mass ? ms : uint64_t(cs)) >= goal);
+      const int l = hits ? __builtin_ctzll(hits) : 63;
+      if (lane == l) {
+        uint64_t am = ms - m;
+        uint32_t ac = cs - c;
+        int b = lane * per;
+        for (int i = 0; i + 1 < per; ++i) {
+          if ((by_mass ? am + mass[b] : uint64_t(ac) + count[b]) >= goal) break;
+          am += mass[b];
+          ac += count[b];
+          ++b;
+        }
+        at.bin = b;
+        at.count = ac;
+        at.mass = am;
+      }
+    }
+    __syncthreads();
+  };
+  auto sum_of = [&](uint64_t m) -> uint64_t {
+    m = wave_sum_u64(m);
+    if (lane == 0) red64[wave] = m;
+    __syncthreads();
+    uint64_t s = 0;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) s += red64[i];
+    __syncthreads();
+    return s;
+  };
+  // bins of the tokens of `each` that `in` takes
+  auto fill = [&](auto each, auto in, auto where) {
+    clear();
+    each([&](float x, int) {
+      if (in(x)) {
+        const uint32_t b = where(x);
+        atomicAdd(&count[b], 1u);
+        const uint64_t m = w(x);
+        if (m) atomicAdd(&mass[b], (unsigned long long)m);
+      }
+    });
+  };
+  // the exact end of a prefix of `goal` tokens or weight, in bin b0, with so much above the bin
+  auto end_in = [&](auto each, bool by_mass, uint64_t goal, uint32_t b0, uint64_t am, uint64_t ac, uint64_t &above_mass) -> Cut {
+    // the keys of that bin
+    uint32_t lo = 0xffffffffu, hi = 0;
+    each([&](float x, int) {
+      if (bin_of(x) == b0) {
+        const uint32_t kk = value_key(x);
+        lo = min(lo, kk);
+        hi = max(hi, kk);
+      }
+    });
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+      lo = min(lo, uint32_t(__shfl_xor(lo, o, 64)));
+      hi = max(hi, uint32_t(__shfl_xor(hi, o, 64)));
+    }
+    if (lane == 0) {
+      red[0][wave] = lo;
+      red[1][wave] = hi;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NW; ++i) {
+      lo = min(lo, red[0][i]);
+      hi = max(hi, red[1][i]);
+    }
+    __syncthreads();
+    for (;;) {
+      int sh = 0;
+      while (((hi - lo) >> sh) >= uint32_t(kBins)) ++sh;
+      fill(each, [&](float x) { const uint32_t kk = value_key(x); return bin_of(x) == b0 && kk >= lo && kk <= hi; },
+           [&](float x) { return (hi - value_key(x)) >> sh; });
+      find(by_mass, by_mass ? goal - am : goal - ac);
+      const uint32_t sb = at.bin;
+      am += at.mass;
+      ac += at.count;
+      __syncthreads();
+      if (sh == 0) {
+        const uint32_t K = hi - sb;
+        above_mass = am;
+        uint64_t ties = goal - ac;
+        if (by_mass) {
+          const uint64_t one = w(key_value(K));
+          ties = one ? (goal - am + one - 1) / one : 1;
+        }
+        return Cut{K, uint32_t(ties > 0xffffffffu ? 0xffffffffu : ties)};
+      }
+      hi -= sb << sh;
+      const uint32_t span = (1u << sh) - 1u;
+      lo = hi - lo > span ? hi - span : lo;
+    }
+  };
+  auto goal_p = [&](uint64_t total) -> uint64_t {  // the weight that top-p's prefix reaches
+    const double g = __builtin_ceil(double(fmaxf(tp, 0.f)) * double(total));
+    return g < 1.0 ? 1 : min(uint64_t(g), total);
+  };
+  auto shorter = [](Cut a, Cut b) { return b.K > a.K || (b.K == a.K && b.ties < a.ties) ? b : a; };
+  // top-k's prefix over `each`, and top-p's of what it leaves
+  auto of_top_k = [&](auto each) -> Cut {
+    fill(each, [&](float) { return true; }, bin_of);
+    find(false, uint64_t(k));
+    uint64_t above = 0;
+    const Cut c = end_in(each, false, uint64_t(k), at.bin, at.mass, at.count, above);
+    if (!by_p) return c;
+    const uint64_t goal = goal_p(above + uint64_t(c.ties) * w(key_value(c.K)));
+    fill(each, [&](float) { return true; }, bin_of);
+    find(true, goal);
+    return shorter(c, end_in(each, true, goal, at.bin, at.mass, at.count, above));
+  };
+  // The index at which the running sum of `weight` over `each`, in index order,
+  // passes goal: bins of consecutive indexes, refined to one.
+  auto select = [&](auto each, uint64_t goal, auto weight) -> int {
+    int lo = 0, bits = 0;
+    while ((int64_t(kBins) << bits) < V) ++bits;
+    for (;; bits = bits > 11 ? bits - 11 : 0) {
+      __syncthreads();
+      clear();
+      each([&](float x, int i) {
+        const int b = (i - lo) >> bits;
+        if (i >= lo && b < kBins) {
+          const uint64_t v = weight(x, i);
+          if (v) atomicAdd(&mass[b], (unsigned long long)v);
+        }
+      });
+      find(true, goal + 1);
+      lo += int(at.bin) << bits;
+      goal -= at.mass;
+      if (bits == 0) return lo;
+    }
+  };
+  // The threshold, and the index of its last tie that is kept.
+  Cut cut{0u, 0xffffffffu};
+  int last_tie = V;
+  auto weight = [&](float x, int i) -> uint64_t {
+    const uint32_t kk = value_key(x);
+    if (kk < cut.K || (kk == cut.K && i > last_tie)) return 0;
+    const double s = w.scaled(x);
+    return s < least ? 0 : Weigh::whole(s);
+  };
+  auto cut_ties = [&](auto each) {
+    uint32_t ties = 0;
+    each([&](float x, int) { ties += value_key(x) == cut.K; });
+    if (sum_of(ties) > cut.ties)
+      last_tie = select(each, uint64_t(cut.ties) - 1, [&](float x, int) { return uint64_t(value_key(x) == cut.K); });
+  };
+  auto put = [&](int i, float x, uint64_t total) {
+    p.ids[r] = i;
+    // log(w / sum) from the logit itself: the whole weight has few bits where w is small
+    if (p.logprob)
+      p.logprob[r] = float((double(x) == w.max ? 0.0 : (double(x) - w.max) / double(T_)) - log(double(total) * __builtin_ldexp(1.0, -S)));
+  };
+  float u = p.u[r];
+  u = u > 0.f ? u : 0.f;
+  auto goal_of = [&](uint64_t total) -> uint64_t {
+    const uint64_t g = uint64_t(double(u) * double(total));
+    return g < total ? g : total - 1;  // u = 1: the last kept token
+  };
+
+  auto over_row = [&](auto f) { each_value<DT, NT>(row, V, f); };
+  // Groups of consecutive tokens: f(logit, index) over one by a wave, in any order.
   int gs = 512;
   while ((V + gs - 1) / gs > kMaxGroups) gs *= 2;
   const int groups = (V + gs - 1) / gs;
-  // (mass / count are reused: kMaxGroups <= kBins)
-  auto kept = [&](float x, uint64_t &m) -> int {  // 0 no, 1 above the threshold, 2 equal to it
-    m = 0;
-    const uint32_t kk = value_key(x);
-    if (kk < cut.K) return 0;
-    const double s = w.scaled(x);
-    if (s < least) return 0;
-    m = Weigh::whole(s);
-    return kk > cut.K ? 1 : 2;
-  };
-  for (int g = wave; g < groups; g += NW) {
-    uint64_t m = 0;
-    uint32_t ties = 0;
-    const int end = min(g * gs + gs, V);
-#pragma unroll 4
-    for (int i = g * gs + lane; i < end; i += 64) {
-      uint64_t one;
-      const int how = kept(logit<DT>(row[i]), one);
-      if (how == 1) m += one;
-      if (how == 2) ++ties;
-    }
-    m = wave_sum_u64(m);
+  const bool chunks = ((uintptr_t(row) & 15) == 0);
+  auto over_group = [&](int g, auto f) {
+    const int from = g * gs, to = min(from + gs, V);
+    if (chunks && to - from == gs) {
+#pragma unroll 2
+      for (int i = from + lane * 8; i < to; i += 512) {
+        float v[8];
+        if constexpr (DT == F32) {
+          ld4<F32>(row + i, v);
+          ld4<F32>(row + i + 4, v + 4);
+        } else {
+          dec8<DT>(*reinterpret_cast<const uint4 *>(row + i), v);
+        }
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) ties += __shfl_xor(ties, o, 64);
-    if (lane == 0) {
-      mass[g] = m;
-      count[g] = ties;
+        for (int e = 0; e < 8; ++e) f(v[e] == v[e] ? v[e] : -__builtin_inff(), i + e);
+      }
+    } else {
+      for (int i = from + lane; i < to; i += 64) f(logit<DT>(row[i]), i);
     }
-  }
-  __syncthreads();
-  if (wave != 0) return;
+  };
+  bool grouped = false;  // group_mass is filled
 
-  // ---- the draw (one wave)
-  const uint64_t tie_weight = w(key_value(cut.K));  // (unused where nothing ties)
-  const int per = (groups + 63) / 64;
-  uint32_t my_ties = 0;
-  for (int i = 0; i < per; ++i)
-    if (lane * per + i < groups) my_ties += count[lane * per + i];
-  uint64_t before = uint64_t(wave_scan((unsigned long long)my_ties, lane)) - my_ties;
-  uint64_t sum = 0, left_ties = before;
-  for (int i = 0; i < per; ++i) {
-    const int g = lane * per + i;
-    if (g >= groups) break;
-    const uint64_t left = left_ties < cut.ties ? cut.ties - left_ties : 0, n = min(left, uint64_t(count[g]));
-    left_ties += count[g];
-    mass[g] += n * tie_weight;
-    sum += mass[g];
+  // ---- the threshold
+  if (by_p && !by_k) {
+    clear();
+    over_row([&](float x, int) {
+      const uint64_t m = w(x);
+      if (m) atomicAdd(&mass[bin_of(x)], (unsigned long long)m);
+    });
+    __syncthreads();
+    uint64_t m = 0;
+    for (int i = tid; i < kBins; i += NT) m += mass[i];
+    const uint64_t goal = goal_p(sum_of(m));
+    find(true, goal);
+    const uint32_t b0 = at.bin;
+    const uint64_t am = at.mass;
+    if (tid == 0) listed = 0;
+    __syncthreads();
+    for (int g = wave; g < groups; g += NW) {
+      uint64_t gm = 0;
+      over_group(g, [&](float x, int i) {
+        const uint32_t b = bin_of(x);
+        if (b < b0) {
+          const double s = w.scaled(x);
+          gm += s < least ? 0 : Weigh::whole(s);
+        } else if (b == b0) {
+          const int n = atomicAdd(&listed, 1);
+          if (n < kList) {
+            list_key[n] = value_key(x);
+            list_at[n] = i;
+          }
+        }
+      });
+      gm = wave_sum_u64(gm);
+      if (lane == 0) group_mass[g] = gm;
+    }
+    __syncthreads();
+    const int n = listed;
+    uint64_t above = 0;
+    if (n <= kList) {
+      auto each = [&](auto f) {
+        for (int i = tid; i < n; i += NT) f(key_value(list_key[i]), list_at[i]);
+      };
+      cut = end_in(each, true, goal, b0, am, 0, above);
+      cut_ties(each);
+      each([&](float x, int i) {
+        const uint64_t v = weight(x, i);
+        if (v) atomicAdd(&group_mass[i / gs], (unsigned long long)v);
+      });
+      grouped = true;
+    } else {
+      cut = end_in(over_row, true, goal, b0, am, 0, above);
+      cut_ties(over_row);
+    }
+    __syncthreads();
+  } else if (by_k || by_m) {
+    uint32_t bound = kBins - 1;
+    if (by_k && V > kList) {
+      const int owners = int(sum_of(own != 0));  // (threads with a logit)
+      clear();
+      if (own) atomicAdd(&count[bin_of(key_value(own))], 1u);
+      find(false, uint64_t(min(k, owners)));
+      if (k <= owners) bound = at.bin;
+    }
+    if (by_m) bound = min(bound, uint32_t(fminf(float(-log2(double(fminf(mp, 1.f)))) * per_bin + 2.f, float(kBins - 1))));
+    if (tid == 0) listed = 0;
+    __syncthreads();
+    over_row([&](float x, int i) {
+      if (bin_of(x) <= bound) {
+        const int n = atomicAdd(&listed, 1);
+        if (n < kList) {
+          list_key[n] = value_key(x);
+          list_at[n] = i;
+        }
+      }
+    });
+    __syncthreads();
+    const int n = listed;
+    // (fewer than k where min-p leaves fewer: then it decides)
+    const bool holds = n <= kList && (n >= k || by_m || V <= kList);
+    auto each = [&](auto f) {
+      for (int i = tid; i < n; i += NT) f(key_value(list_key[i]), list_at[i]);
+    };
+    if (holds && !(by_k && by_p && n < k)) {
+      if (by_k && n >= k) {
+        cut = of_top_k(each);
+        cut_ties(each);
+      }
+      uint64_t total = 0;
+      each([&](float x, int i) { total += weight(x, i); });
+      total = sum_of(total);
+      const int id = select(each, goal_of(total), weight);
+      if (tid == 0) put(id, logit<DT>(row[id]), total);
+      return;
+    }
+    if (by_k) {
+      cut = of_top_k(over_row);
+      cut_ties(over_row);
+    }
+    __syncthreads();
   }
+
+  // ---- the draw from the groups
+  if (!grouped) {
+    for (int g = wave; g < groups; g += NW) {
+      uint64_t gm = 0;
+      over_group(g, [&](float x, int i) { gm += weight(x, i); });
+      gm = wave_sum_u64(gm);
+      if (lane == 0) group_mass[g] = gm;
+    }
+    __syncthreads();
+  }
+  if (wave != 0) return;
+  const int per = (groups + 63) / 64;
+  uint64_t sum = 0;
+  for (int i = 0; i < per; ++i)
+    if (lane * per + i < groups) sum += group_mass[lane * per + i];
   const uint64_t run = wave_scan((unsigned long long)sum, lane);
   const uint64_t total = __shfl((unsigned long long)run, 63, 64);
-  float u = p.u[r];
-  u = u > 0.f ? u : 0.f;
-  uint64_t goal = uint64_t(double(u) * double(total));
-  if (goal >= total) goal = total - 1;  // u = 1: the last kept token
+  const uint64_t goal = goal_of(total);
   const int hl = __builtin_ctzll(__ballot(run > goal));
   int g0 = 0;
-  uint64_t g_goal = 0, g_ties = 0;
+  uint64_t left = 0;
   if (lane == hl) {
     uint64_t m = run - sum;
-    uint64_t ties = before;
     g0 = lane * per;
-    while (m + mass[g0] <= goal) {
-      m += mass[g0];
-      ties += count[g0];
-      ++g0;
-    }
-    g_goal = goal - m;
-    g_ties = ties;
+    while (m + group_mass[g0] <= goal) m += group_mass[g0++];
+    left = goal - m;
   }
   g0 = __shfl(g0, hl, 64);
-  g_goal = __shfl((unsigned long long)g_goal, hl, 64);
-  g_ties = __shfl((unsigned long long)g_ties, hl, 64);
-  uint64_t have = 0, ties = g_ties;
+  left = __shfl((unsigned long long)left, hl, 64);
+  uint64_t have = 0;
   for (int base = g0 * gs; base < min(g0 * gs + gs, V); base += 64) {
     const int i = base + lane;
-    uint64_t one = 0;
-    int how = 0;
-    float x = 0.f;
-    if (i < V) {
-      x = logit<DT>(row[i]);
-      how = kept(x, one);
-    }
-    const uint64_t tied = __ballot(how == 2);
-    if (how == 2 && ties + __builtin_popcountll(tied & ((uint64_t(1) << lane) - 1)) >= cut.ties) one = 0;
-    ties += __builtin_popcountll(tied);
-    const uint64_t run2 = have + uint64_t(wave_scan((unsigned long long)one, lane));
-    const uint64_t hit = __ballot(run2 > g_goal);
+    const float x = i < V ? logit<DT>(row[i]) : -__builtin_inff();
+    const uint64_t run2 = have + uint64_t(wave_scan((unsigned long long)(i < V ? weight(x, i) : 0), lane));
+    const uint64_t hit = __ballot(run2 > left);
     if (hit) {
-      if (lane == __builtin_ctzll(hit)) {
-        p.ids[r] = i;
-        // log(w / sum) from the logit itself: the whole weight has few bits where w is small
-        if (p.logprob)
-          p.logprob[r] = greedy ? 0.f
-                                : float((double(x) == w.max ? 0.0 : (double(x) - w.max) / double(T_)) -
-                                        log(double(total) * __builtin_ldexp(1.0, -S)));
-      }
+      if (lane == __builtin_ctzll(hit)) put(i, x, total);
       return;
     }
     have = __shfl((unsigned long long)run2, 63, 64);
