@@ -34,37 +34,47 @@ __device__ __forceinline__ float key_value(uint32_t k) {
   return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
 }
 
-// 2^y for y <= 0 as a whole multiple of 2^-S, and before that rounding (times
-// 2^S): 2^y = 2^n e^(f ln 2), |f| <= 1/2, by the exponential's series to the
-// twelfth power (the next term is below 2^-52).
+// 2^(S + y), y = (x - max) log2(e) / T <= 0, and rounded to a whole number.  With
+// 128 (S + y) = n + r, n whole and |r| <= 1/2: 2^(n >> 7) times the table's 2^(n mod 128
+// / 128) times e^(r ln 2 / 128) by its series to the third power (the next term is
+// below 2^-38: one in 10^8 draws from 10^5 equal tokens could move).  Eleven 64-bit
+// operations, where the series without a table takes twenty (sums of 131072
+// weights in 200 rows 92 us | 60).
+constexpr int kTable = 128;
 struct Weigh {
-  double max, per;  // z log2(e) = (x - max) * per
+  const double *table;  // 2^(j / 128)
+  double max, per;      // y = (x - max) * per
+  float least;          // logits below weigh nothing
   int S;
+  bool inf;  // the largest logit is infinite: it weighs 1, all others nothing
+  __device__ __forceinline__ void start(float xmax, float T) {
+    max = double(xmax);
+    per = 1.4426950408889634074 / double(T);
+    inf = xmax == __builtin_inff();
+    least = inf ? xmax : float(max - double(S) / per);
+  }
   __device__ __forceinline__ double scaled(float x) const {
-    if (double(x) == max) return __builtin_ldexp(1.0, S);
-    const double y = (double(x) - max) * per;
-    if (!(y > -64.0)) return 0.0;
-    const double n = __builtin_rint(y), t = (y - n) * 0.69314718055994530942;
-    double r = 1.0 / 479001600.0;
-    r = fma(r, t, 1.0 / 39916800.0);
-    r = fma(r, t, 1.0 / 3628800.0);
-    r = fma(r, t, 1.0 / 362880.0);
-    r = fma(r, t, 1.0 / 40320.0);
-    r = fma(r, t, 1.0 / 5040.0);
-    r = fma(r, t, 1.0 / 720.0);
-    r = fma(r, t, 1.0 / 120.0);
-    r = fma(r, t, 1.0 / 24.0);
-    r = fma(r, t, 1.0 / 6.0);
-    r = fma(r, t, 0.5);
-    r = fma(r, t, 1.0);
-    r = fma(r, t, 1.0);
-    return __builtin_ldexp(r, int(n) + S);
+    constexpr double round = 6755399441055744.0;  // 1.5 * 2^52: a sum's low bits are the number rounded
+    constexpr double c1 = 0.69314718055994530942 / kTable, c2 = c1 * c1 / 2, c3 = c1 * c1 * c1 / 6;
+    const double t = inf ? double(kTable) * S : fma(double(x) - max, per * kTable, double(kTable) * S), m = t + round;
+    const int n = int(uint32_t(__double_as_longlong(m)));
+    const double r = t - (m - round), e = r * fma(r, fma(r, c3, c2), c1), b = table[n & (kTable - 1)];
+    const uint64_t v = uint64_t(__double_as_longlong(fma(b, e, b))) + (uint64_t(uint32_t(n >> 7)) << 52);
+    return x >= least ? __longlong_as_double((long long)v) : 0.0;
   }
   static __device__ __forceinline__ uint64_t whole(double v) {
     // (below 2^52: the sum's low bits are the number rounded to nearest)
     return uint64_t(__double_as_longlong(v + 4503599627370496.0)) & ((uint64_t(1) << 52) - 1);
   }
   __device__ __forceinline__ uint64_t operator()(float x) const { return whole(scaled(x)); }
+  // the table's entry j: e^(j ln 2 / 128) by its series
+  static __device__ __forceinline__ double entry(int j) {
+    const double t = j * (0.69314718055994530942 / kTable);
+    double r = 1.0;
+#pragma unroll
+    for (int i = 20; i > 0; --i) r = fma(r, t / i, 1.0);
+    return r;
+  }
 };
 
 __device__ __forceinline__ uint64_t wave_sum_u64(uint64_t v) {
@@ -144,6 +154,9 @@ __global__ void __launch_bounds__(NT) sample_kernel(Sampling p, int S) {
   __shared__ uint32_t list_key[kList];
   __shared__ int list_at[kList];
   __shared__ int listed;
+  __shared__ double table[kTable];
+  __shared__ unsigned long long scan_mass[NW];
+  __shared__ unsigned int scan_count[NW];
   __shared__ struct {
     uint32_t bin;
     uint32_t count;  // tokens above the bin
@@ -186,6 +199,7 @@ __global__ void __launch_bounds__(NT) sample_kernel(Sampling p, int S) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) top = max(top, uint32_t(__shfl_xor(top, o, 64)));
   if (lane == 0) red[0][wave] = top;
+  if (tid < kTable) table[tid] = Weigh::entry(tid);
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < NW; ++w) top = max(top, red[0][w]);
@@ -198,9 +212,9 @@ __global__ void __launch_bounds__(NT) sample_kernel(Sampling p, int S) {
     return;
   }
   Weigh w;
-  w.max = double(xmax);
-  w.per = 1.4426950408889634074 / double(T_);
+  w.table = table;
   w.S = S;
+  w.start(xmax, T_);
   // min-p: a weight below this (times 2^S) is dropped
   const double least = by_m ? double(fminf(mp, 1.f)) * __builtin_ldexp(1.0, S) : 0.0;
   // bins of equal width in z over the S bits that weigh anything
@@ -214,36 +228,44 @@ __global__ void __launch_bounds__(NT) sample_kernel(Sampling p, int S) {
     }
     __syncthreads();
   };
-  // where a prefix of `goal` tokens or weight of the bins ends, and what lies above
+  // Where a prefix of `goal` tokens or weight of the bins ends, and what lies above:
+  // kBins / NT bins to a thread, its wave's sums before it, the waves' before those.
   auto find = [&](bool by_mass, uint64_t goal) {
+    constexpr int PB = kBins / NT;
     __syncthreads();
-    if (wave == 0) {
-      constexpr int per = kBins / 64;
-      uint64_t m = 0;
-      uint32_t c = 0;
-#pragma unroll 8
-      for (int i = 0; i < per; ++i) {
-        m += mass[lane * per + i];
-        c += count[lane * per + i];
-      }
-      const uint64_t ms = wave_scan((unsigned long long)m, lane);
-      const uint32_t cs = wave_scan(c, lane);
-      const uint64_t hits = __ballot((by_mass ? ms : uint64_t(cs)) >= goal);
-      const int l = hits ? __builtin_ctzll(hits) : 63;
-      if (lane == l) {
-        uint64_t am = ms - m;
-        uint32_t ac = cs - c;
-        int b = lane * per;
-        for (int i = 0; i + 1 < per; ++i) {
-          if ((by_mass ? am + mass[b] : uint64_t(ac) + count[b]) >= goal) break;
-          am += mass[b];
-          ac += count[b];
+    uint64_t bm[PB], m = 0;
+    uint32_t bc[PB], c = 0;
+#pragma unroll
+    for (int i = 0; i < PB; ++i) {
+      m += bm[i] = mass[tid * PB + i];
+      c += bc[i] = count[tid * PB + i];
+    }
+    uint64_t ms = wave_scan((unsigned long long)m, lane);
+    uint32_t cs = wave_scan(c, lane);
+    if (lane == 63) {
+      scan_mass[wave] = ms;
+      scan_count[wave] = cs;
+    }
+    __syncthreads();
+    for (int v = 0; v < wave; ++v) {
+      ms += scan_mass[v];
+      cs += scan_count[v];
+    }
+    const uint64_t up = by_mass ? ms : uint64_t(cs), down = by_mass ? ms - m : uint64_t(cs - c);
+    if ((down < goal && up >= goal) || (tid == NT - 1 && up < goal)) {
+      uint64_t am = ms - m;
+      uint32_t ac = cs - c;
+      int b = 0;
+#pragma unroll
+      for (int i = 0; i + 1 < PB; ++i)
+        if (b == i && (by_mass ? am + bm[i] : uint64_t(ac) + bc[i]) < goal) {
+          am += bm[i];
+          ac += bc[i];
           ++b;
         }
-        at.bin = b;
-        at.count = ac;
-        at.mass = am;
-      }
+      at.bin = tid * PB + b;
+      at.count = ac;
+      at.mass = am;
     }
     __syncthreads();
   };
@@ -388,6 +410,66 @@ __global__ void __launch_bounds__(NT) sample_kernel(Sampling p, int S) {
   };
 
   auto over_row = [&](auto f) { each_value<DT, NT>(row, V, f); };
+  // A list of one token per thread is ordered by counting, for each, those before
+  // it: a few steps over LDS where the histograms take a dozen barriers each
+  // (top 50 of 131072: 57 us | 48).
+  constexpr int kShort = NT < 512 ? NT : 512;
+  // inclusive sums over the threads, and the last one's
+  auto scan = [&](uint64_t v, uint64_t &total) -> uint64_t {
+    uint64_t run = wave_scan((unsigned long long)v, lane);
+    if (lane == 63) scan_mass[wave] = run;
+    __syncthreads();
+    total = 0;
+    for (int i = 0; i < NW; ++i) {
+      if (i < wave) run += scan_mass[i];
+      total += scan_mass[i];
+    }
+    __syncthreads();
+    return run;
+  };
+  // The list's token that ends the prefix: of k tokens; then of weight `goal`, with
+  // `above` before the list (0: top-p's share of those k).
+  auto short_cut = [&](int n, uint32_t k_, uint64_t above, uint64_t goal) {
+    uint32_t rank = 0;
+    if (tid < n) {
+      const uint32_t kk = list_key[tid];
+      const int i = list_at[tid];
+      for (int j = 0; j < n; ++j) rank += list_key[j] > kk || (list_key[j] == kk && list_at[j] < i);
+      mass[rank] = w(key_value(kk));
+      count[rank] = uint32_t(tid);
+    }
+    __syncthreads();
+    const uint64_t mine = uint32_t(tid) < k_ ? mass[tid] : 0;
+    uint64_t total;
+    const uint64_t run = scan(mine, total);
+    if (goal == 0) goal = goal_p(total);
+    const uint64_t need = goal > above + total ? total : goal - above;  // (~0: all k)
+    if (tid == int(k_) - 1) at.bin = k_ - 1;
+    __syncthreads();
+    if (uint32_t(tid) < k_ && goal != ~uint64_t(0) && run >= need && run - mine < need) at.bin = uint32_t(tid);
+    __syncthreads();
+    const int last = int(count[at.bin]);
+    cut.K = list_key[last];
+    last_tie = list_at[last];
+    __syncthreads();
+  };
+  auto draw_short = [&](int n) {
+    if (tid < n) {
+      const int i = list_at[tid];
+      uint32_t rank = 0;
+      for (int j = 0; j < n; ++j) rank += list_at[j] < i;
+      mass[rank] = weight(key_value(list_key[tid]), i);
+      count[rank] = uint32_t(tid);
+    }
+    __syncthreads();
+    const uint64_t mine = tid < n ? mass[tid] : 0;
+    uint64_t total;
+    const uint64_t run = scan(mine, total), goal = goal_of(total);
+    if (run > goal && run - mine <= goal) {
+      const int e = int(count[tid]);
+      put(list_at[e], key_value(list_key[e]), total);
+    }
+  };
   // Groups of consecutive tokens: f(logit, index) over one by a wave, in any order.
   int gs = 512;
   while ((V + gs - 1) / gs > kMaxGroups) gs *= 2;
@@ -455,8 +537,12 @@ __global__ void __launch_bounds__(NT) sample_kernel(Sampling p, int S) {
       auto each = [&](auto f) {
         for (int i = tid; i < n; i += NT) f(key_value(list_key[i]), list_at[i]);
       };
-      cut = end_in(each, true, goal, b0, am, 0, above);
-      cut_ties(each);
+      if (n <= kShort) {
+        short_cut(n, uint32_t(n), am, goal);
+      } else {
+        cut = end_in(each, true, goal, b0, am, 0, above);
+        cut_ties(each);
+      }
       each([&](float x, int i) {
         const uint64_t v = weight(x, i);
         if (v) atomicAdd(&group_mass[i / gs], (unsigned long long)v);
@@ -469,14 +555,22 @@ __global__ void __launch_bounds__(NT) sample_kernel(Sampling p, int S) {
     __syncthreads();
   } else if (by_k || by_m) {
     uint32_t bound = kBins - 1;
-    if (by_k && V > kList) {
+    if (by_k && V > kShort) {
       const int owners = int(sum_of(own != 0));  // (threads with a logit)
       clear();
-      if (own) atomicAdd(&count[bin_of(key_value(own))], 1u);
-      find(false, uint64_t(min(k, owners)));
-      if (k <= owners) bound = at.bin;
+      // (of n threads' largest the k-th is passed by about -n log(1 - k / n) logits:
+      // near n that is no bound, and the logits are counted instead)
+      const bool bounded = k <= owners - owners / 10;
+      if (bounded) {
+        if (own) atomicAdd(&count[bin_of(key_value(own))], 1u);
+      } else {
+        over_row([&](float x, int) { atomicAdd(&count[bin_of(x)], 1u); });
+      }
+      find(false, uint64_t(k));
+      bound = at.bin;
     }
-    if (by_m) bound = min(bound, uint32_t(fminf(float(-log2(double(fminf(mp, 1.f)))) * per_bin + 2.f, float(kBins - 1))));
+    // (top-p goes by the weight of all that top-k leaves)
+    if (by_m && !(by_k && by_p)) bound = min(bound, uint32_t(fminf(float(-log2(double(fminf(mp, 1.f)))) * per_bin + 2.f, float(kBins - 1))));
     if (tid == 0) listed = 0;
     __syncthreads();
     over_row([&](float x, int i) {
@@ -495,7 +589,12 @@ __global__ void __launch_bounds__(NT) sample_kernel(Sampling p, int S) {
     auto each = [&](auto f) {
       for (int i = tid; i < n; i += NT) f(key_value(list_key[i]), list_at[i]);
     };
-    if (holds && !(by_k && by_p && n < k)) {
+    if (holds && n <= kShort) {
+      if (by_k && n >= k) short_cut(n, uint32_t(k), 0, by_p ? 0 : ~uint64_t(0));
+      draw_short(n);
+      return;
+    }
+    if (holds) {
       if (by_k && n >= k) {
         cut = of_top_k(each);
         cut_ties(each);
