@@ -239,7 +239,8 @@ int mh_attention_textbook(int dt, const void *q, const void *k, const void *v, v
  * needed).  A token whose page does not exist (the free pages or the table's
  * width are exhausted, a held entry lies outside the pool) gets slot -1, a page
  * that could not be had the entry -1, tokens past n_slots are left out (cu stops
- * there), and the error flag is raised.  Outputs overlap no input but tables. */
+ * there), and the error flag is raised.  Outputs overlap no input and no other
+ * output.  Nothing is done for B = 0; B is below 2^24. */
 int mh_page_plan(const int32_t *lens, const int32_t *new_lens, const int32_t *free_pages, int32_t *tables,
                  int32_t *total_lens, int32_t *cu, int32_t *slots, int32_t *positions, int32_t *used, int B, int n_free,
                  int width, int page, int n_pages, int n_slots, void *stream);
@@ -254,7 +255,7 @@ int mh_page_plan(const int32_t *lens, const int32_t *new_lens, const int32_t *fr
  * page's first token is among them, else the larger of e and the scale held,
  * and if it grows the page's earlier tokens are rounded to it; values are
  * rounded to the nearest e4m3, ties to even.  Infinities and NaN become NaN and do not
- * count towards the magnitude. */
+ * count towards the magnitude.  n is at most 2^29, Hkv 65535. */
 int mh_kv_store_paged(int dt, const void *k, const void *v, int64_t ldk, int64_t ldv, const int32_t *slots,
                       void *k_cache, void *v_cache, float *k_scale, float *v_scale, int n, int Hkv, int hd, int page,
                       int n_pages, void *stream);
@@ -296,7 +297,8 @@ int mh_attention_paged(int dt, const void *q, int64_t ldq, const void *k_cache, 
  * exceeds u times their sum.  Sums are whole 64-bit numbers: results do not vary
  * from run to run.  NaN logits count as -inf; a row of nothing else gives -1.
  * logprob [rows] (may be NULL): log of the drawn token's share of the kept w
- * (-inf with -1).  workspace: mh_sample_workspace bytes, as in mh_attention_paged. */
+ * (-inf with -1).  rows is below 2^22.  workspace: mh_sample_workspace bytes, as
+ * in mh_attention_paged (0, whatever the size: no row needs one yet). */
 int mh_sample_workspace(int dt, int rows, int cols, size_t *bytes);
 int mh_sample(int dt, const void *logits, int64_t ld, int rows, int cols, const float *u, const float *temperature,
               const int32_t *top_k, const float *top_p, const float *min_p, int32_t *out, float *logprob, void *workspace,

@@ -586,6 +586,7 @@ int mh_page_plan(const int32_t *lens, const int32_t *new_lens, const int32_t *fr
   MH_TRY({
     check_page("page_plan", page, n_pages);
     if (B < 0 || n_free < 0 || width < 0 || n_slots < 0) throw Error("page_plan: negative size");
+    if (B >= 1 << 24) throw Error("page_plan: more requests than one launch takes (2^24 - 1)");
     if (int64_t(width) * page > 0x7fffffff) throw Error("page_plan: a table row must hold at most 2^31 - 1 tokens");
     if (B == 0) return 0;
     if (!lens || !new_lens || !total_lens || !cu || !used || (width && !tables) || (n_free && !free_pages) ||
@@ -617,6 +618,7 @@ int mh_kv_store_paged(int dt, const void *k, const void *v, int64_t ldk, int64_t
     check_dt(dt);
     check_pool("kv_store_paged", k_cache, v_cache, k_scale, v_scale, Hkv, hd, page, n_pages);
     if (n < 0) throw Error("kv_store_paged: negative size");
+    if (n > 1 << 29) throw Error("kv_store_paged: more tokens than one launch takes (2^29)");
     if (n == 0) return 0;
     if (!slots) throw Error("kv_store_paged: null slots");
     check_rows("kv_store_paged", "k", dt, k, ldk, int64_t(Hkv) * hd);
@@ -688,6 +690,7 @@ int mh_sample_workspace(int dt, int rows, int cols, size_t *bytes) {
     check_dt(dt);
     if (!bytes) throw Error("sample_workspace: null output");
     if (rows < 0 || cols < 1) throw Error("sample: bad row count or empty rows");
+    if (rows >= 1 << 22) throw Error("sample: more rows than one launch takes (2^22 - 1)");
     *bytes = 0;
   })
 }
@@ -697,6 +700,7 @@ int mh_sample(int dt, const void *logits, int64_t ld, int rows, int cols, const 
   MH_TRY({
     check_dt(dt);
     if (rows < 0 || cols < 1) throw Error("sample: bad row count or empty rows");
+    if (rows >= 1 << 22) throw Error("sample: more rows than one launch takes (2^22 - 1)");
     if (rows == 0) return 0;
     if (!logits || !u || !out) throw Error("sample: null argument");
     if (ld < cols) throw Error("sample: rows overlap");

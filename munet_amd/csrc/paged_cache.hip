@@ -26,15 +26,16 @@ __device__ __forceinline__ Need need_of(const PagePlan &p, int b) {
   return Need{n.fresh, n.need - n.have};
 }
 
-// One workgroup per kPlanRequests requests, and the slots behind the last token
-// by whoever comes to them.
+// blockIdx.x is the request; its workgroups (blockIdx.y) go round its tokens, the
+// last request's also round the slots behind the last token.  The first one
+// writes the rest.
 __global__ void __launch_bounds__(256) page_plan_kernel(PagePlan p, int *err) {
   __shared__ int64_t part[2][4];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int b0 = blockIdx.x * kPlanRequests, b1 = min(b0 + kPlanRequests, p.B);
+  const int b = blockIdx.x, turn = 256 * gridDim.y, at0 = 256 * blockIdx.y + tid;
   Need before{0, 0};
-  for (int b = tid; b < b0; b += 256) {
-    const Need n = need_of(p, b);
+  for (int o = tid; o < b; o += 256) {
+    const Need n = need_of(p, o);
     before.tokens += n.tokens;
     before.pages += n.pages;
   }
@@ -44,46 +45,43 @@ __global__ void __launch_bounds__(256) page_plan_kernel(PagePlan p, int *err) {
     part[1][wave] = g;
   }
   __syncthreads();
-  int64_t tok = part[0][0] + part[0][1] + part[0][2] + part[0][3], pg = part[1][0] + part[1][1] + part[1][2] + part[1][3];
-  if (blockIdx.x == 0 && tid == 0) p.cu[0] = 0;
+  const int64_t tok = part[0][0] + part[0][1] + part[0][2] + part[0][3];
+  const int64_t first = part[1][0] + part[1][1] + part[1][2] + part[1][3];
+  const PlanNeed n = plan_need(p.lens[b], p.fresh[b], p.page, p.width);
+  int32_t *table = p.tables + int64_t(b) * p.width;
+  // a page of this request's list: held before, or the next free one
+  auto page_at = [&](int i) -> int {
+    int page = -1;
+    if (i < n.have) page = i < p.width ? table[i] : -1;
+    else if (i < n.need) page = first + i - n.have < p.n_free ? p.free_pages[first + i - n.have] : -1;
+    return page_in_pool(page, p.n_pages) ? page : -1;
+  };
   int bad = 0;
-  for (int b = b0; b < b1; ++b) {
-    const PlanNeed n = plan_need(p.lens[b], p.fresh[b], p.page, p.width);
-    int32_t *table = p.tables + int64_t(b) * p.width;
-    const int64_t first = pg;
-    // a page of this request's list: held before, or the next free one
-    auto page_at = [&](int i) -> int {
-      int page = -1;
-      if (i < n.have) page = i < p.width ? table[i] : -1;
-      else if (i < n.need) page = first + i - n.have < p.n_free ? p.free_pages[first + i - n.have] : -1;
-      return page_in_pool(page, p.n_pages) ? page : -1;
-    };
-    for (int i = n.have + tid; i < n.need; i += 256) table[i] = page_at(i);
-    if (n.fresh > 0) {
-      for (int64_t i = tid; i < n.fresh; i += 256) {
-        const int64_t at = tok + i, pos = int64_t(n.len) + i;
-        if (at >= p.cap) {
-          bad = 1;
-          break;
-        }
-        const int page = pos / p.page < p.width ? page_at(int(pos / p.page)) : -1;
-        if (page < 0) bad = 1;
-        p.slots[at] = page < 0 ? -1 : page * p.page + int(pos % p.page);
-        if (p.positions) p.positions[at] = int(pos);
-      }
+  for (int64_t i = at0; i < n.fresh; i += turn) {
+    const int64_t at = tok + i, pos = int64_t(n.len) + i;
+    if (at >= p.cap) {
+      bad = 1;
+      break;
     }
-    tok += n.fresh;
-    pg += n.need - n.have;
-    if (tid == 0) {
-      p.total[b] = int(int64_t(n.len) + n.fresh);
-      p.cu[b + 1] = int(tok < p.cap ? tok : p.cap);
-      if (b + 1 == p.B) p.used[0] = int(pg);
-    }
+    const int nth = int(pos) / p.page, page = nth < p.width ? page_at(nth) : -1;  // (pos is below 2^31)
+    if (page < 0) bad = 1;
+    p.slots[at] = page < 0 ? -1 : page * p.page + int(pos) % p.page;
+    if (p.positions) p.positions[at] = int(pos);
   }
   if (bad) atomicOr(err, kErrPlan);
+  const int64_t end = tok + n.fresh;
+  if (blockIdx.y == 0) {
+    for (int i = n.have + tid; i < n.need; i += 256) table[i] = page_at(i);
+    if (tid == 0) {
+      p.total[b] = int(int64_t(n.len) + n.fresh);
+      if (b == 0) p.cu[0] = 0;
+      p.cu[b + 1] = int(end < p.cap ? end : p.cap);
+      if (b + 1 == p.B) p.used[0] = int(first + n.need - n.have);
+    }
+  }
   // the slots behind the last token (a batch padded to a captured graph's size)
-  if (b1 == p.B)
-    for (int64_t i = tok + tid; i < p.cap; i += 256) {
+  if (b + 1 == p.B)
+    for (int64_t i = end + at0; i < p.cap; i += turn) {
       p.slots[i] = -1;
       if (p.positions) p.positions[i] = 0;
     }
@@ -140,6 +138,23 @@ __device__ __forceinline__ float amax8(const float v[8], float big) {
   return big;
 }
 
+// eight consecutive values as they lie
+template <int DT> struct Raw {
+  uint4 a, b;
+  __device__ __forceinline__ void load(const typename Store<DT>::T *p) {
+    a = reinterpret_cast<const uint4 *>(p)[0];
+    if constexpr (DT == F32) b = reinterpret_cast<const uint4 *>(p)[1];
+  }
+  __device__ __forceinline__ void get(float v[8]) const {
+    if constexpr (DT == F32) {
+      v[0] = __uint_as_float(a.x); v[1] = __uint_as_float(a.y); v[2] = __uint_as_float(a.z); v[3] = __uint_as_float(a.w);
+      v[4] = __uint_as_float(b.x); v[5] = __uint_as_float(b.y); v[6] = __uint_as_float(b.z); v[7] = __uint_as_float(b.w);
+    } else {
+      dec8<DT>(a, v);
+    }
+  }
+};
+
 struct StoreArgs {
   const void *k, *v;
   const int32_t *slots;
@@ -159,7 +174,8 @@ __global__ void __launch_bounds__(256) kv_store_paged_kernel(StoreArgs a) {
   typedef typename Store<DT>::T T;
   constexpr int VT = 64;  // tokens of a value tile
   __shared__ float red[2][4];
-  __shared__ __align__(16) uint8_t vt[kPagedHeadMax][VT + 4];
+  // (rows of VT + 4 bytes; of the run's quads in the short form)
+  __shared__ __align__(16) uint8_t vt[kPagedHeadMax * (VT + 4)];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, head = blockIdx.y;
   const int t0 = blockIdx.x * a.per, hd = a.hd, P = a.page, h8 = hd / 8;
   const int64_t limit = int64_t(a.n_pages) * P;
@@ -179,6 +195,8 @@ __global__ void __launch_bounds__(256) kv_store_paged_kernel(StoreArgs a) {
     const int t = t0 + __builtin_ctzll(starts);
     starts &= starts - 1;
     const int slot = a.slots[t], page = slot / P, place = slot - page * P;
+    const int64_t sc = int64_t(page) * a.Hkv + head;
+    const float held[2] = {a.ks[sc], a.vs[sc]};
     int n = 0;  // tokens of the run
     for (;;) {
       const int i = n + lane;
@@ -194,8 +212,33 @@ __global__ void __launch_bounds__(256) kv_store_paged_kernel(StoreArgs a) {
     const T *vp = static_cast<const T *>(a.v) + int64_t(t) * a.ldv + int64_t(head) * hd;
     uint8_t *kd = a.kc + page_base(page, a.Hkv, head, P, hd), *vd = a.vc + page_base(page, a.Hkv, head, P, hd);
 
+    // A run of at most 256 pieces of 4 places and 8 head values (64 tokens of heads of
+    // 128) is held in registers, a piece to a thread: loaded once, its values
+    // transposed four places at a time (17k tokens, 8 heads of 128: 39 us, against 44
+    // with two passes over memory and single bytes).
+    const int q0 = place / 4, nq = (place + n - 1) / 4 - q0 + 1;
+    const bool held_run = nq * h8 <= 256;
+    const int pq = tid / h8, pd = 8 * (tid - pq * h8), pi = 4 * (q0 + pq) - place;  // this thread's piece: first token
+    const bool mine = held_run && pq < nq;
+    Raw<DT> kr[4], vr[4];
     float big[2] = {0.f, 0.f};
-    for (int c = tid; c < n * h8; c += 256) {
+    if (mine) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int64_t i = min(max(pi + j, 0), n - 1);  // (places beside the run repeat its tokens, not stored)
+        kr[j].load(kp + i * a.ldk + pd);
+        vr[j].load(vp + i * a.ldv + pd);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float v[8];
+        kr[j].get(v);
+        big[0] = amax8(v, big[0]);
+        vr[j].get(v);
+        big[1] = amax8(v, big[1]);
+      }
+    }
+    for (int c = held_run ? n * h8 : tid; c < n * h8; c += 256) {
       const int i = c / h8, d = 8 * (c - i * h8);
       float v[8];
       ld8<DT>(kp + int64_t(i) * a.ldk + d, v);
@@ -203,9 +246,7 @@ __global__ void __launch_bounds__(256) kv_store_paged_kernel(StoreArgs a) {
       ld8<DT>(vp + int64_t(i) * a.ldv + d, v);
       big[1] = amax8(v, big[1]);
     }
-    const int64_t sc = int64_t(page) * a.Hkv + head;
     float now[2], inv[2], ratio[2];
-    const float held[2] = {a.ks[sc], a.vs[sc]};
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
       const float m = wave_max(big[x]);
@@ -248,6 +289,53 @@ __global__ void __launch_bounds__(256) kv_store_paged_kernel(StoreArgs a) {
     }
     __syncthreads();
 
+    if (held_run) {
+      const int rs = 4 * nq + 4;  // LDS bytes of a head value's places
+      if (mine) {
+        uint32_t w[4][2];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float v[8];
+          kr[j].get(v);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] *= inv[0];
+          if (pi + j >= 0 && pi + j < n)
+            *reinterpret_cast<uint2 *>(kd + int64_t(place + pi + j) * hd + pd) = make_uint2(e4m3x4(v), e4m3x4(v + 4));
+          vr[j].get(v);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] *= inv[1];
+          w[j][0] = e4m3x4(v);
+          w[j][1] = e4m3x4(v + 4);
+        }
+        // four places of each head value to a word
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          uint32_t x = 0;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x |= ((w[j][e >> 2] >> (8 * (e & 3))) & 0xffu) << (8 * j);
+          *reinterpret_cast<uint32_t *>(&vt[(pd + e) * rs + 4 * pq]) = x;
+        }
+      }
+      __syncthreads();
+      const int lo = place, hi = place + n, first = lo & ~15, pieces = (hi + 15) / 16 - lo / 16;
+      for (int c = tid; c < hd * pieces; c += 256) {
+        const int d = c / pieces, at = first + 16 * (c - d * pieces);
+        const uint8_t *src = &vt[d * rs] + (at - 4 * q0);  // (before the row where the run starts inside the piece)
+        uint8_t *dst = vd + int64_t(d) * P + at;
+        if (at >= lo && at + 16 <= hi) {
+          const uint32_t *s4 = reinterpret_cast<const uint32_t *>(src);
+          *reinterpret_cast<uint4 *>(dst) = make_uint4(s4[0], s4[1], s4[2], s4[3]);
+        } else {
+          for (int e = max(lo - at, 0); e < min(hi - at, 16); ++e) dst[e] = src[e];
+        }
+      }
+      __syncthreads();
+      if (tid == 0) {
+        a.ks[sc] = now[0];
+        a.vs[sc] = now[1];
+      }
+      continue;
+    }
     // keys, in their rows
     for (int c = tid; c < n * h8; c += 256) {
       const int i = c / h8, d = 8 * (c - i * h8);
@@ -268,18 +356,18 @@ __global__ void __launch_bounds__(256) kv_store_paged_kernel(StoreArgs a) {
         for (int e = 0; e < 8; ++e) v[e] *= inv[1];
         const uint32_t w[2] = {e4m3x4(v), e4m3x4(v + 4)};
 #pragma unroll
-        for (int e = 0; e < 8; ++e) vt[d + e][lo - c0 + i] = uint8_t(w[e >> 2] >> (8 * (e & 3)));
+        for (int e = 0; e < 8; ++e) vt[(d + e) * (VT + 4) + lo - c0 + i] = uint8_t(w[e >> 2] >> (8 * (e & 3)));
       }
       __syncthreads();
       const int first = lo & ~15, pieces = ((hi + 15) / 16) - lo / 16;
       for (int c = tid; c < hd * pieces; c += 256) {
         const int d = c / pieces, at = first + 16 * (c - d * pieces);
-        const uint32_t *src = reinterpret_cast<const uint32_t *>(&vt[d][at - c0]);
+        const uint32_t *src = reinterpret_cast<const uint32_t *>(&vt[d * (VT + 4) + at - c0]);
         uint8_t *dst = vd + int64_t(d) * P + at;
         if (at >= lo && at + 16 <= hi) {
           *reinterpret_cast<uint4 *>(dst) = make_uint4(src[0], src[1], src[2], src[3]);
         } else {
-          for (int e = max(lo - at, 0); e < min(hi - at, 16); ++e) dst[e] = vt[d][at - c0 + e];
+          for (int e = max(lo - at, 0); e < min(hi - at, 16); ++e) dst[e] = vt[d * (VT + 4) + at - c0 + e];
         }
       }
       __syncthreads();
@@ -294,16 +382,16 @@ __global__ void __launch_bounds__(256) kv_store_paged_kernel(StoreArgs a) {
 }  // namespace
 
 hipError_t page_plan(const PagePlan &p, int *err, hipStream_t st) {
-  if (p.B < 1) return hipErrorInvalidValue;
-  const int blocks = (p.B + kPlanRequests - 1) / kPlanRequests;
-  hipLaunchKernelGGL(page_plan_kernel, dim3(unsigned(blocks)), dim3(256), 0, st, p, err);
+  if (p.B < 1 || p.B >= 1 << 24) return hipErrorInvalidValue;
+  const dim3 grid(unsigned(p.B), unsigned(plan_groups(p.B, p.cap)));
+  hipLaunchKernelGGL(page_plan_kernel, grid, dim3(256), 0, st, p, err);
   return hipGetLastError();
 }
 
 hipError_t kv_store_paged(int dt, const void *k, const void *v, long ldk, long ldv, const int32_t *slots, void *k_cache,
                           void *v_cache, float *k_scale, float *v_scale, int n, int Hkv, int hd, int page, int n_pages, int *err,
                           hipStream_t st) {
-  if (n < 1 || Hkv < 1 || Hkv > 65535) return hipErrorInvalidValue;
+  if (n < 1 || n > 1 << 29 || Hkv < 1 || Hkv > 65535) return hipErrorInvalidValue;
   StoreArgs a{k, v, slots, static_cast<uint8_t *>(k_cache), static_cast<uint8_t *>(v_cache), k_scale, v_scale, err, ldk, ldv,
               n, Hkv, hd, page, n_pages, store_tokens(n, Hkv)};
   const dim3 grid(unsigned((n + a.per - 1) / a.per), unsigned(Hkv));

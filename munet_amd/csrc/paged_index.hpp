@@ -72,13 +72,18 @@ __host__ __device__ __forceinline__ PlanNeed plan_need(int len, int fresh, int p
   if (n.need < n.have) n.need = n.have;
   return n;
 }
-// Requests per workgroup of the plan: each adds up the ones before its own.
-constexpr int kPlanRequests = 1;
+// Workgroups per request of the plan, which go round its tokens: one for each
+// 1024 tokens that there may be, at most 1024 in all (one prompt of 131072
+// tokens 6 us, 302 with one workgroup; 12 of 2500 4.0 against 6.6).
+inline int plan_groups(int B, int64_t cap) {
+  return int(std::max<int64_t>(1, std::min<int64_t>(1024 / std::max(B, 1), (cap + 1023) / 1024)));
+}
 
-// Tokens per workgroup of the store: one while that leaves at most 16384
+// Tokens per workgroup of the store: one while that leaves at most 4096
 // workgroups (a decode step: every token starts a run), up to 64 for prompts,
-// where one token in a page does.
-inline int store_tokens(int n, int heads) { return int(std::min<int64_t>(64, std::max<int64_t>(1, int64_t(n) * heads / 16384))); }
+// where one token in a page does (17k tokens, 8 heads of 128, pages of 64: 34 us;
+// at most 2048 workgroups 37, 8192 38, 16384 39).
+inline int store_tokens(int n, int heads) { return int(std::min<int64_t>(64, std::max<int64_t>(1, int64_t(n) * heads / 4096))); }
 
 // Workgroup i of a launch over `pairs` (sequence, key/value head) pairs of `per`
 // items each.  Workgroups go round the eight XCDs, each with an L2 of its own:

@@ -39,7 +39,7 @@ __device__ __forceinline__ float key_value(uint32_t k) {
 // / 128) times e^(r ln 2 / 128) by its series to the third power (the next term is
 // below 2^-38: one in 10^8 draws from 10^5 equal tokens could move).  Eleven 64-bit
 // operations, where the series without a table takes twenty (sums of 131072
-// weights in 200 rows 92 us | 60).
+// weights in 200 rows 92 us | 77).
 constexpr int kTable = 128;
 struct Weigh {
   const double *table;  // 2^(j / 128)
@@ -51,7 +51,8 @@ struct Weigh {
     max = double(xmax);
     per = 1.4426950408889634074 / double(T);
     inf = xmax == __builtin_inff();
-    least = inf ? xmax : float(max - double(S) / per);
+    // (-inf weighs nothing at any temperature)
+    least = inf ? xmax : fmaxf(float(max - double(S) / per), -3.402823466e38f);
   }
   __device__ __forceinline__ double scaled(float x) const {
     constexpr double round = 6755399441055744.0;  // 1.5 * 2^52: a sum's low bits are the number rounded
@@ -412,7 +413,7 @@ __global__ void __launch_bounds__(NT) sample_kernel(Sampling p, int S) {
   auto over_row = [&](auto f) { each_value<DT, NT>(row, V, f); };
   // A list of one token per thread is ordered by counting, for each, those before
   // it: a few steps over LDS where the histograms take a dozen barriers each
-  // (top 50 of 131072: 57 us | 48).
+  // (top 50 of 131072: 57 us | 52).
   constexpr int kShort = NT < 512 ? NT : 512;
   // inclusive sums over the threads, and the last one's
   auto scan = [&](uint64_t v, uint64_t &total) -> uint64_t {
@@ -659,7 +660,7 @@ __global__ void __launch_bounds__(NT) sample_kernel(Sampling p, int S) {
 }  // namespace
 
 hipError_t sample_rows(int dt, const Sampling &p, hipStream_t st) {
-  if (p.rows < 1 || p.cols < 1) return hipErrorInvalidValue;
+  if (p.rows < 1 || p.rows >= 1 << 22 || p.cols < 1) return hipErrorInvalidValue;
   // sums of p.cols weights of at most 2^S stay below 2^63
   int bits = 0;
   while ((int64_t(1) << bits) < p.cols) ++bits;

@@ -230,6 +230,7 @@ def check(torch, hip, c, heads, dtype, seed=1, what="", extra=0, **kw):
     ([0], [1], 4, 4, 1), ([15, 16, 17, 0], [1, 1, 1, 1], 9, 3, 4), ([0, 5, 300, 31], [700, 0, 1, 33], 70, 50, 740),
     ([3] * 300, [1] * 300, 0, 1, 300), ([64] * 300, [2] * 300, 400, 6, 700), ([0, 0], [0, 0], 0, 0, 3),
     ([-4, 10], [5, -6], 2, 2, 8),                       # negative counts are none
+    ([77], [20000], 1300, 1400, 30000), ([9, 0, 40], [1, 9000, 2000], 700, 600, 11500),  # several workgroups to a request
     ([0, 0, 0], [100, 100, 100], 5, 20, 300),           # free pages end
     ([10, 10], [400, 20], 60, 2, 500),                  # the table's width ends
     ([0, 0], [30, 30], 9, 9, 41)])                      # the slots end

@@ -40,6 +40,7 @@ def reference(torch, logits, u, T=None, k=None, p=None, m=None):
             logprob.append(0.0)
             continue
         w = torch.where(x == best, 1.0, torch.exp((x - best) / t))
+        w = torch.where(x == -math.inf, 0.0, w)  # (also where T is infinite)
         order = torch.argsort(-x, stable=True)
         order = order[:kk] if 0 < kk < len(order) else order
         n = len(order)
@@ -152,6 +153,20 @@ def test_ends_of_the_range(torch, hip, dtype):
     run(torch, hip, x, [0.0, 1 - 2.0 ** -24, 1.0, 2.0, -1.0, 0.5], what="u")
     run(torch, hip, x, uniform(torch, 6), T=[math.nan, math.inf, 1.0, 1.0, 1.0, 1.0], k=[-3, 0, 2 ** 31 - 1, 1000, 999, 5],
         p=[-1.0, 2.0, -1.0, 0.999, 1.0, -0.5], m=[-1.0, 5.0, 0.0, -0.0, 2.0, 0.1], what="settings")
+
+
+@pytest.mark.parametrize("V", [300, 6000])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_masked_tokens_at_any_temperature(torch, hip, dtype, V):
+    """-inf is never drawn, however flat the rest; without a limit all others are alike (sums exact)."""
+    g = torch.Generator().manual_seed(V)
+    x = torch.randn((8, V), generator=g).to(getattr(torch, dtype))
+    x[:, torch.rand(V, generator=g) < 0.6] = -math.inf
+    x[0, 1:] = -math.inf
+    u = [0.0, 0.25, 0.5, 0.75, 0.9375, 0.0078125, 0.998046875, 1.0]
+    for T in (1e37, 3e38, math.inf):
+        for k, p in ((None, None), ([V] * 8, None), ([V // 4] * 8, None), (None, [0.625] * 8)):
+            run(torch, hip, x.cuda(), u, [T] * 8, k, p, what=f"T {T} k {k and k[0]} p {p and p[0]}")
 
 
 @pytest.mark.parametrize("dtype", DTYPES)

@@ -36,7 +36,7 @@ def _plan(**kw):
     (dict(page=48), "16, 32, 64, 128 or 256"), (dict(page=8), "16, 32"), (dict(page=512), "16, 32"),
     (dict(n_pages=0), "pool"), (dict(n_pages=1 << 27), "pool"), (dict(B=-1), "negative"), (dict(width=-2), "negative"),
     (dict(n_slots=-1), "negative"), (dict(width=1 << 27), "table row"), (dict(lens=None), "null"), (dict(used=None), "null"),
-    (dict(slots=None), "null"), (dict(tables=None), "null"), (dict(free_pages=None), "null")])
+    (dict(slots=None), "null"), (dict(tables=None), "null"), (dict(free_pages=None), "null"), (dict(B=1 << 24), "one launch")])
 def test_page_plan_refusals(kw, match):
     with pytest.raises(_lib.HipError, match=match):
         _plan(**kw)
@@ -52,7 +52,8 @@ def _store(**kw):
     (dict(dt=3), "dtype"), (dict(hd=24), "multiple of 16"), (dict(hd=272), "multiple of 16"), (dict(hd=0), "multiple of 16"),
     (dict(Hkv=0), "head count"), (dict(page=100), "page holds"), (dict(n=-1), "negative"), (dict(slots=None), "null"),
     (dict(k=None), "null k"), (dict(v=A + 8), "aligned"), (dict(ldk=1023), "multiple of 16"), (dict(ldv=1016), "whole"),
-    (dict(kc=A + 4), "aligned"), (dict(vs=None), "null cache"), (dict(dt=F32, ldk=1026), "multiple of 16")])
+    (dict(kc=A + 4), "aligned"), (dict(vs=None), "null cache"), (dict(dt=F32, ldk=1026), "multiple of 16"),
+    (dict(n=(1 << 29) + 1), "one launch"), (dict(Hkv=65536), "head count")])
 def test_kv_store_paged_refusals(kw, match):
     with pytest.raises(_lib.HipError, match=match):
         _store(**kw)
@@ -86,7 +87,8 @@ def _sample(**kw):
 
 @pytest.mark.parametrize("kw,match", [
     (dict(dt=3), "dtype"), (dict(rows=-1), "bad row count"), (dict(cols=0), "empty rows"), (dict(ld=99), "overlap"),
-    (dict(logits=None), "null"), (dict(u=None), "null"), (dict(out=None), "null"), (dict(logits=A + 1), "aligned")])
+    (dict(logits=None), "null"), (dict(u=None), "null"), (dict(out=None), "null"), (dict(logits=A + 1), "aligned"),
+    (dict(rows=1 << 22), "one launch")])
 def test_sample_refusals(kw, match):
     with pytest.raises(_lib.HipError, match=match):
         _sample(**kw)
