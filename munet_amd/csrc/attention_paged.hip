@@ -617,6 +617,8 @@ __global__ void __launch_bounds__(256, DT == F32 || HDP > 128 ? 1 : 2) attn_page
   // value, 16 keys; neighbours within a page follow each other).  The pieces of a wave
   // lie in one page, whatever the page holds: its number and the page's address
   // are scalars, and a thread adds a constant.
+  static_assert(NK % NT == 0, "a thread's i-th piece is of keys or of values for the whole workgroup");
+  auto of_keys = [](int i) { return NT * i < NK; };
   const int ql = min(a.plog - 4, 2);  // log2 of the runs of 16 keys per page and block
   uint32_t off[CH];                   // byte within the page's keys or values, less the scalar part
   int l0[CH];                         // LDS byte of its first chunk; the second one's is l0 ^ 16
@@ -630,21 +632,19 @@ __global__ void __launch_bounds__(256, DT == F32 || HDP > 128 ? 1 : 2) attn_page
 #pragma unroll
   for (int i = 0; i < CH; ++i) {
     const int e = tid + NT * i;
-    if (e < NK) {
+    if (of_keys(i)) {
       const int row = e / XK, x = e % XK, k = row & 15, R = (row & 32) + 8 * (k >> 2) + 4 * ((row >> 4) & 1) + (k & 3);
       off[i] = uint32_t(k * a.hd + min(16 * x, a.hd - 16));
       l0[i] = k_at(R, 2 * x);
-      grp0[i] = __builtin_amdgcn_readfirstlane(row >> 4);
+      grp0[i] = (64 * wave + NT * i) / (16 * XK);
     } else {
       int row, grp;
       const int lo = value_piece(i, row, grp);
       off[i] = uint32_t(min(row, a.hd - 1) * P + 16 * lo);
       l0[i] = v_at(row, 2 * grp);
-      grp0[i] = __builtin_amdgcn_readfirstlane(grp - lo);
+      grp0[i] = ((64 * wave + NT * i - NK) >> ql) / HDP << ql;
     }
   }
-  // (pieces of keys come first; a wave's i-th pieces are all of one kind)
-  auto of_keys = [&](int i) { return wave * 64 + NT * i < NK; };
 
   // (the last rows first: with causal masks they have the most keys)
   for (int tile = a.tiles - 1 - it.item / a.splits; long(tile) * RB < w.rows; tile += a.tiles) {
@@ -702,11 +702,8 @@ __global__ void __launch_bounds__(256, DT == F32 || HDP > 128 ? 1 : 2) attn_page
     }
 
     // ---- the loader.  Every load is made, at an address that exists (see above).
-    auto page_of = [&](int base, int grp) {
-      const int p = table[min(base + 16 * grp, mine.hi - 1) >> a.plog];
-      return page_in_pool(p, a.n_pages) ? p : -1;
-    };
-    int page[CH], ipage = -1, holes = 0;  // holes: pieces of the fetched block whose page is outside the pool
+    int page[CH], ipage = -1;  // of the block asked for
+    int ip = -1, holes = 0;    // of the block fetched; holes: pieces whose page is outside the pool
     const int last = __builtin_amdgcn_readfirstlane(mine.hi) - 1;
     const auto table_s = scalar_ptr(table);
     uint4 raw[CH];
@@ -714,24 +711,27 @@ __global__ void __launch_bounds__(256, DT == F32 || HDP > 128 ? 1 : 2) attn_page
     auto ask = [&](int base) {  // pages of the block
 #pragma unroll
       for (int i = 0; i < CH; ++i) page[i] = table_s[min(base + 16 * grp0[i], last) >> a.plog];
-      if (wave == 0) ipage = page_of(base, tid & 3);
+      if (wave == 0) ipage = table[min(base + 16 * (tid & 3), last) >> a.plog];
     };
     auto fetch = [&](int base) {  // its bytes and scales
       holes = 0;
+      ip = page_in_pool(ipage, a.n_pages) ? ipage : -1;
 #pragma unroll
       for (int i = 0; i < CH; ++i) {
         const bool in = page_in_pool(page[i], a.n_pages);
         const int p = in ? page[i] : 0, at = (base + 16 * grp0[i]) & (P - 1);
         if (!in) holes |= 1 << i;
         const uint8_t *from = (of_keys(i) ? kc + at * a.hd : vc + at) + p * stride;
-        raw[i] = *reinterpret_cast<const uint4 *>(from + off[i]);
+        uint32_t o = off[i];
+        asm volatile("" : "+v"(o));  // (a scalar address and 32 bits, not a 64-bit sum kept for each piece)
+        raw[i] = *reinterpret_cast<const uint4 *>(from + o);
       }
       if (wave == 0) {
-        isc = a.ks[long(max(ipage, 0)) * a.Hkv + w.kvh];
-        ivs = a.vs[long(max(ipage, 0)) * a.Hkv + w.kvh];
+        isc = a.ks[long(max(ip, 0)) * a.Hkv + w.kvh];
+        ivs = a.vs[long(max(ip, 0)) * a.Hkv + w.kvh];
       }
     };
-    auto place = [&](int base, int ip, int buf) {  // into LDS as fp16
+    auto place = [&](int base, int buf) {  // into LDS as fp16
       uint32_t any = 0;
       if (base < all_lo || base + kKeyBlock > all_hi || holes) {
 #pragma unroll
@@ -776,19 +776,19 @@ __global__ void __launch_bounds__(256, DT == F32 || HDP > 128 ? 1 : 2) attn_page
       const int first = mine.lo & ~(kKeyBlock - 1);
       ask(first);
       fetch(first);
-      int ip = ipage;
       ask(first + kKeyBlock);
-      place(first, ip, 0);
+      place(first, 0);
+      if (first + kKeyBlock < mine.hi) fetch(first + kKeyBlock);
+      ask(first + 2 * kKeyBlock);
       __syncthreads();
       int buf = 0;
       for (int base = first; base < mine.hi; base += kKeyBlock, buf ^= 1) {
-        const bool more = base + kKeyBlock < mine.hi;
-        ip = ipage;
+        // The next block into LDS, and the one behind it on its way: its bytes have
+        // the whole of this block to arrive (TODO).
+        if (base + kKeyBlock < mine.hi) place(base + kKeyBlock, buf ^ 1);
+        if (base + 2 * kKeyBlock < mine.hi) fetch(base + 2 * kKeyBlock);
         const bool busy = on && base < some.hi && base + kKeyBlock > some.lo;
-        if (more && !busy) {
-          fetch(base + kKeyBlock);
-          ask(base + 2 * kKeyBlock);
-        }
+        if (!busy) ask(base + 3 * kKeyBlock);
         if (busy) {
           // LDS bytes of this lane's first operands; the chunks of a row differ in an
           // exclusive or (hidden from the compiler, which would keep every sum)
@@ -803,34 +803,27 @@ __global__ void __launch_bounds__(256, DT == F32 || HDP > 128 ? 1 : 2) attn_page
             for (int j = 0; j < 16; ++j) s[t][j] = 0.f;
           // Operands are read two steps ahead of their products (left alone, the
           // compiler reads one, waits, multiplies: 1.2 of 3 us a block).
-          f16x8 kf[2][2][2];
-          auto read_keys = [&](int b) {
+          f16x8 kf[3][2];
+          auto read_keys = [&](int c) {
 #pragma unroll
-            for (int c = 0; c < 2; ++c)
-#pragma unroll
-              for (int t = 0; t < 2; ++t)
-                kf[b & 1][c][t] = *reinterpret_cast<const f16x8 *>(lds[0] + (at_k ^ (32 * (2 * b + c))) + 32 * t * KROW);
+            for (int t = 0; t < 2; ++t)
+              kf[c % 3][t] = *reinterpret_cast<const f16x8 *>(lds[0] + (at_k ^ (32 * c)) + 32 * t * KROW);
           };
           read_keys(0);
+          read_keys(1);
 #pragma unroll
-          for (int b = 0; b < KS / 2; ++b) {
-            if (b + 1 < KS / 2) read_keys(b + 1);
+          for (int c = 0; c < KS; ++c) {
+            if (c + 2 < KS) read_keys(c + 2);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int c = 0; c < 2; ++c)
+            for (int t = 0; t < 2; ++t)
 #pragma unroll
-              for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int p = NP - 1; p >= 0; --p)
-                  s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[b & 1][c][t], qf[p][2 * b + c], s[t], 0, 0, 0);
+              for (int p = NP - 1; p >= 0; --p)
+                s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[c % 3][t], qf[p][c], s[t], 0, 0, 0);
           }
-          // (here, where the operands of the scores have left their registers; and
-          // scalar loads where no LDS read is on its way: the two share a counter and
+          // (scalar loads, where no LDS read is on its way: the two share a counter and
           // come back in any order)
-          if (more) {
-            fetch(base + kKeyBlock);
-            ask(base + 2 * kKeyBlock);
-          }
+          ask(base + 3 * kKeyBlock);
           float lv[2] = {in[0].y, in[1].y}, lv_top = in[0].w;
           const bool ok0 = in[0].z != 0.f, ok1 = in[1].z != 0.f;
           auto seen = [&](int t) -> uint32_t {  // bit i: this row sees key 32 t + 16 h + i
@@ -947,7 +940,6 @@ __global__ void __launch_bounds__(256, DT == F32 || HDP > 128 ? 1 : 2) attn_page
                 if (nan_at[buf][32 * i + 8 * (j >> 2) + 4 * h + (j & 3)] & sees) acc[i][j] = __builtin_nanf("");
           }
         }
-        if (more) place(base + kKeyBlock, ip, buf ^ 1);
         __syncthreads();
       }
     }
