@@ -221,8 +221,8 @@ int mh_attention_textbook(int dt, const void *q, const void *k, const void *v, v
  * those that mh_kv_store_paged writes are powers of two.  A slot is
  * page number * page + place.  A request's pages are its row of the block
  * table [B][width]: token t lies in page table[t / page], place t % page.
- * hd is a multiple of 16, at most 256; n_pages * page and width * page are
- * below 2^31.  Caches are 16-byte aligned.
+ * hd is a multiple of 16, at most 256; n_pages * page is below 2^31, width * page
+ * at most 2^31 - 4096.  Caches are 16-byte aligned.
  * Device-side data that cannot be checked on the host never leads outside the
  * buffers: what is done instead is said below, and mh_check_device_errors
  * reports it.  None of these calls allocates; all may be captured into graphs

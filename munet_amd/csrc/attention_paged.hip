@@ -567,9 +567,13 @@ __global__ void __launch_bounds__(256) attn_paged_kernel(PagedArgs a) {
 // of 16 rows find them in different banks: chunk c of a row of 256 bytes or more
 // lies at c ^ (row & 15), of 128 bytes (values: a head value's 64 keys) at c ^
 // (row / 2 & 7).
+// ONE: pages of 64 tokens or more, where a block lies in one: one page number, two
+// addresses and two scales, scalars that each wave has.  With smaller pages the first
+// wave puts the runs' scales into LDS for the others, who wait for it (6 prompts of
+// 1200 to 8000 tokens, 32 heads on 8 of 128, pages of 64: 622 us so, 561 with ONE).
 // Registers bound the waves: 64 outputs, 32 of q and 32 scores a lane at hd 128
 // leave two waves to a SIMD; fp32 and heads above 128 take all registers for one.
-template <int DT, int HDP>
+template <int DT, int HDP, bool ONE>
 __global__ void __launch_bounds__(256, DT == F32 || HDP > 128 ? 1 : 2) attn_paged_wide_kernel(PagedArgs a) {
   typedef typename Store<DT>::T T;
   constexpr int NT = 256, NW = 4, RW = 32, RB = NW * RW;
@@ -634,9 +638,9 @@ __global__ void __launch_bounds__(256, DT == F32 || HDP > 128 ? 1 : 2) attn_page
     const int e = tid + NT * i;
     if (of_keys(i)) {
       const int row = e / XK, x = e % XK, k = row & 15, R = (row & 32) + 8 * (k >> 2) + 4 * ((row >> 4) & 1) + (k & 3);
-      off[i] = uint32_t(k * a.hd + min(16 * x, a.hd - 16));
-      l0[i] = k_at(R, 2 * x);
       grp0[i] = (64 * wave + NT * i) / (16 * XK);
+      off[i] = uint32_t((ONE ? row : k) * a.hd + min(16 * x, a.hd - 16));
+      l0[i] = k_at(R, 2 * x);
     } else {
       int row, grp;
       const int lo = value_piece(i, row, grp);
@@ -708,25 +712,56 @@ __global__ void __launch_bounds__(256, DT == F32 || HDP > 128 ? 1 : 2) attn_page
     const auto table_s = scalar_ptr(table);
     uint4 raw[CH];
     float isc = 0.f, ivs = 0.f;
+    const auto ks_s = scalar_ptr(reinterpret_cast<const int32_t *>(a.ks)), vs_s = scalar_ptr(reinterpret_cast<const int32_t *>(a.vs));
+    int p_far = -1, p_near = -1;        // (one page a block) pages of the block fetched, of the block before it
+    float ks_next = 0.f, vs_next = 0.f;  // scales of the block that comes next
     auto ask = [&](int base) {  // pages of the block
+      if constexpr (ONE) {
+        page[0] = table_s[uint32_t(min(base, last)) >> a.plog];
+      } else {
 #pragma unroll
-      for (int i = 0; i < CH; ++i) page[i] = table_s[min(base + 16 * grp0[i], last) >> a.plog];
-      if (wave == 0) ipage = table[min(base + 16 * (tid & 3), last) >> a.plog];
+        for (int i = 0; i < CH; ++i) page[i] = table_s[uint32_t(min(base + 16 * grp0[i], last)) >> a.plog];
+        if (wave == 0) ipage = table[uint32_t(min(base + 16 * (tid & 3), last)) >> a.plog];
+      }
+    };
+    auto ask_scales = [&]() {  // of the block before the one that was fetched last
+      if constexpr (ONE) {
+        const int64_t at = int64_t(max(p_near, 0)) * a.Hkv + w.kvh;
+        ks_next = __int_as_float(ks_s[at]);
+        vs_next = __int_as_float(vs_s[at]);
+      }
+    };
+    auto load_piece = [&](int i, const uint8_t *from) {
+      uint32_t o = off[i];
+      asm volatile("" : "+v"(o));  // (a scalar address and 32 bits, not a 64-bit sum kept for each piece)
+      raw[i] = *reinterpret_cast<const uint4 *>(from + o);
     };
     auto fetch = [&](int base) {  // its bytes and scales
       holes = 0;
-      ip = page_in_pool(ipage, a.n_pages) ? ipage : -1;
+      if constexpr (ONE) {
+        const bool in = page_in_pool(page[0], a.n_pages);
+        p_near = p_far;
+        p_far = __builtin_amdgcn_readfirstlane(in ? page[0] : -1);
+        const int at = base & (P - 1);
+        const int64_t from = (in ? page[0] : 0) * stride;
+        const uint8_t *const kb = kc + from + at * a.hd, *const vb = vc + from + at;
+#pragma unroll
+        for (int i = 0; i < CH; ++i) load_piece(i, of_keys(i) ? kb : vb);
+        if (!in) {
+          holes = -1;
+          if (tid == 0) atomicOr(a.err, kErrPage);
+        }
+        return;
+      }
 #pragma unroll
       for (int i = 0; i < CH; ++i) {
         const bool in = page_in_pool(page[i], a.n_pages);
         const int p = in ? page[i] : 0, at = (base + 16 * grp0[i]) & (P - 1);
         if (!in) holes |= 1 << i;
-        const uint8_t *from = (of_keys(i) ? kc + at * a.hd : vc + at) + p * stride;
-        uint32_t o = off[i];
-        asm volatile("" : "+v"(o));  // (a scalar address and 32 bits, not a 64-bit sum kept for each piece)
-        raw[i] = *reinterpret_cast<const uint4 *>(from + o);
+        load_piece(i, (of_keys(i) ? kc + at * a.hd : vc + at) + p * stride);
       }
       if (wave == 0) {
+        ip = page_in_pool(ipage, a.n_pages) ? ipage : -1;
         isc = a.ks[long(max(ip, 0)) * a.Hkv + w.kvh];
         ivs = a.vs[long(max(ip, 0)) * a.Hkv + w.kvh];
       }
@@ -760,7 +795,7 @@ __global__ void __launch_bounds__(256, DT == F32 || HDP > 128 ? 1 : 2) attn_page
         *reinterpret_cast<f16x8 *>(&lds[buf][l0[i] ^ 16]) = cvt8(raw[i].z, raw[i].w);
       }
       if (lane == 0) dirty[buf][wave] = any;
-      if (wave == 0) {
+      if (!ONE && wave == 0) {
         const float lv = ip >= 0 ? fmaxf(__builtin_amdgcn_logf(ivs), -126.f) : -126.f;
         float m = lv;
         m = fmaxf(m, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(m), 0xb1, 0xf, 0xf, false)));  // quad [1,0,3,2]
@@ -778,31 +813,45 @@ __global__ void __launch_bounds__(256, DT == F32 || HDP > 128 ? 1 : 2) attn_page
       fetch(first);
       ask(first + kKeyBlock);
       place(first, 0);
-      if (first + kKeyBlock < mine.hi) fetch(first + kKeyBlock);
+      fetch(first + kKeyBlock);
+      ask_scales();
       ask(first + 2 * kKeyBlock);
       __syncthreads();
       int buf = 0;
       for (int base = first; base < mine.hi; base += kKeyBlock, buf ^= 1) {
         // The next block into LDS, and the one behind it on its way: its bytes have
-        // the whole of this block to arrive (TODO).
+        // the whole of this block to arrive (loaded after the scores and placed behind the
+        // values' product, 672 us where this took 660).
+        const float ks_now = ks_next, vs_now = vs_next;
+        const bool ok_now = p_near >= 0;
         if (base + kKeyBlock < mine.hi) place(base + kKeyBlock, buf ^ 1);
-        if (base + 2 * kKeyBlock < mine.hi) fetch(base + 2 * kKeyBlock);
+        fetch(base + 2 * kKeyBlock);
         const bool busy = on && base < some.hi && base + kKeyBlock > some.lo;
-        if (!busy) ask(base + 3 * kKeyBlock);
+        if (!busy) {
+          ask_scales();
+          ask(base + 3 * kKeyBlock);
+        }
         if (busy) {
           // LDS bytes of this lane's first operands; the chunks of a row differ in an
           // exclusive or (hidden from the compiler, which would keep every sum)
           uint32_t at_k = uint32_t(buf) * (KB + VB) + k_at(n, h), at_v = uint32_t(buf) * (KB + VB) + v_at(n, 2 * h);
           asm volatile("" : "+v"(at_k), "+v"(at_v));
           // this lane half's two runs of keys: 16 h of either tile
-          const float4 in[2] = {info[buf][h], info[buf][2 + h]};
+          float4 in[2];
+          if constexpr (ONE) {
+            const float lv = ok_now ? fmaxf(__builtin_amdgcn_logf(vs_now), -126.f) : -126.f;
+            in[0] = in[1] = make_float4(ks_now, lv, ok_now ? 1.f : 0.f, lv);
+          } else {
+            in[0] = info[buf][h];
+            in[1] = info[buf][2 + h];
+          }
           f32x16 s[2];
 #pragma unroll
           for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int j = 0; j < 16; ++j) s[t][j] = 0.f;
           // Operands are read two steps ahead of their products (left alone, the
-          // compiler reads one, waits, multiplies: 1.2 of 3 us a block).
+          // compiler reads one, waits, multiplies).
           f16x8 kf[3][2];
           auto read_keys = [&](int c) {
 #pragma unroll
@@ -823,6 +872,7 @@ __global__ void __launch_bounds__(256, DT == F32 || HDP > 128 ? 1 : 2) attn_page
           }
           // (scalar loads, where no LDS read is on its way: the two share a counter and
           // come back in any order)
+          ask_scales();
           ask(base + 3 * kKeyBlock);
           float lv[2] = {in[0].y, in[1].y}, lv_top = in[0].w;
           const bool ok0 = in[0].z != 0.f, ok1 = in[1].z != 0.f;
@@ -1013,7 +1063,10 @@ hipError_t launch(const PagedArgs &a, const PagedShape &s, hipStream_t st) {
   if (blocks * 512 > 0xffffffffL) return hipErrorInvalidValue;
   const dim3 grid{unsigned(blocks)};
   if (s.wide)
-    hipLaunchKernelGGL((attn_paged_wide_kernel<DT, HDP>), grid, dim3(256), 0, st, a);
+    if (a.plog >= 6)
+      hipLaunchKernelGGL((attn_paged_wide_kernel<DT, HDP, true>), grid, dim3(256), 0, st, a);
+    else
+      hipLaunchKernelGGL((attn_paged_wide_kernel<DT, HDP, false>), grid, dim3(256), 0, st, a);
   else
     hipLaunchKernelGGL((attn_paged_kernel<DT, HDP>), grid, dim3(256), 0, st, a);
   hipError_t e = hipGetLastError();

@@ -587,7 +587,7 @@ int mh_page_plan(const int32_t *lens, const int32_t *new_lens, const int32_t *fr
     check_page("page_plan", page, n_pages);
     if (B < 0 || n_free < 0 || width < 0 || n_slots < 0) throw Error("page_plan: negative size");
     if (B >= 1 << 24) throw Error("page_plan: more requests than one launch takes (2^24 - 1)");
-    if (int64_t(width) * page > 0x7fffffff) throw Error("page_plan: a table row must hold at most 2^31 - 1 tokens");
+    if (int64_t(width) * page > kPagedMaxKeys) throw Error("page_plan: a table row must hold at most 2^31 - 4096 tokens");
     if (B == 0) return 0;
     if (!lens || !new_lens || !total_lens || !cu || !used || (width && !tables) || (n_free && !free_pages) ||
         (n_slots && !slots))
@@ -644,8 +644,8 @@ int mh_attention_paged(int dt, const void *q, int64_t ldq, const void *k_cache, 
   MH_TRY({
     const PagedShape s = paged_call_shape(dt, B, n_rows, Hq, Hkv, hd, max_q, max_len, window);
     check_pool("attention_paged", k_cache, v_cache, k_scale, v_scale, Hkv, hd, page, n_pages);
-    if (width < 0 || int64_t(width) * page > 0x7fffffff)
-      throw Error("attention_paged: a table row must hold at most 2^31 - 1 tokens");
+    if (width < 0 || int64_t(width) * page > kPagedMaxKeys)
+      throw Error("attention_paged: a table row must hold at most 2^31 - 4096 tokens");
     if (!(std::fabs(scale) <= 3.4e38f)) throw Error("attention_paged: the scale must be finite");
     if (B == 0 || n_rows == 0) return 0;
     if (!lens || !cu || (width && !tables)) throw Error("attention_paged: null argument");

@@ -109,6 +109,9 @@ __host__ __device__ __forceinline__ PairItem pair_item(uint32_t i, int pairs, in
   return r;
 }
 
+// Tokens of a table row: the kernels look a few blocks past the last one in 32 bits.
+constexpr int kPagedMaxKeys = 0x7fffffff - 4095;
+
 // How a call is cut: rows of one (sequence, key/value head) in tiles, and each
 // tile's keys in `splits` shares of `chunk`.
 struct PagedShape {

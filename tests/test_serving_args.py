@@ -35,7 +35,7 @@ def _plan(**kw):
 @pytest.mark.parametrize("kw,match", [
     (dict(page=48), "16, 32, 64, 128 or 256"), (dict(page=8), "16, 32"), (dict(page=512), "16, 32"),
     (dict(n_pages=0), "pool"), (dict(n_pages=1 << 27), "pool"), (dict(B=-1), "negative"), (dict(width=-2), "negative"),
-    (dict(n_slots=-1), "negative"), (dict(width=1 << 27), "table row"), (dict(lens=None), "null"), (dict(used=None), "null"),
+    (dict(n_slots=-1), "negative"), (dict(width=1 << 27), "table row"), (dict(width=(1 << 27) - 1), "table row"), (dict(lens=None), "null"), (dict(used=None), "null"),
     (dict(slots=None), "null"), (dict(tables=None), "null"), (dict(free_pages=None), "null"), (dict(B=1 << 24), "one launch")])
 def test_page_plan_refusals(kw, match):
     with pytest.raises(_lib.HipError, match=match):
@@ -70,7 +70,7 @@ def _attend(**kw):
     (dict(dt=4), "dtype"), (dict(Hq=15), "multiple of key/value heads"), (dict(hd=136), "multiple of 16"), (dict(page=0), "page holds"),
     (dict(q=None), "null q"), (dict(out=A + 2), "aligned"), (dict(ldq=2047), "multiple of 16"), (dict(ldo=1024), "whole"),
     (dict(B=-1), "negative"), (dict(window=-1), "negative"), (dict(max_len=-5), "negative"), (dict(lens=None), "null"),
-    (dict(cu=None), "null"), (dict(tables=None), "null"), (dict(width=1 << 26), "table row"), (dict(scale=float("nan")), "finite"),
+    (dict(cu=None), "null"), (dict(tables=None), "null"), (dict(width=1 << 26), "table row"), (dict(width=(1 << 25) - 1), "table row"), (dict(scale=float("nan")), "finite"),
     (dict(scale=float("inf")), "finite"), (dict(n_rows=1 << 29), "2\\^30"), (dict(max_len=100000), "workspace"),
     (dict(max_len=100000, ws=A, nbytes=100), "workspace"), (dict(max_len=100000, ws=A + 8, nbytes=1 << 40), "aligned")])
 def test_attention_paged_refusals(kw, match):
