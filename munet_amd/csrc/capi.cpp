@@ -592,6 +592,24 @@ int mh_page_plan(const int32_t *lens, const int32_t *new_lens, const int32_t *fr
     if (!lens || !new_lens || !total_lens || !cu || !used || (width && !tables) || (n_free && !free_pages) ||
         (n_slots && !slots))
       throw Error("page_plan: null argument");
+    {  // (requests read those before them while others write)
+      struct Range {
+        const void *at;
+        int64_t n;
+      };
+      const Range in[] = {{lens, B}, {new_lens, B}, {free_pages, n_free}},
+                  out[] = {{tables, int64_t(B) * width}, {total_lens, B}, {cu, int64_t(B) + 1}, {slots, n_slots}, {positions, n_slots}, {used, 1}};
+      auto meet = [](const Range &x, const Range &y) {
+        const uintptr_t a = reinterpret_cast<uintptr_t>(x.at), b = reinterpret_cast<uintptr_t>(y.at);
+        return a && b && a < b + 4 * uintptr_t(y.n) && b < a + 4 * uintptr_t(x.n);
+      };
+      for (const Range &o : out) {
+        for (const Range &i : in)
+          if (meet(o, i)) throw Error("page_plan: an output overlaps an input");
+        for (const Range &other : out)
+          if (&other != &o && meet(o, other)) throw Error("page_plan: two outputs overlap");
+      }
+    }
     PagePlan p;
     p.lens = lens;
     p.fresh = new_lens;

@@ -429,6 +429,20 @@ def test_value_scales_far_apart(torch, hip, spread):
     check(torch, hip, Cache(torch, 2, 64, 16, [200, 90], [1, 30], spread=spread, seed=4), 4, "bfloat16", what="value scales")
 
 
+@pytest.mark.parametrize("P", [32, 64, 128])
+@pytest.mark.parametrize("dtype,hd", [("bfloat16", 128), ("float32", 64), ("float16", 256)])
+def test_prompts_over_pages_outside_the_pool(torch, hip, P, dtype, hd):
+    """Prompts whose blocks lie in one page each and in several, some pages missing, scales far apart."""
+    from munet_amd._lib import HipError
+    c = Cache(torch, 2, hd, P, [700, 333, 64], [200, 333, 40], spread=4.0 if dtype == "float16" else 40.0, seed=P)
+    c.tables[0][2], c.tables[0][-1], c.tables[1][0] = -1, c.n_pages + 5, 2 ** 31 - 1
+    c.sync(torch)
+    hip.check_device_errors()
+    check(torch, hip, c, 4, dtype, what="prompts, bad pages")
+    with pytest.raises(HipError, match="paged KV cache"):
+        hip.check_device_errors()
+
+
 def test_pages_outside_the_pool_hold_no_keys(torch, hip):
     from munet_amd._lib import HipError
     c = Cache(torch, 2, 64, 16, [100, 40], [1, 30], seed=6)

@@ -42,6 +42,17 @@ def test_page_plan_refusals(kw, match):
         _plan(**kw)
 
 
+def test_page_plan_refuses_operands_that_overlap():
+    """Lengths updated in place, outputs inside one another."""
+    apart = dict(lens=A, new_lens=A + 64, free_pages=A + 128, tables=A + 256, total=A + 512, cu=A + 576, slots=A + 640,
+                 positions=A + 704, used=A + 768)
+    for kw, match in ((dict(total=A), "an input"), (dict(total=A + 12), "an input"), (dict(slots=A + 64 - 36), "an input"),
+                      (dict(used=A + 128 + 28), "an input"), (dict(positions=A + 640), "two outputs"), (dict(cu=A + 512 - 16), "two outputs"),
+                      (dict(tables=A + 512 - 60), "two outputs")):
+        with pytest.raises(_lib.HipError, match=match):
+            _plan(**{**apart, **kw})
+
+
 def _store(**kw):
     a = dict(dt=BF16, k=A, v=A, ldk=1024, ldv=1024, slots=A, kc=A, vc=A, ks=A, vs=A, n=4, Hkv=8, hd=128, page=64, n_pages=16)
     a.update(kw)
