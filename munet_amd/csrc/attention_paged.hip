@@ -21,8 +21,8 @@
 // page and take one key scale and one value scale.
 //
 // Precision: e4m3 converts to fp16 exactly.  A row of q is scaled by a power of
-// two to below 2^14 and is then exact in fp16 for bf16 and fp16 inputs (down to
-// 2^-38 of the row's largest value); fp32 inputs are the sum of two fp16 parts
+// two to below 2^14 and is then exact in fp16 for bf16 and fp16 inputs (but for at
+// most 2^-38 of the row's largest value); fp32 inputs are the sum of two fp16 parts
 // (22 bits and a sign).  Scores, the running maximum, the sum and the outputs are
 // fp32.  A probability enters the second product as 2^9 w times its page's value
 // scale over the largest one that the row has seen, rounded to fp16 (half a unit
@@ -569,8 +569,9 @@ __global__ void __launch_bounds__(256) attn_paged_kernel(PagedArgs a) {
 // (row / 2 & 7).
 // ONE: pages of 64 tokens or more, where a block lies in one: one page number, two
 // addresses and two scales, scalars that each wave has.  With smaller pages the first
-// wave puts the runs' scales into LDS for the others, who wait for it (6 prompts of
-// 1200 to 8000 tokens, 32 heads on 8 of 128, pages of 64: 622 us so, 561 with ONE).
+// wave puts the runs' scales into LDS for the others, who wait for it (6 chunks
+// of 6700 tokens in all that end at 1200 to 8000 keys, 32 heads on 8 of 128, pages of
+// 64: 622 us so, 561 with ONE).
 // Registers bound the waves: 64 outputs, 32 of q and 32 scores a lane at hd 128
 // leave two waves to a SIMD; fp32 and heads above 128 take all registers for one.
 template <int DT, int HDP, bool ONE>

@@ -88,9 +88,9 @@ inline int store_tokens(int n, int heads) { return int(std::min<int64_t>(64, std
 // Workgroup i of a launch over `pairs` (sequence, key/value head) pairs of `per`
 // items each.  Workgroups go round the eight XCDs, each with an L2 of its own:
 // eight pairs at a time, one to an XCD, so that the items that read the same
-// keys find them there (6 requests of 8000 tokens, 8 heads: 1029 us with a pair's
-// items in any XCD and items of all pairs at once, 820 with one pair's items
-// after another over all XCDs).  The pairs left over go round all of them.
+// keys find them there (6 chunks of prompts, 8 heads, when this was chosen: 816 us; a
+// pair's items after another over all XCDs 820, all pairs' first items, then all
+// second ones 1029).  The pairs left over go round all of them.
 constexpr int kXcds = 8;
 struct PairItem {
   int pair, item;
