@@ -255,7 +255,7 @@ int mh_page_plan(const int32_t *lens, const int32_t *new_lens, const int32_t *fr
  * page's first token is among them, else the larger of e and the scale held,
  * and if it grows the page's earlier tokens are rounded to it; values are
  * rounded to the nearest e4m3, ties to even.  Infinities and NaN become NaN and do not
- * count towards the magnitude.  n is at most 2^29, Hkv 65535. */
+ * count towards the magnitude.  n is at most 2^27, Hkv 65535. */
 int mh_kv_store_paged(int dt, const void *k, const void *v, int64_t ldk, int64_t ldv, const int32_t *slots,
                       void *k_cache, void *v_cache, float *k_scale, float *v_scale, int n, int Hkv, int hd, int page,
                       int n_pages, void *stream);

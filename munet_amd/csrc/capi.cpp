@@ -636,7 +636,7 @@ int mh_kv_store_paged(int dt, const void *k, const void *v, int64_t ldk, int64_t
     check_dt(dt);
     check_pool("kv_store_paged", k_cache, v_cache, k_scale, v_scale, Hkv, hd, page, n_pages);
     if (n < 0) throw Error("kv_store_paged: negative size");
-    if (n > 1 << 29) throw Error("kv_store_paged: more tokens than one launch takes (2^29)");
+    if (n > 1 << 27) throw Error("kv_store_paged: more tokens than one launch takes (2^27)");
     if (n == 0) return 0;
     if (!slots) throw Error("kv_store_paged: null slots");
     check_rows("kv_store_paged", "k", dt, k, ldk, int64_t(Hkv) * hd);

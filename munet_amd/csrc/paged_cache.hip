@@ -169,13 +169,14 @@ struct StoreArgs {
 // workgroup that holds a run's first token writes all of it for one head, and
 // so owns the page's two scales.  Tokens at `per` consecutive places per
 // workgroup.
-template <int DT>
-__global__ void __launch_bounds__(256) kv_store_paged_kernel(StoreArgs a) {
+template <int DT, int NT>
+__global__ void __launch_bounds__(NT) kv_store_paged_kernel(StoreArgs a) {
   typedef typename Store<DT>::T T;
   constexpr int VT = 64;  // tokens of a value tile
-  __shared__ float red[2][4];
+  constexpr int NW = NT / 64;
+  __shared__ float red[2][NW];
   // (rows of VT + 4 bytes; of the run's quads in the short form)
-  __shared__ __align__(16) uint8_t vt[kPagedHeadMax * (VT + 4)];
+  __shared__ __align__(16) uint8_t vt[NT == 256 ? kPagedHeadMax * (VT + 4) : 32 * NT + 4 * kPagedHeadMax];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, head = blockIdx.y;
   const int t0 = blockIdx.x * a.per, hd = a.hd, P = a.page, h8 = hd / 8;
   const int64_t limit = int64_t(a.n_pages) * P;
@@ -212,12 +213,12 @@ __global__ void __launch_bounds__(256) kv_store_paged_kernel(StoreArgs a) {
     const T *vp = static_cast<const T *>(a.v) + int64_t(t) * a.ldv + int64_t(head) * hd;
     uint8_t *kd = a.kc + page_base(page, a.Hkv, head, P, hd), *vd = a.vc + page_base(page, a.Hkv, head, P, hd);
 
-    // A run of at most 256 pieces of 4 places and 8 head values (64 tokens of heads of
-    // 128) is held in registers, a piece to a thread: loaded once, its values
+    // A run of at most NT pieces of 4 places and 8 head values (NT 256: 64 tokens of
+    // heads of 128) is held in registers, a piece to a thread: loaded once, its values
     // transposed four places at a time (17k tokens, 8 heads of 128: 39 us, against 44
     // with two passes over memory and single bytes).
     const int q0 = place / 4, nq = (place + n - 1) / 4 - q0 + 1;
-    const bool held_run = nq * h8 <= 256;
+    const bool held_run = nq * h8 <= NT;
     const int pq = tid / h8, pd = 8 * (tid - pq * h8), pi = 4 * (q0 + pq) - place;  // this thread's piece: first token
     const bool mine = held_run && pq < nq;
     Raw<DT> kr[4], vr[4];
@@ -238,7 +239,7 @@ __global__ void __launch_bounds__(256) kv_store_paged_kernel(StoreArgs a) {
         big[1] = amax8(v, big[1]);
       }
     }
-    for (int c = held_run ? n * h8 : tid; c < n * h8; c += 256) {
+    for (int c = held_run ? n * h8 : tid; c < n * h8; c += NT) {
       const int i = c / h8, d = 8 * (c - i * h8);
       float v[8];
       ld8<DT>(kp + int64_t(i) * a.ldk + d, v);
@@ -255,7 +256,10 @@ __global__ void __launch_bounds__(256) kv_store_paged_kernel(StoreArgs a) {
     __syncthreads();
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-      const float want = e4m3_scale(fmaxf(fmaxf(red[x][0], red[x][1]), fmaxf(red[x][2], red[x][3])));
+      float top = red[x][0];
+#pragma unroll
+      for (int v = 1; v < NW; ++v) top = fmaxf(top, red[x][v]);
+      const float want = e4m3_scale(top);
       const bool keep = place > 0 && held[x] > want && held[x] < __builtin_inff();
       now[x] = keep ? held[x] : want;
       inv[x] = 1.0f / now[x];
@@ -263,7 +267,7 @@ __global__ void __launch_bounds__(256) kv_store_paged_kernel(StoreArgs a) {
     }
     // the page's earlier tokens in the larger scale
     if (ratio[0] != 1.f)
-      for (int c = tid; c < place * hd / 16; c += 256) {
+      for (int c = tid; c < place * hd / 16; c += NT) {
         uint4 *p = reinterpret_cast<uint4 *>(kd) + c;
         const uint4 w = *p;
         *p = make_uint4(rescale4(w.x, ratio[0]), rescale4(w.y, ratio[0]), rescale4(w.z, ratio[0]), rescale4(w.w, ratio[0]));
@@ -272,7 +276,7 @@ __global__ void __launch_bounds__(256) kv_store_paged_kernel(StoreArgs a) {
       // (whole 16-byte pieces of a row: what lies behind the earlier tokens is
       // kept, or written by the run below)
       const int pieces = (place + 15) / 16;
-      for (int c = tid; c < hd * pieces; c += 256) {
+      for (int c = tid; c < hd * pieces; c += NT) {
         const int d = c / pieces, i = c - d * pieces;
         uint4 *p = reinterpret_cast<uint4 *>(vd + int64_t(d) * P + 16 * i);
         const uint4 w = *p;
@@ -318,7 +322,7 @@ __global__ void __launch_bounds__(256) kv_store_paged_kernel(StoreArgs a) {
       }
       __syncthreads();
       const int lo = place, hi = place + n, first = lo & ~15, pieces = (hi + 15) / 16 - lo / 16;
-      for (int c = tid; c < hd * pieces; c += 256) {
+      for (int c = tid; c < hd * pieces; c += NT) {
         const int d = c / pieces, at = first + 16 * (c - d * pieces);
         const uint8_t *src = &vt[d * rs] + (at - 4 * q0);  // (before the row where the run starts inside the piece)
         uint8_t *dst = vd + int64_t(d) * P + at;
@@ -337,7 +341,7 @@ __global__ void __launch_bounds__(256) kv_store_paged_kernel(StoreArgs a) {
       continue;
     }
     // keys, in their rows
-    for (int c = tid; c < n * h8; c += 256) {
+    for (int c = tid; c < n * h8; c += NT) {
       const int i = c / h8, d = 8 * (c - i * h8);
       float v[8];
       ld8<DT>(kp + int64_t(i) * a.ldk + d, v);
@@ -348,7 +352,7 @@ __global__ void __launch_bounds__(256) kv_store_paged_kernel(StoreArgs a) {
     // values, transposed through LDS in tiles of VT places
     for (int c0 = place & ~(VT - 1); c0 < place + n; c0 += VT) {
       const int lo = max(c0, place), hi = min(c0 + VT, place + n);
-      for (int c = tid; c < (hi - lo) * h8; c += 256) {
+      for (int c = tid; c < (hi - lo) * h8; c += NT) {
         const int i = c / h8, d = 8 * (c - i * h8);
         float v[8];
         ld8<DT>(vp + int64_t(lo - place + i) * a.ldv + d, v);
@@ -360,7 +364,7 @@ __global__ void __launch_bounds__(256) kv_store_paged_kernel(StoreArgs a) {
       }
       __syncthreads();
       const int first = lo & ~15, pieces = ((hi + 15) / 16) - lo / 16;
-      for (int c = tid; c < hd * pieces; c += 256) {
+      for (int c = tid; c < hd * pieces; c += NT) {
         const int d = c / pieces, at = first + 16 * (c - d * pieces);
         const uint32_t *src = reinterpret_cast<const uint32_t *>(&vt[d * (VT + 4) + at - c0]);
         uint8_t *dst = vd + int64_t(d) * P + at;
@@ -391,16 +395,28 @@ hipError_t page_plan(const PagePlan &p, int *err, hipStream_t st) {
 hipError_t kv_store_paged(int dt, const void *k, const void *v, long ldk, long ldv, const int32_t *slots, void *k_cache,
                           void *v_cache, float *k_scale, float *v_scale, int n, int Hkv, int hd, int page, int n_pages, int *err,
                           hipStream_t st) {
-  if (n < 1 || n > 1 << 29 || Hkv < 1 || Hkv > 65535) return hipErrorInvalidValue;
+  if (n < 1 || n > 1 << 27 || Hkv < 1 || Hkv > 65535) return hipErrorInvalidValue;
   StoreArgs a{k, v, slots, static_cast<uint8_t *>(k_cache), static_cast<uint8_t *>(v_cache), k_scale, v_scale, err, ldk, ldv,
               n, Hkv, hd, page, n_pages, store_tokens(n, Hkv)};
   const dim3 grid(unsigned((n + a.per - 1) / a.per), unsigned(Hkv));
+  // Threads for a page's pieces at once where workgroups take many tokens (17k
+  // tokens, 8 heads of 128: pages of 128 42 us, 56 with 256 threads; of 256 56, 60);
+  // where they take one, most would be idle.
+  const int pieces = page / 4 * (hd / 8), nt = a.per == 1 || pieces <= 256 ? 256 : pieces <= 512 ? 512 : 1024;
+#define MH_STORE(DTV)                                                                                     \
+  if (nt == 256)                                                                                          \
+    hipLaunchKernelGGL((kv_store_paged_kernel<DTV, 256>), grid, dim3(256), 0, st, a);                     \
+  else if (nt == 512)                                                                                     \
+    hipLaunchKernelGGL((kv_store_paged_kernel<DTV, 512>), grid, dim3(512), 0, st, a);                     \
+  else                                                                                                    \
+    hipLaunchKernelGGL((kv_store_paged_kernel<DTV, 1024>), grid, dim3(1024), 0, st, a);
   switch (dt) {
-  case F32: hipLaunchKernelGGL(kv_store_paged_kernel<F32>, grid, dim3(256), 0, st, a); break;
-  case F16: hipLaunchKernelGGL(kv_store_paged_kernel<F16>, grid, dim3(256), 0, st, a); break;
-  case BF16: hipLaunchKernelGGL(kv_store_paged_kernel<BF16>, grid, dim3(256), 0, st, a); break;
+  case F32: MH_STORE(F32) break;
+  case F16: MH_STORE(F16) break;
+  case BF16: MH_STORE(BF16) break;
   default: return hipErrorInvalidValue;
   }
+#undef MH_STORE
   return hipGetLastError();
 }
 

@@ -305,6 +305,26 @@ def test_kv_store(torch, hip, dtype, P, kv, hd, runs):
     _store(torch, hip, (rows[:, 0], rows[:, 1]), slots, cache, scales, P)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("P,hd", [(64, 128), (128, 128), (128, 80), (256, 64), (256, 128), (256, 256), (64, 256)])
+def test_kv_store_prompts(torch, hip, dtype, P, hd):
+    """Tokens enough for workgroups that look after several: whole pages, and parts of pages behind and before others."""
+    g, kv = torch.Generator().manual_seed(P + hd), 8
+    runs, pages = [(1, P - 3, 3), (2, 5, P // 2), (3, P // 4 + 1, 2)], 24
+    runs += [(p, 0, P) for p in range(4, 4 + 1024 // P)] + [(20, 0, P - 1), (21, 0, 1), (22, 13, P - 13)]
+    slots = []
+    for page, place, n in runs:
+        slots += [page * P + place + i for i in range(n)]
+    assert len(slots) * kv >= 8192
+    rows = torch.randn((len(slots), 2, kv, hd), generator=g)
+    rows *= torch.exp2(torch.randint(-3, 4, (len(slots), 1, 1, 1), generator=g).float())
+    rows = rows.to(getattr(torch, dtype)).cuda()
+    cache = [torch.randn((pages, kv, P, hd), generator=g).to(torch.float8_e4m3fn).view(torch.uint8) for _ in range(2)]
+    scales = [torch.exp2(torch.randint(-12, -2, (pages, kv), generator=g).float()) for _ in range(2)]
+    print(f"kv_store prompts {dtype} P {P} hd {hd}", flush=True)
+    _store(torch, hip, (rows[:, 0], rows[:, 1]), slots, cache, scales, P)
+
+
 def test_kv_store_rounds_every_value(torch, hip):
     """All fp16 values: ties, subnormals of e4m3, NaN and infinities, and each magnitude as its own page's largest."""
     bits = torch.arange(65536, dtype=torch.int32).to(torch.int16).view(torch.float16)

@@ -64,7 +64,7 @@ def _store(**kw):
     (dict(Hkv=0), "head count"), (dict(page=100), "page holds"), (dict(n=-1), "negative"), (dict(slots=None), "null"),
     (dict(k=None), "null k"), (dict(v=A + 8), "aligned"), (dict(ldk=1023), "multiple of 16"), (dict(ldv=1016), "whole"),
     (dict(kc=A + 4), "aligned"), (dict(vs=None), "null cache"), (dict(dt=F32, ldk=1026), "multiple of 16"),
-    (dict(n=(1 << 29) + 1), "one launch"), (dict(Hkv=65536), "head count")])
+    (dict(n=(1 << 27) + 1), "one launch"), (dict(Hkv=65536), "head count")])
 def test_kv_store_paged_refusals(kw, match):
     with pytest.raises(_lib.HipError, match=match):
         _store(**kw)
