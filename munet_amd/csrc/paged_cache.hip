@@ -9,9 +9,8 @@ namespace {
 
 // ---- page_plan ---------------------------------------------------------------
 
-// Exclusive sums over the requests before `b0` and the block's own 256: every
-// workgroup adds up the requests before its own instead of waiting for another
-// (8 bytes a request, from the caches; one launch).
+// Sums over the requests before its own: every workgroup adds them up itself
+// instead of waiting for another (8 bytes a request, from the caches; one launch).
 struct Need {
   int64_t tokens, pages;
 };
