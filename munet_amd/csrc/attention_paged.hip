@@ -1010,20 +1010,20 @@ __global__ void __launch_bounds__(256, DT == F32 || HDP > 128 ? 1 : 2) attn_page
 }
 
 // The shares of a row joined: M the largest maximum, o = sum_s o_s 2^(m_s - M) /
-// sum_s l_s 2^(m_s - M).  hd / 4 threads take a share's values; `groups` of them a row,
-// each every groups-th share, added in group order (with one, a row of 64 shares
-// took 31 us for 128 rows).
+// sum_s l_s 2^(m_s - M).  The cut of a workgroup is JoinShape's; a row's groups are
+// added in group order.
 template <int DT>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(kJoinThreads)
 paged_join_kernel(const float *__restrict__ part_o, const float2 *__restrict__ part_ml, const int32_t *__restrict__ cu, void *out,
-                  long ldo, int B, int Hq, int hd, int splits, int groups, int n_rows) {
+                  long ldo, int B, int Hq, int hd, int splits, JoinShape cut, int n_rows) {
   typedef typename Store<DT>::T T;
-  __shared__ f32x4 so[256];
-  __shared__ float2 sm[256];
-  const int tid = threadIdx.x, per = hd / 4, rpb = 256 / (per * groups), unit = tid / per;  // unit: (row, group)
-  const int rr = unit / groups, grp = unit - rr * groups, d = 4 * (tid - unit * per);
-  const long row = long(blockIdx.x) * rpb + rr, t = row / Hq;
-  const bool live = rr < rpb && t >= cu[0] && t < min(cu[B], n_rows);  // rows of no request are left as they are
+  __shared__ f32x4 so[kJoinThreads];
+  __shared__ float2 sm[kJoinThreads];
+  const int tid = threadIdx.x, per = cut.per, groups = cut.groups;
+  const JoinUnit unit = join_unit(tid, per, groups, cut.rows);
+  const int grp = unit.group, d = unit.d;
+  const long row = long(blockIdx.x) * cut.rows + unit.row, t = row / Hq;
+  const bool live = unit.on && t >= cu[0] && t < min(cu[B], n_rows);  // rows of no request are left as they are
   float top = -__builtin_inff(), sum = 0.f;
   f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
   auto add = [&](float m, float l, f32x4 v) {  // one more share
@@ -1049,7 +1049,7 @@ paged_join_kernel(const float *__restrict__ part_o, const float2 *__restrict__ p
     so[tid] = o;
     sm[tid] = make_float2(top, sum);
     __syncthreads();
-    if (grp != 0) return;
+    if (grp != 0 || !live) return;
     for (int k = 1; k < groups; ++k) add(sm[tid + k * per].x, sm[tid + k * per].y, so[tid + k * per]);
   }
   if (!live) return;
@@ -1072,11 +1072,11 @@ hipError_t launch(const PagedArgs &a, const PagedShape &s, hipStream_t st) {
     hipLaunchKernelGGL((attn_paged_kernel<DT, HDP>), grid, dim3(256), 0, st, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || s.splits == 1) return e;
-  const int per = a.hd / 4, groups = std::max(1, std::min((s.splits + 3) / 4, 256 / per)), rpb = 256 / (per * groups);
-  const long rows = long(a.n_rows) * a.Hq, jb = (rows + rpb - 1) / rpb;
-  if (jb * 256 > 0xffffffffL) return hipErrorInvalidValue;
-  hipLaunchKernelGGL(paged_join_kernel<DT>, dim3(unsigned(jb)), dim3(256), 0, st, a.part_o, a.part_ml, a.cu, a.out, a.ldo, a.B, a.Hq,
-                     a.hd, a.splits, groups, a.n_rows);
+  const JoinShape cut = join_shape(a.hd, s.splits);
+  const long rows = long(a.n_rows) * a.Hq, jb = (rows + cut.rows - 1) / cut.rows;
+  if (jb * kJoinThreads > 0xffffffffL) return hipErrorInvalidValue;
+  hipLaunchKernelGGL(paged_join_kernel<DT>, dim3(unsigned(jb)), dim3(kJoinThreads), 0, st, a.part_o, a.part_ml, a.cu, a.out, a.ldo,
+                     a.B, a.Hq, a.hd, a.splits, cut, a.n_rows);
   return hipGetLastError();
 }
 

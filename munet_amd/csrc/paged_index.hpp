@@ -147,4 +147,33 @@ inline size_t paged_workspace_bytes(int n_rows, int Hq, int hd, int splits) {
   return splits > 1 ? paged_part_bytes(n_rows, Hq, hd, splits) + size_t(n_rows) * Hq * splits * 8 : 0;
 }
 
+// How a workgroup of the join is cut: hd / 4 threads take a share's values, `groups`
+// of them a row, each every groups-th share (with one, a row of 64 shares took
+// 31 us for 128 rows), and `rows` rows.  Where hd / 4 * groups does not divide
+// the workgroup, its last threads have no row, and no partners to read from.
+constexpr int kJoinThreads = 256;
+struct JoinShape {
+  int per, groups, rows;
+};
+inline JoinShape join_shape(int hd, int splits) {
+  JoinShape s;
+  s.per = hd / 4;
+  s.groups = std::max(1, std::min((splits + 3) / 4, kJoinThreads / s.per));
+  s.rows = kJoinThreads / (s.per * s.groups);
+  return s;
+}
+struct JoinUnit {
+  int row, group, d;  // d: the first of its four head values
+  bool on;
+};
+__host__ __device__ __forceinline__ JoinUnit join_unit(int tid, int per, int groups, int rows) {
+  const int unit = tid / per;
+  JoinUnit u;
+  u.row = unit / groups;
+  u.group = unit - u.row * groups;
+  u.d = 4 * (tid - unit * per);
+  u.on = u.row < rows;
+  return u;
+}
+
 }  // namespace mh
