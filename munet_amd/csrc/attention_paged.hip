@@ -974,8 +974,10 @@ __global__ void __launch_bounds__(256, DT == F32 || HDP > 128 ? 1 : 2) attn_page
               }
             }
           }
+          // (NaN values are cleared for the whole workgroup: where some row of another
+          // wave does not see the block, too)
           uint32_t nans = 0;
-          if (masked)
+          if (base < all_lo || base + kKeyBlock > all_hi || __any(!ok0 || !ok1))
 #pragma unroll
             for (int v = 0; v < NW; ++v) nans |= dirty[buf][v];
           if (__builtin_amdgcn_readfirstlane(nans)) {

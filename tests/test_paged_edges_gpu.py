@@ -4,7 +4,7 @@ nobody wrote.  Against the formula in 64 bits, with the tolerance of
 test_paged_gpu.py."""
 import pytest
 
-from test_paged_gpu import Cache, check, torch  # noqa: F401
+from test_paged_gpu import DTYPES, E4M3_NAN, Cache, check, torch  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -14,3 +14,15 @@ pytestmark = pytest.mark.gpu
 def test_joins_that_leave_threads_over(torch, hip, dtype, hd, keys):  # noqa: F811
     """Head sizes and shares whose product does not divide the joining workgroup."""
     check(torch, hip, Cache(torch, 1, hd, 64, [keys, 70], [1, 1], seed=hd), 2, dtype, what="join")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("heads,P,n,new,window", [(1, 16, 256, 256, 0), (1, 64, 300, 200, 0), (4, 32, 230, 200, 0), (2, 64, 400, 300, 150),
+                                                  (4, 128, 261, 261, 90), (1, 16, 333, 290, 200)])
+def test_nan_values_in_long_prompts(torch, hip, dtype, heads, P, n, new, window):  # noqa: F811
+    """A NaN value reaches every row that sees it, whichever wave's rows the mask ends in."""
+    c = Cache(torch, 1, 64, P, [n, 40], [new, 1], seed=P + n, window=window)
+    for d, t in ((5, 3), (17, 40), (33, 120), (63, 200), (5, n - 1)):
+        c.vc[c.tables[0][t // P], 0, d, t % P] = E4M3_NAN
+    out = check(torch, hip, c, heads, dtype, what="NaN values, prompts")
+    assert bool(torch.isnan(out).any()) and not bool(torch.isnan(out[:, :, 6]).any())
