@@ -589,7 +589,9 @@ __global__ void __launch_bounds__(256, DT == F32 || HDP > 128 ? 1 : 2) attn_page
   // NaN values of a block at the edge of some row's mask (they are zeros in
   // LDS): bit k of nan_at, key k of the block
   __shared__ uint64_t nan_at[2][HDP];
-  __shared__ uint32_t dirty[2][NW];  // whether there are any
+  // the runs of 16 keys (bits 0..3) of which a wave noted some: a wave without a missing page
+  // notes nothing in blocks that all rows see, and what nan_at has of its runs is old
+  __shared__ uint32_t dirty[2][NW];
   // (the wave's number as a scalar: what follows from it are scalar tests)
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 31, h = lane >> 5;
   Part w;
@@ -768,7 +770,7 @@ __global__ void __launch_bounds__(256, DT == F32 || HDP > 128 ? 1 : 2) attn_page
       }
     };
     auto place = [&](int base, int buf) {  // into LDS as fp16
-      uint32_t any = 0;
+      uint32_t any = 0, runs = 0;
       if (base < all_lo || base + kKeyBlock > all_hi || holes) {
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
@@ -786,9 +788,10 @@ __global__ void __launch_bounds__(256, DT == F32 || HDP > 128 ? 1 : 2) attn_page
           }
           raw[i] = make_uint4(b[0], b[1], b[2], b[3]);
           any |= bits;
+          runs |= ((1u << (1 << ql)) - 1u) << grp0[i];
           reinterpret_cast<uint16_t *>(nan_at[buf])[vrow * 4 + grp] = uint16_t(bits);
         }
-        any = __any(any != 0);
+        any = __any(any != 0) ? runs : 0u;
       }
 #pragma unroll
       for (int i = 0; i < CH; ++i) {
@@ -980,12 +983,16 @@ __global__ void __launch_bounds__(256, DT == F32 || HDP > 128 ? 1 : 2) attn_page
           if (base < all_lo || base + kKeyBlock > all_hi || __any(!ok0 || !ok1))
 #pragma unroll
             for (int v = 0; v < NW; ++v) nans |= dirty[buf][v];
-          if (__builtin_amdgcn_readfirstlane(nans)) {
+          nans = __builtin_amdgcn_readfirstlane(nans);
+          if (nans) {
             // outputs of rows that see a NaN value (a zero probability alone would
             // not keep it from the others)
             uint64_t sees = uint64_t(seen(0)) << (16 * h) | uint64_t(seen(1)) << (32 + 16 * h);
             sees |= uint64_t(uint32_t(__shfl_xor(int(uint32_t(sees)), 32, 64))) |
                     uint64_t(uint32_t(__shfl_xor(int(uint32_t(sees >> 32)), 32, 64))) << 32;
+            // (bit r of nans: the 16 keys of run r)
+            sees &= uint64_t((nans & 1u) * 0xffffu | (nans >> 1 & 1u) * 0xffff0000u) |
+                    uint64_t((nans >> 2 & 1u) * 0xffffu | (nans >> 3 & 1u) * 0xffff0000u) << 32;
 #pragma unroll
             for (int i = 0; i < MT; ++i)
 #pragma unroll

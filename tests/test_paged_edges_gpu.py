@@ -26,3 +26,21 @@ def test_nan_values_in_long_prompts(torch, hip, dtype, heads, P, n, new, window)
         c.vc[c.tables[0][t // P], 0, d, t % P] = E4M3_NAN
     out = check(torch, hip, c, heads, dtype, what="NaN values, prompts")
     assert bool(torch.isnan(out).any()) and not bool(torch.isnan(out[:, :, 6]).any())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hd,P", [(128, 16), (128, 32), (64, 16), (256, 16)])
+def test_nan_values_beside_pages_outside_the_pool(torch, hip, dtype, hd, P):  # noqa: F811
+    """Marks of an earlier block do not reach rows that see only a later one, part of whose pages is missing."""
+    from munet_amd._lib import HipError
+    c = Cache(torch, 1, hd, P, [640], [128], seed=hd, window=400)
+    c.vc[c.tables[0][144 // P], 0, 5, 144 % P] = E4M3_NAN
+    c.vc[c.tables[0][290 // P], 0, 9, 290 % P] = E4M3_NAN
+    c.tables[0][256 // P] = -1
+    c.sync(torch)
+    hip.check_device_errors()
+    try:
+        check(torch, hip, c, 1, dtype, what="NaN values beside holes")
+    finally:
+        with pytest.raises(HipError, match="paged KV cache"):
+            hip.check_device_errors()
