@@ -159,8 +159,8 @@ template <int DT, int HDP, int NQ> struct RowTiles {
         }
         big = finite_max8(v[s], big);
       }
-      const float up = row_lift(xor32_max(xor16_max(big)));
-      c_row[x] = a.c / up;  // (a power of two)
+      const float lift = row_lift(xor32_max(xor16_max(big))), up = __builtin_copysignf(lift, a.c);
+      c_row[x] = __builtin_fabsf(a.c) / lift;  // (a power of two; the scale's sign is q's)
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
 #pragma unroll
@@ -214,7 +214,7 @@ template <int DT, int HDP, int NQ> struct RowTiles {
       const float rescale = lnew == lref[x] ? 1.f : __builtin_amdgcn_exp2f(lref[x] - lnew);
       const float unscale = __builtin_amdgcn_exp2f(-lf), lift = __builtin_amdgcn_exp2f(lf + kLift);
       lref[x] = lnew;
-      // (a page's scale is positive: the largest raw score is the largest score)
+      // (c_row and a page's scale are positive: the largest raw score is the largest score)
       float f = ksc * c_row[x];
       f = f == 0.f ? 1e-37f : f;  // (so that a masked score stays -inf)
       float top = s[0][x][0];
@@ -695,8 +695,8 @@ __global__ void __launch_bounds__(256, DT == F32 || HDP > 128 ? 1 : 2) attn_page
         for (int e8 = 0; e8 < 8; ++e8) v[s][e8] = d < a.hd ? v[s][e8] : 0.f;
         big = finite_max8(v[s], big);
       }
-      const float up = row_lift(xor32_max(big));
-      c_row = a.c / up;  // (a power of two)
+      const float lift = row_lift(xor32_max(big)), up = __builtin_copysignf(lift, a.c);
+      c_row = __builtin_fabsf(a.c) / lift;  // (a power of two; the scale's sign is q's)
 #pragma unroll
       for (int s = 0; s < KS; ++s)
 #pragma unroll
@@ -899,7 +899,7 @@ __global__ void __launch_bounds__(256, DT == F32 || HDP > 128 ? 1 : 2) attn_page
           const float lnew = fmaxf(lv_top, lref);
           const float rescale = lnew == lref ? 1.f : __builtin_amdgcn_exp2f(lref - lnew);
           lref = lnew;
-          // (a page's scale is positive: the largest raw score is its largest score)
+          // (c_row and a page's scale are positive: the largest raw score is its largest score)
           float f[2] = {in[0].x * c_row, in[1].x * c_row}, top = -__builtin_inff();
 #pragma unroll
           for (int t = 0; t < 2; ++t) {

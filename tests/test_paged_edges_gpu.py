@@ -44,3 +44,11 @@ def test_nan_values_beside_pages_outside_the_pool(torch, hip, dtype, hd, P):  # 
     finally:
         with pytest.raises(HipError, match="paged KV cache"):
             hip.check_device_errors()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lens,new,window,causal", [([1, 70, 300, 0], [1, 1, 1, 1], 0, True), ([70, 200, 33], [70, 60, 33], 0, True),
+                                                    ([70, 200, 33], [70, 60, 33], 50, True), ([70, 200, 33], [70, 60, 33], 0, False)])
+def test_negative_scale(torch, hip, dtype, lens, new, window, causal):  # noqa: F811
+    for scale in (-0.125, -2.0):
+        check(torch, hip, Cache(torch, 2, 64, 16, lens, new, seed=3, window=window, causal=causal), 4, dtype, what=f"scale {scale}", scale=scale)
