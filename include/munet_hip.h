@@ -266,9 +266,10 @@ int mh_kv_store_paged(int dt, const void *k, const void *v, int64_t ldk, int64_t
  * p = lens[b] - (cu[b+1] - cu[b]) + i.  Head h reads key/value head
  * h / (Hq / Hkv).  It sees keys j < lens[b]; with `causal` only j <= p, with
  * window > 0 only j > p - window.  out = softmax(scale q k) v over those, zeros
- * for a query that sees none; scale 0 means 1 / sqrt(hd).  Rows of no request
- * are left as they are.  Scores, softmax and sums are fp32, for fp16 and bf16
- * probabilities enter the product with the values as fp16.
+ * for a query that sees none; scale 0 means 1 / sqrt(hd), and |scale| is at most
+ * 2^127.  Rows of no request are left as they are.  Scores, softmax and sums are
+ * fp32, for fp16 and bf16 probabilities enter the product with the values as
+ * fp16.
  * max_q and max_len bound the requests' query and key counts; they size the
  * launch (larger ones on the device are still served, more slowly).
  * Table entries outside the pool hold no keys, and lengths past width * page

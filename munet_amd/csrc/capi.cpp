@@ -664,7 +664,8 @@ int mh_attention_paged(int dt, const void *q, int64_t ldq, const void *k_cache, 
     check_pool("attention_paged", k_cache, v_cache, k_scale, v_scale, Hkv, hd, page, n_pages);
     if (width < 0 || int64_t(width) * page > kPagedMaxKeys)
       throw Error("attention_paged: a table row must hold at most 2^31 - 4096 tokens");
-    if (!(std::fabs(scale) <= 3.4e38f)) throw Error("attention_paged: the scale must be finite");
+    // (its product with log2(e) is a float)
+    if (!(std::fabs(scale) <= 0x1p127f)) throw Error("attention_paged: the scale must be finite, of at most 2^127");
     if (B == 0 || n_rows == 0) return 0;
     if (!lens || !cu || (width && !tables)) throw Error("attention_paged: null argument");
     check_rows("attention_paged", "q", dt, q, ldq, int64_t(Hq) * hd);
