@@ -188,9 +188,10 @@ template <int DT, int HDP, int NQ> struct RowTiles {
   // masked: some row does not see some key.
   __device__ __forceinline__ void probabilities(f32x4 (&s)[4][NQ], float ksc, float lv, float lv_block, bool page_ok, int tv,
                                                 bool masked) {
-    float lvs[NQ], tops[NQ];
+    float lvs[NQ], tops[NQ], ks[NQ];
 #pragma unroll
     for (int x = 0; x < NQ; ++x) {
+      ks[x] = ksc;
       lvs[x] = lv;
       tops[x] = lv_block;
     }
@@ -202,7 +203,8 @@ template <int DT, int HDP, int NQ> struct RowTiles {
         for (int t = 0; t < 4; ++t)
 #pragma unroll
           for (int r = 0; r < 4; ++r) s[t][x][r] = (ok >> (4 * t + r)) & 1u ? s[t][x][r] : -__builtin_inff();
-        // a page of which the row sees nothing does not count for its values' scale
+        // a page of which the row sees nothing may have anything as scales
+        ks[x] = ok ? ksc : 1.f;
         tops[x] = xor32_max(xor16_max(ok ? lv : -126.f));
         lvs[x] = ok ? lv : fmaxf(tops[x], lref[x]);
       }
@@ -215,7 +217,7 @@ template <int DT, int HDP, int NQ> struct RowTiles {
       const float unscale = __builtin_amdgcn_exp2f(-lf), lift = __builtin_amdgcn_exp2f(lf + kLift);
       lref[x] = lnew;
       // (c_row and a page's scale are positive: the largest raw score is the largest score)
-      float f = ksc * c_row[x];
+      float f = ks[x] * c_row[x];
       f = f == 0.f ? 1e-37f : f;  // (so that a masked score stays -inf)
       float top = s[0][x][0];
 #pragma unroll
@@ -891,10 +893,13 @@ __global__ void __launch_bounds__(256, DT == F32 || HDP > 128 ? 1 : 2) attn_page
             for (int t = 0; t < 2; ++t)
 #pragma unroll
               for (int j = 0; j < 16; ++j) s[t][j] = (ok[t] >> j) & 1u ? s[t][j] : -__builtin_inff();
-            // a page of which the row sees nothing does not count for its values' scale
+            // a page of which the row sees nothing may have anything as scales
             lv_top = xor32_max(fmaxf(ok[0] ? lv[0] : -126.f, ok[1] ? lv[1] : -126.f));
 #pragma unroll
-            for (int t = 0; t < 2; ++t) lv[t] = ok[t] ? lv[t] : fmaxf(lv_top, lref);
+            for (int t = 0; t < 2; ++t) {
+              in[t].x = ok[t] ? in[t].x : 1.f;
+              lv[t] = ok[t] ? lv[t] : fmaxf(lv_top, lref);
+            }
           }
           const float lnew = fmaxf(lv_top, lref);
           const float rescale = lnew == lref ? 1.f : __builtin_amdgcn_exp2f(lref - lnew);

@@ -2,6 +2,8 @@
 of odd cuts, values that are not numbers, masks that differ from wave to wave, pages
 nobody wrote.  Against the formula in 64 bits, with the tolerance of
 test_paged_gpu.py."""
+import math
+
 import pytest
 
 from test_paged_gpu import DTYPES, E4M3_NAN, Cache, check, torch  # noqa: F401
@@ -52,3 +54,23 @@ def test_nan_values_beside_pages_outside_the_pool(torch, hip, dtype, hd, P):  # 
 def test_negative_scale(torch, hip, dtype, lens, new, window, causal):  # noqa: F811
     for scale in (-0.125, -2.0):
         check(torch, hip, Cache(torch, 2, 64, 16, lens, new, seed=3, window=window, causal=causal), 4, dtype, what=f"scale {scale}", scale=scale)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("junk", [math.nan, math.inf, -1.0, 0.0])
+@pytest.mark.parametrize("new,P", [(1, 16), (40, 16), (40, 64)])
+def test_scales_of_pages_nobody_sees(torch, hip, dtype, junk, new, P):  # noqa: F811
+    """Page 0, which no table names, and pages behind the window may hold anything as scales."""
+    from munet_amd._lib import HipError
+    c = Cache(torch, 2, 64, P, [300, 90], [new, new], seed=7, window=100)
+    c.kc, c.vc = (torch.cat([torch.full_like(x[:1], E4M3_NAN), x]) for x in (c.kc, c.vc))
+    c.ks, c.vs = (torch.cat([torch.full_like(x[:1], junk), x]) for x in (c.ks, c.vs))
+    c.n_pages += 1
+    c.tables = [[p + 1 if p >= 0 else p for p in row] for row in c.tables]
+    behind = c.tables[0][:(300 - new - 100 + 1) // P]
+    c.ks[behind], c.vs[behind] = junk, junk
+    c.tables[0][-1 if P == 16 else 3] = -1
+    c.sync(torch)
+    check(torch, hip, c, 4, dtype, what="scales nobody sees")
+    with pytest.raises(HipError, match="paged KV cache"):
+        hip.check_device_errors()
