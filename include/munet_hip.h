@@ -273,7 +273,8 @@ int mh_kv_store_paged(int dt, const void *k, const void *v, int64_t ldk, int64_t
  * max_q and max_len bound the requests' query and key counts; they size the
  * launch (larger ones on the device are still served, more slowly).
  * Table entries outside the pool hold no keys, and lengths past width * page
- * are cut there, raising the error flag.
+ * are cut there, raising the error flag; an entry none of whose keys a query of
+ * the request sees (behind the window) may be anything.
  * workspace: mh_attention_paged_workspace bytes, 16-byte aligned, in use until the
  * call's work on the stream has ended; calls that may overlap need one each.  out
  * may not overlap another operand. */

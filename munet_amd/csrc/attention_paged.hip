@@ -403,7 +403,7 @@ __global__ void __launch_bounds__(256) attn_paged_kernel(PagedArgs a) {
   for (int tile = it.pair % a.tiles; long(tile) * RW < w.rows; tile += a.tiles) {
     const int r_first = tile * RW;
     const int i0 = r_first / a.G, i1 = (min(r_first + RW, w.rows) - 1) / a.G;
-    const KeyRange mine = key_share(seen_keys(w.len, w.nq, i0, i1, a.causal, a.window), w.split, a.splits, a.chunk);
+    const KeyRange all = seen_keys(w.len, w.nq, i0, i1, a.causal, a.window), mine = key_share(all, w.split, a.splits, a.chunk);
     // A block's keys are on their way while the probabilities and values of the block
     // before are worked on, its values during its scores: they take the registers
     // that those have left.  Every load is made, at an address that exists, and
@@ -435,7 +435,8 @@ __global__ void __launch_bounds__(256) attn_paged_kernel(PagedArgs a) {
       int pk = of_run(n >> 2);  // of this lane's key rows
       pv = of_run(g);
       next_ok = page_in_pool(pv, a.n_pages);
-      if (!next_ok && tv < mine.hi && n == 0) atomicOr(a.err, kErrPage);
+      // (pages behind the window may be gone)
+      if (!next_ok && tv < mine.hi && tv + 16 > all.lo && n == 0) atomicOr(a.err, kErrPage);
       pk = page_in_pool(pk, a.n_pages) ? pk : 0;
       pv = next_ok ? pv : 0;
       const uint8_t *kp = kc + pk * stride + (tk & (P - 1)) * a.hd;
@@ -807,7 +808,8 @@ __global__ void __launch_bounds__(256, DT == F32 || HDP > 128 ? 1 : 2) attn_page
         m = fmaxf(m, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(m), 0xb1, 0xf, 0xf, false)));  // quad [1,0,3,2]
         m = fmaxf(m, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(m), 0x4e, 0xf, 0xf, false)));  // quad [2,3,0,1]
         if (tid < 4) {
-          if (ip < 0 && base + 16 * tid < mine.hi) atomicOr(a.err, kErrPage);
+          // (pages behind the window may be gone)
+          if (ip < 0 && base + 16 * tid < mine.hi && base + 16 * tid + 16 > any_lo) atomicOr(a.err, kErrPage);
           info[buf][tid] = make_float4(isc, lv, ip >= 0 ? 1.f : 0.f, m);
         }
       }

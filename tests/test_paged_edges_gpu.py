@@ -74,3 +74,23 @@ def test_scales_of_pages_nobody_sees(torch, hip, dtype, junk, new, P):  # noqa: 
     check(torch, hip, c, 4, dtype, what="scales nobody sees")
     with pytest.raises(HipError, match="paged KV cache"):
         hip.check_device_errors()
+
+
+@pytest.mark.parametrize("P,window", [(16, 20), (32, 20), (16, 70), (64, 90)])
+@pytest.mark.parametrize("new", [1, 20])
+def test_pages_behind_the_window_may_be_gone(torch, hip, P, window, new):  # noqa: F811
+    """Entries before the first key that a query sees are no error, and the page of that key is one."""
+    from munet_amd._lib import HipError
+    c = Cache(torch, 2, 64, P, [200, 127], [new, new], window=window, seed=P)
+    first = [max(n - new - window + 1, 0) // P for n in c.lens]
+    for row, p in zip(c.tables, first):
+        row[:p] = [-1 - i for i in range(p)]
+    c.sync(torch)
+    hip.check_device_errors()
+    check(torch, hip, c, 4, "bfloat16", what="pages behind the window")
+    hip.check_device_errors()
+    c.tables[0][first[0]] = -1
+    c.sync(torch)
+    check(torch, hip, c, 4, "bfloat16", what="the window's first page")
+    with pytest.raises(HipError, match="paged KV cache"):
+        hip.check_device_errors()
