@@ -186,7 +186,7 @@ __global__ void __launch_bounds__(NT) kv_store_paged_kernel(StoreArgs a) {
     bool first = false;
     if (lane < a.per && t < a.n) {
       const int s = a.slots[t];
-      if (s >= limit && head == 0 && wave == 0) atomicOr(a.err, kErrPage);
+      if ((s < -1 || s >= limit) && head == 0 && wave == 0) atomicOr(a.err, kErrPage);
       first = s >= 0 && s < limit && (s % P == 0 || t == 0 || a.slots[t - 1] != s - 1);
     }
     starts = __ballot(first);

@@ -1,7 +1,7 @@
 """Attention over the paged 8-bit KV cache where its forms meet their ends: joins
 of odd cuts, values that are not numbers, masks that differ from wave to wave, pages
 nobody wrote.  Against the formula in 64 bits, with the tolerance of
-test_paged_gpu.py."""
+test_paged_gpu.py.  And what the error flag tells."""
 import math
 
 import pytest
@@ -94,3 +94,22 @@ def test_pages_behind_the_window_may_be_gone(torch, hip, P, window, new):  # noq
     check(torch, hip, c, 4, "bfloat16", what="the window's first page")
     with pytest.raises(HipError, match="paged KV cache"):
         hip.check_device_errors()
+
+
+def _small_pool(torch):
+    kc, vc = (torch.zeros((3, 1, 16, 16), dtype=torch.uint8, device="cuda") for _ in range(2))
+    return kc, vc, torch.ones((3, 1), device="cuda"), torch.ones((3, 1), device="cuda")
+
+
+@pytest.mark.parametrize("slot", [-2, -2 ** 31, 48])
+def test_slots_outside_the_pool_raise(torch, hip, slot):  # noqa: F811
+    """Any but -1, which is skipped in silence."""
+    from munet_amd._lib import HipError
+    x, pool = torch.ones((3, 1, 16), device="cuda"), _small_pool(torch)
+    slots = lambda *s: torch.tensor(s, dtype=torch.int32, device="cuda")  # noqa: E731
+    hip.kv_store_paged(x, x, slots(-1, 5, -1), *pool)
+    hip.check_device_errors()
+    hip.kv_store_paged(x, x, slots(-1, slot, 6), *pool)
+    with pytest.raises(HipError, match="paged KV cache"):
+        hip.check_device_errors()
+    assert pool[0][0].any(-1)[0].nonzero().flatten().tolist() == [5, 6] and not bool(pool[0][1:].any())
