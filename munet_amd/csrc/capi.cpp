@@ -30,7 +30,7 @@ namespace {
 thread_local std::string g_last_error;
 
 struct DeviceState {
-  int *err_flag = nullptr;  // device int, embedding index errors
+  int *err_flag = nullptr;  // two device ints: embedding index errors, those of the paged cache
   void *workspace = nullptr;
   size_t workspace_bytes = 0;
 };
@@ -85,13 +85,14 @@ static DeviceState &state() {
   std::lock_guard<std::mutex> lk(g_mu);
   DeviceState &s = g_devices[d];
   if (!s.err_flag) {
-    hip_check(hipMalloc(&s.err_flag, sizeof(int)), "hipMalloc(error flag)");
-    hip_check(hipMemset(s.err_flag, 0, sizeof(int)), "hipMemset(error flag)");
+    hip_check(hipMalloc(&s.err_flag, 2 * sizeof(int)), "hipMalloc(error flag)");
+    hip_check(hipMemset(s.err_flag, 0, 2 * sizeof(int)), "hipMemset(error flag)");
   }
   return s;
 }
 
 int *device_error_flag() { return state().err_flag; }
+int *serving_error_flag() { return state().err_flag + 1; }
 
 void *workspace(size_t bytes) {
   DeviceState &s = state();
@@ -323,11 +324,12 @@ int mh_init(int device) {
 int mh_check_device_errors(void) {
   MH_TRY({
     int *flag = device_error_flag();
-    int h = 0;
+    int both[2] = {0, 0};
     hip_check(hipDeviceSynchronize(), "hipDeviceSynchronize");
-    hip_check(hipMemcpy(&h, flag, sizeof(int), hipMemcpyDeviceToHost), "hipMemcpy(error flag)");
+    hip_check(hipMemcpy(both, flag, sizeof both, hipMemcpyDeviceToHost), "hipMemcpy(error flag)");
+    const int h = both[0] | both[1];
     if (h) {
-      hip_check(hipMemset(flag, 0, sizeof(int)), "hipMemset(error flag)");
+      hip_check(hipMemset(flag, 0, sizeof both), "hipMemset(error flag)");
       if (h & kErrEmbedding) throw Error("Embedding index out of range");
       if (h & kErrPage) throw Error("paged KV cache: page, slot or length out of range");
       if (h & kErrPlan) throw Error("page_plan: out of free pages, table width or slots");
@@ -626,7 +628,7 @@ int mh_page_plan(const int32_t *lens, const int32_t *new_lens, const int32_t *fr
     p.page = page;
     p.n_pages = n_pages;
     p.cap = n_slots;
-    hip_check(page_plan(p, device_error_flag(), S_(stream)), "page_plan");
+    hip_check(page_plan(p, serving_error_flag(), S_(stream)), "page_plan");
   })
 }
 int mh_kv_store_paged(int dt, const void *k, const void *v, int64_t ldk, int64_t ldv, const int32_t *slots,
@@ -642,7 +644,7 @@ int mh_kv_store_paged(int dt, const void *k, const void *v, int64_t ldk, int64_t
     check_rows("kv_store_paged", "k", dt, k, ldk, int64_t(Hkv) * hd);
     check_rows("kv_store_paged", "v", dt, v, ldv, int64_t(Hkv) * hd);
     hip_check(kv_store_paged(dt, k, v, long(ldk), long(ldv), slots, k_cache, v_cache, k_scale, v_scale, n, Hkv, hd, page, n_pages,
-                             device_error_flag(), S_(stream)),
+                             serving_error_flag(), S_(stream)),
               "kv_store_paged");
   })
 }
@@ -685,7 +687,7 @@ int mh_attention_paged(int dt, const void *q, int64_t ldq, const void *k_cache, 
     p.lens = lens;
     p.cu = cu;
     p.workspace = workspace;
-    p.err = device_error_flag();
+    p.err = serving_error_flag();
     p.ldq = long(ldq);
     p.ldo = long(ldo);
     p.B = B;

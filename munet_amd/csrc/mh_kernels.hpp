@@ -243,7 +243,7 @@ hipError_t nchw_to_nhwc(int dt, const void *in, void *out, int B, int C, int HW,
 hipError_t nchw_to_nhwc_pad(int dt, const void *in, void *out, int B, int C, int HW, int Cp, hipStream_t st);
 hipError_t nhwc_to_nchw(int dt, const void *in, void *out, int B, int C, int HW, hipStream_t st);
 
-// Bits of the device error flag.
+// Bits of the device error flags (the last two: of the paged cache's).
 constexpr int kErrEmbedding = 1, kErrPage = 2, kErrPlan = 4;
 
 // Attention over the paged 8-bit KV cache (attention_paged.hip); layouts and

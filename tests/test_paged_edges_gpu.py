@@ -113,3 +113,24 @@ def test_slots_outside_the_pool_raise(torch, hip, slot):  # noqa: F811
     with pytest.raises(HipError, match="paged KV cache"):
         hip.check_device_errors()
     assert pool[0][0].any(-1)[0].nonzero().flatten().tolist() == [5, 6] and not bool(pool[0][1:].any())
+
+
+def test_engine_runs_go_on(torch, hip):  # noqa: F811
+    """An error of the paged calls is not the engine's, and neither takes the other's away."""
+    from munet_amd import models
+    from munet_amd._lib import HipError
+    from munet_amd.engine import Engine
+    cfg = models.decoder_config(vocab=100, ctx=16, d_model=64, num_heads=2, num_layers=1, ffn=128)
+    eng = Engine(0).load(cfg, models.init_params(cfg, "gpt", scope="p")).compile((1, 16))
+    ids = models.make_input(cfg, (1, 16), "gpt", scope="p_in")
+    before, x = eng.run(ids), torch.ones((1, 1, 16), device="cuda")
+    hip.kv_store_paged(x, x, torch.tensor([48], dtype=torch.int32, device="cuda"), *_small_pool(torch))
+    assert (eng.run(ids) == before).all()
+    bad = ids.copy()
+    bad[0, 3] = 100
+    with pytest.raises(HipError, match="Embedding index out of range"):
+        eng.run(bad)
+    with pytest.raises(HipError, match="paged KV cache"):
+        hip.check_device_errors()
+    hip.check_device_errors()
+    assert (eng.run(ids) == before).all()
