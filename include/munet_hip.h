@@ -77,7 +77,8 @@ int mh_init(int device);
 #define MH_POLICY_CONVERSION_FALLBACK 2
 int mh_query_support(int feature, int dtype, int *available, int *fallback_policy, int *accumulation_dtype);
 /* Poll and clear device-side error flags (embedding ids out of range, pages
- * and slots of the paged KV cache); synchronises the device.  Returns non-zero with a message if any was set. */
+ * and slots of the paged KV cache); synchronises the device.  Returns non-zero
+ * with a message that names all kinds of error that were set. */
 int mh_check_device_errors(void);
 
 /* ---- BackendAllocationTransferCapability (src/core/backend.hpp:190-205) --- */

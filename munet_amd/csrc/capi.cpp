@@ -330,10 +330,15 @@ int mh_check_device_errors(void) {
     const int h = both[0] | both[1];
     if (h) {
       hip_check(hipMemset(flag, 0, sizeof both), "hipMemset(error flag)");
-      if (h & kErrEmbedding) throw Error("Embedding index out of range");
-      if (h & kErrPage) throw Error("paged KV cache: page, slot or length out of range");
-      if (h & kErrPlan) throw Error("page_plan: out of free pages, table width or slots");
-      throw Error("device error flag set");
+      // all that is set: one error often brings the next
+      std::string told;
+      auto tell = [&](int bit, const char *what) {
+        if (h & bit) told += std::string(told.empty() ? "" : "; ") + what;
+      };
+      tell(kErrEmbedding, "Embedding index out of range");
+      tell(kErrPlan, "page_plan: out of free pages, table width or slots");
+      tell(kErrPage, "paged KV cache: page, slot or length out of range");
+      throw Error(told.empty() ? "device error flag set" : told);
     }
   })
 }

@@ -6,7 +6,7 @@ import math
 
 import pytest
 
-from test_paged_gpu import DTYPES, E4M3_NAN, Cache, check, torch  # noqa: F401
+from test_paged_gpu import DTYPES, E4M3_NAN, Cache, check, queries, torch  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -134,3 +134,22 @@ def test_engine_runs_go_on(torch, hip):  # noqa: F811
         hip.check_device_errors()
     hip.check_device_errors()
     assert (eng.run(ids) == before).all()
+
+
+def test_all_errors_are_told(torch, hip):  # noqa: F811
+    """A plan that runs out of pages, the attention over its table and a bad token id, checked once."""
+    from munet_amd._lib import HipError
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    c = Cache(torch, 1, 64, 16, [20], [1], junk=False)
+    tables, total, cu, slots, used = i32(0, -1, -1)[None], i32(0), i32(0, 0), i32(*[0] * 20), i32(0)
+    hip.check_device_errors()
+    hip.page_plan(i32(10), i32(20), i32(), tables, total, cu, slots, None, used, 16, c.n_pages)
+    q = queries(torch, 20, 1, 64, "bfloat16")
+    hip.attention_paged(q, c.kc, c.vc, c.ks, c.vs, tables, total, cu, torch.empty_like(q), 20, 30)
+    w = torch.zeros((10, 8), device="cuda")
+    hip.embedding(i32(1, 10, 3), w, torch.zeros((3, 8), device="cuda"), 3, 10, 8)
+    with pytest.raises(HipError) as e:
+        hip.check_device_errors()
+    for what in ("Embedding index", "page_plan", "paged KV cache"):
+        assert what in str(e.value)
+    hip.check_device_errors()
