@@ -300,8 +300,9 @@ int mh_attention_paged(int dt, const void *q, int64_t ldq, const void *k_cache, 
  * exceeds u times their sum.  Sums are whole 64-bit numbers: results do not vary
  * from run to run.  NaN logits count as -inf; a row of nothing else gives -1.
  * logprob [rows] (may be NULL): log of the drawn token's share of the kept w
- * (-inf with -1).  rows is below 2^22.  workspace: mh_sample_workspace bytes, as
- * in mh_attention_paged (0, whatever the size: no row needs one yet). */
+ * (-inf with -1).  rows is below 2^22, cols at most 2^31 - 2^21.  workspace:
+ * mh_sample_workspace bytes, as in mh_attention_paged (0, whatever the size: no
+ * row needs one yet). */
 int mh_sample_workspace(int dt, int rows, int cols, size_t *bytes);
 int mh_sample(int dt, const void *logits, int64_t ld, int rows, int cols, const float *u, const float *temperature,
               const int32_t *top_k, const float *top_p, const float *min_p, int32_t *out, float *logprob, void *workspace,

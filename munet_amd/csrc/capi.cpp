@@ -248,6 +248,11 @@ void check_rows(const char *op, const char *what, int dt, const void *p, int64_t
   if (ld < cols || ld * int64_t(dt_size(dt)) % 16)
     throw Error(std::string(op) + ": rows of " + what + " must be whole, a multiple of 16 bytes apart");
 }
+void check_sample_size(int rows, int cols) {
+  if (rows < 0 || cols < 1) throw Error("sample: bad row count or empty rows");
+  if (rows >= 1 << 22) throw Error("sample: more rows than one launch takes (2^22 - 1)");
+  if (cols > kSampleMaxCols) throw Error("sample: more tokens than indexes of 32 bits go round (2^31 - 2^21)");
+}
 // The cut of an attention_paged call, its sizes checked.
 PagedShape paged_call_shape(int dt, int B, int n_rows, int Hq, int Hkv, int hd, int max_q, int max_len, int window) {
   check_dt(dt);
@@ -715,8 +720,7 @@ int mh_sample_workspace(int dt, int rows, int cols, size_t *bytes) {
   MH_TRY({
     check_dt(dt);
     if (!bytes) throw Error("sample_workspace: null output");
-    if (rows < 0 || cols < 1) throw Error("sample: bad row count or empty rows");
-    if (rows >= 1 << 22) throw Error("sample: more rows than one launch takes (2^22 - 1)");
+    check_sample_size(rows, cols);
     *bytes = 0;
   })
 }
@@ -725,8 +729,7 @@ int mh_sample(int dt, const void *logits, int64_t ld, int rows, int cols, const 
               size_t workspace_bytes, void *stream) {
   MH_TRY({
     check_dt(dt);
-    if (rows < 0 || cols < 1) throw Error("sample: bad row count or empty rows");
-    if (rows >= 1 << 22) throw Error("sample: more rows than one launch takes (2^22 - 1)");
+    check_sample_size(rows, cols);
     if (rows == 0) return 0;
     if (!logits || !u || !out) throw Error("sample: null argument");
     if (ld < cols) throw Error("sample: rows overlap");

@@ -272,7 +272,10 @@ struct PagePlan {
   int B = 0, n_free = 0, width = 0, page = 0, n_pages = 0, cap = 0;
 };
 hipError_t page_plan(const PagePlan &p, int *err, hipStream_t st);
-// The next tokens of rows of logits (sample.hip).
+// The next tokens of rows of logits (sample.hip).  Tokens of a row: the end of a group
+// (of 2^21 tokens in rows of that length) and the tokens that a workgroup looks at past
+// the row's last chunk have 32-bit indexes.
+constexpr int kSampleMaxCols = 0x7fffffff - (1 << 21) + 1;
 struct Sampling {
   const void *logits = nullptr;
   long ld = 0;
