@@ -272,7 +272,8 @@ int mh_kv_store_paged(int dt, const void *k, const void *v, int64_t ldk, int64_t
  * fp32, for fp16 and bf16 probabilities enter the product with the values as
  * fp16.
  * max_q and max_len bound the requests' query and key counts; they size the
- * launch (larger ones on the device are still served, more slowly).
+ * launch (larger ones on the device are still served, more slowly).  B * Hkv is
+ * below 2^23, n_rows * Hq at most 2^30.
  * Table entries outside the pool hold no keys, and lengths past width * page
  * are cut there, raising the error flag; an entry none of whose keys a query of
  * the request sees (behind the window) may be anything.

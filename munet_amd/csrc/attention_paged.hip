@@ -1076,9 +1076,7 @@ paged_join_kernel(const float *__restrict__ part_o, const float2 *__restrict__ p
 
 template <int DT, int HDP>
 hipError_t launch(const PagedArgs &a, const PagedShape &s, hipStream_t st) {
-  const long blocks = long(s.tiles) * s.splits * a.Hkv * a.B;
-  if (blocks * 512 > 0xffffffffL) return hipErrorInvalidValue;
-  const dim3 grid{unsigned(blocks)};
+  const dim3 grid{unsigned(long(s.tiles) * s.splits * a.Hkv * a.B)};
   if (s.wide)
     if (a.plog >= 6)
       hipLaunchKernelGGL((attn_paged_wide_kernel<DT, HDP, true>), grid, dim3(256), 0, st, a);
@@ -1090,7 +1088,6 @@ hipError_t launch(const PagedArgs &a, const PagedShape &s, hipStream_t st) {
   if (e != hipSuccess || s.splits == 1) return e;
   const JoinShape cut = join_shape(a.hd, s.splits);
   const long rows = long(a.n_rows) * a.Hq, jb = (rows + cut.rows - 1) / cut.rows;
-  if (jb * kJoinThreads > 0xffffffffL) return hipErrorInvalidValue;
   hipLaunchKernelGGL(paged_join_kernel<DT>, dim3(unsigned(jb)), dim3(kJoinThreads), 0, st, a.part_o, a.part_ml, a.cu, a.out, a.ldo,
                      a.B, a.Hq, a.hd, a.splits, cut, a.n_rows);
   return hipGetLastError();

@@ -260,7 +260,11 @@ PagedShape paged_call_shape(int dt, int B, int n_rows, int Hq, int Hkv, int hd, 
   if (Hkv < 1 || Hq < 1 || Hq % Hkv) throw Error("attention_paged: query heads must be a multiple of key/value heads");
   if (hd < 16 || hd > kPagedHeadMax || hd % 16) throw Error("attention_paged: head_dim must be a multiple of 16, at most 256");
   if (int64_t(n_rows) * Hq > (1 << 30)) throw Error("attention_paged: more than 2^30 query rows");
-  return paged_shape(B, Hq, Hkv, std::min(max_q, n_rows), max_len, window);
+  if (int64_t(B) * Hkv > kPagedMaxBlocks) throw Error("attention_paged: more requests times key/value heads than one launch takes (2^23 - 1)");
+  PagedShape s = paged_shape(B, Hq, Hkv, std::min(max_q, n_rows), max_len, window);
+  // (a batch padded with more rows than one launch joins: no shares)
+  if (s.splits > 1 && int64_t(n_rows) * Hq > kJoinMaxBlocks * join_shape(hd, s.splits).rows) s.splits = 1;
+  return s;
 }
 
 }  // namespace

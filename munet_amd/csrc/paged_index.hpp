@@ -117,6 +117,8 @@ constexpr int kPagedMaxKeys = 0x7fffffff - 4095;
 struct PagedShape {
   int wide, tiles, splits, chunk;
 };
+// Workgroups of a launch: kernels walk the tiles past those that it has.
+constexpr int kPagedMaxBlocks = (1 << 23) - 1;
 // Rows that a workgroup of the wide form takes: 32 to each of four waves.
 constexpr int kPagedWideRows = 128;
 inline PagedShape paged_shape(int B, int Hq, int Hkv, int max_q, int max_len, int window) {
@@ -130,13 +132,15 @@ inline PagedShape paged_shape(int B, int Hq, int Hkv, int max_q, int max_len, in
   // join 5, four 145 + 6; 2 requests of which one has 131072: 32 shares 85 + 6,
   // 64 74 + 7, 128 83 + 12), none shorter than one block per wave.
   const int64_t whole = std::max<int64_t>(1, int64_t(B) * Hkv * s.tiles);
-  const int64_t keys = window > 0 ? std::min<int64_t>(max_len, int64_t(window) + max_q + kKeyBlock) : max_len;
+  const int64_t longest = std::min(max_len, kPagedMaxKeys);
+  const int64_t keys = window > 0 ? std::min<int64_t>(longest, int64_t(window) + max_q + kKeyBlock) : longest;
   const int64_t least = 4 * kKeyBlock;
   int64_t n = std::min<int64_t>((keys + least - 1) / least, 1025 / (whole + 1));
   n = std::max<int64_t>(1, std::min<int64_t>(n, 256));
-  s.chunk = int(std::min<int64_t>(((keys + n - 1) / n + least - 1) / least * least, 1 << 30));
+  s.chunk = int(((keys + n - 1) / n + least - 1) / least * least);
   if (s.chunk == 0) s.chunk = int(least);
   s.splits = int(std::max<int64_t>(1, (keys + s.chunk - 1) / s.chunk));
+  s.tiles = int(std::min<int64_t>(s.tiles, std::max<int64_t>(1, kPagedMaxBlocks / std::max<int64_t>(1, int64_t(B) * Hkv * s.splits))));
   return s;
 }
 // Workspace: the shares' outputs, then their (maximum, sum) pairs.
@@ -155,6 +159,7 @@ constexpr int kJoinThreads = 256;
 struct JoinShape {
   int per, groups, rows;
 };
+constexpr int64_t kJoinMaxBlocks = (1 << 24) - 1;  // 2^32 threads
 inline JoinShape join_shape(int hd, int splits) {
   JoinShape s;
   s.per = hd / 4;

@@ -32,7 +32,25 @@ static void check_join() {
     }
 }
 
+// Every cut fits a launch, whatever the bounds; as many tiles as the bounds ask
+// for where they fit.
+static void check_launches() {
+  for (int B : {1, 2, 7, 256, 4096, 100000, kPagedMaxBlocks / 8})
+    for (int kv : {1, 2, 8})
+      for (int G : {1, 4, 64})
+        for (int max_q : {0, 1, 2, 17, 300, 5000, 131072, 1 << 30 >> 6})
+          for (int max_len : {0, 1, 100, 70000, 0x7fffffff})
+            for (int window : {0, 1, 5000}) {
+              const PagedShape s = paged_shape(B, kv * G, kv, max_q, max_len, window);
+              const int64_t pairs = int64_t(B) * kv;
+              need(pairs * s.tiles * s.splits <= kPagedMaxBlocks && s.tiles >= 1 && s.splits >= 1, "a call's workgroups fit a launch");
+              const int64_t per = s.wide ? kPagedWideRows : 16, tiles = std::max<int64_t>(1, (int64_t(max_q) * G + per - 1) / per);
+              need(s.tiles == tiles || pairs * s.splits * (s.tiles + 1) > kPagedMaxBlocks, "fewer tiles only where a launch ends");
+            }
+}
+
 int main() {
   check_join();
+  check_launches();
   std::puts("ok");
 }

@@ -6,7 +6,7 @@ import math
 
 import pytest
 
-from test_paged_gpu import DTYPES, E4M3_NAN, Cache, check, queries, torch  # noqa: F401
+from test_paged_gpu import DTYPES, E4M3_NAN, Cache, assert_within, attend_reference, check, queries, torch  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -153,3 +153,16 @@ def test_all_errors_are_told(torch, hip):  # noqa: F811
     for what in ("Embedding index", "page_plan", "paged KV cache"):
         assert what in str(e.value)
     hip.check_device_errors()
+
+
+def test_bounds_past_a_launch(torch, hip):  # noqa: F811
+    """Bounds that ask for more workgroups than a launch has: fewer, which walk."""
+    B, heads, kv, n_rows = 256, 64, 8, 65600
+    lens, new = [300] + [1 + 3 * i for i in range(B - 1)], [300] + [1] * (B - 1)
+    c = Cache(torch, kv, 16, 16, lens, new, seed=12)
+    q = queries(torch, n_rows, heads, 16, "bfloat16")
+    out, rows = torch.full_like(q, 7.0), c.cu[-1]
+    ref, tol = attend_reference(torch, c, q[:rows], out[:rows])
+    c.attend(hip, q, out, max_q=n_rows, max_len=n_rows)
+    assert_within(torch, out[:rows], ref, tol, "many workgroups")
+    assert bool((out[rows:] == 7.0).all())

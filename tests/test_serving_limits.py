@@ -23,3 +23,17 @@ def test_rows_of_tokens_past_32_bits(cols):
     with pytest.raises(_lib.HipError, match="2\\^31 - 2\\^21"):
         _lib.call("mh_sample_workspace", 0, 1, cols, ctypes.byref(n))
     _lib.call("mh_sample_workspace", 0, 1, 2 ** 31 - 2 ** 21, ctypes.byref(n))
+
+
+def test_launch_limits():
+    """More workgroups than a launch has are refused by name where tiles cannot be walked instead."""
+    with pytest.raises(_lib.HipError, match="one launch takes"):
+        _attend(B=1 << 21, n_rows=1 << 21)
+    n = ctypes.c_size_t()
+
+    def workspace(n_rows):
+        _lib.call("mh_attention_paged_workspace", 2, 1, n_rows, 16, 16, 256, 1, 100000, 0, ctypes.byref(n))
+        return n.value
+
+    assert workspace(1 << 16) > 0
+    assert workspace(1 << 26) == 0  # (rows that pad the batch, more than one launch joins: no shares)
