@@ -38,8 +38,11 @@ namespace {
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
 // Probabilities are taken times 2^kLift, against a reference that the row's
-// largest score passes by at most kRaise (log2): below 2^15 in fp16.
-constexpr float kLift = 9.f, kRaise = 5.f;
+// largest score passes by at most kRaise (log2): below 2^15 in fp16.  A page's
+// value scale counts as no less than 2^-kApart of the largest: its probabilities are
+// zeros in fp16 long before, but the sum goes by them times the inverse, which has to
+// stay a float (a page of zeros has scale 2^-100).
+constexpr float kLift = 9.f, kRaise = 5.f, kApart = 60.f;
 
 struct PagedArgs {
   const void *q;
@@ -212,7 +215,7 @@ template <int DT, int HDP, int NQ> struct RowTiles {
 #pragma unroll
     for (int x = 0; x < NQ; ++x) {
       // the value scales: this lane group's over the largest that the row has seen
-      const float lnew = fmaxf(tops[x], lref[x]), lf = lvs[x] - lnew;
+      const float lnew = fmaxf(tops[x], lref[x]), lf = fmaxf(lvs[x] - lnew, -kApart);
       const float rescale = lnew == lref[x] ? 1.f : __builtin_amdgcn_exp2f(lref[x] - lnew);
       const float unscale = __builtin_amdgcn_exp2f(-lf), lift = __builtin_amdgcn_exp2f(lf + kLift);
       lref[x] = lnew;
@@ -954,7 +957,7 @@ __global__ void __launch_bounds__(256, DT == F32 || HDP > 128 ? 1 : 2) attn_page
           read_values(0);
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
-            const float lf = lv[t] - lnew, unscale = __builtin_amdgcn_exp2f(-lf), lift = __builtin_amdgcn_exp2f(lf + kLift),
+            const float lf = fmaxf(lv[t] - lnew, -kApart), unscale = __builtin_amdgcn_exp2f(-lf), lift = __builtin_amdgcn_exp2f(lf + kLift),
                         shift = lf + kLift - ref;
             float sum = 0.f;
             f16x8 pf[NP][2];

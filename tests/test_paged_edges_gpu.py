@@ -166,3 +166,18 @@ def test_bounds_past_a_launch(torch, hip):  # noqa: F811
     c.attend(hip, q, out, max_q=n_rows, max_len=n_rows)
     assert_within(torch, out[:rows], ref, tol, "many workgroups")
     assert bool((out[rows:] == 7.0).all())
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("P", [16, 64])
+@pytest.mark.parametrize("low,high", [(-100, 30), (-100, 90), (-100, 28)])
+def test_zero_pages_beside_large_values(torch, hip, dtype, new, P, low, high):  # noqa: F811
+    """Pages of zeros (scale 2^-100) beside large values: their weights stay in the sum."""
+    c = Cache(torch, 2, 64, P, [200, 90, 64], [new, new, 1], seed=4, spread=1.0)
+    c.vs[:] = 2.0 ** high
+    for b, p in ((0, 0), (0, 2), (1, 1), (2, 0)):
+        g = c.tables[b][p]
+        c.vs[g] = 2.0 ** low
+        c.vc[g] = torch.where(c.vc[g] == E4M3_NAN, E4M3_NAN, 0).to(torch.uint8)
+    check(torch, hip, c, 4, dtype, what="zero pages")
