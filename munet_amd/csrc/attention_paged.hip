@@ -115,6 +115,9 @@ __device__ __forceinline__ float row_lift(float big) {
   return __uint_as_float(uint32_t(k + 127) << 23);
 }
 
+// 1 / a row's sum; 0 where it saw no key
+__device__ __forceinline__ float over(float sum) { return sum == 0.f ? 0.f : 1.f / sum; }
+
 // The query rows of a wave: NQ tiles of 16 (column n of tile x is row r_first + 16 x
 // + n of the packed rows; past the last row, that row again, not stored), their
 // running softmax and their outputs O^T.
@@ -319,29 +322,30 @@ template <int DT, int HDP, int NQ> struct RowTiles {
     }
   }
 
-  // the sums over the lane groups, the outputs in the values' scale
+  // The sums over the lane groups, the outputs over them (zero where no key was seen)
+  // and in the values' scale, in this order: an output is no larger than the
+  // largest value, its product with the sum may pass a float.
   __device__ __forceinline__ void finish() {
 #pragma unroll
     for (int x = 0; x < NQ; ++x) {
       l[x] = xor32_add(xor16_add(l[x]));
+      const float inv = over(l[x]), up = __builtin_amdgcn_exp2f(lref[x]);
 #pragma unroll
-      for (int i = 0; i < MT; ++i) acc[i][x] *= __builtin_amdgcn_exp2f(lref[x]);
+      for (int i = 0; i < MT; ++i) acc[i][x] = acc[i][x] * inv * up;
     }
   }
 };
 
-// Where a packed row's output goes: o / sum, or this share's (o, maximum, sum)
-// for the join.
+// Where a packed row's output goes: to the caller, or with the share's maximum and
+// sum to the join.
 template <int DT> struct RowOut {
   typedef typename Store<DT>::T T;
   T *out;
   float *part;
-  float inv;
   __device__ __forceinline__ RowOut(const PagedArgs &a, int row0, int kvh, int split, int r, float m, float sum, bool first) {
     const int i = r / a.G, h = kvh * a.G + r - i * a.G;
     out = nullptr;
     part = nullptr;
-    inv = sum == 0.f ? 0.f : 1.f / sum;  // (a row that sees no key is zero)
     if (a.splits == 1) {
       out = static_cast<T *>(a.out) + long(row0 + i) * a.ldo + long(h) * a.hd;
     } else {
@@ -352,7 +356,7 @@ template <int DT> struct RowOut {
   }
   __device__ __forceinline__ void put(int d, f32x4 o) const {
     if (out) {
-      const float v[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
+      const float v[4] = {o[0], o[1], o[2], o[3]};
       st4<DT>(out + d, v);
     } else if (part) {
       *reinterpret_cast<f32x4 *>(part + d) = o;
@@ -541,14 +545,18 @@ __global__ void __launch_bounds__(256) attn_paged_kernel(PagedArgs a) {
           float top = wml[0][rr].x;
 #pragma unroll
           for (int v = 1; v < 4; ++v) top = fmaxf(top, wml[v][rr].x);
-          float sum = 0.f;
-          f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+          float of[4], sum = 0.f;  // (0: this wave saw no key)
 #pragma unroll
           for (int v = 0; v < 4; ++v) {
             const float2 ml = wml[v][rr];
-            if (ml.y == 0.f) continue;  // (this wave saw no key)
-            const float f = ml.x == top ? 1.f : __builtin_amdgcn_exp2f(ml.x - top);
-            sum = fmaf(ml.y, f, sum);
+            of[v] = ml.y == 0.f ? 0.f : ml.x == top ? ml.y : ml.y * __builtin_amdgcn_exp2f(ml.x - top);
+            sum += of[v];
+          }
+          const float inv = over(sum);
+          f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            const float f = of[v] * inv;
             const f32x4 y = *reinterpret_cast<const f32x4 *>(&wo[v][rr][d]);
 #pragma unroll
             for (int c = 0; c < 4; ++c) o[c] = fmaf(y[c], f, o[c]);
@@ -1016,20 +1024,20 @@ __global__ void __launch_bounds__(256, DT == F32 || HDP > 128 ? 1 : 2) attn_page
     l = xor32_add(l);
     if (r_first + n < w.rows) {
       const RowOut<DT> to(a, w.row0, w.kvh, w.split, row, mx, l, h == 0);
-      const float vref = __builtin_amdgcn_exp2f(lref);
+      const float inv = over(l), up = __builtin_amdgcn_exp2f(lref);  // (in this order: see above)
 #pragma unroll
       for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int d = 32 * i + 8 * j + 4 * h;
-          if (d < a.hd) to.put(d, f32x4{acc[i][4 * j], acc[i][4 * j + 1], acc[i][4 * j + 2], acc[i][4 * j + 3]} * vref);
+          if (d < a.hd) to.put(d, f32x4{acc[i][4 * j], acc[i][4 * j + 1], acc[i][4 * j + 2], acc[i][4 * j + 3]} * inv * up);
         }
     }
   }
 }
 
-// The shares of a row joined: M the largest maximum, o = sum_s o_s 2^(m_s - M) /
-// sum_s l_s 2^(m_s - M).  The cut of a workgroup is JoinShape's; a row's groups are
+// The shares of a row joined: M the largest maximum, o = sum_s o_s l_s 2^(m_s - M) /
+// sum_s l_s 2^(m_s - M), divided at each step (the sum may pass a float).  The cut of a workgroup is JoinShape's; a row's groups are
 // added in group order.
 template <int DT>
 __global__ void __launch_bounds__(kJoinThreads)
@@ -1047,11 +1055,14 @@ paged_join_kernel(const float *__restrict__ part_o, const float2 *__restrict__ p
   f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
   auto add = [&](float m, float l, f32x4 v) {  // one more share
     if (l == 0.f) return;                      // (of no key)
-    const float up = fmaxf(top, m), f0 = top == up ? 1.f : __builtin_amdgcn_exp2f(top - up), f1 = m == up ? 1.f : __builtin_amdgcn_exp2f(m - up);
+    const float up = fmaxf(top, m);
+    float s0 = top == up ? sum : sum * __builtin_amdgcn_exp2f(top - up), s1 = m == up ? l : l * __builtin_amdgcn_exp2f(m - up);
     top = up;
-    sum = fmaf(l, f1, sum * f0);
+    sum = s0 + s1;
+    s0 /= sum;
+    s1 /= sum;
 #pragma unroll
-    for (int c = 0; c < 4; ++c) o[c] = fmaf(v[c], f1, o[c] * f0);
+    for (int c = 0; c < 4; ++c) o[c] = fmaf(v[c], s1, o[c] * s0);
   };
   if (live) {
     const float2 *ml = part_ml + row * splits;
@@ -1072,8 +1083,7 @@ paged_join_kernel(const float *__restrict__ part_o, const float2 *__restrict__ p
     for (int k = 1; k < groups; ++k) add(sm[tid + k * per].x, sm[tid + k * per].y, so[tid + k * per]);
   }
   if (!live) return;
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  const float v[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
+  const float v[4] = {o[0], o[1], o[2], o[3]};
   st4<DT>(static_cast<T *>(out) + t * ldo + long(row - t * Hq) * hd + d, v);
 }
 

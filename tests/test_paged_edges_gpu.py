@@ -181,3 +181,14 @@ def test_zero_pages_beside_large_values(torch, hip, dtype, new, P, low, high):  
         c.vs[g] = 2.0 ** low
         c.vc[g] = torch.where(c.vc[g] == E4M3_NAN, E4M3_NAN, 0).to(torch.uint8)
     check(torch, hip, c, 4, dtype, what="zero pages")
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("lens,new", [([200, 90, 64], [1, 1, 1]), ([200, 90, 64], [40, 40, 1]), ([3000, 700], [1, 1]), ([900, 700], [40, 1])])
+def test_values_near_the_largest(torch, hip, dtype, lens, new):  # noqa: F811
+    """Outputs that a float holds, and whose products with the softmax's sum it does not, in one share and joined ones."""
+    for P in (16, 64):
+        c = Cache(torch, 1, 64, P, lens, new, seed=4, spread=1.0)
+        c.vs[:] = 2.0 ** 118
+        c.vs[c.tables[0][1]] = 2.0 ** -12
+        check(torch, hip, c, 2, dtype, what="large values")
