@@ -25,9 +25,9 @@
 // most 2^-38 of the row's largest value); fp32 inputs are the sum of two fp16 parts
 // (22 bits and a sign).  Scores, the running maximum, the sum and the outputs are
 // fp32.  A probability enters the second product as 2^9 w times its page's value
-// scale over the largest one that the row has seen, rounded to fp16 (half a unit
-// of 11 bits down to 2^-23 of the reference; outputs of 16 bits are rounded as
-// much once more), or as two such parts for fp32 inputs.
+// scale over the row's largest product of the two so far (a reference near it),
+// rounded to fp16 (half a unit of 11 bits down to 2^-23 of that; outputs of 16 bits
+// are rounded as much once more), or as two such parts for fp32 inputs.
 #include "mh_common.hpp"
 #include "mh_kernels.hpp"
 #include "paged_index.hpp"
@@ -37,12 +37,35 @@ namespace {
 
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
-// Probabilities are taken times 2^kLift, against a reference that the row's
-// largest score passes by at most kRaise (log2): below 2^15 in fp16.  A page's
-// value scale counts as no less than 2^-kApart of the largest: its probabilities are
-// zeros in fp16 long before, but the sum goes by them times the inverse, which has to
-// stay a float (a page of zeros has scale 2^-100).
-constexpr float kLift = 9.f, kRaise = 5.f, kApart = 60.f;
+// Probabilities times value scales are taken times 2^kLift, against a reference that
+// the row's largest passes by at most kRaise (log2): below 2^15 in fp16.
+constexpr float kLift = 9.f, kRaise = 5.f;
+// The references: mx of the scores (log2), to which the sum goes, and mx + lref of
+// scores + log2 of value scales, to which the outputs go; lref is a whole number, so
+// that powers of two alone lie between the two.  The first moves when a score
+// passes it by kRaise, the second then too or when a product passes it: sums and
+// outputs are seldom scaled.  (Against the largest value scale alone, outputs of
+// small values went lost beside large ones of no weight.)
+__device__ __forceinline__ bool passes(float top, float both, float &mx, float &lref, float &down, float &down_both) {
+  const float m = top > mx + kRaise ? top : mx;
+  const bool moved = m != mx || both > mx + lref + kRaise;
+  down = down_both = 1.f;
+  if (moved) {
+    const float by = mx - m, l = __builtin_ceilf(fmaxf(mx + lref, both) - m);
+    down = __builtin_amdgcn_exp2f(by);
+    down_both = __builtin_amdgcn_exp2f(by + (lref - l));
+    mx = m;
+    lref = l;
+  }
+  return moved;
+}
+// A run's value scale over lref, to what the probabilities can take: at least 2^-60,
+// where they are zeros in fp16, since the sum goes by them times the inverse, which has
+// to stay a float (a page of zeros has scale 2^-100); and for two parts, which
+// are scaled after the exponential, at most 2^110.
+template <int NP> __device__ __forceinline__ float apart(float lv, float lref) {
+  return __builtin_amdgcn_fmed3f(lv - lref, -60.f, NP == 2 ? 110.f : 250.f);
+}
 
 struct PagedArgs {
   const void *q;
@@ -129,7 +152,7 @@ template <int DT, int HDP, int NQ> struct RowTiles {
   f16x8 pf[NP][NQ][2];
   f32x4 acc[MT][NQ];
   float c_row[NQ], mx[NQ], l[NQ];
-  float lref[NQ];  // log2 of the largest value scale that the row has seen
+  float lref[NQ];  // outputs are in units of 2^lref
   int lo_row[NQ], hi_row[NQ];
   int every_lo, every_hi;  // keys that every row sees
   int some_lo, some_hi;    // keys that some row sees
@@ -189,18 +212,13 @@ template <int DT, int HDP, int NQ> struct RowTiles {
   }
 
   // Raw scores of a block (this lane group's keys tv .. tv + 15, with their
-  // page's key scale and log2 of its value scale, and the block's largest) to
-  // probabilities pf; the sums and outputs so far scaled to the new reference.
+  // page's key scale and log2 of its value scale) to probabilities pf; the sums and
+  // outputs so far scaled to the new references.
   // masked: some row does not see some key.
-  __device__ __forceinline__ void probabilities(f32x4 (&s)[4][NQ], float ksc, float lv, float lv_block, bool page_ok, int tv,
-                                                bool masked) {
-    float lvs[NQ], tops[NQ], ks[NQ];
+  __device__ __forceinline__ void probabilities(f32x4 (&s)[4][NQ], float ksc, float lv, bool page_ok, int tv, bool masked) {
+    float ks[NQ];
 #pragma unroll
-    for (int x = 0; x < NQ; ++x) {
-      ks[x] = ksc;
-      lvs[x] = lv;
-      tops[x] = lv_block;
-    }
+    for (int x = 0; x < NQ; ++x) ks[x] = ksc;
     if (masked) {
 #pragma unroll
       for (int x = 0; x < NQ; ++x) {
@@ -211,17 +229,10 @@ template <int DT, int HDP, int NQ> struct RowTiles {
           for (int r = 0; r < 4; ++r) s[t][x][r] = (ok >> (4 * t + r)) & 1u ? s[t][x][r] : -__builtin_inff();
         // a page of which the row sees nothing may have anything as scales
         ks[x] = ok ? ksc : 1.f;
-        tops[x] = xor32_max(xor16_max(ok ? lv : -126.f));
-        lvs[x] = ok ? lv : fmaxf(tops[x], lref[x]);
       }
     }
 #pragma unroll
     for (int x = 0; x < NQ; ++x) {
-      // the value scales: this lane group's over the largest that the row has seen
-      const float lnew = fmaxf(tops[x], lref[x]), lf = fmaxf(lvs[x] - lnew, -kApart);
-      const float rescale = lnew == lref[x] ? 1.f : __builtin_amdgcn_exp2f(lref[x] - lnew);
-      const float unscale = __builtin_amdgcn_exp2f(-lf), lift = __builtin_amdgcn_exp2f(lf + kLift);
-      lref[x] = lnew;
       // (c_row and a page's scale are positive: the largest raw score is the largest score)
       float f = ks[x] * c_row[x];
       f = f == 0.f ? 1e-37f : f;  // (so that a masked score stays -inf)
@@ -230,19 +241,19 @@ template <int DT, int HDP, int NQ> struct RowTiles {
       for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r) top = fmaxf(top, s[t][x][r]);
-      top = top > -__builtin_inff() ? top * f : -__builtin_inff();
+      const bool none = !(top > -__builtin_inff());
+      top = none ? -__builtin_inff() : top * f;
+      const float both = xor32_max(xor16_max(none ? top : top + lv));
       top = xor32_max(xor16_max(top));
-      // the reference moves only when a score passes it by 2^kRaise: sums and
-      // outputs are seldom scaled
-      top = top > mx[x] + kRaise ? top : mx[x];
-      float ref = top > -__builtin_inff() ? top : 0.f;
-      const float down = mx[x] == top ? 1.f : __builtin_amdgcn_exp2f(mx[x] - ref);
-      mx[x] = top;
-      if (__any(down * rescale != 1.f)) {
+      float down, down_both;
+      if (__any(passes(top, both, mx[x], lref[x], down, down_both))) {
         l[x] *= down;
 #pragma unroll
-        for (int i = 0; i < MT; ++i) acc[i][x] *= down * rescale;
+        for (int i = 0; i < MT; ++i) acc[i][x] *= down_both;
       }
+      float ref = mx[x] > -__builtin_inff() ? mx[x] : 0.f;
+      const float lf = apart<NP>(lv, lref[x]);
+      const float unscale = __builtin_amdgcn_exp2f(-lf), lift = __builtin_amdgcn_exp2f(lf + kLift);
       // The product below is not rounded before the maximum, which is, goes off it.
       // Where that could leave much (scores past 2^16), both are rounded.
       const bool far = __builtin_fabsf(ref) > 65536.f;
@@ -268,8 +279,8 @@ template <int DT, int HDP, int NQ> struct RowTiles {
             // power of two applied to the result
             p[y] = __builtin_amdgcn_exp2f(NP == 2 ? fmaf(raw, f, -ref) : fmaf(raw, f, lf + kLift - ref));
             if constexpr (NP == 2) p[y] *= lift;
-            // (not of the rounded values: those of a page whose value scale is far
-            // below the largest are zero)
+            // (not of the rounded values: those of small weights and value scales are
+            // zero)
             sum += p[y];
           }
 #pragma unroll
@@ -496,7 +507,7 @@ __global__ void __launch_bounds__(256) attn_paged_kernel(PagedArgs a) {
       pages(after(then));
       __builtin_amdgcn_sched_barrier(0);
       const bool masked = base < q.every_lo || base + kKeyBlock > q.every_hi || __any(!page_ok);
-      q.probabilities(s, kscale, lv, xor32_max(xor16_max(lv)), page_ok, tv, masked);
+      q.probabilities(s, kscale, lv, page_ok, tv, masked);
 
       // Keys that no row sees may hold anything, NaN among it: their bytes are
       // cleared.
@@ -598,7 +609,7 @@ __global__ void __launch_bounds__(256, DT == F32 || HDP > 128 ? 1 : 2) attn_page
   constexpr int NK = 64 * XK, CH = 2 * NK / NT;  // pieces of a block's keys; pieces (keys and values) per thread
   constexpr int KROW = HDP * 2, KB = 64 * KROW, VB = HDP * 128;
   __shared__ __align__(16) uint8_t lds[2][KB + VB];
-  // per 16 keys: key scale, log2 of the value scale, page in the pool, the block's largest log2
+  // per 16 keys: key scale, log2 of the value scale, page in the pool
   __shared__ float4 info[2][4];
   // NaN values of a block at the edge of some row's mask (they are zeros in
   // LDS): bit k of nan_at, key k of the block
@@ -687,7 +698,7 @@ __global__ void __launch_bounds__(256, DT == F32 || HDP > 128 ? 1 : 2) attn_page
     const int every_lo = max(seen_keys(w.len, w.nq, i1, i1, a.causal, a.window).lo, mine.lo);
     const int every_hi = min(seen_keys(w.len, w.nq, i0, i0, a.causal, a.window).hi, mine.hi);
     f16x8 qf[NP][KS];
-    float c_row, mx = -__builtin_inff(), l = 0.f, lref = -126.f;  // lref: log2 of the largest value scale seen
+    float c_row, mx = -__builtin_inff(), l = 0.f, lref = -126.f;
     f32x16 acc[MT];
 #pragma unroll
     for (int i = 0; i < MT; ++i)
@@ -815,13 +826,10 @@ __global__ void __launch_bounds__(256, DT == F32 || HDP > 128 ? 1 : 2) attn_page
       if (lane == 0) dirty[buf][wave] = any;
       if (!ONE && wave == 0) {
         const float lv = ip >= 0 ? fmaxf(__builtin_amdgcn_logf(ivs), -126.f) : -126.f;
-        float m = lv;
-        m = fmaxf(m, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(m), 0xb1, 0xf, 0xf, false)));  // quad [1,0,3,2]
-        m = fmaxf(m, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(m), 0x4e, 0xf, 0xf, false)));  // quad [2,3,0,1]
         if (tid < 4) {
           // (pages behind the window may be gone)
           if (ip < 0 && base + 16 * tid < mine.hi && base + 16 * tid + 16 > any_lo) atomicOr(a.err, kErrPage);
-          info[buf][tid] = make_float4(isc, lv, ip >= 0 ? 1.f : 0.f, m);
+          info[buf][tid] = make_float4(isc, lv, ip >= 0 ? 1.f : 0.f, 0.f);
         }
       }
     };
@@ -859,7 +867,7 @@ __global__ void __launch_bounds__(256, DT == F32 || HDP > 128 ? 1 : 2) attn_page
           float4 in[2];
           if constexpr (ONE) {
             const float lv = ok_now ? fmaxf(__builtin_amdgcn_logf(vs_now), -126.f) : -126.f;
-            in[0] = in[1] = make_float4(ks_now, lv, ok_now ? 1.f : 0.f, lv);
+            in[0] = in[1] = make_float4(ks_now, lv, ok_now ? 1.f : 0.f, 0.f);
           } else {
             in[0] = info[buf][h];
             in[1] = info[buf][2 + h];
@@ -893,7 +901,7 @@ __global__ void __launch_bounds__(256, DT == F32 || HDP > 128 ? 1 : 2) attn_page
           // come back in any order)
           ask_scales();
           ask(base + 3 * kKeyBlock);
-          float lv[2] = {in[0].y, in[1].y}, lv_top = in[0].w;
+          const float lv[2] = {in[0].y, in[1].y};
           const bool ok0 = in[0].z != 0.f, ok1 = in[1].z != 0.f;
           auto seen = [&](int t) -> uint32_t {  // bit i: this row sees key 32 t + 16 h + i
             const int k0 = base + 32 * t + 16 * h, lo = min(max(row_lo - k0, 0), 16), hi = min(max(row_hi - k0, 0), 16);
@@ -907,36 +915,30 @@ __global__ void __launch_bounds__(256, DT == F32 || HDP > 128 ? 1 : 2) attn_page
 #pragma unroll
               for (int j = 0; j < 16; ++j) s[t][j] = (ok[t] >> j) & 1u ? s[t][j] : -__builtin_inff();
             // a page of which the row sees nothing may have anything as scales
-            lv_top = xor32_max(fmaxf(ok[0] ? lv[0] : -126.f, ok[1] ? lv[1] : -126.f));
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-              in[t].x = ok[t] ? in[t].x : 1.f;
-              lv[t] = ok[t] ? lv[t] : fmaxf(lv_top, lref);
-            }
+            for (int t = 0; t < 2; ++t) in[t].x = ok[t] ? in[t].x : 1.f;
           }
-          const float lnew = fmaxf(lv_top, lref);
-          const float rescale = lnew == lref ? 1.f : __builtin_amdgcn_exp2f(lref - lnew);
-          lref = lnew;
           // (c_row and a page's scale are positive: the largest raw score is its largest score)
-          float f[2] = {in[0].x * c_row, in[1].x * c_row}, top = -__builtin_inff();
+          float f[2] = {in[0].x * c_row, in[1].x * c_row}, top = -__builtin_inff(), both = -__builtin_inff();
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
             f[t] = f[t] == 0.f ? 1e-37f : f[t];  // (so that a masked score stays -inf)
             float m = s[t][0];
 #pragma unroll
             for (int j = 1; j < 16; ++j) m = fmaxf(m, s[t][j]);
-            top = fmaxf(top, m > -__builtin_inff() ? m * f[t] : m);
+            m = m > -__builtin_inff() ? m * f[t] : -__builtin_inff();
+            top = fmaxf(top, m);
+            if constexpr (!ONE) both = fmaxf(both, m > -__builtin_inff() ? m + lv[t] : m);
           }
           top = xor32_max(top);
-          top = top > mx + kRaise ? top : mx;
-          float ref = top > -__builtin_inff() ? top : 0.f;
-          const float down = mx == top ? 1.f : __builtin_amdgcn_exp2f(mx - ref);
-          mx = top;
-          if (__any(down * rescale != 1.f)) {
+          both = ONE ? top + lv[0] : xor32_max(both);
+          float down, down_both;
+          if (__any(passes(top, both, mx, lref, down, down_both))) {
             l *= down;
 #pragma unroll
-            for (int i = 0; i < MT; ++i) acc[i] *= down * rescale;
+            for (int i = 0; i < MT; ++i) acc[i] *= down_both;
           }
+          float ref = mx > -__builtin_inff() ? mx : 0.f;
           const bool far = __builtin_fabsf(ref) > 65536.f;
           if (__any(far)) {
 #pragma clang fp contract(off)
@@ -965,7 +967,7 @@ __global__ void __launch_bounds__(256, DT == F32 || HDP > 128 ? 1 : 2) attn_page
           read_values(0);
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
-            const float lf = fmaxf(lv[t] - lnew, -kApart), unscale = __builtin_amdgcn_exp2f(-lf), lift = __builtin_amdgcn_exp2f(lf + kLift),
+            const float lf = apart<NP>(lv[t], lref), unscale = __builtin_amdgcn_exp2f(-lf), lift = __builtin_amdgcn_exp2f(lf + kLift),
                         shift = lf + kLift - ref;
             float sum = 0.f;
             f16x8 pf[NP][2];

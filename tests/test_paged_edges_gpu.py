@@ -192,3 +192,25 @@ def test_values_near_the_largest(torch, hip, dtype, lens, new):  # noqa: F811
         c.vs[:] = 2.0 ** 118
         c.vs[c.tables[0][1]] = 2.0 ** -12
         check(torch, hip, c, 2, dtype, what="large values")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("P", [16, 64])
+@pytest.mark.parametrize("apart", [20, 40, 100])
+def test_large_values_of_no_weight(torch, hip, dtype, new, P, apart):  # noqa: F811
+    """Pages of values 2^apart larger, whose scores lie 56 (168) below the others', leave the others' precision alone."""
+    low = -9 if dtype == "float16" else -30  # (an fp16 output stays above its type's least step)
+    c = Cache(torch, 2, 64, P, [300, 150], [new, new], seed=5, spread=1.0)
+    c.ks[:], c.vs[:] = 2.0 ** -6, 2.0 ** low
+    c.kc[..., 0] = torch.where(c.kc[..., 0] == E4M3_NAN, E4M3_NAN, 0).to(torch.uint8)
+    for b, p in ((0, 0), (0, 3), (1, 1)):
+        g = c.tables[b][p]
+        c.vs[g] = 2.0 ** (apart + low)
+        c.kc[g, :, :, 0] = torch.where(c.kc[g, :, :, 0] == E4M3_NAN, E4M3_NAN, 0xFE).to(torch.uint8)  # -448
+    q = queries(torch, c.cu[-1], 4, 64, dtype)
+    q[:, :, 0] = 8.0 if apart < 100 else 24.0
+    out = torch.full_like(q, 7.0)
+    ref, tol = attend_reference(torch, c, q, out, 1.0)
+    c.attend(hip, q, out, scale=1.0)
+    assert_within(torch, out, ref, tol, "large values of no weight")
