@@ -241,7 +241,8 @@ int mh_attention_textbook(int dt, const void *q, const void *k, const void *v, v
  * width are exhausted, a held entry lies outside the pool) gets slot -1, a page
  * that could not be had the entry -1, tokens past n_slots are left out (cu stops
  * there), and the error flag is raised.  Outputs overlap no input and no other
- * output.  Nothing is done for B = 0; B is below 2^24. */
+ * output.  Nothing is done for B = 0; B is at most 2^20 (above some 10^4 requests
+ * the time grows with B^2). */
 int mh_page_plan(const int32_t *lens, const int32_t *new_lens, const int32_t *free_pages, int32_t *tables,
                  int32_t *total_lens, int32_t *cu, int32_t *slots, int32_t *positions, int32_t *used, int B, int n_free,
                  int width, int page, int n_pages, int n_slots, void *stream);

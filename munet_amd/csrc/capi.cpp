@@ -602,7 +602,7 @@ int mh_page_plan(const int32_t *lens, const int32_t *new_lens, const int32_t *fr
   MH_TRY({
     check_page("page_plan", page, n_pages);
     if (B < 0 || n_free < 0 || width < 0 || n_slots < 0) throw Error("page_plan: negative size");
-    if (B >= 1 << 24) throw Error("page_plan: more requests than one launch takes (2^24 - 1)");
+    if (B > kPlanMaxRequests) throw Error("page_plan: more requests than one launch takes (2^20)");
     if (int64_t(width) * page > kPagedMaxKeys) throw Error("page_plan: a table row must hold at most 2^31 - 4096 tokens");
     if (B == 0) return 0;
     if (!lens || !new_lens || !total_lens || !cu || !used || (width && !tables) || (n_free && !free_pages) ||

@@ -72,6 +72,8 @@ __host__ __device__ __forceinline__ PlanNeed plan_need(int len, int fresh, int p
   if (n.need < n.have) n.need = n.have;
   return n;
 }
+// Requests of a plan: its work grows with their square (2^18 take 46 ms).
+constexpr int kPlanMaxRequests = 1 << 20;
 // Workgroups per request of the plan, which go round its tokens: one for each
 // 1024 tokens that there may be, at most 1024 in all (one prompt of 131072
 // tokens 6 us, 302 with one workgroup; 12 of 2500 4.0 against 6.6).

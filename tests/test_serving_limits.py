@@ -5,7 +5,7 @@ import ctypes
 import pytest
 
 from munet_amd import _lib
-from test_serving_args import _attend, _sample
+from test_serving_args import _attend, _plan, _sample
 
 
 @pytest.mark.parametrize("scale", [2.0 ** 127 * 1.0001, -3e38, 3.4e38])
@@ -37,3 +37,9 @@ def test_launch_limits():
 
     assert workspace(1 << 16) > 0
     assert workspace(1 << 26) == 0  # (rows that pad the batch, more than one launch joins: no shares)
+
+
+def test_plans_of_millions_of_requests():
+    """Work that grows with the square of the requests ends in time."""
+    with pytest.raises(_lib.HipError, match="one launch takes"):
+        _plan(B=(1 << 20) + 1)
