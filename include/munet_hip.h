@@ -270,8 +270,9 @@ int mh_kv_store_paged(int dt, const void *k, const void *v, int64_t ldk, int64_t
  * window > 0 only j > p - window.  out = softmax(scale q k) v over those, zeros
  * for a query that sees none; scale 0 means 1 / sqrt(hd), and |scale| is at most
  * 2^127.  Rows of no request are left as they are.  Scores, softmax and sums are
- * fp32, for fp16 and bf16 probabilities enter the product with the values as
- * fp16.
+ * fp32; a probability times its page's value scale enters the product with the
+ * values as fp16 (for float32 as two fp16 parts, as does q), relative to the
+ * row's largest.
  * max_q and max_len bound the requests' query and key counts; they size the
  * launch (larger ones on the device are still served, more slowly).  B * Hkv is
  * below 2^23, n_rows * Hq at most 2^30.

@@ -602,9 +602,10 @@ __global__ void __launch_bounds__(256) attn_paged_kernel(PagedArgs a) {
 // addresses and two scales, scalars that each wave has.  With smaller pages the first
 // wave puts the runs' scales into LDS for the others, who wait for it (6 chunks
 // of 6700 tokens in all that end at 1200 to 8000 keys, 32 heads on 8 of 128, pages of
-// 64: 622 us so, 561 with ONE).
+// 64: 520 us a pass so, 452 with ONE).
 // Registers bound the waves: 64 outputs, 32 of q and 32 scores a lane at hd 128
-// leave two waves to a SIMD; fp32 and heads above 128 take all registers for one.
+// leave two waves to a SIMD, with 11 to 21 of 256 spilled; fp32 and heads above 128
+// take all registers for one.
 template <int DT, int HDP, bool ONE>
 __global__ void __launch_bounds__(256, DT == F32 || HDP > 128 ? 1 : 2) attn_paged_wide_kernel(PagedArgs a) {
   typedef typename Store<DT>::T T;
@@ -854,7 +855,7 @@ __global__ void __launch_bounds__(256, DT == F32 || HDP > 128 ? 1 : 2) attn_page
       for (int base = first; base < mine.hi; base += kKeyBlock, buf ^= 1) {
         // The next block into LDS, and the one behind it on its way: its bytes have
         // the whole of this block to arrive (loaded after the scores and placed behind the
-        // values' product, 672 us where this took 660).
+        // values' product, 672 us where this took 660, when small pages' form served all).
         const float ks_now = ks_next, vs_now = vs_next;
         const bool ok_now = p_near >= 0;
         if (base + kKeyBlock < mine.hi) place(base + kKeyBlock, buf ^ 1);
