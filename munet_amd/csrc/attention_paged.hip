@@ -1046,8 +1046,8 @@ __global__ void __launch_bounds__(256, DT == F32 || HDP > 128 ? 1 : 2) attn_page
 }
 
 // The shares of a row joined: M the largest maximum, o = sum_s o_s l_s 2^(m_s - M) /
-// sum_s l_s 2^(m_s - M), divided at each step (the sum may pass a float).  The cut of a workgroup is JoinShape's; a row's groups are
-// added in group order.
+// sum_s l_s 2^(m_s - M), divided at each step (the products may pass a float).  The
+// cut of a workgroup is JoinShape's; a row's groups are added in group order.
 template <int DT>
 __global__ void __launch_bounds__(kJoinThreads)
 paged_join_kernel(const float *__restrict__ part_o, const float2 *__restrict__ part_ml, const int32_t *__restrict__ cu, void *out,
