@@ -290,6 +290,77 @@ int mh_attention_paged(int dt, const void *q, int64_t ldq, const void *k_cache, 
                        int max_len, int causal, int window, float scale, void *workspace, size_t workspace_bytes,
                        void *stream);
 
+/* ---- rotary positions ----------------------------------------------------------
+ * No counterpart in the reference, whose positions are learned vectors
+ * (mh_embedding_pos).  A head's first 2 * half values are `half` pairs, each turned
+ * by position * frequency: pair j is (x_j, x_{j + half}), or with `interleaved`
+ * (x_2j, x_{2j + 1}); what lies behind them stays.  The angles of a step's tokens
+ * are worked out once (mh_rotary_table) and read by every layer.  None of the calls
+ * on a stream allocates; all may be captured. */
+
+/* Frequencies of a rotation of `rot` values (even) of each head, on the host: freq
+ * [rot / 2] gets base^(-2 j / rot), changed for contexts longer than the trained:
+ *   MH_ROTARY_PLAIN   as they are;
+ *   MH_ROTARY_LINEAR  divided by `factor` (positions drawn together);
+ *   MH_ROTARY_BASE    of the base times factor^(rot / (rot - 2)) (rot from 4 on): the
+ *                     fastest stays, the slowest is divided by factor;
+ *   MH_ROTARY_TURNS   by the turns r = original freq / (2 pi) that a pair makes over
+ *                     the `original` trained positions: from `high` turns on as it
+ *                     is, up to `low` divided by factor, between in proportion
+ *                     (g f + (1 - g) f / factor, g = (r - low) / (high - low)).
+ * *magnitude (may be NULL) gets what tables are to be multiplied by: 1 + 0.1
+ * ln(factor) for MH_ROTARY_TURNS with a factor above 1, else 1. */
+#define MH_ROTARY_PLAIN 0
+#define MH_ROTARY_LINEAR 1
+#define MH_ROTARY_BASE 2
+#define MH_ROTARY_TURNS 3
+int mh_rotary_frequencies(double *freq, double *magnitude, int rot, double base, int scaling, double factor, double original,
+                          double low, double high);
+/* table [n][half][2] = magnitude * (cos a, sin a), a = positions[t] * freq[j] (device
+ * arrays; the angles in 64 bits, any int32 position).  table is 16-byte aligned. */
+int mh_rotary_table(const int32_t *positions, const double *freq, float *table, int n, int half, double magnitude, void *stream);
+/* out = x with its pairs (a, b) turned to (a c - b s, a s + b c); with `inverse` s
+ * counts negative, which is also the gradient.  x, out: n token rows of heads * hd
+ * values of `dt`, ldx / ldo values apart; table [n][half][2], 2 half <= hd.  out is
+ * x (with ldo = ldx) or does not overlap it.  heads * hd is at most 2^30. */
+int mh_rotary(int dt, const void *x, int64_t ldx, const float *table, void *out, int64_t ldo, int n, int heads, int hd, int half,
+              int interleaved, int inverse, void *stream);
+/* mh_kv_store_paged of keys that are rotated on the way (the cache's 8 bits are
+ * their only rounding; mh_kv_store_paged has the other arguments and what is
+ * written), and in the same launch q [n][Hq * hd] (rows ldq values apart) rotated
+ * into q_out (ldqo apart; q itself, or not overlapping q, k or v).  q NULL: none.
+ * Rows of q whose slot is -1 or outside the pool are left as they are in q_out.
+ * Rows of q and q_out are multiples of 16 bytes apart, as are the pointers. */
+int mh_kv_store_rotary_paged(int dt, const void *k, const void *v, int64_t ldk, int64_t ldv, const float *table,
+                             const int32_t *slots, void *k_cache, void *v_cache, float *k_scale, float *v_scale, int n, int Hkv,
+                             int hd, int half, int interleaved, int page, int n_pages, const void *q, int64_t ldq, void *q_out,
+                             int64_t ldqo, int Hq, void *stream);
+
+/* ---- products in 8-bit integers --------------------------------------------------
+ * No counterpart in the reference.  Rows of values (a token's activations, an output
+ * channel's weights) as int8 with one float scale each, and nn::Linear on them.
+ * None of these calls allocates; all may be captured. */
+
+/* q = the whole numbers nearest to 127 x / a (ties to even), scale = a / 127, a the
+ * row's largest magnitude, at least 127 * 2^-126.  A row with NaN or infinities
+ * gets the scale NaN (and q = 0): what is computed from it is NaN.  x [rows][cols]
+ * of `dt`, rows ldx values apart, q ldq apart, of any alignment; q may not overlap
+ * x. */
+int mh_quantize_rows(int dt, const void *x, int64_t ldx, int8_t *q, int64_t ldq, float *scale, int rows, int cols, void *stream);
+/* out = q * scale of its row, rounded to `dt`. */
+int mh_dequantize_rows(int dt, const int8_t *q, int64_t ldq, const float *scale, void *out, int64_t ldo, int rows, int cols,
+                       void *stream);
+/* out[m][n] = act(x_scale[m] w_scale[n] sum_k x[m][k] w[n][k] + bias[n]) + resid[m][n]:
+ * mh_linear with both operands in int8, [M][K] rows ldx and [N][K] rows ldw apart, of
+ * any alignment (multiples of 16 bytes are faster).  bias (may be NULL), resid (may be
+ * NULL; rows ldr apart) and out (ldo apart) are of `dt`; act is MH_ACT_*, GELU
+ * x * sigmoid(1.702 x).  The sum is exact in int32 (K is at most 2^17 - 1), the rest
+ * in fp32, rounded once.  out may be resid (with ldo = ldr), else it overlaps
+ * neither it nor x or w. */
+int mh_linear_i8(int dt, const int8_t *x, int64_t ldx, const float *x_scale, const int8_t *w, int64_t ldw, const float *w_scale,
+                 const void *bias, const void *resid, int64_t ldr, void *out, int64_t ldo, int M, int N, int K, int act,
+                 void *stream);
+
 /* ---- sampling ----------------------------------------------------------------
  * No counterpart in the reference (its demos take np.argmax, mh_argmax here):
  * one token per row of logits [rows][cols] (rows ld values apart), drawn with

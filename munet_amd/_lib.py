@@ -71,6 +71,13 @@ _SIGS = {
     "mh_attention_paged": [_i, _vp, _i64] + [_vp] * 8 + [_i64] + [_i] * 12 + [_f, _vp, _sz, _vp],
     "mh_sample_workspace": [_i, _i, _i, ctypes.POINTER(_sz)],
     "mh_sample": [_i, _vp, _i64, _i, _i] + [_vp] * 8 + [_sz, _vp],
+    "mh_rotary_frequencies": [ctypes.POINTER(_d), ctypes.POINTER(_d), _i, _d, _i, _d, _d, _d, _d],
+    "mh_rotary_table": [_vp, _vp, _vp, _i, _i, _d, _vp],
+    "mh_rotary": [_i, _vp, _i64, _vp, _vp, _i64] + [_i] * 6 + [_vp],
+    "mh_kv_store_rotary_paged": [_i, _vp, _vp, _i64, _i64] + [_vp] * 6 + [_i] * 7 + [_vp, _i64, _vp, _i64, _i, _vp],
+    "mh_quantize_rows": [_i, _vp, _i64, _vp, _i64, _vp, _i, _i, _vp],
+    "mh_dequantize_rows": [_i, _vp, _i64, _vp, _vp, _i64, _i, _i, _vp],
+    "mh_linear_i8": [_i, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _vp, _i64, _i, _i, _i, _i, _vp],
     "mh_concat": [_i, ctypes.POINTER(_vp), _i, _vp, _i, _i, _ip, _vp],
     "mh_transpose2d": [_i, _vp, _vp, _i, _i, _i, _vp],
     "mh_conv2d": [_i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _i, _vp],

@@ -99,6 +99,16 @@ def _token_rows(op, d, name, x, dtype, shape):
     return x.data_ptr(), n if shape[0] > 1 else shape[1] * shape[2]
 
 
+def _rows(op, d, name, x, dtype, shape):
+    """(address, values between rows) of a matrix on GPU d whose rows are contiguous."""
+    if x.get_device() != d or x.dtype is not dtype or x.shape != shape:
+        _refuse(op, d, name, x, (dtype,), shape, False)
+    n, e = x.stride()
+    if e != 1 and shape[1] > 1:
+        raise ValueError(f"{op}: the rows of {name} must be contiguous")
+    return x.data_ptr(), n if shape[0] > 1 else shape[1]
+
+
 def _pool(op, d, k_cache, v_cache, k_scale, v_scale):
     """Addresses and (pages, Hkv, page, hd) of the paged cache's four tensors."""
     if k_cache.dim() != 4:
@@ -219,6 +229,19 @@ def query_support(feature: str, dtype: int) -> BackendSupport:
     call("mh_query_support", FEATURES.get(feature, -1), dtype, ctypes.byref(av), ctypes.byref(pol),
          ctypes.byref(acc))
     return BackendSupport(bool(av.value), POLICIES[pol.value], acc.value)
+
+
+ROTARY_SCALINGS = {None: 0, "linear": 1, "base": 2, "turns": 3}
+
+
+def rotary_frequencies(rot, base=10000.0, scaling=None, factor=1.0, original=0, low=1.0, high=32.0):
+    """(frequencies, magnitude) for ``rotary_table`` (mh_rotary_frequencies): float64
+    [rot / 2] on the host; ``scaling`` None, "linear", "base" or "turns"."""
+    if scaling not in ROTARY_SCALINGS:
+        raise ValueError(f"rotary_frequencies: scaling must be None, 'linear', 'base' or 'turns', not {scaling!r}")
+    freq, m = (ctypes.c_double * max(1, rot // 2))(), ctypes.c_double()
+    call("mh_rotary_frequencies", freq, ctypes.byref(m), rot, base, ROTARY_SCALINGS[scaling], factor, original, low, high)
+    return np.array(freq, dtype=np.float64), m.value
 
 
 class HipBackend:
@@ -443,6 +466,83 @@ class HipBackend:
         _launch("mh_attention_paged", d, dt, qp, ldq, kc, vc, ks, vs, _operand(op, d, "tables", tables, i32, (B, width)),
                 _operand(op, d, "lens", lens, i32, (B,)), _operand(op, d, "cu", cu, i32, (B + 1,)), po, ldo, B, rows, Hq, Hkv, hd, page,
                 n_pages, width, max_q, max_len, causal, window, scale, wp, wn)
+
+    # ---- rotary positions (no MuNet counterpart) --------------------------------
+    def rotary_table(self, positions, freq, table, magnitude=1.0):
+        """Angles of a step's tokens (mh_rotary_table): ``positions`` [n] int32,
+        ``freq`` [pairs] float64 (``rotary_frequencies``) -> ``table`` [n, pairs, 2]
+        float32, the cosines and sines times ``magnitude``."""
+        op, d, t = "rotary_table", positions.get_device(), _torch()
+        (n,), (half,) = _rank(op, d, "positions", positions, 1), _rank(op, d, "freq", freq, 1)
+        _launch("mh_rotary_table", d, _operand(op, d, "positions", positions, t.int32, (n,)),
+                _operand(op, d, "freq", freq, t.float64, (half,)), _operand(op, d, "table", table, t.float32, (n, half, 2)), n, half,
+                magnitude)
+
+    def rotary(self, x, table, out, interleaved=False, inverse=False):
+        """The first pairs of each head of ``x`` [n, heads, hd] (heads contiguous)
+        turned by ``table`` [n, pairs, 2] into ``out``, which may be ``x``
+        (mh_rotary).  Pairs lie half of the rotated part apart, or ``interleaved``
+        next to each other; ``inverse`` turns back, which is also the gradient."""
+        op, d = "rotary", x.get_device()
+        shape = (n, heads, hd) = _rank(op, d, "x", x, 3)
+        half = _rank(op, d, "table", table, 3)[1]
+        dt = _float_dt(op, "x", x)
+        (xp, ldx), (po, ldo) = _token_rows(op, d, "x", x, x.dtype, shape), _token_rows(op, d, "out", out, x.dtype, shape)
+        _launch("mh_rotary", d, dt, xp, ldx, _operand(op, d, "table", table, _torch().float32, (n, half, 2)), po, ldo, n, heads, hd,
+                half, interleaved, inverse)
+
+    def kv_store_rotary_paged(self, k, v, table, slots, k_cache, v_cache, k_scale, v_scale, q=None, q_out=None, interleaved=False):
+        """``kv_store_paged`` of keys rotated by ``table`` [n, pairs, 2] on the way, and
+        ``q`` [n, Hq, hd] rotated into ``q_out`` (which may be ``q``) in the same launch
+        (mh_kv_store_rotary_paged).  Rows without a slot are left alone."""
+        op, d, t = "kv_store_rotary_paged", k.get_device(), _torch()
+        kc, vc, ks, vs, n_pages, Hkv, page, hd = _pool(op, d, k_cache, v_cache, k_scale, v_scale)
+        n, half = _rank(op, d, "k", k, 3)[0], _rank(op, d, "table", table, 3)[1]
+        shape, dt = (n, Hkv, hd), _float_dt(op, "k", k)
+        (kp, ldk), (vp, ldv) = _token_rows(op, d, "k", k, k.dtype, shape), _token_rows(op, d, "v", v, k.dtype, shape)
+        qp, ldq, po, ldo, Hq = None, 0, None, 0, 0
+        if q is not None:
+            Hq = _rank(op, d, "q", q, 3)[1]
+            if q_out is None:
+                raise ValueError("kv_store_rotary_paged: q needs q_out")
+            (qp, ldq), (po, ldo) = (_token_rows(op, d, "q", q, k.dtype, (n, Hq, hd)),
+                                    _token_rows(op, d, "q_out", q_out, k.dtype, (n, Hq, hd)))
+        _launch("mh_kv_store_rotary_paged", d, dt, kp, vp, ldk, ldv, _operand(op, d, "table", table, t.float32, (n, half, 2)),
+                _operand(op, d, "slots", slots, t.int32, (n,)), kc, vc, ks, vs, n, Hkv, hd, half, interleaved, page, n_pages, qp, ldq,
+                po, ldo, Hq)
+
+    # ---- products in 8-bit integers (no MuNet counterpart) ------------------------
+    def quantize_rows(self, x, q, scale):
+        """Rows of ``x`` [rows, cols] as int8 ``q`` with float32 ``scale`` [rows]
+        (mh_quantize_rows): a linear_i8's tokens, or its weights [out, in]."""
+        op, d, t = "quantize_rows", x.get_device(), _torch()
+        shape = _rank(op, d, "x", x, 2)
+        dt = _float_dt(op, "x", x)
+        (xp, ldx), (qp, ldq) = _rows(op, d, "x", x, x.dtype, shape), _rows(op, d, "q", q, t.int8, shape)
+        _launch("mh_quantize_rows", d, dt, xp, ldx, qp, ldq, _operand(op, d, "scale", scale, t.float32, shape[:1]), *shape)
+
+    def dequantize_rows(self, q, scale, out):
+        """The values that ``quantize_rows`` left, in ``out``'s type (mh_dequantize_rows)."""
+        op, d, t = "dequantize_rows", q.get_device(), _torch()
+        shape = _rank(op, d, "q", q, 2)
+        dt = _float_dt(op, "out", out)
+        (qp, ldq), (po, ldo) = _rows(op, d, "q", q, t.int8, shape), _rows(op, d, "out", out, out.dtype, shape)
+        _launch("mh_dequantize_rows", d, dt, qp, ldq, _operand(op, d, "scale", scale, t.float32, shape[:1]), po, ldo, *shape)
+
+    def linear_i8(self, x, x_scale, w, w_scale, out, bias=None, act=0, resid=None):
+        """``linear`` of int8 tokens ``x`` [M, K] and weights ``w`` [N, K] with a float32
+        scale each (mh_linear_i8): ``out`` [M, N], ``bias`` [N] and ``resid`` [M, N] of
+        one floating type; ``resid`` may be ``out``."""
+        op, d, t = "linear_i8", x.get_device(), _torch()
+        M, K = _rank(op, d, "x", x, 2)
+        N = _rank(op, d, "w", w, 2)[0]
+        dt, i8, f32 = _float_dt(op, "out", out), t.int8, t.float32
+        (xp, ldx), (wp, ldw) = _rows(op, d, "x", x, i8, (M, K)), _rows(op, d, "w", w, i8, (N, K))
+        po, ldo = _rows(op, d, "out", out, out.dtype, (M, N))
+        rp, ldr = (None, 0) if resid is None else _rows(op, d, "resid", resid, out.dtype, (M, N))
+        _launch("mh_linear_i8", d, dt, xp, ldx, _operand(op, d, "x_scale", x_scale, f32, (M,)), wp, ldw,
+                _operand(op, d, "w_scale", w_scale, f32, (N,)), _optional(op, d, "bias", bias, out.dtype, (N,)), rp, ldr, po, ldo, M, N,
+                K, act)
 
     # ---- sampling (no MuNet counterpart) ---------------------------------------
     def sample_workspace(self, logits) -> int:

@@ -248,6 +248,35 @@ void check_rows(const char *op, const char *what, int dt, const void *p, int64_t
   if (ld < cols || ld * int64_t(dt_size(dt)) % 16)
     throw Error(std::string(op) + ": rows of " + what + " must be whole, a multiple of 16 bytes apart");
 }
+// n rows of cols elements, ld apart, aligned to their type.
+void check_whole_rows(const char *op, const char *what, size_t es, const void *p, int64_t n, int64_t ld, int64_t cols) {
+  if (!p) throw Error(std::string(op) + ": null " + what);
+  if (reinterpret_cast<uintptr_t>(p) % es) throw Error(std::string(op) + ": " + what + " must be aligned to its type");
+  if (ld < cols) throw Error(std::string(op) + ": rows of " + what + " must be whole");
+  if (ld > (int64_t(1) << 56) / n) throw Error(std::string(op) + ": rows of " + what + " too far apart");
+}
+// Whether two sets of rows share a byte; sets of the same spacing that lie beside
+// each other (columns of one buffer) do not.
+struct RowSet {
+  const void *p;
+  int64_t rows, ld, cols;  // (in bytes)
+};
+bool rows_meet(const RowSet &a, const RowSet &b) {
+  if (!a.p || !b.p || a.rows < 1 || b.rows < 1 || a.cols < 1 || b.cols < 1) return false;
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a.p), y = reinterpret_cast<uintptr_t>(b.p);
+  const uintptr_t xe = x + uintptr_t((a.rows - 1) * a.ld + a.cols), ye = y + uintptr_t((b.rows - 1) * b.ld + b.cols);
+  if (xe <= y || ye <= x) return false;
+  if (a.rows > 1 && b.rows > 1 && a.ld == b.ld) {
+    const uintptr_t d = (y >= x ? (y - x) : uintptr_t(a.ld) - (x - y) % uintptr_t(a.ld)) % uintptr_t(a.ld);
+    return d < uintptr_t(a.cols) || uintptr_t(a.ld) - d < uintptr_t(b.cols);
+  }
+  return true;
+}
+void check_rotation(const char *op, const float *table, int hd, int half) {
+  if (half < 1 || hd < 1 || half > hd / 2) throw Error(std::string(op) + ": the rotated part must be 2 values at least and fit the head");
+  if (!table) throw Error(std::string(op) + ": null table");
+  aligned16(table, "table");
+}
 void check_sample_size(int rows, int cols) {
   if (rows < 0 || cols < 1) throw Error("sample: bad row count or empty rows");
   if (rows >= 1 << 22) throw Error("sample: more rows than one launch takes (2^22 - 1)");
@@ -716,6 +745,204 @@ int mh_attention_paged(int dt, const void *q, int64_t ldq, const void *k_cache, 
     p.window = window;
     p.scale = scale == 0.f ? float(1.0 / std::sqrt(double(hd))) : scale;
     hip_check(attention_paged(dt, p, s, S_(stream)), "attention_paged");
+  })
+}
+
+// ---- rotary positions ----------------------------------------------------------
+int mh_rotary_frequencies(double *freq, double *magnitude, int rot, double base, int scaling, double factor, double original,
+                          double low, double high) {
+  MH_TRY({
+    if (!freq) throw Error("rotary_frequencies: null freq");
+    if (rot < 2 || rot % 2) throw Error("rotary_frequencies: the rotated part must be an even number of values");
+    if (!(base > 0) || !std::isfinite(base)) throw Error("rotary_frequencies: the base must be positive");
+    if (scaling < MH_ROTARY_PLAIN || scaling > MH_ROTARY_TURNS) throw Error("rotary_frequencies: unknown scaling");
+    if (scaling != MH_ROTARY_PLAIN && (!(factor > 0) || !std::isfinite(factor)))
+      throw Error("rotary_frequencies: the factor must be positive");
+    if (scaling == MH_ROTARY_BASE && rot < 4) throw Error("rotary_frequencies: a changed base needs a rotated part of 4 at least");
+    if (scaling == MH_ROTARY_TURNS && (!(original > 0) || !std::isfinite(original) || !(low >= 0) || !(high > low) || !std::isfinite(high)))
+      throw Error("rotary_frequencies: needs original > 0 and 0 <= low < high");
+    if (scaling == MH_ROTARY_BASE) base *= std::pow(factor, double(rot) / (rot - 2));
+    for (int j = 0; j < rot / 2; ++j) {
+      double f = std::pow(base, -2.0 * j / rot);
+      if (scaling == MH_ROTARY_LINEAR) f /= factor;
+      if (scaling == MH_ROTARY_TURNS) {
+        const double r = original * f / (2 * M_PI), g = std::min(1.0, std::max(0.0, (r - low) / (high - low)));
+        f = g * f + (1 - g) * f / factor;
+      }
+      freq[j] = f;
+    }
+    if (magnitude) *magnitude = scaling == MH_ROTARY_TURNS && factor > 1 ? 1 + 0.1 * std::log(factor) : 1.0;
+  })
+}
+int mh_rotary_table(const int32_t *positions, const double *freq, float *table, int n, int half, double magnitude, void *stream) {
+  MH_TRY({
+    if (n < 0) throw Error("rotary_table: negative size");
+    if (half < 1) throw Error("rotary_table: no pairs");
+    if (n == 0) return 0;
+    if (!positions || !freq || !table) throw Error("rotary_table: null argument");
+    aligned16(table, "table");
+    hip_check(rotary_table(positions, freq, table, n, half, magnitude, S_(stream)), "rotary_table");
+  })
+}
+int mh_rotary(int dt, const void *x, int64_t ldx, const float *table, void *out, int64_t ldo, int n, int heads, int hd, int half,
+              int interleaved, int inverse, void *stream) {
+  MH_TRY({
+    check_dt(dt);
+    if (n < 0) throw Error("rotary: negative size");
+    if (heads < 1 || hd < 1 || int64_t(heads) * hd > 1 << 30) throw Error("rotary: bad head count or size");
+    if (n == 0) return 0;
+    check_rotation("rotary", table, hd, half);
+    const int64_t es = int64_t(dt_size(dt)), cols = int64_t(heads) * hd;
+    check_whole_rows("rotary", "x", es, x, n, ldx, cols);
+    check_whole_rows("rotary", "out", es, out, n, ldo, cols);
+    if (!(x == out && (ldx == ldo || n == 1)) && rows_meet({x, n, ldx * es, cols * es}, {out, n, ldo * es, cols * es}))
+      throw Error("rotary: out overlaps x without being it");
+    Rotary p;
+    p.x = x;
+    p.out = out;
+    p.table = table;
+    p.ldx = ldx;
+    p.ldo = ldo;
+    p.n = n;
+    p.heads = heads;
+    p.hd = hd;
+    p.half = half;
+    p.interleaved = interleaved != 0;
+    p.inverse = inverse != 0;
+    hip_check(rotary(dt, p, S_(stream)), "rotary");
+  })
+}
+int mh_kv_store_rotary_paged(int dt, const void *k, const void *v, int64_t ldk, int64_t ldv, const float *table,
+                             const int32_t *slots, void *k_cache, void *v_cache, float *k_scale, float *v_scale, int n, int Hkv,
+                             int hd, int half, int interleaved, int page, int n_pages, const void *q, int64_t ldq, void *q_out,
+                             int64_t ldqo, int Hq, void *stream) {
+  MH_TRY({
+    const char *op = "kv_store_rotary_paged";
+    check_dt(dt);
+    check_pool(op, k_cache, v_cache, k_scale, v_scale, Hkv, hd, page, n_pages);
+    if (Hkv > 65535 - kStoreQueryRows) throw Error("kv_store_rotary_paged: bad key/value head count");
+    if (n < 0) throw Error("kv_store_rotary_paged: negative size");
+    if (n > 1 << 27) throw Error("kv_store_rotary_paged: more tokens than one launch takes (2^27)");
+    if (q && (Hq < 1 || int64_t(Hq) * hd > 1 << 30)) throw Error("kv_store_rotary_paged: bad query head count");
+    if (n == 0) return 0;
+    if (!slots) throw Error("kv_store_rotary_paged: null slots");
+    check_rotation(op, table, hd, half);
+    check_rows(op, "k", dt, k, ldk, int64_t(Hkv) * hd);
+    check_rows(op, "v", dt, v, ldv, int64_t(Hkv) * hd);
+    Rotary p;
+    p.table = table;
+    p.n = n;
+    p.hd = hd;
+    p.half = half;
+    p.interleaved = interleaved != 0;
+    if (q) {
+      const int64_t es = int64_t(dt_size(dt)), cols = int64_t(Hq) * hd * es;
+      check_rows(op, "q", dt, q, ldq, int64_t(Hq) * hd);
+      check_rows(op, "q_out", dt, q_out, ldqo, int64_t(Hq) * hd);
+      for (int64_t ld : {ldk, ldv, ldq, ldqo})
+        if (ld > (int64_t(1) << 56) / n) throw Error("kv_store_rotary_paged: rows too far apart");
+      const RowSet o{q_out, n, ldqo * es, cols};
+      if ((!(q == q_out && (ldq == ldqo || n == 1)) && rows_meet(o, {q, n, ldq * es, cols})) ||
+          rows_meet(o, {k, n, ldk * es, int64_t(Hkv) * hd * es}) || rows_meet(o, {v, n, ldv * es, int64_t(Hkv) * hd * es}))
+        throw Error("kv_store_rotary_paged: q_out overlaps q without being it, or k or v");
+      p.x = q;
+      p.out = q_out;
+      p.ldx = ldq;
+      p.ldo = ldqo;
+      p.heads = Hq;
+    }
+    hip_check(kv_store_paged(dt, k, v, long(ldk), long(ldv), slots, k_cache, v_cache, k_scale, v_scale, n, Hkv, hd, page, n_pages,
+                             serving_error_flag(), S_(stream), &p),
+              op);
+  })
+}
+
+// ---- products in 8-bit integers ---------------------------------------------------
+int mh_quantize_rows(int dt, const void *x, int64_t ldx, int8_t *q, int64_t ldq, float *scale, int rows, int cols, void *stream) {
+  MH_TRY({
+    check_dt(dt);
+    if (rows < 0 || cols < 1) throw Error("quantize_rows: bad row count or empty rows");
+    if (rows == 0) return 0;
+    const int64_t es = int64_t(dt_size(dt));
+    check_whole_rows("quantize_rows", "x", es, x, rows, ldx, cols);
+    check_whole_rows("quantize_rows", "q", 1, q, rows, ldq, cols);
+    if (!scale) throw Error("quantize_rows: null scale");
+    if (rows_meet({x, rows, ldx * es, cols * es}, {q, rows, ldq, cols})) throw Error("quantize_rows: q overlaps x");
+    QuantRows p;
+    p.x = x;
+    p.q = q;
+    p.scale = scale;
+    p.ldx = ldx;
+    p.ldq = ldq;
+    p.rows = rows;
+    p.cols = cols;
+    hip_check(quantize_rows(dt, p, S_(stream)), "quantize_rows");
+  })
+}
+int mh_dequantize_rows(int dt, const int8_t *q, int64_t ldq, const float *scale, void *out, int64_t ldo, int rows, int cols,
+                       void *stream) {
+  MH_TRY({
+    check_dt(dt);
+    if (rows < 0 || cols < 1) throw Error("dequantize_rows: bad row count or empty rows");
+    if (rows == 0) return 0;
+    const int64_t es = int64_t(dt_size(dt));
+    check_whole_rows("dequantize_rows", "q", 1, q, rows, ldq, cols);
+    check_whole_rows("dequantize_rows", "out", es, out, rows, ldo, cols);
+    if (!scale) throw Error("dequantize_rows: null scale");
+    if (rows_meet({out, rows, ldo * es, cols * es}, {q, rows, ldq, cols})) throw Error("dequantize_rows: out overlaps q");
+    QuantRows p;
+    p.out = out;
+    p.q = const_cast<int8_t *>(q);
+    p.scale = const_cast<float *>(scale);
+    p.ldx = ldo;
+    p.ldq = ldq;
+    p.rows = rows;
+    p.cols = cols;
+    hip_check(dequantize_rows(dt, p, S_(stream)), "dequantize_rows");
+  })
+}
+int mh_linear_i8(int dt, const int8_t *x, int64_t ldx, const float *x_scale, const int8_t *w, int64_t ldw, const float *w_scale,
+                 const void *bias, const void *resid, int64_t ldr, void *out, int64_t ldo, int M, int N, int K, int act,
+                 void *stream) {
+  MH_TRY({
+    check_dt(dt);
+    if (act < 0 || act > 2) throw Error("linear_i8: bad activation code");
+    if (M < 0 || N < 0 || K < 1) throw Error("linear_i8: negative size or empty rows");
+    if (K > kI8MaxK) throw Error("linear_i8: the sums of more than 2^17 - 1 products may pass 32 bits");
+    if (int64_t((int64_t(M) + 63) / 64) * ((int64_t(N) + 63) / 64) > kI8MaxTiles) throw Error("linear_i8: more outputs than one launch takes (2^34)");
+    if (M == 0 || N == 0) return 0;
+    const int64_t es = int64_t(dt_size(dt));
+    check_whole_rows("linear_i8", "x", 1, x, M, ldx, K);
+    check_whole_rows("linear_i8", "w", 1, w, N, ldw, K);
+    check_whole_rows("linear_i8", "out", es, out, M, ldo, N);
+    if (!x_scale || !w_scale) throw Error("linear_i8: null scale");
+    if (bias) check_whole_rows("linear_i8", "bias", es, bias, 1, N, N);
+    const RowSet o{out, M, ldo * es, N * es};
+    if (resid) {
+      check_whole_rows("linear_i8", "resid", es, resid, M, ldr, N);
+      if (!(resid == out && (ldr == ldo || M == 1)) && rows_meet(o, {resid, M, ldr * es, N * es}))
+        throw Error("linear_i8: out overlaps the residual without being it");
+    }
+    if (rows_meet(o, {x, M, ldx, K}) || rows_meet(o, {w, N, ldw, K})) throw Error("linear_i8: out overlaps x or w");
+    LinearI8 p;
+    p.x = x;
+    p.w = w;
+    p.sx = x_scale;
+    p.sw = w_scale;
+    p.bias = bias;
+    p.resid = resid;
+    p.out = out;
+    p.ldx = ldx;
+    p.ldw = ldw;
+    p.ldo = ldo;
+    p.ldr = ldr;
+    p.M = M;
+    p.N = N;
+    p.K = K;
+    p.act = act;
+    const uintptr_t any = reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(bias) | reinterpret_cast<uintptr_t>(resid);
+    p.quads = any % (4 * es) == 0 && (ldo % 4 == 0 || M == 1) && (!resid || ldr % 4 == 0 || M == 1);
+    hip_check(linear_i8(dt, p, S_(stream)), "linear_i8");
   })
 }
 

@@ -262,16 +262,51 @@ struct PagedAttention {
   float scale = 1.f;
 };
 hipError_t attention_paged(int dt, const PagedAttention &p, const PagedShape &s, hipStream_t st);
+// Rotary positions (rotary.hip): token rows of heads * hd values, their first
+// 2 * half of each head rotated by rows of `half` (cosine, sine) pairs
+struct Rotary {
+  const void *x = nullptr;
+  void *out = nullptr;
+  const float *table = nullptr;
+  int64_t ldx = 0, ldo = 0;
+  int n = 0, heads = 0, hd = 0, half = 0, interleaved = 0, inverse = 0;
+};
 // n rows of keys and values (rows ld apart) into their slots (paged_cache.hip)
 hipError_t kv_store_paged(int dt, const void *k, const void *v, long ldk, long ldv, const int32_t *slots, void *k_cache,
                           void *v_cache, float *k_scale, float *v_scale, int n, int Hkv, int hd, int page, int n_pages, int *err,
-                          hipStream_t st);
+                          hipStream_t st, const Rotary *rot = nullptr);  // rot: k is rotated on the way, and rot's rows beside it
 struct PagePlan {
   const int32_t *lens = nullptr, *fresh = nullptr, *free_pages = nullptr;
   int32_t *tables = nullptr, *total = nullptr, *cu = nullptr, *slots = nullptr, *positions = nullptr, *used = nullptr;
   int B = 0, n_free = 0, width = 0, page = 0, n_pages = 0, cap = 0;
 };
 hipError_t page_plan(const PagePlan &p, int *err, hipStream_t st);
+hipError_t rotary_table(const int32_t *positions, const double *freq, float *table, int n, int half, double magnitude,
+                        hipStream_t st);
+hipError_t rotary(int dt, const Rotary &p, hipStream_t st);
+// Rows as 8-bit integers with a scale each, and back (rows_i8.hip)
+struct QuantRows {
+  const void *x = nullptr;  // quantize: the values; ldx is their (and out's) row spacing
+  void *out = nullptr;      // dequantize: the values
+  int8_t *q = nullptr;
+  float *scale = nullptr;
+  int64_t ldx = 0, ldq = 0;
+  int rows = 0, cols = 0;
+};
+hipError_t quantize_rows(int dt, const QuantRows &p, hipStream_t st);
+hipError_t dequantize_rows(int dt, const QuantRows &p, hipStream_t st);
+// Products of 8-bit integers with scales for each row and column (gemm_i8.hip)
+constexpr int kI8MaxK = (1 << 17) - 1;      // K products of magnitude 2^14 in int32
+constexpr int64_t kI8MaxTiles = 1 << 22;    // workgroups of a launch
+struct LinearI8 {
+  const int8_t *x = nullptr, *w = nullptr;
+  const float *sx = nullptr, *sw = nullptr;
+  const void *bias = nullptr, *resid = nullptr;
+  void *out = nullptr;
+  int64_t ldx = 0, ldw = 0, ldo = 0, ldr = 0;
+  int M = 0, N = 0, K = 0, act = 0, quads = 0;  // quads: bias, residual and output go four values at a time
+};
+hipError_t linear_i8(int dt, const LinearI8 &p, hipStream_t st);
 // The next tokens of rows of logits (sample.hip).  Tokens of a row: the end of a group
 // (of 2^21 tokens in rows of that length) and the tokens that a workgroup looks at past
 // the row's last chunk have 32-bit indexes.

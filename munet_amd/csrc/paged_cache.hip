@@ -3,6 +3,7 @@
 #include "mh_common.hpp"
 #include "mh_kernels.hpp"
 #include "paged_index.hpp"
+#include "rotary.hpp"
 
 namespace mh {
 namespace {
@@ -155,6 +156,25 @@ template <int DT> struct Raw {
   }
 };
 
+// A token's eight key values from d on: as they lie, or rotated on the way (ROT 1:
+// pairs half a head apart, 2: neighbours).  Rotated keys are held as floats, so that
+// the cache's 8 bits are their only rounding.
+template <int DT, int ROT> struct Key {
+  float f[8];
+  __device__ __forceinline__ void load(const typename Store<DT>::T *head, const float2 *tab, int half, int d) {
+    turned8<DT, ROT == 2>(head, tab, half, d, f);
+  }
+  __device__ __forceinline__ void get(float v[8]) const {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = f[e];
+  }
+};
+template <int DT> struct Key<DT, 0> {
+  Raw<DT> r;
+  __device__ __forceinline__ void load(const typename Store<DT>::T *head, const float2 *, int, int d) { r.load(head + d); }
+  __device__ __forceinline__ void get(float v[8]) const { r.get(v); }
+};
+
 struct StoreArgs {
   const void *k, *v;
   const int32_t *slots;
@@ -163,13 +183,14 @@ struct StoreArgs {
   int *err;
   long ldk, ldv;
   int n, Hkv, hd, page, n_pages, per;
+  Rotary q;  // the table and, where there are queries, their rotation (workgroups behind the heads')
 };
 
 // A run is a stretch of tokens with consecutive slots inside one page.  The
 // workgroup that holds a run's first token writes all of it for one head, and
 // so owns the page's two scales.  Tokens at `per` consecutive places per
 // workgroup.
-template <int DT, int NT>
+template <int DT, int NT, int ROT>
 __global__ void __launch_bounds__(NT) kv_store_paged_kernel(StoreArgs a) {
   typedef typename Store<DT>::T T;
   constexpr int VT = 64;  // tokens of a value tile
@@ -180,6 +201,14 @@ __global__ void __launch_bounds__(NT) kv_store_paged_kernel(StoreArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, head = blockIdx.y;
   const int t0 = blockIdx.x * a.per, hd = a.hd, P = a.page, h8 = hd / 8;
   const int64_t limit = int64_t(a.n_pages) * P;
+  if constexpr (ROT != 0) {
+    if (head >= a.Hkv) {
+      const int64_t step = int64_t(gridDim.y - a.Hkv) * gridDim.x;
+      for (int64_t t = int64_t(head - a.Hkv) * gridDim.x + blockIdx.x; t < a.n; t += step)
+        if (a.slots[t] >= 0 && a.slots[t] < limit) rotate_token<DT, NT>(a.q, t);
+      return;
+    }
+  }
   // the run starts among this workgroup's tokens (every wave finds the same)
   uint64_t starts;
   {
@@ -211,7 +240,13 @@ __global__ void __launch_bounds__(NT) kv_store_paged_kernel(StoreArgs a) {
     }
     const T *kp = static_cast<const T *>(a.k) + int64_t(t) * a.ldk + int64_t(head) * hd;
     const T *vp = static_cast<const T *>(a.v) + int64_t(t) * a.ldv + int64_t(head) * hd;
+    const float2 *tab = ROT ? reinterpret_cast<const float2 *>(a.q.table) + int64_t(t) * a.q.half : nullptr;
     uint8_t *kd = a.kc + page_base(page, a.Hkv, head, P, hd), *vd = a.vc + page_base(page, a.Hkv, head, P, hd);
+
+    auto key8 = [&](int i, int d, float v[8]) {
+      if constexpr (ROT) turned8<DT, ROT == 2>(kp + int64_t(i) * a.ldk, tab + int64_t(i) * a.q.half, a.q.half, d, v);
+      else ld8<DT>(kp + int64_t(i) * a.ldk + d, v);
+    };
 
     // A run of at most NT pieces of 4 places and 8 head values (NT 256: 64 tokens of
     // heads of 128) is held in registers, a piece to a thread: loaded once, its values
@@ -221,13 +256,14 @@ __global__ void __launch_bounds__(NT) kv_store_paged_kernel(StoreArgs a) {
     const bool held_run = nq * h8 <= NT;
     const int pq = tid / h8, pd = 8 * (tid - pq * h8), pi = 4 * (q0 + pq) - place;  // this thread's piece: first token
     const bool mine = held_run && pq < nq;
-    Raw<DT> kr[4], vr[4];
+    Key<DT, ROT> kr[4];
+    Raw<DT> vr[4];
     float big[2] = {0.f, 0.f};
     if (mine) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int64_t i = min(max(pi + j, 0), n - 1);  // (places beside the run repeat its tokens, not stored)
-        kr[j].load(kp + i * a.ldk + pd);
+        kr[j].load(kp + i * a.ldk, tab + (ROT ? i * a.q.half : 0), a.q.half, pd);
         vr[j].load(vp + i * a.ldv + pd);
       }
 #pragma unroll
@@ -242,7 +278,7 @@ __global__ void __launch_bounds__(NT) kv_store_paged_kernel(StoreArgs a) {
     for (int c = held_run ? n * h8 : tid; c < n * h8; c += NT) {
       const int i = c / h8, d = 8 * (c - i * h8);
       float v[8];
-      ld8<DT>(kp + int64_t(i) * a.ldk + d, v);
+      key8(i, d, v);
       big[0] = amax8(v, big[0]);
       ld8<DT>(vp + int64_t(i) * a.ldv + d, v);
       big[1] = amax8(v, big[1]);
@@ -344,7 +380,7 @@ __global__ void __launch_bounds__(NT) kv_store_paged_kernel(StoreArgs a) {
     for (int c = tid; c < n * h8; c += NT) {
       const int i = c / h8, d = 8 * (c - i * h8);
       float v[8];
-      ld8<DT>(kp + int64_t(i) * a.ldk + d, v);
+      key8(i, d, v);
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] *= inv[0];
       *reinterpret_cast<uint2 *>(kd + int64_t(place + i) * hd + d) = make_uint2(e4m3x4(v), e4m3x4(v + 4));
@@ -394,28 +430,41 @@ hipError_t page_plan(const PagePlan &p, int *err, hipStream_t st) {
 
 hipError_t kv_store_paged(int dt, const void *k, const void *v, long ldk, long ldv, const int32_t *slots, void *k_cache,
                           void *v_cache, float *k_scale, float *v_scale, int n, int Hkv, int hd, int page, int n_pages, int *err,
-                          hipStream_t st) {
+                          hipStream_t st, const Rotary *rot) {
   if (n < 1 || n > 1 << 27 || Hkv < 1 || Hkv > 65535) return hipErrorInvalidValue;
   StoreArgs a{k, v, slots, static_cast<uint8_t *>(k_cache), static_cast<uint8_t *>(v_cache), k_scale, v_scale, err, ldk, ldv,
-              n, Hkv, hd, page, n_pages, store_tokens(n, Hkv)};
-  const dim3 grid(unsigned((n + a.per - 1) / a.per), unsigned(Hkv));
+              n, Hkv, hd, page, n_pages, store_tokens(n, Hkv), rot ? *rot : Rotary{}};
+  dim3 grid(unsigned((n + a.per - 1) / a.per), unsigned(Hkv));
+  if (rot && rot->heads) {
+    if (Hkv > 65535 - kStoreQueryRows) return hipErrorInvalidValue;
+    grid.y += unsigned(std::min(kStoreQueryRows, a.per));
+  }
   // Threads for a page's pieces at once where workgroups take many tokens (17k
   // tokens, 8 heads of 128: pages of 128 42 us, 56 with 256 threads; of 256 56, 60);
   // where they take one, most would be idle.
   const int pieces = page / 4 * (hd / 8), nt = a.per == 1 || pieces <= 256 ? 256 : pieces <= 512 ? 512 : 1024;
-#define MH_STORE(DTV)                                                                                     \
+#define MH_STORE(DTV, ROT)                                                                                \
   if (nt == 256)                                                                                          \
-    hipLaunchKernelGGL((kv_store_paged_kernel<DTV, 256>), grid, dim3(256), 0, st, a);                     \
+    hipLaunchKernelGGL((kv_store_paged_kernel<DTV, 256, ROT>), grid, dim3(256), 0, st, a);                \
   else if (nt == 512)                                                                                     \
-    hipLaunchKernelGGL((kv_store_paged_kernel<DTV, 512>), grid, dim3(512), 0, st, a);                     \
+    hipLaunchKernelGGL((kv_store_paged_kernel<DTV, 512, ROT>), grid, dim3(512), 0, st, a);                \
   else                                                                                                    \
-    hipLaunchKernelGGL((kv_store_paged_kernel<DTV, 1024>), grid, dim3(1024), 0, st, a);
+    hipLaunchKernelGGL((kv_store_paged_kernel<DTV, 1024, ROT>), grid, dim3(1024), 0, st, a);
+#define MH_STORE_ROT(DTV)                                                                                 \
+  if (!rot) {                                                                                             \
+    MH_STORE(DTV, 0)                                                                                      \
+  } else if (rot->interleaved) {                                                                          \
+    MH_STORE(DTV, 2)                                                                                      \
+  } else {                                                                                                \
+    MH_STORE(DTV, 1)                                                                                      \
+  }
   switch (dt) {
-  case F32: MH_STORE(F32) break;
-  case F16: MH_STORE(F16) break;
-  case BF16: MH_STORE(BF16) break;
+  case F32: MH_STORE_ROT(F32) break;
+  case F16: MH_STORE_ROT(F16) break;
+  case BF16: MH_STORE_ROT(BF16) break;
   default: return hipErrorInvalidValue;
   }
+#undef MH_STORE_ROT
 #undef MH_STORE
   return hipGetLastError();
 }

@@ -1,0 +1,56 @@
+// Rotary positions: the angles of a step's tokens, worked out once for all
+// layers, and the rotation of token rows by them (rotary.hpp has the pairs).
+#include <algorithm>
+
+#include "mh_common.hpp"
+#include "mh_kernels.hpp"
+#include "rotary.hpp"
+
+namespace mh {
+namespace {
+
+// ---- rotary_table --------------------------------------------------------------
+
+// (m cos a, m sin a) of a = position * frequency, in 64 bits: a document's
+// position is a million turns of the fastest pair, of which 32 bits would leave
+// four digits of the last one.
+__global__ void __launch_bounds__(256) rotary_table_kernel(const int32_t *__restrict__ pos, const double *__restrict__ freq,
+                                                           float2 *__restrict__ table, int64_t total, int half, double m) {
+  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < total; i += int64_t(gridDim.x) * 256) {
+    const int64_t t = i / half;
+    const int j = int(i - t * half);
+    double s, c;
+    sincos(double(pos[t]) * freq[j], &s, &c);
+    table[i] = make_float2(float(m * c), float(m * s));
+  }
+}
+
+// ---- rotary --------------------------------------------------------------------
+
+template <int DT> __global__ void __launch_bounds__(256) rotary_kernel(Rotary p) {
+  for (int64_t t = blockIdx.x; t < p.n; t += gridDim.x) rotate_token<DT, 256>(p, t);
+}
+
+}  // namespace
+
+hipError_t rotary_table(const int32_t *positions, const double *freq, float *table, int n, int half, double magnitude,
+                        hipStream_t st) {
+  const int64_t total = int64_t(n) * half;
+  const unsigned grid = unsigned(std::min<int64_t>((total + 255) / 256, 1 << 20));
+  hipLaunchKernelGGL(rotary_table_kernel, dim3(grid), dim3(256), 0, st, positions, freq, reinterpret_cast<float2 *>(table), total,
+                     half, magnitude);
+  return hipGetLastError();
+}
+
+hipError_t rotary(int dt, const Rotary &p, hipStream_t st) {
+  const unsigned grid = unsigned(std::min(p.n, 1 << 20));
+  switch (dt) {
+  case F32: hipLaunchKernelGGL(rotary_kernel<F32>, dim3(grid), dim3(256), 0, st, p); break;
+  case F16: hipLaunchKernelGGL(rotary_kernel<F16>, dim3(grid), dim3(256), 0, st, p); break;
+  case BF16: hipLaunchKernelGGL(rotary_kernel<BF16>, dim3(grid), dim3(256), 0, st, p); break;
+  default: return hipErrorInvalidValue;
+  }
+  return hipGetLastError();
+}
+
+}  // namespace mh
