@@ -809,7 +809,7 @@ int mh_rotary(int dt, const void *x, int64_t ldx, const float *table, void *out,
     p.half = half;
     p.interleaved = interleaved != 0;
     p.inverse = inverse != 0;
-    hip_check(rotary(dt, p, S_(stream)), "rotary");
+    hip_check(rotary(dt, p, nullptr, 0, S_(stream)), "rotary");
   })
 }
 int mh_kv_store_rotary_paged(int dt, const void *k, const void *v, int64_t ldk, int64_t ldv, const float *table,
@@ -820,7 +820,6 @@ int mh_kv_store_rotary_paged(int dt, const void *k, const void *v, int64_t ldk, 
     const char *op = "kv_store_rotary_paged";
     check_dt(dt);
     check_pool(op, k_cache, v_cache, k_scale, v_scale, Hkv, hd, page, n_pages);
-    if (Hkv > 65535 - kStoreQueryRows) throw Error("kv_store_rotary_paged: bad key/value head count");
     if (n < 0) throw Error("kv_store_rotary_paged: negative size");
     if (n > 1 << 27) throw Error("kv_store_rotary_paged: more tokens than one launch takes (2^27)");
     if (q && (Hq < 1 || int64_t(Hq) * hd > 1 << 30)) throw Error("kv_store_rotary_paged: bad query head count");

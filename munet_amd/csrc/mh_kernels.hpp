@@ -270,6 +270,7 @@ struct Rotary {
   const float *table = nullptr;
   int64_t ldx = 0, ldo = 0;
   int n = 0, heads = 0, hd = 0, half = 0, interleaved = 0, inverse = 0;
+  int units = 0, lanes = 0, tokens = 0;  // the cut (rotary.hpp)
 };
 // n rows of keys and values (rows ld apart) into their slots (paged_cache.hip)
 hipError_t kv_store_paged(int dt, const void *k, const void *v, long ldk, long ldv, const int32_t *slots, void *k_cache,
@@ -283,7 +284,8 @@ struct PagePlan {
 hipError_t page_plan(const PagePlan &p, int *err, hipStream_t st);
 hipError_t rotary_table(const int32_t *positions, const double *freq, float *table, int n, int half, double magnitude,
                         hipStream_t st);
-hipError_t rotary(int dt, const Rotary &p, hipStream_t st);
+// slots (may be null): tokens without a slot in 0 .. limit - 1 are left alone
+hipError_t rotary(int dt, Rotary p, const int32_t *slots, int64_t limit, hipStream_t st);
 // Rows as 8-bit integers with a scale each, and back (rows_i8.hip)
 struct QuantRows {
   const void *x = nullptr;  // quantize: the values; ldx is their (and out's) row spacing

@@ -183,7 +183,8 @@ struct StoreArgs {
   int *err;
   long ldk, ldv;
   int n, Hkv, hd, page, n_pages, per;
-  Rotary q;  // the table and, where there are queries, their rotation (workgroups behind the heads')
+  const float2 *table;  // rotated keys: their angles
+  int half;
 };
 
 // A run is a stretch of tokens with consecutive slots inside one page.  The
@@ -201,14 +202,6 @@ __global__ void __launch_bounds__(NT) kv_store_paged_kernel(StoreArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, head = blockIdx.y;
   const int t0 = blockIdx.x * a.per, hd = a.hd, P = a.page, h8 = hd / 8;
   const int64_t limit = int64_t(a.n_pages) * P;
-  if constexpr (ROT != 0) {
-    if (head >= a.Hkv) {
-      const int64_t step = int64_t(gridDim.y - a.Hkv) * gridDim.x;
-      for (int64_t t = int64_t(head - a.Hkv) * gridDim.x + blockIdx.x; t < a.n; t += step)
-        if (a.slots[t] >= 0 && a.slots[t] < limit) rotate_token<DT, NT>(a.q, t);
-      return;
-    }
-  }
   // the run starts among this workgroup's tokens (every wave finds the same)
   uint64_t starts;
   {
@@ -240,11 +233,11 @@ __global__ void __launch_bounds__(NT) kv_store_paged_kernel(StoreArgs a) {
     }
     const T *kp = static_cast<const T *>(a.k) + int64_t(t) * a.ldk + int64_t(head) * hd;
     const T *vp = static_cast<const T *>(a.v) + int64_t(t) * a.ldv + int64_t(head) * hd;
-    const float2 *tab = ROT ? reinterpret_cast<const float2 *>(a.q.table) + int64_t(t) * a.q.half : nullptr;
+    const float2 *tab = ROT ? a.table + int64_t(t) * a.half : nullptr;
     uint8_t *kd = a.kc + page_base(page, a.Hkv, head, P, hd), *vd = a.vc + page_base(page, a.Hkv, head, P, hd);
 
     auto key8 = [&](int i, int d, float v[8]) {
-      if constexpr (ROT) turned8<DT, ROT == 2>(kp + int64_t(i) * a.ldk, tab + int64_t(i) * a.q.half, a.q.half, d, v);
+      if constexpr (ROT) turned8<DT, ROT == 2>(kp + int64_t(i) * a.ldk, tab + int64_t(i) * a.half, a.half, d, v);
       else ld8<DT>(kp + int64_t(i) * a.ldk + d, v);
     };
 
@@ -263,7 +256,7 @@ __global__ void __launch_bounds__(NT) kv_store_paged_kernel(StoreArgs a) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int64_t i = min(max(pi + j, 0), n - 1);  // (places beside the run repeat its tokens, not stored)
-        kr[j].load(kp + i * a.ldk, tab + (ROT ? i * a.q.half : 0), a.q.half, pd);
+        kr[j].load(kp + i * a.ldk, tab + (ROT ? i * a.half : 0), a.half, pd);
         vr[j].load(vp + i * a.ldv + pd);
       }
 #pragma unroll
@@ -433,12 +426,12 @@ hipError_t kv_store_paged(int dt, const void *k, const void *v, long ldk, long l
                           hipStream_t st, const Rotary *rot) {
   if (n < 1 || n > 1 << 27 || Hkv < 1 || Hkv > 65535) return hipErrorInvalidValue;
   StoreArgs a{k, v, slots, static_cast<uint8_t *>(k_cache), static_cast<uint8_t *>(v_cache), k_scale, v_scale, err, ldk, ldv,
-              n, Hkv, hd, page, n_pages, store_tokens(n, Hkv), rot ? *rot : Rotary{}};
-  dim3 grid(unsigned((n + a.per - 1) / a.per), unsigned(Hkv));
+              n, Hkv, hd, page, n_pages, store_tokens(n, Hkv), rot ? reinterpret_cast<const float2 *>(rot->table) : nullptr, rot ? rot->half : 0};
   if (rot && rot->heads) {
-    if (Hkv > 65535 - kStoreQueryRows) return hipErrorInvalidValue;
-    grid.y += unsigned(std::min(kStoreQueryRows, a.per));
+    const hipError_t e = rotary(dt, *rot, slots, int64_t(n_pages) * page, st);
+    if (e != hipSuccess) return e;
   }
+  const dim3 grid(unsigned((n + a.per - 1) / a.per), unsigned(Hkv));
   // Threads for a page's pieces at once where workgroups take many tokens (17k
   // tokens, 8 heads of 128: pages of 128 42 us, 56 with 256 threads; of 256 56, 60);
   // where they take one, most would be idle.

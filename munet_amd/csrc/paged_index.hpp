@@ -87,9 +87,6 @@ inline int plan_groups(int B, int64_t cap) {
 // at most 2048 workgroups 37, 8192 38, 16384 39).
 inline int store_tokens(int n, int heads) { return int(std::min<int64_t>(64, std::max<int64_t>(1, int64_t(n) * heads / 4096))); }
 
-// Rows of workgroups behind the heads' that rotate queries beside the store.
-constexpr int kStoreQueryRows = 64;
-
 // Workgroup i of a launch over `pairs` (sequence, key/value head) pairs of `per`
 // items each.  Workgroups go round the eight XCDs, each with an L2 of its own:
 // eight pairs at a time, one to an XCD, so that the items that read the same

@@ -27,8 +27,17 @@ __global__ void __launch_bounds__(256) rotary_table_kernel(const int32_t *__rest
 
 // ---- rotary --------------------------------------------------------------------
 
-template <int DT> __global__ void __launch_bounds__(256) rotary_kernel(Rotary p) {
-  for (int64_t t = blockIdx.x; t < p.n; t += gridDim.x) rotate_token<DT, 256>(p, t);
+template <int DT, int U, bool INTERLEAVED>
+__global__ void __launch_bounds__(256) rotary_kernel(Rotary p, const int32_t *slots, int64_t limit) {
+  for (int64_t t = int64_t(blockIdx.x) * p.tokens; t < p.n; t += int64_t(gridDim.x) * p.tokens)
+    rotate_tokens<DT, U, INTERLEAVED, 256>(p, t, slots, limit);
+}
+
+template <int DT, int U>
+void launch(const Rotary &p, const int32_t *slots, int64_t limit, unsigned grid, hipStream_t st) {
+  constexpr int V = U == 1 ? 1 : U / 2;  // (interleaved pairs lie in one load)
+  if (p.interleaved) hipLaunchKernelGGL((rotary_kernel<DT, V, true>), dim3(grid), dim3(256), 0, st, p, slots, limit);
+  else hipLaunchKernelGGL((rotary_kernel<DT, U, false>), dim3(grid), dim3(256), 0, st, p, slots, limit);
 }
 
 }  // namespace
@@ -42,12 +51,14 @@ hipError_t rotary_table(const int32_t *positions, const double *freq, float *tab
   return hipGetLastError();
 }
 
-hipError_t rotary(int dt, const Rotary &p, hipStream_t st) {
-  const unsigned grid = unsigned(std::min(p.n, 1 << 20));
+hipError_t rotary(int dt, Rotary p, const int32_t *slots, int64_t limit, hipStream_t st) {
+  const int unit = rotary_unit(dt, p);
+  rotary_cut(dt, unit, 256, p);
+  const unsigned grid = unsigned(std::min<int64_t>((int64_t(p.n) + p.tokens - 1) / p.tokens, 1 << 22));
   switch (dt) {
-  case F32: hipLaunchKernelGGL(rotary_kernel<F32>, dim3(grid), dim3(256), 0, st, p); break;
-  case F16: hipLaunchKernelGGL(rotary_kernel<F16>, dim3(grid), dim3(256), 0, st, p); break;
-  case BF16: hipLaunchKernelGGL(rotary_kernel<BF16>, dim3(grid), dim3(256), 0, st, p); break;
+  case F32: unit == 1 ? launch<F32, 1>(p, slots, limit, grid, st) : launch<F32, 4>(p, slots, limit, grid, st); break;
+  case F16: unit == 1 ? launch<F16, 1>(p, slots, limit, grid, st) : launch<F16, 8>(p, slots, limit, grid, st); break;
+  case BF16: unit == 1 ? launch<BF16, 1>(p, slots, limit, grid, st) : launch<BF16, 8>(p, slots, limit, grid, st); break;
   default: return hipErrorInvalidValue;
   }
   return hipGetLastError();
