@@ -1,5 +1,8 @@
+// Products of 8-bit integers with a scale for each row of both operands:
 // out[M, N] = act(sx_m sw_n sum_k x[m, k] w[n, k] + bias_n) + resid[m, n] with x and w
 // in 8-bit integers (v_mfma_i32_16x16x64_i8: 64 products of K per instruction).
+#include <cstdlib>
+
 #include "gemm_i8.hpp"
 
 namespace mh {
@@ -73,18 +76,137 @@ __global__ void __launch_bounds__(256) gemm_i8_any_kernel(LinearI8 p) {
     if (kt + 1 < KT) put((kt + 1) & 1);
     __syncthreads();
   }
+  i8_store<DT, G>(p, g, m0, n0, acc);
+}
+
+// 64 lanes x 16 bytes from a buffer resource into LDS bytes [m0, m0 + 1024); lanes past
+// the resource's end write zeros.
+__device__ __forceinline__ void dma16_at(__amdgpu_buffer_rsrc_t res, uint32_t voff, uint32_t soff, uint32_t ldsaddr) {
+  asm volatile("s_mov_b32 m0, %3\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds" ::"v"(voff), "s"(res), "s"(soff), "s"(ldsaddr)
+               : "memory", "m0");
+}
+
+// Rows and addresses in whole 16-byte blocks: slabs of 128 bytes of K go straight
+// into S LDS stages, as in gemm_dma_kernel (gemm_pipe.hpp has the layout, the
+// schedule of a step and why its loads are inline assembly).  A slab of 128 int8
+// takes as many MFMA cycles as one of 64 16-bit values for twice the products.
+// Where the last slab is not whole, its blocks past K are read from past the
+// end of the resource, as zeros.
+template <int DT, int BM, int BN, int WGM, int WGN, int S>
+__global__ void __launch_bounds__(WGM * WGN * 64) gemm_i8_kernel(LinearI8 p, int gn) {
+  typedef PipeGeom<BM, BN, WGM, WGN> G;
+  constexpr int NW = G::NW, FM = G::FM, FN = G::FN;
+  constexpr int ABLK = BM / 8 / NW, BBLK = BN / 8 / NW, NDMA = ABLK + BBLK;
+  static_assert(BM % (8 * NW) == 0 && BN % (8 * NW) == 0, "the waves share the loads evenly");
+  static_assert(S >= 2 && NDMA * (S - 1) < 64, "stages");
+  constexpr uint32_t STAGE = (BM + BN) * 128;
+  __shared__ u32x4 lds[S][(BM + BN) * 8];
+  int m0, n0;
+  pipe_tile<BM, BN>(p.M, p.N, gn, m0, n0);
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const G g(wave, lane);
+  const int lr = lane >> 3, lc = (lane & 7) ^ lr;
+  const int KT = (p.K + 127) / 128;
+  // (a tile's rows span less than 2^31 bytes: the host checks; rows past the end
+  // read the last one, their results are not stored)
+  const int rx = min(BM, p.M - m0), rw = min(BN, p.N - n0);
+  const __amdgpu_buffer_rsrc_t xres = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t *>(p.x + int64_t(m0) * p.ldx), 0,
+                                                                        int((rx - 1) * p.ldx) + p.K, 0x00020000);
+  const __amdgpu_buffer_rsrc_t wres = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t *>(p.w + int64_t(n0) * p.ldw), 0,
+                                                                        int((rw - 1) * p.ldw) + p.K, 0x00020000);
+  uint32_t aoff[ABLK], boff[BBLK];
 #pragma unroll
-  for (int j = 0; j < G::FN; ++j) {
-    const int n = n0 + g.wn * G::WTN + j * 16 + 4 * g.lg;
-    Scale sw[4];
+  for (int i = 0; i < ABLK; ++i) aoff[i] = uint32_t(min((wave * ABLK + i) * 8 + lr, rx - 1)) * uint32_t(p.ldx) + lc * 16;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) sw[i] = Scale(p.sw[min(n + i, p.N - 1)]);
-#pragma unroll
-    for (int i = 0; i < G::FM; ++i) {
-      const int m = m0 + g.wm * G::WTM + i * 16 + g.li;
-      if (m < p.M && n < p.N) i8_store4<DT>(p, m, n, acc[i][j], Scale(p.sx[m]), sw);
-    }
+  for (int i = 0; i < BBLK; ++i) boff[i] = uint32_t(min((wave * BBLK + i) * 8 + lr, rw - 1)) * uint32_t(p.ldw) + lc * 16;
+  const uint32_t lds0 = uint32_t(reinterpret_cast<uintptr_t>((lds_void_t *)&lds[0][0]));
+  const uint32_t wa = lds0 + wave * ABLK * 1024, wb = lds0 + BM * 128 + wave * BBLK * 1024;
+  const uint32_t past = lc * 16 >= p.K - (KT - 1) * 128 ? 0x80000000u : 0u;  // this lane's block of the last slab
+#define MH_DMA(T, KT_, TAIL, ST)                                                                               \
+  {                                                                                                           \
+    if ((T) < ABLK) dma16_at(xres, aoff[(T) % ABLK] | (TAIL), (KT_) * 128, wa + (ST) * STAGE + ((T) % ABLK) * 1024);  \
+    else dma16_at(wres, boff[((T) - ABLK) % BBLK] | (TAIL), (KT_) * 128, wb + (ST) * STAGE + (((T) - ABLK) % BBLK) * 1024); \
   }
+  i32x4 acc[FM][FN];
+  u32x4 af0[FM], bf0[FN], af1[FM], bf1[FN];
+#pragma unroll
+  for (int s = 0; s < S - 1; ++s) {
+    const int kt = min(s, KT - 1);
+    const uint32_t tail = kt == KT - 1 ? past : 0u;
+#pragma unroll
+    for (int t = 0; t < NDMA; ++t) MH_DMA(t, kt, tail, s);
+  }
+  dma_wait<NDMA *(S - 2)>();
+  __syncthreads();
+  g.template frags<0>(lds[0], af0, bf0);
+
+  constexpr int NMM = FM * FN, NRD = FM + FN, RPM = 2;
+  constexpr int LATE = S == 2 ? (NRD + RPM - 1) / RPM : 0;  // two stages: the wait comes late in the second half
+  static_assert(LATE <= NMM, "late wait");
+  constexpr int STAGE4 = (BM + BN) * 8;
+  const int c1 = 4 + g.lg, c0f = g.lg;
+  auto mma = [](i32x4 &c, u32x4 b, u32x4 a) {
+    c = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, b), __builtin_bit_cast(i32x4, a), c, 0, 0, 0);
+  };
+#define MH_FRAG(L, C, X, AF, BF)                                                                               \
+  {                                                                                                           \
+    if ((X) < FM) {                                                                                           \
+      const int r = g.wm * G::WTM + ((X) % FM) * 16 + g.li;                                                   \
+      AF[(X) % FM] = (L)[r * 8 + ((C) ^ (r & 7))];                                                            \
+    } else {                                                                                                  \
+      const int r = g.wn * G::WTN + (((X) - FM) % FN) * 16 + g.li;                                            \
+      BF[((X) - FM) % FN] = (L)[BM * 8 + r * 8 + ((C) ^ (r & 7))];                                            \
+    }                                                                                                         \
+  }
+  int stg = 0;
+#define MH_STEP(KK, FIRST)                                                                                     \
+  {                                                                                                           \
+    const int s_ = stg, sn_ = s_ + 1 == S ? 0 : s_ + 1, sf_ = s_ == 0 ? S - 1 : s_ - 1;                        \
+    const int kf_ = min((KK) + S - 1, KT - 1);                                                                \
+    const uint32_t tail_ = kf_ == KT - 1 ? past : 0u;                                                         \
+    const u32x4 *Ls_ = &lds[0][0] + s_ * STAGE4, *Ln_ = &lds[0][0] + sn_ * STAGE4;                             \
+    _Pragma("unroll") for (int t = 0; t < NMM; ++t) {                                                         \
+      if (FIRST) acc[t / FN][t % FN] = i32x4{0, 0, 0, 0};                                                     \
+      mma(acc[t / FN][t % FN], bf0[t % FN], af0[t / FN]);                                                     \
+      if (t < NDMA) MH_DMA(t, kf_, tail_, sf_)                                                                \
+      else if (t < NDMA + NRD) MH_FRAG(Ls_, c1, t - NDMA, af1, bf1)                                           \
+      __builtin_amdgcn_sched_barrier(0);                                                                      \
+    }                                                                                                         \
+    _Pragma("unroll") for (int t = NMM; t < NDMA + NRD; ++t) {                                                \
+      if (t < NDMA) MH_DMA(t, kf_, tail_, sf_)                                                                \
+      else MH_FRAG(Ls_, c1, t - NDMA, af1, bf1)                                                               \
+    }                                                                                                         \
+    if constexpr (LATE == 0) {                                                                                \
+      dma_wait<NDMA *(S - 2)>();                                                                              \
+      __syncthreads();                                                                                        \
+    }                                                                                                         \
+    _Pragma("unroll") for (int t = 0; t < NMM; ++t) {                                                         \
+      if (LATE > 0 && t == NMM - LATE) {                                                                      \
+        dma_wait<0>();                                                                                        \
+        __syncthreads();                                                                                      \
+      }                                                                                                       \
+      mma(acc[t / FN][t % FN], bf1[t % FN], af1[t / FN]);                                                     \
+      if (LATE == 0) {                                                                                        \
+        if (t < NRD) MH_FRAG(Ln_, c0f, t, af0, bf0)                                                           \
+      } else if (t >= NMM - LATE) {                                                                           \
+        _Pragma("unroll") for (int q_ = 0; q_ < RPM; ++q_)                                                    \
+          if (RPM * (t - (NMM - LATE)) + q_ < NRD) MH_FRAG(Ln_, c0f, RPM * (t - (NMM - LATE)) + q_, af0, bf0)  \
+      }                                                                                                       \
+      __builtin_amdgcn_sched_barrier(0);                                                                      \
+    }                                                                                                         \
+    if constexpr (LATE == 0) {                                                                                \
+      _Pragma("unroll") for (int t = NMM; t < NRD; ++t) MH_FRAG(Ln_, c0f, t, af0, bf0)                         \
+    }                                                                                                         \
+    stg = sn_;                                                                                                \
+  }
+  MH_STEP(0, true);
+  for (int k = 1; k < KT; ++k) MH_STEP(k, false);
+#undef MH_STEP
+#undef MH_FRAG
+#undef MH_DMA
+  dma_wait<0>();  // no load is in flight when the workgroup ends
+  i8_store<DT, G>(p, g, m0, n0, acc);
 }
 
 template <int DT> hipError_t launch_any(const LinearI8 &p, hipStream_t st) {
@@ -94,13 +216,49 @@ template <int DT> hipError_t launch_any(const LinearI8 &p, hipStream_t st) {
   return hipGetLastError();
 }
 
+template <int DT, int BM, int BN, int WGM, int WGN, int S> hipError_t launch(const LinearI8 &p, hipStream_t st) {
+  const int64_t tiles = int64_t((p.M + BM - 1) / BM) * ((p.N + BN - 1) / BN);
+  if (tiles > kI8MaxTiles) return hipErrorInvalidValue;
+  const int gn = 2L * p.N >= p.M ? (p.N >= 4L * p.M ? 16 : 8) : 0;
+  hipLaunchKernelGGL((gemm_i8_kernel<DT, BM, BN, WGM, WGN, S>), dim3(unsigned(tiles)), dim3(WGM * WGN * 64), 0, st, p, gn);
+  return hipGetLastError();
+}
+
+// Whether rows and addresses go in 16-byte blocks, tiles of up to 256 rows within the
+// 31 bits of a buffer resource.
+bool blocks(const LinearI8 &p) {
+  return p.K % 16 == 0 && p.ldx % 16 == 0 && p.ldw % 16 == 0 && reinterpret_cast<uintptr_t>(p.x) % 16 == 0 &&
+         reinterpret_cast<uintptr_t>(p.w) % 16 == 0 && p.ldx < (1 << 22) && p.ldw < (1 << 22);
+}
+
+template <int DT> hipError_t run(const LinearI8 &p, hipStream_t st) {
+  int tile = blocks(p) ? 1 : 0;
+  // (MUNET_HIP_I8_TILE names a kernel for tests and tuning, where the operands allow it)
+  if (const char *force = std::getenv("MUNET_HIP_I8_TILE"))
+    if (blocks(p)) tile = std::atoi(force);
+  switch (tile) {
+  case 1: return launch<DT, 128, 128, 2, 2, 2>(p, st);
+  case 2: return launch<DT, 256, 256, 4, 2, 2>(p, st);
+  case 3: return launch<DT, 256, 256, 2, 4, 2>(p, st);
+  case 4: return launch<DT, 256, 128, 4, 2, 2>(p, st);
+  case 5: return launch<DT, 256, 128, 4, 2, 3>(p, st);
+  case 6: return launch<DT, 128, 128, 4, 2, 4>(p, st);
+  case 7: return launch<DT, 64, 64, 2, 2, 8>(p, st);
+  case 8: return launch<DT, 32, 64, 2, 2, 10>(p, st);
+  case 9: return launch<DT, 32, 32, 2, 2, 16>(p, st);
+  case 10: return launch<DT, 256, 256, 2, 2, 2>(p, st);
+  case 11: return launch<DT, 128, 64, 4, 2, 6>(p, st);
+  default: return launch_any<DT>(p, st);
+  }
+}
+
 }  // namespace
 
 hipError_t linear_i8(int dt, const LinearI8 &p, hipStream_t st) {
   switch (dt) {
-  case F32: return launch_any<F32>(p, st);
-  case F16: return launch_any<F16>(p, st);
-  case BF16: return launch_any<BF16>(p, st);
+  case F32: return run<F32>(p, st);
+  case F16: return run<F16>(p, st);
+  case BF16: return run<BF16>(p, st);
   default: return hipErrorInvalidValue;
   }
 }
