@@ -939,8 +939,6 @@ int mh_linear_i8(int dt, const int8_t *x, int64_t ldx, const float *x_scale, con
     p.N = N;
     p.K = K;
     p.act = act;
-    const uintptr_t any = reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(bias) | reinterpret_cast<uintptr_t>(resid);
-    p.quads = any % (4 * es) == 0 && (ldo % 4 == 0 || M == 1) && (!resid || ldr % 4 == 0 || M == 1);
     hip_check(linear_i8(dt, p, S_(stream)), "linear_i8");
   })
 }

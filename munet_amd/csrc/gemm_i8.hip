@@ -25,7 +25,7 @@ __device__ __forceinline__ i32x4 row_chunk(const int8_t *row, int k, int K) {
 template <int DT>
 __global__ void __launch_bounds__(256) gemm_i8_any_kernel(LinearI8 p) {
   constexpr int BM = 64, BN = 64;
-  typedef PipeGeom<BM, BN, 2, 2> G;
+  typedef I8Geom<BM, BN, 2, 2> G;
   __shared__ u32x4 lds[2][(BM + BN) * 8];
   int m0, n0;
   pipe_tile<BM, BN>(p.M, p.N, 0, m0, n0);
@@ -50,8 +50,8 @@ __global__ void __launch_bounds__(256) gemm_i8_any_kernel(LinearI8 p) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int r = r0 + 32 * i;
-      lds[b][r * 8 + (c0 ^ (r & 7))] = __builtin_bit_cast(u32x4, ra[i]);
-      lds[b][BM * 8 + r * 8 + (c0 ^ (r & 7))] = __builtin_bit_cast(u32x4, rb[i]);
+      lds[b][r * 8 + (c0 ^ G::xswizzle(r))] = __builtin_bit_cast(u32x4, ra[i]);
+      lds[b][BM * 8 + r * 8 + (c0 ^ G::wswizzle(r))] = __builtin_bit_cast(u32x4, rb[i]);
     }
   };
   i32x4 acc[G::FM][G::FN] = {};
@@ -64,8 +64,10 @@ __global__ void __launch_bounds__(256) gemm_i8_any_kernel(LinearI8 p) {
     u32x4 af[G::FM], bf[G::FN];
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
-      if (ks == 0) g.template frags<0>(lds[kt & 1], af, bf);
-      else g.template frags<1>(lds[kt & 1], af, bf);
+#pragma unroll
+      for (int i = 0; i < G::FM; ++i) af[i] = g.xfrag(lds[kt & 1], i, 4 * ks + g.lg);
+#pragma unroll
+      for (int j = 0; j < G::FN; ++j) bf[j] = g.wfrag(lds[kt & 1], j, 4 * ks + g.lg);
 #pragma unroll
       for (int i = 0; i < G::FM; ++i)
 #pragma unroll
@@ -94,7 +96,7 @@ __device__ __forceinline__ void dma16_at(__amdgpu_buffer_rsrc_t res, uint32_t vo
 // end of the resource, as zeros.
 template <int DT, int BM, int BN, int WGM, int WGN, int S>
 __global__ void __launch_bounds__(WGM * WGN * 64) gemm_i8_kernel(LinearI8 p, int gn) {
-  typedef PipeGeom<BM, BN, WGM, WGN> G;
+  typedef I8Geom<BM, BN, WGM, WGN> G;
   constexpr int NW = G::NW, FM = G::FM, FN = G::FN;
   constexpr int ABLK = BM / 8 / NW, BBLK = BN / 8 / NW, NDMA = ABLK + BBLK;
   static_assert(BM % (8 * NW) == 0 && BN % (8 * NW) == 0, "the waves share the loads evenly");
@@ -106,7 +108,9 @@ __global__ void __launch_bounds__(WGM * WGN * 64) gemm_i8_kernel(LinearI8 p, int
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const G g(wave, lane);
-  const int lr = lane >> 3, lc = (lane & 7) ^ lr;
+  // lane l of a load fetches block row l / 8's chunk that lies at LDS slot l % 8
+  const int lr = lane >> 3, lc = (lane & 7) ^ G::xswizzle(lr);
+  auto wchunk = [&](int i) { return (lane & 7) ^ G::wswizzle((wave * BBLK + i) * 8 + lr); };
   const int KT = (p.K + 127) / 128;
   // (a tile's rows span less than 2^31 bytes: the host checks; rows past the end
   // read the last one, their results are not stored)
@@ -119,27 +123,38 @@ __global__ void __launch_bounds__(WGM * WGN * 64) gemm_i8_kernel(LinearI8 p, int
 #pragma unroll
   for (int i = 0; i < ABLK; ++i) aoff[i] = uint32_t(min((wave * ABLK + i) * 8 + lr, rx - 1)) * uint32_t(p.ldx) + lc * 16;
 #pragma unroll
-  for (int i = 0; i < BBLK; ++i) boff[i] = uint32_t(min((wave * BBLK + i) * 8 + lr, rw - 1)) * uint32_t(p.ldw) + lc * 16;
+  for (int i = 0; i < BBLK; ++i) boff[i] = uint32_t(min((wave * BBLK + i) * 8 + lr, rw - 1)) * uint32_t(p.ldw) + wchunk(i) * 16;
   const uint32_t lds0 = uint32_t(reinterpret_cast<uintptr_t>((lds_void_t *)&lds[0][0]));
   const uint32_t wa = lds0 + wave * ABLK * 1024, wb = lds0 + BM * 128 + wave * BBLK * 1024;
-  const uint32_t past = lc * 16 >= p.K - (KT - 1) * 128 ? 0x80000000u : 0u;  // this lane's block of the last slab
-#define MH_DMA(T, KT_, TAIL, ST)                                                                               \
+  // this lane's blocks of the last slab that lie past K
+  const int rest = p.K - (KT - 1) * 128;
+  const uint32_t xpast = lc * 16 >= rest ? 0x80000000u : 0u;
+  uint32_t wpast[2];  // (the chunk alternates at most between two of a wave's blocks)
+#pragma unroll
+  for (int i = 0; i < 2; ++i) wpast[i] = wchunk(i < BBLK ? i : 0) * 16 >= rest ? 0x80000000u : 0u;
+  // load T of a slab into a stage; LAST: of the last slab
+#define MH_DMA(T, KT_, LAST, ST)                                                                               \
   {                                                                                                           \
-    if ((T) < ABLK) dma16_at(xres, aoff[(T) % ABLK] | (TAIL), (KT_) * 128, wa + (ST) * STAGE + ((T) % ABLK) * 1024);  \
-    else dma16_at(wres, boff[((T) - ABLK) % BBLK] | (TAIL), (KT_) * 128, wb + (ST) * STAGE + (((T) - ABLK) % BBLK) * 1024); \
+    if ((T) < ABLK)                                                                                           \
+      dma16_at(xres, aoff[(T) % ABLK] | ((LAST) ? xpast : 0u), (KT_) * 128, wa + (ST) * STAGE + ((T) % ABLK) * 1024);  \
+    else                                                                                                      \
+      dma16_at(wres, boff[((T) - ABLK) % BBLK] | ((LAST) ? wpast[((T) - ABLK) % BBLK % 2] : 0u), (KT_) * 128,  \
+               wb + (ST) * STAGE + (((T) - ABLK) % BBLK) * 1024);                                             \
   }
   i32x4 acc[FM][FN];
   u32x4 af0[FM], bf0[FN], af1[FM], bf1[FN];
 #pragma unroll
   for (int s = 0; s < S - 1; ++s) {
     const int kt = min(s, KT - 1);
-    const uint32_t tail = kt == KT - 1 ? past : 0u;
 #pragma unroll
-    for (int t = 0; t < NDMA; ++t) MH_DMA(t, kt, tail, s);
+    for (int t = 0; t < NDMA; ++t) MH_DMA(t, kt, kt == KT - 1, s);
   }
   dma_wait<NDMA *(S - 2)>();
   __syncthreads();
-  g.template frags<0>(lds[0], af0, bf0);
+#pragma unroll
+  for (int i = 0; i < FM; ++i) af0[i] = g.xfrag(lds[0], i, g.lg);
+#pragma unroll
+  for (int j = 0; j < FN; ++j) bf0[j] = g.wfrag(lds[0], j, g.lg);
 
   constexpr int NMM = FM * FN, NRD = FM + FN, RPM = 2;
   constexpr int LATE = S == 2 ? (NRD + RPM - 1) / RPM : 0;  // two stages: the wait comes late in the second half
@@ -151,30 +166,25 @@ __global__ void __launch_bounds__(WGM * WGN * 64) gemm_i8_kernel(LinearI8 p, int
   };
 #define MH_FRAG(L, C, X, AF, BF)                                                                               \
   {                                                                                                           \
-    if ((X) < FM) {                                                                                           \
-      const int r = g.wm * G::WTM + ((X) % FM) * 16 + g.li;                                                   \
-      AF[(X) % FM] = (L)[r * 8 + ((C) ^ (r & 7))];                                                            \
-    } else {                                                                                                  \
-      const int r = g.wn * G::WTN + (((X) - FM) % FN) * 16 + g.li;                                            \
-      BF[((X) - FM) % FN] = (L)[BM * 8 + r * 8 + ((C) ^ (r & 7))];                                            \
-    }                                                                                                         \
+    if ((X) < FM) AF[(X) % FM] = g.xfrag(L, (X) % FM, C);                                                     \
+    else BF[((X) - FM) % FN] = g.wfrag(L, ((X) - FM) % FN, C);                                                \
   }
   int stg = 0;
 #define MH_STEP(KK, FIRST)                                                                                     \
   {                                                                                                           \
     const int s_ = stg, sn_ = s_ + 1 == S ? 0 : s_ + 1, sf_ = s_ == 0 ? S - 1 : s_ - 1;                        \
     const int kf_ = min((KK) + S - 1, KT - 1);                                                                \
-    const uint32_t tail_ = kf_ == KT - 1 ? past : 0u;                                                         \
+    const bool last_ = kf_ == KT - 1;                                                                         \
     const u32x4 *Ls_ = &lds[0][0] + s_ * STAGE4, *Ln_ = &lds[0][0] + sn_ * STAGE4;                             \
     _Pragma("unroll") for (int t = 0; t < NMM; ++t) {                                                         \
       if (FIRST) acc[t / FN][t % FN] = i32x4{0, 0, 0, 0};                                                     \
       mma(acc[t / FN][t % FN], bf0[t % FN], af0[t / FN]);                                                     \
-      if (t < NDMA) MH_DMA(t, kf_, tail_, sf_)                                                                \
+      if (t < NDMA) MH_DMA(t, kf_, last_, sf_)                                                                \
       else if (t < NDMA + NRD) MH_FRAG(Ls_, c1, t - NDMA, af1, bf1)                                           \
       __builtin_amdgcn_sched_barrier(0);                                                                      \
     }                                                                                                         \
     _Pragma("unroll") for (int t = NMM; t < NDMA + NRD; ++t) {                                                \
-      if (t < NDMA) MH_DMA(t, kf_, tail_, sf_)                                                                \
+      if (t < NDMA) MH_DMA(t, kf_, last_, sf_)                                                                \
       else MH_FRAG(Ls_, c1, t - NDMA, af1, bf1)                                                               \
     }                                                                                                         \
     if constexpr (LATE == 0) {                                                                                \

@@ -20,121 +20,195 @@ struct Scale {
   __device__ __forceinline__ explicit Scale(float s) : f(__builtin_amdgcn_frexp_mantf(s)), e(__builtin_amdgcn_frexp_expf(s)) {}
 };
 
-// Four values of a bias or residual, zeros past the row.
-template <int DT>
-__device__ __forceinline__ void i8_load4(const typename Store<DT>::T *p, int left, bool quads, float v[4]) {
-  if (quads && left >= 4) {
-    ld4<DT>(p, v);
-  } else {
+// A wave's tile of BM x BN / (WGM x WGN) outputs.  The sums of fragment (i, j) lie in
+// lane (li, lg) as four of row 16 i + li; which four columns they are is decided by
+// the rows of w that the fragment is given: fragments 2 q and 2 q + 1 take
+// alternate fours of 32 columns, so that a lane ends with eight consecutive
+// columns, 32 q + 8 lg .. + 7, and four lanes with 64 consecutive bytes of 16-bit
+// results (with a fragment to 16 consecutive columns, stores of 8 bytes took
+// 4096 x 2304 outputs 9 us longer than no stores: STORE_FIGURES).
+template <int BM, int BN, int WGM, int WGN> struct I8Geom : PipeGeom<BM, BN, WGM, WGN> {
+  typedef PipeGeom<BM, BN, WGM, WGN> P;
+  static constexpr int FM = P::FM, FN = P::FN;
+  static constexpr int COLS = FN == 1 ? 4 : 8, GROUPS = FN * 4 / COLS;  // consecutive columns of a lane
+  static_assert(FN == 1 || FN % 2 == 0, "fragments go in pairs");
+  __device__ __forceinline__ I8Geom(int wave, int lane) : P(wave, lane) {}
+  // LDS: row r's chunk c lies at c ^ swizzle(r), so that the eight rows that eight
+  // consecutive lanes read spread over the banks
+  static __device__ __forceinline__ int xswizzle(int r) { return r & 7; }
+  static __device__ __forceinline__ int wswizzle(int r) { return FN == 1 ? r & 7 : (r & 3) | ((r >> 1) & 4); }
+  __device__ __forceinline__ u32x4 xfrag(const u32x4 *L, int i, int c) const {
+    const int r = this->wm * P::WTM + i * 16 + this->li;
+    return L[r * 8 + (c ^ xswizzle(r))];
+  }
+  __device__ __forceinline__ u32x4 wfrag(const u32x4 *L, int j, int c) const {
+    const int r = this->wn * P::WTN + (FN == 1 ? this->li : 32 * (j / 2) + 8 * (this->li >> 2) + 4 * (j & 1) + (this->li & 3));
+    return L[BM * 8 + r * 8 + (c ^ wswizzle(r))];
+  }
+  __device__ __forceinline__ int row(int m0, int i) const { return m0 + this->wm * P::WTM + i * 16 + this->li; }
+  __device__ __forceinline__ int col(int n0, int q) const { return n0 + this->wn * P::WTN + 32 * q + COLS * this->lg; }
+};
+
+// C consecutive values, aligned to their type alone, and their stores.
+template <int DT, int C> __device__ __forceinline__ void i8_get(const typename Store<DT>::T *p, float (&v)[C]) {
+  struct __attribute__((packed, aligned(4))) F4 { f32x4 v; };
+  struct __attribute__((packed, aligned(2))) H8 { uint4 v; };
+  struct __attribute__((packed, aligned(2))) H4 { uint2 v; };
+  if constexpr (DT == F32) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = i < left ? Store<DT>::dec(p[i]) : 0.f;
+    for (int i = 0; i < C; i += 4) {
+      const f32x4 x = reinterpret_cast<const F4 *>(p + i)->v;
+      v[i] = x[0]; v[i + 1] = x[1]; v[i + 2] = x[2]; v[i + 3] = x[3];
+    }
+  } else if constexpr (C == 8) {
+    dec8<DT>(reinterpret_cast<const H8 *>(p)->v, v);
+  } else {
+    const uint2 x = reinterpret_cast<const H4 *>(p)->v;
+    v[0] = Store<DT>::dec(uint16_t(x.x)); v[1] = Store<DT>::dec(uint16_t(x.x >> 16));
+    v[2] = Store<DT>::dec(uint16_t(x.y)); v[3] = Store<DT>::dec(uint16_t(x.y >> 16));
   }
 }
-
-// Columns n .. n + 3 of row m from their scaled sums, with the bias and the residual.
-template <int DT>
-__device__ __forceinline__ void i8_store4(const LinearI8 &p, int m, int n, float (&v)[4], const float (&bias)[4], const float (&resid)[4]) {
-  typedef typename Store<DT>::T T;
-  T *out = static_cast<T *>(p.out) + int64_t(m) * p.ldo + n;
-  if (p.bias) {
+template <int DT, int C> __device__ __forceinline__ void i8_put(typename Store<DT>::T *p, float (&v)[C]) {
+  struct __attribute__((packed, aligned(4))) F4 { f32x4 v; };
+  struct __attribute__((packed, aligned(2))) H8 { uint4 v; };
+  struct __attribute__((packed, aligned(2))) H4 { uint2 v; };
+  if constexpr (DT == F32) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = __fadd_rn(v[i], bias[i]);
-  }
-  if (p.act == ACT_RELU) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = v[i] < 0.f ? 0.f : v[i];  // (NaN stays)
-  } else if (p.act == ACT_GELU) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = __fmul_rn(v[i], sigmoidf_ref(1.702f * v[i]));
-  }
-  if (p.resid) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = __fadd_rn(v[i], resid[i]);
-  }
-  if (p.quads && n + 4 <= p.N) {
-    if constexpr (DT == BF16) {
-      *reinterpret_cast<uint2 *>(out) = pack4_bf16(v);
-    } else if constexpr (DT == F16) {
-      round4_f16(v);
-      *reinterpret_cast<uint2 *>(out) = make_uint2(pack_f16x2_exact(v[0], v[1]), pack_f16x2_exact(v[2], v[3]));
-    } else {
-      st4<DT>(out, v);
-    }
+    for (int i = 0; i < C; i += 4) reinterpret_cast<F4 *>(p + i)->v = f32x4{v[i], v[i + 1], v[i + 2], v[i + 3]};
   } else {
+    uint32_t w[C / 2];
+    if constexpr (DT == F16) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (n + i < p.N) out[i] = Store<DT>::enc(v[i]);
+      for (int i = 0; i < C; i += 4) round4_f16(v + i);
+    }
+#pragma unroll
+    for (int i = 0; i < C / 2; ++i) w[i] = DT == F16 ? pack_f16x2_exact(v[2 * i], v[2 * i + 1]) : pack_bf16x2(v[2 * i], v[2 * i + 1]);
+    if constexpr (C == 8) reinterpret_cast<H8 *>(p)->v = make_uint4(w[0], w[1], w[2], w[3]);
+    else reinterpret_cast<H4 *>(p)->v = make_uint2(w[0], w[1]);
   }
+}
+template <int ACT> __device__ __forceinline__ float i8_act(float v) {
+  if constexpr (ACT == ACT_RELU) return v < 0.f ? 0.f : v;  // (NaN stays)
+  if constexpr (ACT == ACT_GELU) return __fmul_rn(v, sigmoidf_ref(__fmul_rn(1.702f, v)));
+  return v;
 }
 
 // Whether sums times any two scales of this size, one after the other, stay normal floats or
 // overflow where the result does.
 __device__ __forceinline__ bool plain_scale(float s) { return s == 0.f || (s >= 0x1p-60f && s <= 0x1p60f); }
 
-// A wave's tile: lane (li, lg) of fragment (i, j) has row 16 i + li, columns
-// 16 j + 4 lg .. + 3.  What is the same for several fragments is loaded before
-// the first store (a load behind a store waits for it: out might be what is read), a
-// row's residual before its stores.  (Whole rows through LDS were slower: 4096 x
-// 4096 x 1024 on 256 x 128 tiles 38 us, 34 so.)
-template <int DT, typename G, bool PLAIN>
-__device__ __forceinline__ void i8_store_as(const LinearI8 &p, int mw, int n0, const i32x4 (&acc)[G::FM][G::FN], const float (&fx)[G::FM],
-                                            const float (&fw)[G::FN][4]) {
+// A wave's results.  What is the same for several fragments is loaded before the
+// first store (a load behind a store waits for it: out might be what is read), a
+// row's residual before its stores.  The code is straight and runs once a tile, so
+// that it is fetched while it runs: what every fragment might need, inline in
+// each, was 100 KB of it.  Hence one path for whole tiles with scales of ordinary
+// size, which multiply as they are, for each activation, and one for all else,
+// where scales are fractions and powers of two: the same bits where both can.
+// Roundings are explicit, a missing bias or residual is a zero: a row's results do
+// not depend on the kernel.  (Whole rows through LDS were slower: 4096 x 4096 x
+// 1024 on 256 x 128 tiles 38 us, 34 from registers.)
+template <int DT, typename G, int ACT>
+__device__ __forceinline__ void i8_store_whole(const LinearI8 &p, const G &g, int m0, int n0, const i32x4 (&acc)[G::FM][G::FN],
+                                               const float (&fx)[G::FM], const float (&fw)[G::GROUPS][G::COLS],
+                                               const float (&bias)[G::GROUPS][G::COLS]) {
   typedef typename Store<DT>::T T;
-  float bias[G::FN][4], resid[G::FN][4];
-  if (p.bias) {
-#pragma unroll
-    for (int j = 0; j < G::FN; ++j)
-      i8_load4<DT>(static_cast<const T *>(p.bias) + n0 + j * 16, p.N - (n0 + j * 16), p.quads, bias[j]);
-  }
 #pragma unroll
   for (int i = 0; i < G::FM; ++i) {
-    const int m = mw + i * 16;
-    if (p.resid && m < p.M) {
+    const int m = g.row(m0, i);
+    if (m < p.M) {
+      float resid[G::GROUPS][G::COLS] = {};
+      if (p.resid) {
+        const T *r = static_cast<const T *>(p.resid) + int64_t(m) * p.ldr + g.col(n0, 0);
 #pragma unroll
-      for (int j = 0; j < G::FN; ++j)
-        i8_load4<DT>(static_cast<const T *>(p.resid) + int64_t(m) * p.ldr + n0 + j * 16, p.N - (n0 + j * 16), p.quads, resid[j]);
-    }
-#pragma unroll
-    for (int j = 0; j < G::FN; ++j) {
-      const int n = n0 + j * 16;
-      float v[4];
-      if constexpr (PLAIN) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = __fmul_rn(__fmul_rn(float(acc[i][j][e]), fx[i]), fw[j][e]);
-      } else {
-        const Scale sx(fx[i]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const Scale sw(fw[j][e]);
-          v[e] = __builtin_amdgcn_ldexpf(__fmul_rn(__fmul_rn(float(acc[i][j][e]), sx.f), sw.f), sx.e + sw.e);
-        }
+        for (int q = 0; q < G::GROUPS; ++q) i8_get<DT>(r + q * 32, resid[q]);
       }
-      if (m < p.M && n < p.N) i8_store4<DT>(p, m, n, v, bias[j], resid[j]);
+      T *out = static_cast<T *>(p.out) + int64_t(m) * p.ldo + g.col(n0, 0);
+#pragma unroll
+      for (int q = 0; q < G::GROUPS; ++q) {
+        float v[G::COLS];
+#pragma unroll
+        for (int e = 0; e < G::COLS; ++e)
+          v[e] = __fadd_rn(i8_act<ACT>(__fadd_rn(__fmul_rn(__fmul_rn(float(acc[i][q * (G::COLS / 4) + e / 4][e % 4]), fx[i]), fw[q][e]), bias[q][e])),
+                           resid[q][e]);
+        i8_put<DT>(out + q * 32, v);
+      }
     }
   }
 }
-// Scales of ordinary size multiply as they are, others as fractions and powers of two: the
-// same bits where both can.  Roundings are explicit: a row's results do not
-// depend on the kernel.
+template <int DT, typename G>
+__device__ __forceinline__ void i8_store_any(const LinearI8 &p, const G &g, int m0, int n0, const i32x4 (&acc)[G::FM][G::FN],
+                                             const float (&fx)[G::FM], const float (&fw)[G::GROUPS][G::COLS],
+                                             const float (&bias)[G::GROUPS][G::COLS]) {
+  typedef typename Store<DT>::T T;
+#pragma unroll
+  for (int i = 0; i < G::FM; ++i) {
+    const int m = g.row(m0, i);
+    const Scale sx(fx[i]);
+#pragma unroll
+    for (int q = 0; q < G::GROUPS; ++q) {
+      const int n = g.col(n0, q), left = p.N - n;
+      if (m < p.M && left > 0) {
+        float v[G::COLS], resid[G::COLS] = {};
+        if (p.resid) {
+          const T *r = static_cast<const T *>(p.resid) + int64_t(m) * p.ldr + n;
+#pragma unroll
+          for (int e = 0; e < G::COLS; ++e)
+            if (e < left) resid[e] = Store<DT>::dec(r[e]);
+        }
+#pragma unroll
+        for (int e = 0; e < G::COLS; ++e) {
+          const Scale sw(fw[q][e]);
+          v[e] = __fadd_rn(__builtin_amdgcn_ldexpf(__fmul_rn(__fmul_rn(float(acc[i][q * (G::COLS / 4) + e / 4][e % 4]), sx.f), sw.f), sx.e + sw.e),
+                           bias[q][e]);
+          v[e] = __fadd_rn(p.act == ACT_RELU ? i8_act<ACT_RELU>(v[e]) : p.act == ACT_GELU ? i8_act<ACT_GELU>(v[e]) : v[e], resid[e]);
+        }
+        T *out = static_cast<T *>(p.out) + int64_t(m) * p.ldo + n;
+        if (left >= G::COLS) {
+          i8_put<DT>(out, v);
+        } else {
+#pragma unroll
+          for (int e = 0; e < G::COLS; ++e)
+            if (e < left) out[e] = Store<DT>::enc(v[e]);
+        }
+      }
+    }
+  }
+}
 template <int DT, typename G>
 __device__ __forceinline__ void i8_store(const LinearI8 &p, const G &g, int m0, int n0, const i32x4 (&acc)[G::FM][G::FN]) {
-  const int mw = m0 + g.wm * G::WTM + g.li, nw = n0 + g.wn * G::WTN + 4 * g.lg;
-  float fx[G::FM], fw[G::FN][4];
+  typedef typename Store<DT>::T T;
+  const bool whole = n0 + (g.wn + 1) * G::WTN <= p.N;
+  float fx[G::FM], fw[G::GROUPS][G::COLS], bias[G::GROUPS][G::COLS] = {};
   bool plain = true;
 #pragma unroll
-  for (int i = 0; i < G::FM; ++i) fx[i] = p.sx[min(mw + i * 16, p.M - 1)];
+  for (int i = 0; i < G::FM; ++i) fx[i] = p.sx[min(g.row(m0, i), p.M - 1)];
 #pragma unroll
-  for (int j = 0; j < G::FN; ++j)
+  for (int q = 0; q < G::GROUPS; ++q) {
+    const int n = g.col(n0, q);
+    if (whole) {
+      i8_get<F32>(p.sw + n, fw[q]);
+      if (p.bias) i8_get<DT>(static_cast<const T *>(p.bias) + n, bias[q]);
+    } else {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) fw[j][e] = p.sw[min(nw + j * 16 + e, p.N - 1)];
+      for (int e = 0; e < G::COLS; ++e) {
+        fw[q][e] = p.sw[min(n + e, p.N - 1)];
+        if (p.bias) bias[q][e] = Store<DT>::dec(static_cast<const T *>(p.bias)[min(n + e, p.N - 1)]);
+      }
+    }
+  }
 #pragma unroll
   for (int i = 0; i < G::FM; ++i) plain &= plain_scale(fx[i]);
 #pragma unroll
-  for (int j = 0; j < G::FN; ++j)
+  for (int q = 0; q < G::GROUPS; ++q)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) plain &= plain_scale(fw[j][e]);
-  if (__all(plain)) i8_store_as<DT, G, true>(p, mw, nw, acc, fx, fw);
-  else i8_store_as<DT, G, false>(p, mw, nw, acc, fx, fw);
+    for (int e = 0; e < G::COLS; ++e) plain &= plain_scale(fw[q][e]);
+  if (whole && __all(plain)) {
+    if (p.act == ACT_NONE) i8_store_whole<DT, G, ACT_NONE>(p, g, m0, n0, acc, fx, fw, bias);
+    else if (p.act == ACT_RELU) i8_store_whole<DT, G, ACT_RELU>(p, g, m0, n0, acc, fx, fw, bias);
+    else i8_store_whole<DT, G, ACT_GELU>(p, g, m0, n0, acc, fx, fw, bias);
+  } else {
+    i8_store_any<DT, G>(p, g, m0, n0, acc, fx, fw, bias);
+  }
 }
 
 }  // namespace

@@ -306,7 +306,7 @@ struct LinearI8 {
   const void *bias = nullptr, *resid = nullptr;
   void *out = nullptr;
   int64_t ldx = 0, ldw = 0, ldo = 0, ldr = 0;
-  int M = 0, N = 0, K = 0, act = 0, quads = 0;  // quads: bias, residual and output go four values at a time
+  int M = 0, N = 0, K = 0, act = 0;
 };
 hipError_t linear_i8(int dt, const LinearI8 &p, hipStream_t st);
 // The next tokens of rows of logits (sample.hip).  Tokens of a row: the end of a group
