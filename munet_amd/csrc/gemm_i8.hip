@@ -8,18 +8,6 @@
 namespace mh {
 namespace {
 
-// 16 bytes of a row from k on, zeros past K.  Rows start anywhere: the loads are
-// not aligned.
-__device__ __forceinline__ i32x4 row_chunk(const int8_t *row, int k, int K) {
-  struct __attribute__((packed)) Any { i32x4 v; };
-  if (k + 16 <= K) return reinterpret_cast<const Any *>(row + k)->v;
-  i32x4 r = {0, 0, 0, 0};
-#pragma unroll
-  for (int i = 0; i < 16; ++i)
-    if (k + i < K) r[i >> 2] |= int(uint32_t(uint8_t(row[k + i])) << (8 * (i & 3)));
-  return r;
-}
-
 // Any K, any row spacing: 64 x 64 tiles of four waves, slabs of 128 bytes of K
 // staged through registers into two LDS buffers (gemm_pipe.hpp's layout).
 template <int DT>
@@ -42,8 +30,8 @@ __global__ void __launch_bounds__(256) gemm_i8_any_kernel(LinearI8 p) {
   auto load = [&](int kt) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      ra[i] = row_chunk(xr[i], kt * 128 + c0 * 16, p.K);
-      rb[i] = row_chunk(wr[i], kt * 128 + c0 * 16, p.K);
+      ra[i] = row_end(xr[i] + kt * 128 + c0 * 16, p.K - (kt * 128 + c0 * 16));
+      rb[i] = row_end(wr[i] + kt * 128 + c0 * 16, p.K - (kt * 128 + c0 * 16));
     }
   };
   auto put = [&](int b) {
@@ -245,7 +233,8 @@ template <int DT> hipError_t run(const LinearI8 &p, hipStream_t st) {
   int tile = blocks(p) ? 1 : 0;
   // (MUNET_HIP_I8_TILE names a kernel for tests and tuning, where the operands allow it)
   if (const char *force = std::getenv("MUNET_HIP_I8_TILE"))
-    if (blocks(p)) tile = std::atoi(force);
+    if (blocks(p) || std::atoi(force) >= 100) tile = std::atoi(force);
+  if (tile >= 100) return linear_i8_few(DT, p, tile - 100, st);
   switch (tile) {
   case 1: return launch<DT, 128, 128, 2, 2, 2>(p, st);
   case 2: return launch<DT, 256, 256, 4, 2, 2>(p, st);

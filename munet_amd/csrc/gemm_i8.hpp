@@ -10,6 +10,21 @@ namespace {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
+// 16 bytes of a row.  Rows start anywhere: the load is not aligned.
+__device__ __forceinline__ i32x4 row_block(const int8_t *p) {
+  struct __attribute__((packed)) Any { i32x4 v; };
+  return reinterpret_cast<const Any *>(p)->v;
+}
+// The same where `left` values are left of the row: zeros behind them.
+__device__ __forceinline__ i32x4 row_end(const int8_t *p, int left) {
+  if (left >= 16) return row_block(p);
+  i32x4 r = {0, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    if (i < left) r[i >> 2] |= int(uint32_t(uint8_t(p[i])) << (8 * (i & 3)));
+  return r;
+}
+
 // A scale as a fraction and a power of two.  The product of two scales may lie
 // outside the floats where the result does not (and below the normal ones, where
 // it loses digits): fractions multiply, powers add.

@@ -309,6 +309,7 @@ struct LinearI8 {
   int M = 0, N = 0, K = 0, act = 0;
 };
 hipError_t linear_i8(int dt, const LinearI8 &p, hipStream_t st);
+hipError_t linear_i8_few(int dt, const LinearI8 &p, int form, hipStream_t st);  // few rows (gemm_i8_few.hip)
 // The next tokens of rows of logits (sample.hip).  Tokens of a row: the end of a group
 // (of 2^21 tokens in rows of that length) and the tokens that a workgroup looks at past
 // the row's last chunk have 32-bit indexes.
