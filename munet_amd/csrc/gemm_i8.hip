@@ -4,46 +4,58 @@
 #include <cstdlib>
 
 #include "gemm_i8.hpp"
+#include "gemm_i8_tiles.hpp"
 
 namespace mh {
 namespace {
 
-// Any K, any row spacing: 64 x 64 tiles of four waves, slabs of 128 bytes of K
-// staged through registers into two LDS buffers (gemm_pipe.hpp's layout).
-template <int DT>
-__global__ void __launch_bounds__(256) gemm_i8_any_kernel(LinearI8 p) {
-  constexpr int BM = 64, BN = 64;
+// Any K, any row spacing: four waves, slabs of 128 bytes of K staged through
+// registers into two LDS buffers (gemm_pipe.hpp's layout).
+template <int DT, int BM, int BN> __global__ void __launch_bounds__(256) gemm_i8_any_kernel(LinearI8 p, int gn) {
+  constexpr int XCH = BM / 32, WCH = BN / 32;
   typedef I8Geom<BM, BN, 2, 2> G;
   __shared__ u32x4 lds[2][(BM + BN) * 8];
   int m0, n0;
-  pipe_tile<BM, BN>(p.M, p.N, 0, m0, n0);
+  pipe_tile<BM, BN>(p.M, p.N, gn, m0, n0);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const G g(wave, lane);
+  // chunk c0 of rows r0 + 32 i; rows past the end read the last one
   const int c0 = tid & 7, r0 = tid >> 3;
-  const int8_t *xr[2], *wr[2];
+  const int8_t *xr[XCH], *wr[WCH];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    xr[i] = p.x + int64_t(min(m0 + r0 + 32 * i, p.M - 1)) * p.ldx;
-    wr[i] = p.w + int64_t(min(n0 + r0 + 32 * i, p.N - 1)) * p.ldw;
-  }
-  i32x4 ra[2], rb[2];
+  for (int i = 0; i < XCH; ++i) xr[i] = p.x + int64_t(min(m0 + r0 + 32 * i, p.M - 1)) * p.ldx + c0 * 16;
+#pragma unroll
+  for (int i = 0; i < WCH; ++i) wr[i] = p.w + int64_t(min(n0 + r0 + 32 * i, p.N - 1)) * p.ldw + c0 * 16;
+  i32x4 ra[XCH], rb[WCH];
+  const int KT = (p.K + 127) / 128;
+  auto end = [](const int8_t *at, int left) {
+    RowBlock<true> r;
+    const int shift = row_shift(at);
+    r.load_end(at, shift, left);
+    return r.get(shift);
+  };
   auto load = [&](int kt) {
+    const int k = kt * 128;
+    if (k + 128 <= p.K) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      ra[i] = row_end(xr[i] + kt * 128 + c0 * 16, p.K - (kt * 128 + c0 * 16));
-      rb[i] = row_end(wr[i] + kt * 128 + c0 * 16, p.K - (kt * 128 + c0 * 16));
+      for (int i = 0; i < XCH; ++i) ra[i] = row_bytes(xr[i] + k);
+#pragma unroll
+      for (int i = 0; i < WCH; ++i) rb[i] = row_bytes(wr[i] + k);
+    } else {
+      const int left = p.K - k - c0 * 16;
+#pragma unroll
+      for (int i = 0; i < XCH; ++i) ra[i] = end(xr[i] + k, left);
+#pragma unroll
+      for (int i = 0; i < WCH; ++i) rb[i] = end(wr[i] + k, left);
     }
   };
   auto put = [&](int b) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int r = r0 + 32 * i;
-      lds[b][r * 8 + (c0 ^ G::xswizzle(r))] = __builtin_bit_cast(u32x4, ra[i]);
-      lds[b][BM * 8 + r * 8 + (c0 ^ G::wswizzle(r))] = __builtin_bit_cast(u32x4, rb[i]);
-    }
+    for (int i = 0; i < XCH; ++i) lds[b][(r0 + 32 * i) * 8 + (c0 ^ G::xswizzle(r0 + 32 * i))] = __builtin_bit_cast(u32x4, ra[i]);
+#pragma unroll
+    for (int i = 0; i < WCH; ++i) lds[b][(BM + r0 + 32 * i) * 8 + (c0 ^ G::wswizzle(r0 + 32 * i))] = __builtin_bit_cast(u32x4, rb[i]);
   };
   i32x4 acc[G::FM][G::FN] = {};
-  const int KT = (p.K + 127) / 128;
   load(0);
   put(0);
   __syncthreads();
@@ -207,18 +219,20 @@ __global__ void __launch_bounds__(WGM * WGN * 64) gemm_i8_kernel(LinearI8 p, int
   i8_store<DT, G>(p, g, m0, n0, acc);
 }
 
-template <int DT> hipError_t launch_any(const LinearI8 &p, hipStream_t st) {
-  const int64_t tiles = int64_t((p.M + 63) / 64) * ((p.N + 63) / 64);
+// Column groups of the tile enumeration, as in gemm_pipe.hip.
+int column_groups(const LinearI8 &p) { return 2L * p.N >= p.M ? (p.N >= 4L * p.M ? 16 : 8) : 0; }
+
+template <int DT, int BM, int BN> hipError_t launch_any(const LinearI8 &p, hipStream_t st) {
+  const int64_t tiles = int64_t((p.M + BM - 1) / BM) * ((p.N + BN - 1) / BN);
   if (tiles > kI8MaxTiles) return hipErrorInvalidValue;
-  hipLaunchKernelGGL(gemm_i8_any_kernel<DT>, dim3(unsigned(tiles)), dim3(256), 0, st, p);
+  hipLaunchKernelGGL((gemm_i8_any_kernel<DT, BM, BN>), dim3(unsigned(tiles)), dim3(256), 0, st, p, column_groups(p));
   return hipGetLastError();
 }
 
 template <int DT, int BM, int BN, int WGM, int WGN, int S> hipError_t launch(const LinearI8 &p, hipStream_t st) {
   const int64_t tiles = int64_t((p.M + BM - 1) / BM) * ((p.N + BN - 1) / BN);
   if (tiles > kI8MaxTiles) return hipErrorInvalidValue;
-  const int gn = 2L * p.N >= p.M ? (p.N >= 4L * p.M ? 16 : 8) : 0;
-  hipLaunchKernelGGL((gemm_i8_kernel<DT, BM, BN, WGM, WGN, S>), dim3(unsigned(tiles)), dim3(WGM * WGN * 64), 0, st, p, gn);
+  hipLaunchKernelGGL((gemm_i8_kernel<DT, BM, BN, WGM, WGN, S>), dim3(unsigned(tiles)), dim3(WGM * WGN * 64), 0, st, p, column_groups(p));
   return hipGetLastError();
 }
 
@@ -230,24 +244,28 @@ bool blocks(const LinearI8 &p) {
 }
 
 template <int DT> hipError_t run(const LinearI8 &p, hipStream_t st) {
-  int tile = blocks(p) ? 1 : 0;
-  // (MUNET_HIP_I8_TILE names a kernel for tests and tuning, where the operands allow it)
-  if (const char *force = std::getenv("MUNET_HIP_I8_TILE"))
-    if (blocks(p) || std::atoi(force) >= 100) tile = std::atoi(force);
-  if (tile >= 100) return linear_i8_few(DT, p, tile - 100, st);
+  const bool whole = blocks(p);
+  int tile = i8_tile(whole, p.M, p.N, p.K);
+  // MUNET_HIP_I8_TILE names a kernel for tests and tuning (read at every call; one that
+  // the operands do not suit takes the automatic choice)
+  if (const char *force = std::getenv("MUNET_HIP_I8_TILE")) {
+    const int f = std::atoi(force);
+    if (f == 0 || f == 10 || (f >= 1 && f <= 9 && whole) || ((f == 100 || f == 101) && p.M <= kI8FewRows)) tile = f;
+  }
   switch (tile) {
-  case 1: return launch<DT, 128, 128, 2, 2, 2>(p, st);
-  case 2: return launch<DT, 256, 256, 4, 2, 2>(p, st);
-  case 3: return launch<DT, 256, 256, 2, 4, 2>(p, st);
-  case 4: return launch<DT, 256, 128, 4, 2, 2>(p, st);
-  case 5: return launch<DT, 256, 128, 4, 2, 3>(p, st);
-  case 6: return launch<DT, 128, 128, 4, 2, 4>(p, st);
-  case 7: return launch<DT, 64, 64, 2, 2, 8>(p, st);
-  case 8: return launch<DT, 32, 64, 2, 2, 10>(p, st);
-  case 9: return launch<DT, 32, 32, 2, 2, 16>(p, st);
-  case 10: return launch<DT, 256, 256, 2, 2, 2>(p, st);
-  case 11: return launch<DT, 128, 64, 4, 2, 6>(p, st);
-  default: return launch_any<DT>(p, st);
+  case 1: return launch<DT, 256, 256, 2, 4, 2>(p, st);
+  case 2: return launch<DT, 256, 128, 4, 2, 3>(p, st);
+  case 3: return launch<DT, 128, 128, 4, 2, 4>(p, st);
+  case 4: return launch<DT, 128, 64, 4, 2, 6>(p, st);
+  case 5: return launch<DT, 64, 64, 2, 2, 5>(p, st);
+  case 6: return launch<DT, 64, 64, 2, 2, 3>(p, st);
+  case 7: return launch<DT, 64, 32, 2, 2, 6>(p, st);
+  case 8: return launch<DT, 32, 32, 2, 2, 9>(p, st);
+  case 9: return launch<DT, 64, 128, 2, 4, 3>(p, st);
+  case 10: return launch_any<DT, 128, 128>(p, st);
+  case 100:
+  case 101: return linear_i8_few(DT, p, tile - 100, st);
+  default: return launch_any<DT, 64, 64>(p, st);
   }
 }
 

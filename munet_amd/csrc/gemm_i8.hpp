@@ -10,19 +10,52 @@ namespace {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
-// 16 bytes of a row.  Rows start anywhere: the load is not aligned.
-__device__ __forceinline__ i32x4 row_block(const int8_t *p) {
+// 16 bytes of a row from anywhere.
+__device__ __forceinline__ i32x4 row_bytes(const int8_t *p) {
   struct __attribute__((packed)) Any { i32x4 v; };
   return reinterpret_cast<const Any *>(p)->v;
 }
-// The same where `left` values are left of the row: zeros behind them.
-__device__ __forceinline__ i32x4 row_end(const int8_t *p, int left) {
-  if (left >= 16) return row_block(p);
-  i32x4 r = {0, 0, 0, 0};
+// 16 bytes of a row.  ODD: rows start anywhere, `shift` bytes behind a word; whole
+// words are loaded, five of them, all of which hold some of the 16 bytes, and
+// shifted when they are used (loads that are not aligned to words take several times as
+// long: UNALIGNED_FIGURES).  Else the row's blocks start at words.
+template <bool ODD> struct RowBlock {
+  i32x4 v;
+  int next;
+  __device__ __forceinline__ void load(const int8_t *p, int shift) {
+    struct __attribute__((packed, aligned(4))) Words { i32x4 v; };
+    const int8_t *w = ODD ? p - shift : p;
+    v = reinterpret_cast<const Words *>(w)->v;
+    if constexpr (ODD) next = reinterpret_cast<const int *>(w)[shift ? 4 : 3];
+  }
+  // where `left` values are left of the row: zeros behind them, and no word without one
+  __device__ __forceinline__ void load_end(const int8_t *p, int shift, int left) {
+    if (left >= 16) {
+      load(p, shift);
+      return;
+    }
+    const int first = ODD ? shift : 0, end = left > 0 ? first + left : 0;
+    const int *w = reinterpret_cast<const int *>(p - first);
+    uint32_t r[5];
 #pragma unroll
-  for (int i = 0; i < 16; ++i)
-    if (i < left) r[i >> 2] |= int(uint32_t(uint8_t(p[i])) << (8 * (i & 3)));
-  return r;
+    for (int q = 0; q < 5; ++q) {
+      const int n = end - 4 * q;
+      const uint32_t x = n > 0 && (ODD || q < 4) ? uint32_t(w[q]) : 0u;
+      r[q] = n >= 4 ? x : n > 0 ? x & ((1u << (8 * n)) - 1u) : 0u;
+    }
+    v = i32x4{int(r[0]), int(r[1]), int(r[2]), int(r[3])};
+    if constexpr (ODD) next = int(r[4]);
+  }
+  __device__ __forceinline__ i32x4 get(int shift) const {
+    if constexpr (!ODD) return v;
+    const uint32_t s = uint32_t(shift);
+    return i32x4{int(__builtin_amdgcn_alignbyte(uint32_t(v[1]), uint32_t(v[0]), s)), int(__builtin_amdgcn_alignbyte(uint32_t(v[2]), uint32_t(v[1]), s)),
+                 int(__builtin_amdgcn_alignbyte(uint32_t(v[3]), uint32_t(v[2]), s)), int(__builtin_amdgcn_alignbyte(uint32_t(next), uint32_t(v[3]), s))};
+  }
+};
+__device__ __forceinline__ int row_shift(const int8_t *p) { return int(reinterpret_cast<uintptr_t>(p) & 3); }
+inline bool odd_rows(const LinearI8 &p) {
+  return ((reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.w)) & 3) || (p.ldx & 3) || (p.ldw & 3);
 }
 
 // A scale as a fraction and a power of two.  The product of two scales may lie

@@ -11,7 +11,7 @@
 namespace mh {
 namespace {
 
-template <int DT, int MF, int NF, int W, int CH>
+template <int DT, int MF, int NF, int W, int CH, bool ODD>
 __global__ void __launch_bounds__(64 * W) gemm_i8_few_kernel(LinearI8 p) {
   __shared__ i32x4 red[W][MF * NF][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -22,17 +22,22 @@ __global__ void __launch_bounds__(64 * W) gemm_i8_few_kernel(LinearI8 p) {
   for (int i = 0; i < MF; ++i) xr[i] = p.x + int64_t(min(m0 + 16 * i + li, p.M - 1)) * p.ldx + 16 * lg;
 #pragma unroll
   for (int j = 0; j < NF; ++j) wr[j] = p.w + int64_t(min(n0 + 16 * j + li, p.N - 1)) * p.ldw + 16 * lg;
+  int xs[MF], ws[NF];
+#pragma unroll
+  for (int i = 0; i < MF; ++i) xs[i] = row_shift(xr[i]);
+#pragma unroll
+  for (int j = 0; j < NF; ++j) ws[j] = row_shift(wr[j]);
   i32x4 acc[MF][NF] = {};
   const int whole = p.K / 64, pieces = whole / CH;  // steps and pieces that every lane has
-  struct Piece { i32x4 x[CH][MF], w[CH][NF]; } a, b;
+  struct Piece { RowBlock<ODD> x[CH][MF], w[CH][NF]; } a, b;
   auto load = [&](Piece &q, int piece) {
 #pragma unroll
     for (int s = 0; s < CH; ++s) {
       const int k = (piece * CH + s) * 64;
 #pragma unroll
-      for (int j = 0; j < NF; ++j) q.w[s][j] = row_block(wr[j] + k);
+      for (int j = 0; j < NF; ++j) q.w[s][j].load(wr[j] + k, ws[j]);
 #pragma unroll
-      for (int i = 0; i < MF; ++i) q.x[s][i] = row_block(xr[i] + k);
+      for (int i = 0; i < MF; ++i) q.x[s][i].load(xr[i] + k, xs[i]);
     }
   };
   auto add = [&](const Piece &q) {
@@ -41,7 +46,7 @@ __global__ void __launch_bounds__(64 * W) gemm_i8_few_kernel(LinearI8 p) {
 #pragma unroll
       for (int i = 0; i < MF; ++i)
 #pragma unroll
-        for (int j = 0; j < NF; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(q.w[s][j], q.x[s][i], acc[i][j], 0, 0, 0);
+        for (int j = 0; j < NF; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(q.w[s][j].get(ws[j]), q.x[s][i].get(xs[i]), acc[i][j], 0, 0, 0);
   };
   int c = wave;
   if (c < pieces) load(a, c);
@@ -54,16 +59,16 @@ __global__ void __launch_bounds__(64 * W) gemm_i8_few_kernel(LinearI8 p) {
   }
   // the steps behind the last whole piece, the last one of them not whole
   for (int s = pieces * CH + wave; s * 64 < p.K; s += W) {
-    i32x4 x[MF], w[NF];
+    RowBlock<ODD> x[MF], w[NF];
     const int k = s * 64, left = p.K - k - 16 * lg;
 #pragma unroll
-    for (int j = 0; j < NF; ++j) w[j] = row_end(wr[j] + k, left);
+    for (int j = 0; j < NF; ++j) w[j].load_end(wr[j] + k, ws[j], left);
 #pragma unroll
-    for (int i = 0; i < MF; ++i) x[i] = row_end(xr[i] + k, left);
+    for (int i = 0; i < MF; ++i) x[i].load_end(xr[i] + k, xs[i], left);
 #pragma unroll
     for (int i = 0; i < MF; ++i)
 #pragma unroll
-      for (int j = 0; j < NF; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[j], x[i], acc[i][j], 0, 0, 0);
+      for (int j = 0; j < NF; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[j].get(ws[j]), x[i].get(xs[i]), acc[i][j], 0, 0, 0);
   }
 #pragma unroll
   for (int i = 0; i < MF; ++i)
@@ -85,24 +90,13 @@ __global__ void __launch_bounds__(64 * W) gemm_i8_few_kernel(LinearI8 p) {
 template <int DT, int MF, int NF, int W, int CH> hipError_t launch(const LinearI8 &p, hipStream_t st) {
   const dim3 grid(unsigned((p.N + 16 * NF - 1) / (16 * NF)), unsigned((p.M + 16 * MF - 1) / (16 * MF)));
   if (grid.y > 65535) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((gemm_i8_few_kernel<DT, MF, NF, W, CH>), grid, dim3(64 * W), 0, st, p);
+  if (odd_rows(p)) hipLaunchKernelGGL((gemm_i8_few_kernel<DT, MF, NF, W, CH, true>), grid, dim3(64 * W), 0, st, p);
+  else hipLaunchKernelGGL((gemm_i8_few_kernel<DT, MF, NF, W, CH, false>), grid, dim3(64 * W), 0, st, p);
   return hipGetLastError();
 }
 
 template <int DT> hipError_t run(const LinearI8 &p, int form, hipStream_t st) {
-  switch (form) {
-  case 0: return launch<DT, 1, 1, 8, 4>(p, st);
-  case 1: return launch<DT, 1, 2, 8, 4>(p, st);
-  case 2: return launch<DT, 2, 1, 8, 4>(p, st);
-  case 3: return launch<DT, 2, 2, 8, 2>(p, st);
-  case 4: return launch<DT, 4, 2, 8, 2>(p, st);
-  case 5: return launch<DT, 4, 4, 8, 1>(p, st);
-  case 6: return launch<DT, 1, 1, 4, 4>(p, st);
-  case 7: return launch<DT, 1, 1, 16, 2>(p, st);
-  case 8: return launch<DT, 4, 1, 8, 2>(p, st);
-  case 9: return launch<DT, 2, 4, 8, 2>(p, st);
-  default: return hipErrorInvalidValue;
-  }
+  return form == 0 ? launch<DT, 1, 1, 4, 4>(p, st) : launch<DT, 1, 2, 8, 4>(p, st);
 }
 
 }  // namespace
