@@ -820,6 +820,7 @@ int mh_kv_store_rotary_paged(int dt, const void *k, const void *v, int64_t ldk, 
     const char *op = "kv_store_rotary_paged";
     check_dt(dt);
     check_pool(op, k_cache, v_cache, k_scale, v_scale, Hkv, hd, page, n_pages);
+    if (Hkv > 65534) throw Error("kv_store_rotary_paged: bad key/value head count");
     if (n < 0) throw Error("kv_store_rotary_paged: negative size");
     if (n > 1 << 27) throw Error("kv_store_rotary_paged: more tokens than one launch takes (2^27)");
     if (q && (Hq < 1 || int64_t(Hq) * hd > 1 << 30)) throw Error("kv_store_rotary_paged: bad query head count");

@@ -156,13 +156,63 @@ template <int DT> struct Raw {
   }
 };
 
-// A token's eight key values from d on: as they lie, or rotated on the way (ROT 1:
-// pairs half a head apart, 2: neighbours).  Rotated keys are held as floats, so that
-// the cache's 8 bits are their only rounding.
+// Piece c of a key: two fours of its values, at `lo` and `hi` of the head.  Eight
+// consecutive ones, but where pairs lie half the rotated part apart (ROT 1) both
+// values of four pairs, so that a thread turns what it has; with ROT 2 (neighbours
+// paired) eight values are four pairs.  Either way the pairs are 4 c .. 4 c + 3, in two
+// loads of the table (eight values of each half and their partners took twice
+// the loads: APPEND_FIGURES).  Rotated keys are floats, so that the cache's 8 bits are their
+// only rounding.
+template <int DT, int ROT> struct KeyPiece {
+  int lo, hi;
+  bool turns;  // four whole pairs
+  __device__ __forceinline__ KeyPiece(int c, int half) {
+    const bool whole = half % 4 == 0;
+    turns = ROT != 0 && whole && 4 * c < half;
+    lo = ROT == 1 && turns ? 4 * c : 8 * c;
+    hi = ROT == 1 && turns ? 4 * c + half : 8 * c + 4;
+  }
+  __device__ __forceinline__ void load(const typename Store<DT>::T *head, const float2 *tab, int half, float v[8]) const {
+    if constexpr (ROT == 0) {
+      ld8<DT>(head + lo, v);
+    } else if (half % 4 != 0) {
+      turned8<DT, ROT == 2>(head, tab, half, lo, v);  // (pairs that straddle pieces)
+    } else {
+      ld4<DT>(head + lo, v);
+      ld4<DT>(head + hi, v + 4);
+      if (!turns) return;
+      const float4 *t = reinterpret_cast<const float4 *>(tab + (ROT == 1 ? lo : lo / 2));
+      const float4 a = t[0], b = t[1];
+      if constexpr (ROT == 1) {
+        turn(v[0], v[4], a.x, a.y);
+        turn(v[1], v[5], a.z, a.w);
+        turn(v[2], v[6], b.x, b.y);
+        turn(v[3], v[7], b.z, b.w);
+      } else {
+        turn(v[0], v[1], a.x, a.y);
+        turn(v[2], v[3], a.z, a.w);
+        turn(v[4], v[5], b.x, b.y);
+        turn(v[6], v[7], b.z, b.w);
+      }
+    }
+  }
+  __device__ __forceinline__ void store(uint8_t *row, const float v[8], float inv) const {
+    float w[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e] = v[e] * inv;
+    if constexpr (ROT == 1) {
+      *reinterpret_cast<uint32_t *>(row + lo) = e4m3x4(w);
+      *reinterpret_cast<uint32_t *>(row + hi) = e4m3x4(w + 4);
+    } else {
+      *reinterpret_cast<uint2 *>(row + lo) = make_uint2(e4m3x4(w), e4m3x4(w + 4));
+    }
+  }
+};
+// A token's key piece as it is held: its bits, or rotated floats.
 template <int DT, int ROT> struct Key {
   float f[8];
-  __device__ __forceinline__ void load(const typename Store<DT>::T *head, const float2 *tab, int half, int d) {
-    turned8<DT, ROT == 2>(head, tab, half, d, f);
+  __device__ __forceinline__ void load(const KeyPiece<DT, ROT> &k, const typename Store<DT>::T *head, const float2 *tab, int half) {
+    k.load(head, tab, half, f);
   }
   __device__ __forceinline__ void get(float v[8]) const {
 #pragma unroll
@@ -171,9 +221,49 @@ template <int DT, int ROT> struct Key {
 };
 template <int DT> struct Key<DT, 0> {
   Raw<DT> r;
-  __device__ __forceinline__ void load(const typename Store<DT>::T *head, const float2 *, int, int d) { r.load(head + d); }
+  __device__ __forceinline__ void load(const KeyPiece<DT, 0> &k, const typename Store<DT>::T *head, const float2 *, int) { r.load(head + k.lo); }
   __device__ __forceinline__ void get(float v[8]) const { r.get(v); }
 };
+
+// The scale of a page (and head) that gets values of largest magnitude `top` from
+// `place` on, and what its earlier tokens are multiplied by.
+struct PageScale {
+  float now, inv, ratio;
+  __device__ __forceinline__ PageScale(float top, float held, int place) {
+    const float want = e4m3_scale(top);
+    const bool keep = place > 0 && held > want && held < __builtin_inff();
+    now = keep ? held : want;
+    inv = 1.0f / now;
+    ratio = place > 0 && held > 0.f && held < now ? held * inv : 1.f;
+  }
+};
+// The page's earlier tokens in a larger scale, by NT threads.
+template <int NT> __device__ __forceinline__ void rescale_keys(uint8_t *kd, int place, int hd, float ratio, int tid) {
+  for (int c = tid; c < place * hd / 16; c += NT) {
+    uint4 *p = reinterpret_cast<uint4 *>(kd) + c;
+    const uint4 w = *p;
+    *p = make_uint4(rescale4(w.x, ratio), rescale4(w.y, ratio), rescale4(w.z, ratio), rescale4(w.w, ratio));
+  }
+}
+template <int NT> __device__ __forceinline__ void rescale_values(uint8_t *vd, int place, int hd, int P, float ratio, int tid) {
+  // (whole 16-byte pieces of a row: what lies behind the earlier tokens is kept, or
+  // written afterwards)
+  const int pieces = (place + 15) / 16;
+  for (int c = tid; c < hd * pieces; c += NT) {
+    const int d = c / pieces, i = c - d * pieces;
+    uint4 *p = reinterpret_cast<uint4 *>(vd + int64_t(d) * P + 16 * i);
+    const uint4 w = *p;
+    const uint32_t o[4] = {w.x, w.y, w.z, w.w};
+    uint32_t r[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int left = place - 16 * i - 4 * q;  // earlier tokens from this word on
+      const uint32_t m = left >= 4 ? 0xffffffffu : left <= 0 ? 0u : (1u << (8 * left)) - 1u;
+      r[q] = (rescale4(o[q], ratio) & m) | (o[q] & ~m);
+    }
+    *p = make_uint4(r[0], r[1], r[2], r[3]);
+  }
+}
 
 struct StoreArgs {
   const void *k, *v;
@@ -185,13 +275,16 @@ struct StoreArgs {
   int n, Hkv, hd, page, n_pages, per;
   const float2 *table;  // rotated keys: their angles
   int half;
+  Rotary q;       // queries to rotate beside them (workgroups behind the heads'), 0 heads: none
+  int q_unit;
+  unsigned q_groups;
 };
 
 // A run is a stretch of tokens with consecutive slots inside one page.  The
 // workgroup that holds a run's first token writes all of it for one head, and
 // so owns the page's two scales.  Tokens at `per` consecutive places per
 // workgroup.
-template <int DT, int NT, int ROT>
+template <int DT, int NT, int ROT, bool ONE>
 __global__ void __launch_bounds__(NT) kv_store_paged_kernel(StoreArgs a) {
   typedef typename Store<DT>::T T;
   constexpr int VT = 64;  // tokens of a value tile
@@ -202,9 +295,69 @@ __global__ void __launch_bounds__(NT) kv_store_paged_kernel(StoreArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, head = blockIdx.y;
   const int t0 = blockIdx.x * a.per, hd = a.hd, P = a.page, h8 = hd / 8;
   const int64_t limit = int64_t(a.n_pages) * P;
-  // the run starts among this workgroup's tokens (every wave finds the same)
+  if constexpr (ROT != 0) {
+    if (head >= a.Hkv) {
+      const unsigned step = (gridDim.y - a.Hkv) * gridDim.x;
+      for (unsigned i = (head - a.Hkv) * gridDim.x + blockIdx.x; i < a.q_groups; i += step) {
+        constexpr int U = ROT == 2 ? (DT == F32 ? 2 : 4) : (DT == F32 ? 4 : 8);
+        if (a.q_unit == 1) rotate_tokens<DT, 1, ROT == 2, NT>(a.q, int64_t(i) * a.q.tokens, a.slots, limit);
+        else rotate_tokens<DT, U, ROT == 2, NT>(a.q, int64_t(i) * a.q.tokens, a.slots, limit);
+      }
+      return;
+    }
+  }
   uint64_t starts;
-  {
+  if constexpr (ONE) {
+    // One token for the workgroup (a decode step).  Where it is a run of its own, the
+    // first wave stores it without LDS or barriers, a key piece or a value piece to
+    // a lane; its row is loaded before its slot is known (64 tokens, 8 heads of 128:
+    // ONE_FIGURES).
+    const int vh = lane >> 5, c = lane & 31;
+    const bool on = wave == 0 && c < h8;
+    const KeyPiece<DT, ROT> piece(c, a.half);
+    float v[8] = {};
+    if (on) {
+      const int64_t hv = int64_t(head) * hd;
+      if (vh) ld8<DT>(static_cast<const T *>(a.v) + int64_t(t0) * a.ldv + hv + 8 * c, v);
+      else piece.load(static_cast<const T *>(a.k) + int64_t(t0) * a.ldk + hv, ROT ? a.table + int64_t(t0) * a.half : nullptr, a.half, v);
+    }
+    const int s = a.slots[t0], before = a.slots[max(t0 - 1, 0)], behind = a.slots[min(t0 + 1, a.n - 1)];
+    if ((s < -1 || s >= limit) && head == 0 && tid == 0) atomicOr(a.err, kErrPage);
+    if (s < 0 || s >= limit) return;
+    const int page = s / P, place = s - page * P;
+    if (place != 0 && t0 != 0 && before == s - 1) return;  // (a run that starts before)
+    if (place + 1 == P || t0 + 1 == a.n || behind != s + 1) {
+      if (wave != 0) return;
+      const int64_t sc = int64_t(page) * a.Hkv + head;
+      float *scale = vh ? a.vs + sc : a.ks + sc;
+      const float held = *scale;
+      float big = on ? amax8(v, 0.f) : 0.f;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor(big, o, 64));
+      const PageScale ps(big, held, place);
+      uint8_t *kd = a.kc + page_base(page, a.Hkv, head, P, hd), *vd = a.vc + page_base(page, a.Hkv, head, P, hd);
+      const float kratio = __shfl(ps.ratio, 0, 64), vratio = __shfl(ps.ratio, 32, 64);
+      if (kratio != 1.f) rescale_keys<64>(kd, place, hd, kratio, lane);
+      if (vratio != 1.f) {
+        rescale_values<64>(vd, place, hd, P, vratio, lane);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the new place lies in a piece that was rewritten
+      }
+      if (on && vh) {
+        float w[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = v[e] * ps.inv;
+        const uint32_t b[2] = {e4m3x4(w), e4m3x4(w + 4)};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) vd[int64_t(8 * c + e) * P + place] = uint8_t(b[e >> 2] >> (8 * (e & 3)));
+      } else if (on) {
+        piece.store(kd + int64_t(place) * hd, v, ps.inv);
+      }
+      if (c == 0) *scale = ps.now;
+      return;
+    }
+    starts = 1;
+  } else {
+    // the run starts among this workgroup's tokens (every wave finds the same)
     const int t = t0 + lane;
     bool first = false;
     if (lane < a.per && t < a.n) {
@@ -236,11 +389,6 @@ __global__ void __launch_bounds__(NT) kv_store_paged_kernel(StoreArgs a) {
     const float2 *tab = ROT ? a.table + int64_t(t) * a.half : nullptr;
     uint8_t *kd = a.kc + page_base(page, a.Hkv, head, P, hd), *vd = a.vc + page_base(page, a.Hkv, head, P, hd);
 
-    auto key8 = [&](int i, int d, float v[8]) {
-      if constexpr (ROT) turned8<DT, ROT == 2>(kp + int64_t(i) * a.ldk, tab + int64_t(i) * a.half, a.half, d, v);
-      else ld8<DT>(kp + int64_t(i) * a.ldk + d, v);
-    };
-
     // A run of at most NT pieces of 4 places and 8 head values (NT 256: 64 tokens of
     // heads of 128) is held in registers, a piece to a thread: loaded once, its values
     // transposed four places at a time (17k tokens, 8 heads of 128: 39 us, against 44
@@ -248,6 +396,7 @@ __global__ void __launch_bounds__(NT) kv_store_paged_kernel(StoreArgs a) {
     const int q0 = place / 4, nq = (place + n - 1) / 4 - q0 + 1;
     const bool held_run = nq * h8 <= NT;
     const int pq = tid / h8, pd = 8 * (tid - pq * h8), pi = 4 * (q0 + pq) - place;  // this thread's piece: first token
+    const KeyPiece<DT, ROT> kpiece(pd / 8, a.half);
     const bool mine = held_run && pq < nq;
     Key<DT, ROT> kr[4];
     Raw<DT> vr[4];
@@ -256,7 +405,7 @@ __global__ void __launch_bounds__(NT) kv_store_paged_kernel(StoreArgs a) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int64_t i = min(max(pi + j, 0), n - 1);  // (places beside the run repeat its tokens, not stored)
-        kr[j].load(kp + i * a.ldk, tab + (ROT ? i * a.half : 0), a.half, pd);
+        kr[j].load(kpiece, kp + i * a.ldk, tab + (ROT ? i * a.half : 0), a.half);
         vr[j].load(vp + i * a.ldv + pd);
       }
 #pragma unroll
@@ -271,7 +420,7 @@ __global__ void __launch_bounds__(NT) kv_store_paged_kernel(StoreArgs a) {
     for (int c = held_run ? n * h8 : tid; c < n * h8; c += NT) {
       const int i = c / h8, d = 8 * (c - i * h8);
       float v[8];
-      key8(i, d, v);
+      KeyPiece<DT, ROT>(d / 8, a.half).load(kp + int64_t(i) * a.ldk, tab + (ROT ? int64_t(i) * a.half : 0), a.half, v);
       big[0] = amax8(v, big[0]);
       ld8<DT>(vp + int64_t(i) * a.ldv + d, v);
       big[1] = amax8(v, big[1]);
@@ -288,38 +437,14 @@ __global__ void __launch_bounds__(NT) kv_store_paged_kernel(StoreArgs a) {
       float top = red[x][0];
 #pragma unroll
       for (int v = 1; v < NW; ++v) top = fmaxf(top, red[x][v]);
-      const float want = e4m3_scale(top);
-      const bool keep = place > 0 && held[x] > want && held[x] < __builtin_inff();
-      now[x] = keep ? held[x] : want;
-      inv[x] = 1.0f / now[x];
-      ratio[x] = place > 0 && held[x] > 0.f && held[x] < now[x] ? held[x] * inv[x] : 1.f;
+      const PageScale ps(top, held[x], place);
+      now[x] = ps.now;
+      inv[x] = ps.inv;
+      ratio[x] = ps.ratio;
     }
     // the page's earlier tokens in the larger scale
-    if (ratio[0] != 1.f)
-      for (int c = tid; c < place * hd / 16; c += NT) {
-        uint4 *p = reinterpret_cast<uint4 *>(kd) + c;
-        const uint4 w = *p;
-        *p = make_uint4(rescale4(w.x, ratio[0]), rescale4(w.y, ratio[0]), rescale4(w.z, ratio[0]), rescale4(w.w, ratio[0]));
-      }
-    if (ratio[1] != 1.f) {
-      // (whole 16-byte pieces of a row: what lies behind the earlier tokens is
-      // kept, or written by the run below)
-      const int pieces = (place + 15) / 16;
-      for (int c = tid; c < hd * pieces; c += NT) {
-        const int d = c / pieces, i = c - d * pieces;
-        uint4 *p = reinterpret_cast<uint4 *>(vd + int64_t(d) * P + 16 * i);
-        const uint4 w = *p;
-        const uint32_t o[4] = {w.x, w.y, w.z, w.w};
-        uint32_t r[4];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int left = place - 16 * i - 4 * q;  // earlier tokens from this word on
-          const uint32_t m = left >= 4 ? 0xffffffffu : left <= 0 ? 0u : (1u << (8 * left)) - 1u;
-          r[q] = (rescale4(o[q], ratio[1]) & m) | (o[q] & ~m);
-        }
-        *p = make_uint4(r[0], r[1], r[2], r[3]);
-      }
-    }
+    if (ratio[0] != 1.f) rescale_keys<NT>(kd, place, hd, ratio[0], tid);
+    if (ratio[1] != 1.f) rescale_values<NT>(vd, place, hd, P, ratio[1], tid);
     __syncthreads();
 
     if (held_run) {
@@ -330,10 +455,7 @@ __global__ void __launch_bounds__(NT) kv_store_paged_kernel(StoreArgs a) {
         for (int j = 0; j < 4; ++j) {
           float v[8];
           kr[j].get(v);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] *= inv[0];
-          if (pi + j >= 0 && pi + j < n)
-            *reinterpret_cast<uint2 *>(kd + int64_t(place + pi + j) * hd + pd) = make_uint2(e4m3x4(v), e4m3x4(v + 4));
+          if (pi + j >= 0 && pi + j < n) kpiece.store(kd + int64_t(place + pi + j) * hd, v, inv[0]);
           vr[j].get(v);
 #pragma unroll
           for (int e = 0; e < 8; ++e) v[e] *= inv[1];
@@ -373,10 +495,9 @@ __global__ void __launch_bounds__(NT) kv_store_paged_kernel(StoreArgs a) {
     for (int c = tid; c < n * h8; c += NT) {
       const int i = c / h8, d = 8 * (c - i * h8);
       float v[8];
-      key8(i, d, v);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] *= inv[0];
-      *reinterpret_cast<uint2 *>(kd + int64_t(place + i) * hd + d) = make_uint2(e4m3x4(v), e4m3x4(v + 4));
+      const KeyPiece<DT, ROT> piece(d / 8, a.half);
+      piece.load(kp + int64_t(i) * a.ldk, tab + (ROT ? int64_t(i) * a.half : 0), a.half, v);
+      piece.store(kd + int64_t(place + i) * hd, v, inv[0]);
     }
     // values, transposed through LDS in tiles of VT places
     for (int c0 = place & ~(VT - 1); c0 < place + n; c0 += VT) {
@@ -426,23 +547,30 @@ hipError_t kv_store_paged(int dt, const void *k, const void *v, long ldk, long l
                           hipStream_t st, const Rotary *rot) {
   if (n < 1 || n > 1 << 27 || Hkv < 1 || Hkv > 65535) return hipErrorInvalidValue;
   StoreArgs a{k, v, slots, static_cast<uint8_t *>(k_cache), static_cast<uint8_t *>(v_cache), k_scale, v_scale, err, ldk, ldv,
-              n, Hkv, hd, page, n_pages, store_tokens(n, Hkv), rot ? reinterpret_cast<const float2 *>(rot->table) : nullptr, rot ? rot->half : 0};
-  if (rot && rot->heads) {
-    const hipError_t e = rotary(dt, *rot, slots, int64_t(n_pages) * page, st);
-    if (e != hipSuccess) return e;
-  }
-  const dim3 grid(unsigned((n + a.per - 1) / a.per), unsigned(Hkv));
+              n, Hkv, hd, page, n_pages, store_tokens(n, Hkv), rot ? reinterpret_cast<const float2 *>(rot->table) : nullptr, rot ? rot->half : 0,
+              Rotary{}, 0, 0};
   // Threads for a page's pieces at once where workgroups take many tokens (17k
   // tokens, 8 heads of 128: pages of 128 42 us, 56 with 256 threads; of 256 56, 60);
   // where they take one, most would be idle.
   const int pieces = page / 4 * (hd / 8), nt = a.per == 1 || pieces <= 256 ? 256 : pieces <= 512 ? 512 : 1024;
+  dim3 grid(unsigned((n + a.per - 1) / a.per), unsigned(Hkv));
+  if (rot && rot->heads) {
+    // the queries behind the heads' workgroups: no more rows of them than a grid has left
+    a.q = *rot;
+    a.q_unit = rotary_unit(dt, a.q);
+    rotary_cut(dt, a.q_unit, nt, a.q);
+    a.q_groups = unsigned((n + a.q.tokens - 1) / a.q.tokens);
+    grid.y += std::min((a.q_groups + grid.x - 1) / grid.x, std::max(1u, 65535u - grid.y));
+  }
 #define MH_STORE(DTV, ROT)                                                                                \
-  if (nt == 256)                                                                                          \
-    hipLaunchKernelGGL((kv_store_paged_kernel<DTV, 256, ROT>), grid, dim3(256), 0, st, a);                \
+  if (a.per == 1)                                                                                         \
+    hipLaunchKernelGGL((kv_store_paged_kernel<DTV, 256, ROT, true>), grid, dim3(256), 0, st, a);          \
+  else if (nt == 256)                                                                                     \
+    hipLaunchKernelGGL((kv_store_paged_kernel<DTV, 256, ROT, false>), grid, dim3(256), 0, st, a);         \
   else if (nt == 512)                                                                                     \
-    hipLaunchKernelGGL((kv_store_paged_kernel<DTV, 512, ROT>), grid, dim3(512), 0, st, a);                \
+    hipLaunchKernelGGL((kv_store_paged_kernel<DTV, 512, ROT, false>), grid, dim3(512), 0, st, a);         \
   else                                                                                                    \
-    hipLaunchKernelGGL((kv_store_paged_kernel<DTV, 1024, ROT>), grid, dim3(1024), 0, st, a);
+    hipLaunchKernelGGL((kv_store_paged_kernel<DTV, 1024, ROT, false>), grid, dim3(1024), 0, st, a);
 #define MH_STORE_ROT(DTV)                                                                                 \
   if (!rot) {                                                                                             \
     MH_STORE(DTV, 0)                                                                                      \

@@ -23,6 +23,11 @@ pytestmark = pytest.mark.gpu
 @pytest.fixture(scope="module")
 def torch(hip):
     import torch as t
+    from munet_amd._lib import HipError
+    try:  # (errors that tests of other files left set)
+        hip.check_device_errors()
+    except HipError:
+        pass
     return t
 
 

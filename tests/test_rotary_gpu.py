@@ -20,6 +20,11 @@ LEAST = {"bfloat16": 2.0 ** -134, "float16": 2.0 ** -25, "float32": 2.0 ** -149}
 @pytest.fixture(scope="module")
 def torch(hip):
     import torch as t
+    from munet_amd._lib import HipError
+    try:  # (errors that tests of other files left set)
+        hip.check_device_errors()
+    except HipError:
+        pass
     return t
 
 

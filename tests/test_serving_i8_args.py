@@ -117,7 +117,7 @@ def _store(**kw):
 
 
 @pytest.mark.parametrize("kw,match", [
-    (dict(dt=3), "dtype"), (dict(hd=24), "multiple of 16"), (dict(Hkv=0), "head count"), (dict(Hkv=65536), "head count"),
+    (dict(dt=3), "dtype"), (dict(hd=24), "multiple of 16"), (dict(Hkv=0), "head count"), (dict(Hkv=65535), "head count"),
     (dict(page=100), "page holds"), (dict(n=-1), "negative"), (dict(n=(1 << 27) + 1), "one launch"), (dict(slots=None), "null slots"),
     (dict(k=None), "null k"), (dict(v=FAR + 8), "aligned"), (dict(ldk=1023), "multiple of 16"), (dict(table=None), "null table"),
     (dict(table=A + 8), "aligned"), (dict(half=0), "rotated part"), (dict(half=65), "rotated part"), (dict(kc=None), "null cache"),
