@@ -291,7 +291,7 @@ __global__ void __launch_bounds__(NT) kv_store_paged_kernel(StoreArgs a) {
   constexpr int NW = NT / 64;
   __shared__ float red[2][NW];
   // (rows of VT + 4 bytes; of the run's quads in the short form)
-  __shared__ __align__(16) uint8_t vt[NT == 256 ? kPagedHeadMax * (VT + 4) : 32 * NT + 4 * kPagedHeadMax];
+  __shared__ __align__(16) uint8_t vt[ONE ? kPagedHeadMax * (VT + 4) : 32 * NT + 4 * kPagedHeadMax];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, head = blockIdx.y;
   const int t0 = blockIdx.x * a.per, hd = a.hd, P = a.page, h8 = hd / 8;
   const int64_t limit = int64_t(a.n_pages) * P;
@@ -300,8 +300,8 @@ __global__ void __launch_bounds__(NT) kv_store_paged_kernel(StoreArgs a) {
       const unsigned step = (gridDim.y - a.Hkv) * gridDim.x;
       for (unsigned i = (head - a.Hkv) * gridDim.x + blockIdx.x; i < a.q_groups; i += step) {
         constexpr int U = ROT == 2 ? (DT == F32 ? 2 : 4) : (DT == F32 ? 4 : 8);
-        if (a.q_unit == 1) rotate_tokens<DT, 1, ROT == 2, NT>(a.q, int64_t(i) * a.q.tokens, a.slots, limit);
-        else rotate_tokens<DT, U, ROT == 2, NT>(a.q, int64_t(i) * a.q.tokens, a.slots, limit);
+        if (a.q_unit == 1) rotate_tokens<DT, 1, ROT == 2, NT, 2>(a.q, int64_t(i) * a.q.tokens, a.slots, limit);
+        else rotate_tokens<DT, U, ROT == 2, NT, 2>(a.q, int64_t(i) * a.q.tokens, a.slots, limit);
       }
       return;
     }
@@ -552,7 +552,7 @@ hipError_t kv_store_paged(int dt, const void *k, const void *v, long ldk, long l
   // Threads for a page's pieces at once where workgroups take many tokens (17k
   // tokens, 8 heads of 128: pages of 128 42 us, 56 with 256 threads; of 256 56, 60);
   // where they take one, most would be idle.
-  const int pieces = page / 4 * (hd / 8), nt = a.per == 1 || pieces <= 256 ? 256 : pieces <= 512 ? 512 : 1024;
+  const int pieces = page / 4 * (hd / 8), nt = a.per == 1 ? 256 : pieces <= 64 ? 64 : pieces <= 128 ? 128 : pieces <= 256 ? 256 : pieces <= 512 ? 512 : 1024;
   dim3 grid(unsigned((n + a.per - 1) / a.per), unsigned(Hkv));
   if (rot && rot->heads) {
     // the queries behind the heads' workgroups: no more rows of them than a grid has left
@@ -565,6 +565,10 @@ hipError_t kv_store_paged(int dt, const void *k, const void *v, long ldk, long l
 #define MH_STORE(DTV, ROT)                                                                                \
   if (a.per == 1)                                                                                         \
     hipLaunchKernelGGL((kv_store_paged_kernel<DTV, 256, ROT, true>), grid, dim3(256), 0, st, a);          \
+  else if (nt == 64)                                                                                      \
+    hipLaunchKernelGGL((kv_store_paged_kernel<DTV, 64, ROT, false>), grid, dim3(64), 0, st, a);           \
+  else if (nt == 128)                                                                                     \
+    hipLaunchKernelGGL((kv_store_paged_kernel<DTV, 128, ROT, false>), grid, dim3(128), 0, st, a);         \
   else if (nt == 256)                                                                                     \
     hipLaunchKernelGGL((kv_store_paged_kernel<DTV, 256, ROT, false>), grid, dim3(256), 0, st, a);         \
   else if (nt == 512)                                                                                     \

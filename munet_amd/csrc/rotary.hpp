@@ -56,10 +56,9 @@ template <int DT, int N> __device__ __forceinline__ void stv(typename Store<DT>:
 // takes U pairs (or, behind the pairs, as many values) of every p.lanes-th head:
 // their angles are loaded once, and HB heads' values are in flight at a time.
 // Where `slots` is given, tokens without one in 0 .. limit - 1 are left alone.
-template <int DT, int U, bool INTERLEAVED, int NT>
+template <int DT, int U, bool INTERLEAVED, int NT, int HB = 4>
 __device__ __forceinline__ void rotate_tokens(const Rotary &p, int64_t first, const int32_t *slots, int64_t limit) {
   typedef typename Store<DT>::T T;
-  constexpr int HB = 4;
   const int pairs = p.half / U, units = p.units, cols = min(units, NT);
   const int lt = threadIdx.x / (cols * p.lanes), r = threadIdx.x - lt * (cols * p.lanes);
   const int64_t t = first + lt;
