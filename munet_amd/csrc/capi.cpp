@@ -17,6 +17,7 @@
 #include <vector>
 
 #include "../../include/munet_hip.h"
+#include "gemm_i8_tiles.hpp"
 #include "host_codec.hpp"
 #include "mh_kernels.hpp"
 #include "mh_runtime.hpp"

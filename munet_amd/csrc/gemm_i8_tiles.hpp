@@ -46,6 +46,9 @@ constexpr I8Tile kI8AnyTiles[] = {
 // Rows that the kernels of few rows take at most.
 constexpr int kI8FewRows = 256;
 
+// Workgroups of a launch; a product's 64 x 64 tiles are no more.
+constexpr int64_t kI8MaxTiles = 1 << 22;
+
 inline double i8_tile_time(const I8Tile &t, int64_t M, int64_t N, int64_t K) {
   const int64_t tm = (M + t.bm - 1) / t.bm, tn = (N + t.bn - 1) / t.bn, n = tm * tn, round = 256 * t.per_cu, rem = n % round;
   double rounds = double(n / round);
@@ -63,6 +66,7 @@ inline int i8_tile(bool blocks, int64_t M, int64_t N, int64_t K) {
   double best_t = 1e300;
   auto look = [&](const I8Tile &t) {
     if (t.code >= 100 && M > kI8FewRows) return;
+    if (((M + t.bm - 1) / t.bm) * ((N + t.bn - 1) / t.bn) > kI8MaxTiles) return;
     const double us = i8_tile_time(t, M, N, K);
     if (us < best_t) {
       best_t = us;

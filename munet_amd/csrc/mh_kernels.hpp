@@ -299,7 +299,6 @@ hipError_t quantize_rows(int dt, const QuantRows &p, hipStream_t st);
 hipError_t dequantize_rows(int dt, const QuantRows &p, hipStream_t st);
 // Products of 8-bit integers with scales for each row and column (gemm_i8.hip)
 constexpr int kI8MaxK = (1 << 17) - 1;      // K products of magnitude 2^14 in int32
-constexpr int64_t kI8MaxTiles = 1 << 22;    // workgroups of a launch
 struct LinearI8 {
   const int8_t *x = nullptr, *w = nullptr;
   const float *sx = nullptr, *sw = nullptr;

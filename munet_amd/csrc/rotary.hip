@@ -13,15 +13,44 @@ namespace {
 
 // (m cos a, m sin a) of a = position * frequency, in 64 bits: a document's
 // position is a million turns of the fastest pair, of which 32 bits would leave
-// four digits of the last one.
+// four digits of the last one.  The angle is taken in turns, p + lo exactly, less
+// the whole ones and then the quarters; what is left, of at most an eighth, goes
+// through the Taylor series to x^17 and x^16 (the next terms are below 2^-58), and the
+// quarters say which is which.  A thread keeps its pair's frequency for all tokens.
+// 17000 tokens of 64 pairs: 5 to 6 us (1.7 TB/s written), 7.7 with a library sincos and a
+// division for each value.
+__device__ __forceinline__ float2 angle(double pos, double turns, double m) {
+  const double p = pos * turns, lo = fma(pos, turns, -p), t = (p - rint(p)) + lo;
+  const double quarters = rint(4.0 * t), x = (t - 0.25 * quarters) * 6.283185307179586476925, y = x * x;
+  double s = 1.0 / 355687428096000.0, c = 1.0 / 20922789888000.0;
+  s = fma(s, y, -1.0 / 1307674368000.0);
+  c = fma(c, y, -1.0 / 87178291200.0);
+  s = fma(s, y, 1.0 / 6227020800.0);
+  c = fma(c, y, 1.0 / 479001600.0);
+  s = fma(s, y, -1.0 / 39916800.0);
+  c = fma(c, y, -1.0 / 3628800.0);
+  s = fma(s, y, 1.0 / 362880.0);
+  c = fma(c, y, 1.0 / 40320.0);
+  s = fma(s, y, -1.0 / 5040.0);
+  c = fma(c, y, -1.0 / 720.0);
+  s = fma(s, y, 1.0 / 120.0);
+  c = fma(c, y, 1.0 / 24.0);
+  s = fma(s, y, -1.0 / 6.0);
+  c = fma(c, y, -0.5);
+  s = m * fma(s * y, x, x);
+  c = m * fma(c, y, 1.0);
+  const int q = int(quarters) & 3;
+  const double u = q & 1 ? -s : c, v = q & 1 ? c : s;  // a quarter on: (-sin, cos)
+  return q & 2 ? make_float2(float(-u), float(-v)) : make_float2(float(u), float(v));
+}
+
 __global__ void __launch_bounds__(256) rotary_table_kernel(const int32_t *__restrict__ pos, const double *__restrict__ freq,
-                                                           float2 *__restrict__ table, int64_t total, int half, double m) {
-  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < total; i += int64_t(gridDim.x) * 256) {
-    const int64_t t = i / half;
-    const int j = int(i - t * half);
-    double s, c;
-    sincos(double(pos[t]) * freq[j], &s, &c);
-    table[i] = make_float2(float(m * c), float(m * s));
+                                                           float2 *__restrict__ table, int n, int half, int cols, int rows, double m) {
+  const int lr = threadIdx.x / cols, lc = threadIdx.x - lr * cols;
+  if (lr >= rows) return;
+  for (int j = lc; j < half; j += cols) {
+    const double turns = freq[j] * 0.159154943091895335768884;
+    for (int64_t t = int64_t(blockIdx.x) * rows + lr; t < n; t += int64_t(gridDim.x) * rows) table[t * half + j] = angle(pos[t], turns, m);
   }
 }
 
@@ -44,10 +73,11 @@ void launch(const Rotary &p, const int32_t *slots, int64_t limit, unsigned grid,
 
 hipError_t rotary_table(const int32_t *positions, const double *freq, float *table, int n, int half, double magnitude,
                         hipStream_t st) {
-  const int64_t total = int64_t(n) * half;
-  const unsigned grid = unsigned(std::min<int64_t>((total + 255) / 256, 1 << 20));
-  hipLaunchKernelGGL(rotary_table_kernel, dim3(grid), dim3(256), 0, st, positions, freq, reinterpret_cast<float2 *>(table), total,
-                     half, magnitude);
+  const int cols = std::min(half, 256), rows = 256 / cols;
+  const int64_t groups = (int64_t(n) + rows - 1) / rows;
+  // (eight workgroups to a CU, then several tokens to a thread)
+  hipLaunchKernelGGL(rotary_table_kernel, dim3(unsigned(std::min<int64_t>(groups, 2048))), dim3(256), 0, st, positions, freq,
+                     reinterpret_cast<float2 *>(table), n, half, cols, rows, magnitude);
   return hipGetLastError();
 }
 

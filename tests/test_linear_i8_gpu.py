@@ -234,6 +234,36 @@ def test_linear_of_views(hip, torch, dtype, M, K, ldx, ldw, fx, fw):
         assert (wide[:, :first] == 5.0).all() and (wide[:, first + N:] == 5.0).all()
 
 
+KERNELS = [0, 1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 100, 101]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("M,N,K", [(1, 40, 16), (70, 264, 208), (256, 300, 1040), (200, 257, 128)])
+def test_every_kernel(hip, torch, monkeypatch, kernel, dtype, M, N, K):
+    """Each kernel and tile on sizes off its own, against the formula; and the bits of the one
+    that the sizes choose."""
+    x, sx, w, sw = operands(torch, M + K, M, N, K)
+    bias, resid = normal(torch, 1, (N,), dtype), normal(torch, 2, (M, N), dtype)
+    for act, r in ((0, resid), (1, None), (2, resid)):
+        own = torch.empty((M, N), dtype=resid.dtype, device="cuda")
+        hip.linear_i8(x, sx, w, sw, own, bias=bias, act=act, resid=r)
+        with monkeypatch.context() as m:
+            m.setenv("MUNET_HIP_I8_TILE", str(kernel))
+            got = check_linear(hip, torch, x, sx, w, sw, dtype, bias=bias, act=act, resid=r)
+        assert torch.equal(got, own)
+
+
+@pytest.mark.parametrize("kernel", [0, 10, 100, 101])
+@pytest.mark.parametrize("K,ldx,ldw,fx,fw", [(1, 3, 5, 1, 2), (15, 21, 18, 2, 3), (65, 70, 66, 5, 1), (130, 131, 137, 0, 7), (255, 259, 260, 3, 4), (1027, 1030, 1031, 1, 2)])
+def test_kernels_of_unaligned_rows(hip, torch, monkeypatch, kernel, K, ldx, ldw, fx, fw):
+    """Rows at every offset from a word, ends inside one."""
+    monkeypatch.setenv("MUNET_HIP_I8_TILE", str(kernel))
+    x, sx, _, _ = operands(torch, K, 37, 1, ldx)
+    w, sw, _, _ = operands(torch, K + 1, 150, 1, ldw)
+    check_linear(hip, torch, x[:, fx:fx + K], sx, w[:, fw:fw + K], sw, "float32")
+
+
 @pytest.mark.parametrize("M", [1, 16, 70])
 def test_linear_sums_fill_32_bits(hip, torch, M):
     """The longest rows of the lowest value: sums of 2^31 - 2^14; and of both signs."""

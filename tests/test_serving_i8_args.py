@@ -2,11 +2,13 @@
 formulas, and calls that must fail before anything reaches a device."""
 import ctypes
 import math
+import os
+import subprocess
 
 import numpy as np
 import pytest
 
-from munet_amd import _lib, synth
+from munet_amd import _lib, build, synth
 from munet_amd.backend import rotary_frequencies
 
 F32, F16, BF16 = synth.F32, synth.F16, synth.BF16
@@ -176,6 +178,16 @@ def _linear(**kw):
 def test_linear_i8_refusals(kw, match):
     with pytest.raises(_lib.HipError, match=match):
         _linear(**kw)
+
+
+def test_tile_rules(tmp_path):
+    exe = str(tmp_path / "check")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run(["g++", "-std=c++17", "-O1", "-fsanitize=undefined", "-fno-sanitize-recover=all", "-I", build.CSRC,
+                        os.path.join(root, "tests", "cxx", "gemm_i8_tiles_check.cpp"), "-o", exe], capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr[-3000:]
+    r = subprocess.run([exe], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0 and r.stdout == "ok\n", r.stdout + r.stderr[-2000:]
 
 
 def test_empty_calls_need_no_device():
