@@ -136,9 +136,15 @@ template <int DT, int C> __device__ __forceinline__ void i8_put(typename Store<D
     else reinterpret_cast<H4 *>(p)->v = make_uint2(w[0], w[1]);
   }
 }
+// A product that no sum is fused with: which of them the compiler fuses differs from one
+// kernel to the next, and so would the bits.
+__device__ __forceinline__ float mul_alone(float a, float b) {
+#pragma clang fp contract(off)
+  return a * b;
+}
 template <int ACT> __device__ __forceinline__ float i8_act(float v) {
   if constexpr (ACT == ACT_RELU) return v < 0.f ? 0.f : v;  // (NaN stays)
-  if constexpr (ACT == ACT_GELU) return __fmul_rn(v, sigmoidf_ref(__fmul_rn(1.702f, v)));
+  if constexpr (ACT == ACT_GELU) return mul_alone(v, sigmoidf_ref(mul_alone(1.702f, v)));
   return v;
 }
 
@@ -153,8 +159,8 @@ __device__ __forceinline__ bool plain_scale(float s) { return s == 0.f || (s >= 
 // each, was 100 KB of it.  Hence one path for whole tiles with scales of ordinary
 // size, which multiply as they are, for each activation, and one for all else,
 // where scales are fractions and powers of two: the same bits where both can.
-// Roundings are explicit, a missing bias or residual is a zero: a row's results do
-// not depend on the kernel.  (Whole rows through LDS were slower: 4096 x 4096 x
+// No sum is fused with a product, a missing bias or residual is a zero: a row's
+// results do not depend on the kernel.  (Whole rows through LDS were slower: 4096 x 4096 x
 // 1024 on 256 x 128 tiles 38 us, 34 from registers.)
 template <int DT, typename G, int ACT>
 __device__ __forceinline__ void i8_store_whole(const LinearI8 &p, const G &g, int m0, int n0, const i32x4 (&acc)[G::FM][G::FN],
@@ -177,8 +183,7 @@ __device__ __forceinline__ void i8_store_whole(const LinearI8 &p, const G &g, in
         float v[G::COLS];
 #pragma unroll
         for (int e = 0; e < G::COLS; ++e)
-          v[e] = __fadd_rn(i8_act<ACT>(__fadd_rn(__fmul_rn(__fmul_rn(float(acc[i][q * (G::COLS / 4) + e / 4][e % 4]), fx[i]), fw[q][e]), bias[q][e])),
-                           resid[q][e]);
+          v[e] = i8_act<ACT>(mul_alone(mul_alone(float(acc[i][q * (G::COLS / 4) + e / 4][e % 4]), fx[i]), fw[q][e]) + bias[q][e]) + resid[q][e];
         i8_put<DT>(out + q * 32, v);
       }
     }
@@ -207,9 +212,8 @@ __device__ __forceinline__ void i8_store_any(const LinearI8 &p, const G &g, int 
 #pragma unroll
         for (int e = 0; e < G::COLS; ++e) {
           const Scale sw(fw[q][e]);
-          v[e] = __fadd_rn(__builtin_amdgcn_ldexpf(__fmul_rn(__fmul_rn(float(acc[i][q * (G::COLS / 4) + e / 4][e % 4]), sx.f), sw.f), sx.e + sw.e),
-                           bias[q][e]);
-          v[e] = __fadd_rn(p.act == ACT_RELU ? i8_act<ACT_RELU>(v[e]) : p.act == ACT_GELU ? i8_act<ACT_GELU>(v[e]) : v[e], resid[e]);
+          v[e] = __builtin_amdgcn_ldexpf(mul_alone(mul_alone(float(acc[i][q * (G::COLS / 4) + e / 4][e % 4]), sx.f), sw.f), sx.e + sw.e) + bias[q][e];
+          v[e] = (p.act == ACT_RELU ? i8_act<ACT_RELU>(v[e]) : p.act == ACT_GELU ? i8_act<ACT_GELU>(v[e]) : v[e]) + resid[e];
         }
         T *out = static_cast<T *>(p.out) + int64_t(m) * p.ldo + n;
         if (left >= G::COLS) {

@@ -13,10 +13,11 @@
 namespace mh {
 namespace {
 
-// (explicit fma and mul: the same bits wherever this is inlined, so that a key
-// rotated on its way into the cache is the key that rotary() gives)
+// (one product fused, the other not: the same bits wherever this is inlined, so
+// that a key rotated on its way into the cache is the key that rotary() gives)
 __device__ __forceinline__ void turn(float &a, float &b, float c, float s) {
-  const float x = __fmaf_rn(a, c, -__fmul_rn(b, s)), y = __fmaf_rn(a, s, __fmul_rn(b, c));
+#pragma clang fp contract(off)
+  const float p = b * s, q = b * c, x = __builtin_fmaf(a, c, -p), y = __builtin_fmaf(a, s, q);
   a = x;
   b = y;
 }

@@ -49,7 +49,7 @@ struct __attribute__((packed)) Bytes8 { uint32_t a, b; };
 // The whole number nearest to 127 x / a, ties to even, where the quotient lies next
 // to a half: 254 |x| and (2 h + 1) a, products of 24 and 8 bits, are exact in 64.
 __device__ __noinline__ float nearest_exact(float x, float a, float inv) {
-  const float h = __builtin_floorf(__builtin_fabsf(__fmul_rn(x, inv)));
+  const float h = __builtin_floorf(__builtin_fabsf(x * inv));
   const double d = 254.0 * double(__builtin_fabsf(x)) - (2.0 * double(h) + 1.0) * double(a);
   const float q = d > 0 ? h + 1.f : d < 0 ? h : 2.f * __builtin_rintf(0.5f * h + 0.25f);
   return __builtin_copysignf(q, x);
@@ -64,15 +64,15 @@ template <int DT> __device__ __forceinline__ Bytes8 to_bytes(const Eight<typenam
   float far = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float x = Store<DT>::dec(e.v[i]), r = __fmaf_rn(x, inv, kWhole);
-    far = fmaxf(far, __builtin_fabsf(__fmaf_rn(x, inv, __fsub_rn(kWhole, r))));
+    const float x = Store<DT>::dec(e.v[i]), r = __builtin_fmaf(x, inv, kWhole);
+    far = fmaxf(far, __builtin_fabsf(__builtin_fmaf(x, inv, kWhole - r)));
     w[i] = __float_as_uint(r);
   }
   if (far > 0.49997f) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float x = Store<DT>::dec(e.v[i]);
-      if (__builtin_fabsf(__fmaf_rn(x, inv, __fsub_rn(kWhole, __uint_as_float(w[i])))) > 0.49997f)
+      if (__builtin_fabsf(__builtin_fmaf(x, inv, kWhole - __uint_as_float(w[i]))) > 0.49997f)
         w[i] = __float_as_uint(nearest_exact(x, a, inv) + kWhole);
     }
   }
