@@ -352,7 +352,8 @@ int mh_dequantize_rows(int dt, const int8_t *q, int64_t ldq, const float *scale,
                        void *stream);
 /* out[m][n] = act(x_scale[m] w_scale[n] sum_k x[m][k] w[n][k] + bias[n]) + resid[m][n]:
  * mh_linear with both operands in int8, [M][K] rows ldx and [N][K] rows ldw apart, of
- * any alignment (multiples of 16 bytes are faster).  bias (may be NULL), resid (may be
+ * any alignment (multiples of 16 bytes are faster; of others whole 4-byte words that
+ * hold a value are read).  bias (may be NULL), resid (may be
  * NULL; rows ldr apart) and out (ldo apart) are of `dt`; act is MH_ACT_*, GELU
  * x * sigmoid(1.702 x).  The sum is exact in int32 (K is at most 2^17 - 1), the rest
  * in fp32, rounded once.  out may be resid (with ldo = ldr), else it overlaps

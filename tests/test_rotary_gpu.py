@@ -261,6 +261,62 @@ def test_append(hip, torch, dtype, interleaved, P, kv, heads, hd, rot):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("P,kv,heads,hd,rot", [(16, 12, 12, 64, 24), (16, 8, 3, 128, 128), (32, 8, 9, 128, 64), (64, 8, 32, 128, 128), (64, 10, 4, 80, 42),
+                                               (128, 8, 5, 128, 128), (256, 8, 2, 128, 20), (256, 6, 1, 256, 256)])
+def test_append_prompts(hip, torch, dtype, interleaved, P, kv, heads, hd, rot):
+    """Several tokens to a workgroup, workgroups of every size: prompts behind prefixes, some
+    tokens without a slot, against the same keys in float32, bit for bit."""
+    runs = [(0, 700), (P - 3, 450), (5, 1), (P // 2, 300), (0, P), (1, 2 * P - 1), (0, 333)]
+    n_pages = sum(-(-(f + n) // P) for f, n in runs) + 5
+    slots = slots_of(torch, hd + P, P, n_pages, runs)
+    n = len(slots)
+    rows, table = normal(torch, P + hd, (n, heads + 2 * kv, hd), dtype), table_of(torch, hd, n, rot // 2)
+    # (sizes that grow along the prompts, so that pages' scales grow behind their prefixes)
+    rows *= torch.linspace(0.1, 8.0, n, device="cuda")[:, None, None].to(rows.dtype)
+    q, k, v = rows[:, :heads], rows[:, heads:heads + kv], rows[:, heads + kv:]
+    got, want = pool(torch, 1, n_pages, kv, P, hd), pool(torch, 1, n_pages, kv, P, hd)
+    q_out = torch.full((n, heads, hd), 3.0, dtype=rows.dtype, device="cuda")
+    hip.kv_store_rotary_paged(k, v, table, slots, *got, q=q, q_out=q_out, interleaved=interleaved)
+    turned = torch.empty((n, kv, hd), device="cuda")
+    hip.rotary(k.float().contiguous(), table, turned, interleaved=interleaved)
+    hip.kv_store_paged(turned, v.float().contiguous(), slots, *want)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    q_want = torch.empty_like(q_out)
+    hip.rotary(q, table, q_want, interleaved=interleaved)
+    q_want[slots < 0] = 3.0
+    assert torch.equal(q_out, q_want)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_single_tokens_beside_runs(hip, torch, dtype):
+    """Batches small enough for a workgroup a token: single tokens at every place of a page, runs
+    of two and three, the last token of the call; the same bits as one call a token or run."""
+    P, kv, hd, n_pages = 16, 2, 48, 40
+    runs = [(i, 1) for i in range(16)] + [(3, 2), (14, 3), (0, 3), (15, 1), (0, 1), (7, 1)]
+    slots = slots_of(torch, 5, P, n_pages, runs)[:-1]
+    n = len(slots)
+    rows = normal(torch, 6, (n, 2, kv, hd), dtype) * 300
+    got, want = pool(torch, 7, n_pages, kv, P, hd), pool(torch, 7, n_pages, kv, P, hd)
+    hip.kv_store_paged(rows[:, 0], rows[:, 1], slots, *got)
+    at = 0
+    for _, m in runs:
+        hip.kv_store_paged(rows[at:at + m, 0], rows[at:at + m, 1], slots[at:at + m], *want)
+        at += m + 1
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    # against many tokens to a workgroup: the same rows among enough others
+    many = 5000
+    filler = torch.full((many,), -1, dtype=torch.int32, device="cuda")
+    big, others = torch.cat([slots, filler]), pool(torch, 7, n_pages, kv, P, hd)
+    wide = torch.cat([rows, torch.zeros((many, 2, kv, hd), dtype=rows.dtype, device="cuda")])
+    hip.kv_store_paged(wide[:, 0], wide[:, 1], big, *others)
+    for a, b in zip(got, others):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_append_against_the_formula(hip, torch, dtype):
     """Keys within half a step of e4m3 (2^-4 of the value, 2^-10 of the scale where it has
     no smaller step) of the rotation in 64 bits, in the least scale that holds them."""
