@@ -156,34 +156,52 @@ template <int DT> struct Raw {
   }
 };
 
-// Piece c of a key: two fours of its values, at `lo` and `hi` of the head.  Eight
-// consecutive ones, but where pairs lie half the rotated part apart (ROT 1) both
-// values of four pairs, so that a thread turns what it has; with ROT 2 (neighbours
-// paired) eight values are four pairs.  Either way the pairs are 4 c .. 4 c + 3, in two
-// loads of the table (with eight values of a half, their partners loaded too and
+// Piece c of a key: eight of its values.  Where pairs lie half the rotated part apart
+// (ROT 1) these are both values of pairs 4 c .. 4 c + 3, two fours at `lo` and `hi`,
+// so that a thread turns what it has; with ROT 2 (neighbours paired) eight consecutive
+// values are those pairs (with eight values of a half, their partners loaded too and
 // the queries in a launch of their own, 17k tokens of 8 heads of 128 and 32 query heads
-// took 132 us, so and in one launch 104).  Rotated keys are floats, so that the cache's 8 bits are their
-// only rounding.
+// took 132 us, so and in one launch 104).  Behind the pairs values go as they lie.  The
+// piece at the pairs' end may be mixed: `few` whole pairs, then (ROT 1) the values
+// behind all pairs, first in the places of the missing first halves, then of the second.
+// Rotated keys are floats, so that the cache's 8 bits are their only rounding.
 template <int DT, int ROT> struct KeyPiece {
-  int lo, hi;
-  bool turns;  // four whole pairs
+  int lo, hi, pair, few;  // few: pairs of this piece (0 to 4)
+  bool mixed;
   __device__ __forceinline__ KeyPiece(int c, int half) {
-    const bool whole = half % 4 == 0;
-    turns = ROT != 0 && whole && 4 * c < half;
-    lo = ROT == 1 && turns ? 4 * c : 8 * c;
-    hi = ROT == 1 && turns ? 4 * c + half : 8 * c + 4;
+    pair = 4 * c;
+    few = ROT ? min(max(half - pair, 0), 4) : 0;
+    mixed = few > 0 && few < 4;
+    lo = ROT == 1 && few == 4 ? pair : 8 * c;
+    hi = ROT == 1 && few == 4 ? pair + half : 8 * c + 4;
+  }
+  // where value e of a mixed piece lies
+  __device__ __forceinline__ int at(int e, int half) const {
+    if (e < 4) return e < few ? pair + e : 2 * half + e - few;
+    return e - 4 < few ? half + pair + e - 4 : 2 * half + (4 - few) + e - 4 - few;
   }
   __device__ __forceinline__ void load(const typename Store<DT>::T *head, const float2 *tab, int half, float v[8]) const {
     if constexpr (ROT == 0) {
       ld8<DT>(head + lo, v);
-    } else if (half % 4 != 0) {
-      turned8<DT, ROT == 2>(head, tab, half, lo, v);  // (pairs that straddle pieces)
+    } else if (ROT == 1 && mixed) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = Store<DT>::dec(head[at(e, half)]);
+#pragma unroll
+      for (int i = 0; i < 3; ++i)
+        if (i < few) turn(v[i], v[4 + i], tab[pair + i].x, tab[pair + i].y);
     } else {
-      ld4<DT>(head + lo, v);
-      ld4<DT>(head + hi, v + 4);
-      if (!turns) return;
-      const float4 *t = reinterpret_cast<const float4 *>(tab + (ROT == 1 ? lo : lo / 2));
-      const float4 a = t[0], b = t[1];
+      ldu4<DT>(head + lo, v);
+      ldu4<DT>(head + hi, v + 4);
+      if (few == 0) return;
+      float4 a, b;
+      if (ROT == 2 && mixed) {
+        const float2 x = tab[pair], y = few > 1 ? tab[pair + 1] : make_float2(1.f, 0.f), z = few > 2 ? tab[pair + 2] : make_float2(1.f, 0.f);
+        a = make_float4(x.x, x.y, y.x, y.y);
+        b = make_float4(z.x, z.y, 1.f, 0.f);
+      } else {
+        a = angles2(tab + pair);
+        b = angles2(tab + pair + 2);
+      }
       if constexpr (ROT == 1) {
         turn(v[0], v[4], a.x, a.y);
         turn(v[1], v[5], a.z, a.w);
@@ -191,21 +209,28 @@ template <int DT, int ROT> struct KeyPiece {
         turn(v[3], v[7], b.z, b.w);
       } else {
         turn(v[0], v[1], a.x, a.y);
-        turn(v[2], v[3], a.z, a.w);
-        turn(v[4], v[5], b.x, b.y);
-        turn(v[6], v[7], b.z, b.w);
+        if (few > 1) turn(v[2], v[3], a.z, a.w);
+        if (few > 2) turn(v[4], v[5], b.x, b.y);
+        if (few > 3) turn(v[6], v[7], b.z, b.w);
       }
     }
   }
-  __device__ __forceinline__ void store(uint8_t *row, const float v[8], float inv) const {
+  __device__ __forceinline__ void store(uint8_t *row, int half, const float v[8], float inv) const {
     float w[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) w[e] = v[e] * inv;
+    const uint32_t first = e4m3x4(w), second = e4m3x4(w + 4);
     if constexpr (ROT == 1) {
-      *reinterpret_cast<uint32_t *>(row + lo) = e4m3x4(w);
-      *reinterpret_cast<uint32_t *>(row + hi) = e4m3x4(w + 4);
+      struct __attribute__((packed)) Any { uint32_t v; };
+      if (mixed) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) row[at(e, half)] = uint8_t((e < 4 ? first : second) >> (8 * (e & 3)));
+      } else {
+        *reinterpret_cast<uint32_t *>(row + lo) = first;
+        reinterpret_cast<Any *>(row + hi)->v = second;
+      }
     } else {
-      *reinterpret_cast<uint2 *>(row + lo) = make_uint2(e4m3x4(w), e4m3x4(w + 4));
+      *reinterpret_cast<uint2 *>(row + lo) = make_uint2(first, second);
     }
   }
 };
@@ -300,9 +325,12 @@ __global__ void __launch_bounds__(NT) kv_store_paged_kernel(StoreArgs a) {
     if (head >= a.Hkv) {
       const unsigned step = (gridDim.y - a.Hkv) * gridDim.x;
       for (unsigned i = (head - a.Hkv) * gridDim.x + blockIdx.x; i < a.q_groups; i += step) {
-        constexpr int U = ROT == 2 ? (DT == F32 ? 2 : 4) : (DT == F32 ? 4 : 8);
-        if (a.q_unit == 1) rotate_tokens<DT, 1, ROT == 2, NT, 2>(a.q, int64_t(i) * a.q.tokens, a.slots, limit);
-        else rotate_tokens<DT, U, ROT == 2, NT, 2>(a.q, int64_t(i) * a.q.tokens, a.slots, limit);
+        const int64_t first = int64_t(i) * a.q.tokens;
+        if constexpr (ONE)
+          rotary_unit_as<DT, ROT == 2>(a.q_unit, [&](auto u, auto inter) {
+            rotate_tokens<DT, decltype(u)::value, decltype(inter)::value, NT, 2>(a.q, first, a.slots, limit);
+          });
+        else rotate_tokens<DT, rotary_most(DT, ROT == 2), ROT == 2, NT, 2>(a.q, first, a.slots, limit);
       }
       return;
     }
@@ -351,7 +379,7 @@ __global__ void __launch_bounds__(NT) kv_store_paged_kernel(StoreArgs a) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) vd[int64_t(8 * c + e) * P + place] = uint8_t(b[e >> 2] >> (8 * (e & 3)));
       } else if (on) {
-        piece.store(kd + int64_t(place) * hd, v, ps.inv);
+        piece.store(kd + int64_t(place) * hd, a.half, v, ps.inv);
       }
       if (c == 0) *scale = ps.now;
       return;
@@ -456,7 +484,7 @@ __global__ void __launch_bounds__(NT) kv_store_paged_kernel(StoreArgs a) {
         for (int j = 0; j < 4; ++j) {
           float v[8];
           kr[j].get(v);
-          if (pi + j >= 0 && pi + j < n) kpiece.store(kd + int64_t(place + pi + j) * hd, v, inv[0]);
+          if (pi + j >= 0 && pi + j < n) kpiece.store(kd + int64_t(place + pi + j) * hd, a.half, v, inv[0]);
           vr[j].get(v);
 #pragma unroll
           for (int e = 0; e < 8; ++e) v[e] *= inv[1];
@@ -498,7 +526,7 @@ __global__ void __launch_bounds__(NT) kv_store_paged_kernel(StoreArgs a) {
       float v[8];
       const KeyPiece<DT, ROT> piece(d / 8, a.half);
       piece.load(kp + int64_t(i) * a.ldk, tab + (ROT ? int64_t(i) * a.half : 0), a.half, v);
-      piece.store(kd + int64_t(place + i) * hd, v, inv[0]);
+      piece.store(kd + int64_t(place + i) * hd, a.half, v, inv[0]);
     }
     // values, transposed through LDS in tiles of VT places
     for (int c0 = place & ~(VT - 1); c0 < place + n; c0 += VT) {
@@ -559,6 +587,15 @@ hipError_t kv_store_paged(int dt, const void *k, const void *v, long ldk, long l
     // the queries behind the heads' workgroups: no more rows of them than a grid has left
     a.q = *rot;
     a.q_unit = rotary_unit(dt, a.q);
+    // Of many tokens only in 16 bytes a thread: narrower ones need the registers of a
+    // launch of their own (17.4k tokens, 32 heads of 128, rotated parts of 120, 100 and
+    // 42 by halves: 169, 194 and 253 us, here 205, 246 and 420; 128: here 109).
+    if (a.per > 1 && a.q_unit < rotary_most(dt, rot->interleaved)) {
+      if (const hipError_t e = rotary(dt, *rot, slots, int64_t(n_pages) * page, st); e != hipSuccess) return e;
+      a.q.heads = 0;
+    }
+  }
+  if (a.q.heads) {
     rotary_cut(dt, a.q_unit, nt, a.q);
     a.q_groups = unsigned((n + a.q.tokens - 1) / a.q.tokens);
     grid.y += std::min((a.q_groups + grid.x - 1) / grid.x, std::max(1u, 65535u - grid.y));

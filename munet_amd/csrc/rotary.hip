@@ -62,11 +62,10 @@ __global__ void __launch_bounds__(256) rotary_kernel(Rotary p, const int32_t *sl
     rotate_tokens<DT, U, INTERLEAVED, 256>(p, t, slots, limit);
 }
 
-template <int DT, int U>
-void launch(const Rotary &p, const int32_t *slots, int64_t limit, unsigned grid, hipStream_t st) {
-  constexpr int V = U == 1 ? 1 : U / 2;  // (interleaved pairs lie in one load)
-  if (p.interleaved) hipLaunchKernelGGL((rotary_kernel<DT, V, true>), dim3(grid), dim3(256), 0, st, p, slots, limit);
-  else hipLaunchKernelGGL((rotary_kernel<DT, U, false>), dim3(grid), dim3(256), 0, st, p, slots, limit);
+template <int DT> void launch(const Rotary &p, int unit, const int32_t *slots, int64_t limit, unsigned grid, hipStream_t st) {
+  rotary_units<DT>(p.interleaved, unit, [&](auto u, auto inter) {
+    hipLaunchKernelGGL((rotary_kernel<DT, decltype(u)::value, decltype(inter)::value>), dim3(grid), dim3(256), 0, st, p, slots, limit);
+  });
 }
 
 }  // namespace
@@ -86,9 +85,9 @@ hipError_t rotary(int dt, Rotary p, const int32_t *slots, int64_t limit, hipStre
   rotary_cut(dt, unit, 256, p);
   const unsigned grid = unsigned(std::min<int64_t>((int64_t(p.n) + p.tokens - 1) / p.tokens, 1 << 22));
   switch (dt) {
-  case F32: unit == 1 ? launch<F32, 1>(p, slots, limit, grid, st) : launch<F32, 4>(p, slots, limit, grid, st); break;
-  case F16: unit == 1 ? launch<F16, 1>(p, slots, limit, grid, st) : launch<F16, 8>(p, slots, limit, grid, st); break;
-  case BF16: unit == 1 ? launch<BF16, 1>(p, slots, limit, grid, st) : launch<BF16, 8>(p, slots, limit, grid, st); break;
+  case F32: launch<F32>(p, unit, slots, limit, grid, st); break;
+  case F16: launch<F16>(p, unit, slots, limit, grid, st); break;
+  case BF16: launch<BF16>(p, unit, slots, limit, grid, st); break;
   default: return hipErrorInvalidValue;
   }
   return hipGetLastError();

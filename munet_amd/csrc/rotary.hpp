@@ -6,6 +6,8 @@
 // becomes (a c - b s, a s + b c).  The rest of the head stays.
 #pragma once
 
+#include <type_traits>
+
 #include "gemm_common.hpp"
 #include "mh_common.hpp"
 #include "mh_kernels.hpp"
@@ -22,36 +24,49 @@ __device__ __forceinline__ void turn(float &a, float &b, float c, float s) {
   b = y;
 }
 
-// N consecutive values (one load or store of up to 16 bytes, aligned to its size).
+// N consecutive values.  N of 16 bytes: one load or store aligned to it; fewer: aligned
+// to the type alone (a rotated part of 100 puts partners 100 bytes apart).
 template <int DT, int N> __device__ __forceinline__ void ldv(const typename Store<DT>::T *p, float v[N]) {
-  if constexpr (N == 1) v[0] = Store<DT>::dec(*p);
-  else if constexpr (DT == F32 && N == 2) {
-    const float2 x = *reinterpret_cast<const float2 *>(p);
-    v[0] = x.x;
-    v[1] = x.y;
-  } else if constexpr (N == 4) ld4<DT>(p, v);
+  typedef typename Store<DT>::T T;
+  if constexpr (DT == F32 && N == 4) ld4<F32>(p, v);
+  else if constexpr (N == 8) dec8<DT>(*reinterpret_cast<const uint4 *>(p), v);
   else {
-    static_assert(DT != F32 && N == 8, "16 bytes at most");
-    dec8<DT>(*reinterpret_cast<const uint4 *>(p), v);
+    struct __attribute__((packed, aligned(sizeof(T)))) Few { T v[N]; };
+    const Few x = *reinterpret_cast<const Few *>(p);
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = Store<DT>::dec(x.v[i]);
   }
 }
 template <int DT, int N> __device__ __forceinline__ void stv(typename Store<DT>::T *p, float v[N]) {
-  if constexpr (N == 1) *p = Store<DT>::enc(v[0]);
-  else if constexpr (DT == F32 && N == 2) *reinterpret_cast<float2 *>(p) = make_float2(v[0], v[1]);
-  else if constexpr (DT == F32) st4<DT>(p, v);
-  else {
-#pragma unroll
-    for (int i = 0; i < N; i += 4) {
-      if constexpr (DT == F16) round4_f16(v + i);
+  typedef typename Store<DT>::T T;
+  if constexpr (DT == F32 && N == 4) st4<F32>(p, v);
+  else if constexpr (N == 8) {
+    if constexpr (DT == F16) {
+      round4_f16(v);
+      round4_f16(v + 4);
     }
-    uint32_t w[N / 2];
+    uint32_t w[4];
 #pragma unroll
-    for (int i = 0; i < N / 2; ++i)
-      w[i] = DT == F16 ? pack_f16x2_exact(v[2 * i], v[2 * i + 1]) : pack_bf16x2(v[2 * i], v[2 * i + 1]);
-    if constexpr (N == 8) *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
-    else *reinterpret_cast<uint2 *>(p) = make_uint2(w[0], w[1]);
+    for (int i = 0; i < 4; ++i) w[i] = DT == F16 ? pack_f16x2_exact(v[2 * i], v[2 * i + 1]) : pack_bf16x2(v[2 * i], v[2 * i + 1]);
+    *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+  } else {
+    struct __attribute__((packed, aligned(sizeof(T)))) Few { T v[N]; };
+    Few x;
+#pragma unroll
+    for (int i = 0; i < N; ++i) x.v[i] = Store<DT>::enc(v[i]);
+    *reinterpret_cast<Few *>(p) = x;
   }
 }
+
+// Two pairs' angles (rows of an odd number of pairs start at 8 bytes).
+__device__ __forceinline__ float4 angles2(const float2 *t) {
+  struct __attribute__((packed, aligned(8))) Two { float4 v; };
+  return reinterpret_cast<const Two *>(t)->v;
+}
+
+// Pairs a thread: 16 bytes of each load at most; and values of a piece behind the pairs.
+constexpr int rotary_most(int dt, bool interleaved) { return (dt == F32 ? 4 : 8) / (interleaved ? 2 : 1); }
+constexpr int rotary_tail(int dt, int unit, bool interleaved) { return unit == rotary_most(dt, interleaved) ? (dt == F32 ? 4 : 8) : unit; }
 
 // One workgroup of NT threads at tokens first .. first + p.tokens - 1.  A thread
 // takes U pairs (or, behind the pairs, as many values) of every p.lanes-th head:
@@ -78,7 +93,7 @@ __device__ __forceinline__ void rotate_tokens(const Rotary &p, int64_t first, co
       if constexpr (U % 2 == 0) {
 #pragma unroll
         for (int i = 0; i < U; i += 2) {
-          const float4 cs = reinterpret_cast<const float4 *>(tab)[i / 2];
+          const float4 cs = angles2(tab + i);
           c[i] = cs.x;
           s[i] = p.inverse ? -cs.y : cs.y;
           c[i + 1] = cs.z;
@@ -96,7 +111,7 @@ __device__ __forceinline__ void rotate_tokens(const Rotary &p, int64_t first, co
           const int hk = h + k * p.lanes;
           if (hk < p.heads) {
             const T *xh = x + hk * p.hd;
-            if constexpr (INTERLEAVED && U > 1) {
+            if constexpr (INTERLEAVED) {
               float v[2 * U];
               ldv<DT, 2 * U>(xh + ia, v);
 #pragma unroll
@@ -117,7 +132,7 @@ __device__ __forceinline__ void rotate_tokens(const Rotary &p, int64_t first, co
             T *o = out + hk * p.hd;
 #pragma unroll
             for (int i = 0; i < U; ++i) turn(a[k][i], b[k][i], c[i], s[i]);
-            if constexpr (INTERLEAVED && U > 1) {
+            if constexpr (INTERLEAVED) {
               float v[2 * U];
 #pragma unroll
               for (int i = 0; i < U; ++i) {
@@ -133,9 +148,9 @@ __device__ __forceinline__ void rotate_tokens(const Rotary &p, int64_t first, co
         }
       }
     } else {
-      // behind the pairs: as they are (units counts these where out is not x)
-      constexpr int W = U == 1 ? 1 : 16 / int(sizeof(T));
-      struct __attribute__((aligned(W * sizeof(T)))) Piece { T v[W]; };
+      // behind the pairs: as they are (units counts these where out is not x), as many values as a thread's pairs
+      constexpr int W = rotary_tail(DT, U, INTERLEAVED);
+      struct __attribute__((packed, aligned(sizeof(T)))) Piece { T v[W]; };
       const int at = 2 * p.half + (u - pairs) * W;
       for (int h = lane; h < p.heads; h += p.lanes)
         *reinterpret_cast<Piece *>(out + h * p.hd + at) = *reinterpret_cast<const Piece *>(x + h * p.hd + at);
@@ -143,74 +158,52 @@ __device__ __forceinline__ void rotate_tokens(const Rotary &p, int64_t first, co
   }
 }
 
-// Eight rotated values of a head from d on (a multiple of 8; the head 16-byte
-// aligned).
-template <int DT, bool INTERLEAVED>
-__device__ __forceinline__ void turned8(const typename Store<DT>::T *head, const float2 *tab, int half, int d, float v[8]) {
-  constexpr int N = DT == F32 ? 4 : 8;
-#pragma unroll
-  for (int e = 0; e < 8; e += N) ldv<DT, N>(head + d + e, v + e);
-  if (d >= 2 * half) return;
-  if constexpr (INTERLEAVED) {
-    if (half % 4 == 0) {
-      const float4 *t = reinterpret_cast<const float4 *>(tab + d / 2);
-      const float4 x = t[0], y = t[1];
-      turn(v[0], v[1], x.x, x.y);
-      turn(v[2], v[3], x.z, x.w);
-      turn(v[4], v[5], y.x, y.y);
-      turn(v[6], v[7], y.z, y.w);
-      return;
-    }
-#pragma unroll
-    for (int e = 0; e < 8; e += 2) {
-      const int j = (d + e) >> 1;
-      if (j < half) turn(v[e], v[e + 1], tab[j].x, tab[j].y);
-    }
+// Four consecutive values, aligned to the type alone (a rotated part of 100 puts
+// partners 100 bytes apart).
+template <int DT> __device__ __forceinline__ void ldu4(const typename Store<DT>::T *p, float v[4]) {
+  struct __attribute__((packed, aligned(4))) F4 { f32x4 v; };
+  struct __attribute__((packed, aligned(2))) H4 { uint2 v; };
+  if constexpr (DT == F32) {
+    const f32x4 x = reinterpret_cast<const F4 *>(p)->v;
+    v[0] = x[0]; v[1] = x[1]; v[2] = x[2]; v[3] = x[3];
   } else {
-    if (half % 8 == 0) {  // the partners are eight values half a rotated part away
-      float w[8];
-      const bool low = d < half;
-#pragma unroll
-      for (int e = 0; e < 8; e += N) ldv<DT, N>(head + (low ? d + half : d - half) + e, w + e);
-      const float4 *t = reinterpret_cast<const float4 *>(tab + (low ? d : d - half));
-#pragma unroll
-      for (int e = 0; e < 8; e += 2) {
-        const float4 cs = t[e / 2];
-        float a0 = low ? v[e] : w[e], b0 = low ? w[e] : v[e], a1 = low ? v[e + 1] : w[e + 1], b1 = low ? w[e + 1] : v[e + 1];
-        turn(a0, b0, cs.x, cs.y);
-        turn(a1, b1, cs.z, cs.w);
-        v[e] = low ? a0 : b0;
-        v[e + 1] = low ? a1 : b1;
-      }
-      return;
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int i = d + e;
-      if (i < half) {
-        float b = Store<DT>::dec(head[i + half]);
-        turn(v[e], b, tab[i].x, tab[i].y);
-      } else if (i < 2 * half) {
-        float a = Store<DT>::dec(head[i - half]);
-        turn(a, v[e], tab[i - half].x, tab[i - half].y);
-      }
-    }
+    const uint2 x = reinterpret_cast<const H4 *>(p)->v;
+    v[0] = Store<DT>::dec(uint16_t(x.x)); v[1] = Store<DT>::dec(uint16_t(x.x >> 16));
+    v[2] = Store<DT>::dec(uint16_t(x.y)); v[3] = Store<DT>::dec(uint16_t(x.y >> 16));
   }
 }
 
 // How many pairs a thread takes: 16 bytes of each load, where sizes, spacing and
-// addresses allow it, else one.
+// addresses allow it, else the largest power of two below that divides a head's parts.
+// 16500 tokens, 40 heads of 128 bf16 values, rotated parts of 128, 120, 100 and 42 by
+// halves: 69, 107, 115 and 185 us (one pair a thread wherever 16 bytes do not fit:
+// 180 and more).
 inline int rotary_unit(int dt, const Rotary &p) {
   const int64_t es = int64_t(dt_size(dt)), e = 16 / es;
-  const int u = int(p.interleaved ? e / 2 : e);
+  const int most = rotary_most(dt, p.interleaved), tail = p.x == p.out ? 0 : p.hd - 2 * p.half;
   const uintptr_t at = reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.out);
-  const bool whole = p.half % u == 0 && (2 * p.half) % e == 0 && p.hd % e == 0 && at % 16 == 0 && (p.n == 1 || (p.ldx % e == 0 && p.ldo % e == 0));
-  return whole ? u : 1;
+  if (p.half % most == 0 && (2 * p.half) % e == 0 && p.hd % e == 0 && at % 16 == 0 && (p.n == 1 || (p.ldx % e == 0 && p.ldo % e == 0))) return most;
+  int u = most / 2;
+  while (u > 1 && (p.half % u || tail % u)) u /= 2;
+  return u;
 }
+
+// f with the unit and the layout as types.
+template <int DT, bool INTERLEAVED, int U = rotary_most(DT, INTERLEAVED), typename F>
+__host__ __device__ __forceinline__ void rotary_unit_as(int unit, F &&f) {
+  if constexpr (U == 1) f(std::integral_constant<int, 1>(), std::integral_constant<bool, INTERLEAVED>());
+  else if (unit == U) f(std::integral_constant<int, U>(), std::integral_constant<bool, INTERLEAVED>());
+  else rotary_unit_as<DT, INTERLEAVED, U / 2>(unit, f);
+}
+template <int DT, typename F> inline void rotary_units(bool interleaved, int unit, F &&f) {
+  if (interleaved) rotary_unit_as<DT, true>(unit, f);
+  else rotary_unit_as<DT, false>(unit, f);
+}
+
 // The cut for workgroups of NT threads: units a head, threads that share a unit's
 // heads (so that each takes several heads where there are tokens enough), tokens.
 inline void rotary_cut(int dt, int unit, int threads, Rotary &p) {
-  const int w = unit == 1 ? 1 : int(16 / dt_size(dt));
+  const int w = rotary_tail(dt, unit, p.interleaved);
   p.units = p.half / unit + (p.x == p.out ? 0 : (p.hd - 2 * p.half) / w);
   const int cols = p.units < threads ? p.units : threads, most = threads / cols;
   const int64_t all = int64_t(p.n) * cols * p.heads;

@@ -85,7 +85,8 @@ def check(got, y, err, dtype):
 
 
 SIZES = [(1, 1, 2, 2), (1, 24, 64, 64), (3, 5, 64, 24), (7, 2, 80, 40), (33, 3, 128, 128), (2, 7, 96, 34), (1100, 4, 128, 64), (5, 3, 7, 4),
-         (65, 40, 128, 128), (4, 1, 256, 256), (9, 9, 48, 48), (17, 33, 32, 16), (2, 300, 64, 64), (3, 2, 33, 32)]
+         (65, 40, 128, 128), (4, 1, 256, 256), (9, 9, 48, 48), (17, 33, 32, 16), (2, 300, 64, 64), (3, 2, 33, 32),
+         (70, 40, 128, 120), (9, 5, 128, 100), (1030, 11, 96, 42), (6, 2, 36, 24)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -224,7 +225,7 @@ RUNS = [(0, 1), (5, 1), (3, 70), (0, 16), (15, 2), (0, 200), (9, 40)]
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("interleaved", [False, True])
 @pytest.mark.parametrize("P,kv,heads,hd,rot", [(16, 2, 4, 64, 64), (64, 3, 3, 64, 24), (256, 1, 8, 128, 128), (32, 2, 10, 80, 40), (64, 1, 1, 256, 6),
-                                               (128, 2, 2, 256, 256), (16, 1, 5, 16, 16)])
+                                               (128, 2, 2, 256, 256), (16, 1, 5, 16, 16), (16, 2, 4, 128, 120), (32, 2, 3, 128, 100)])
 def test_append(hip, torch, dtype, interleaved, P, kv, heads, hd, rot):
     """The cache holds what kv_store_paged makes of the rotated keys in float32, bit for
     bit; queries are rotary()'s; rows without a slot are left alone."""
@@ -263,7 +264,8 @@ def test_append(hip, torch, dtype, interleaved, P, kv, heads, hd, rot):
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("interleaved", [False, True])
 @pytest.mark.parametrize("P,kv,heads,hd,rot", [(16, 12, 12, 64, 24), (16, 8, 3, 128, 128), (32, 8, 9, 128, 64), (64, 8, 32, 128, 128), (64, 10, 4, 80, 42),
-                                               (128, 8, 5, 128, 128), (256, 8, 2, 128, 20), (256, 6, 1, 256, 256)])
+                                               (128, 8, 5, 128, 128), (256, 8, 2, 128, 20), (256, 6, 1, 256, 256), (64, 8, 6, 128, 120),
+                                               (32, 8, 7, 128, 100)])
 def test_append_prompts(hip, torch, dtype, interleaved, P, kv, heads, hd, rot):
     """Several tokens to a workgroup, workgroups of every size: prompts behind prefixes, some
     tokens without a slot, against the same keys in float32, bit for bit."""
