@@ -317,18 +317,18 @@ int mh_attention_paged(int dt, const void *q, int64_t ldq, const void *k_cache, 
 int mh_rotary_frequencies(double *freq, double *magnitude, int rot, double base, int scaling, double factor, double original,
                           double low, double high);
 /* table [n][half][2] = magnitude * (cos a, sin a), a = positions[t] * freq[j] (device
- * arrays; the angles in 64 bits, any int32 position).  table is 16-byte aligned. */
+ * arrays; the angles in 64 bits, any int32 position).  table is 16-byte aligned and overlaps neither of them. */
 int mh_rotary_table(const int32_t *positions, const double *freq, float *table, int n, int half, double magnitude, void *stream);
 /* out = x with its pairs (a, b) turned to (a c - b s, a s + b c); with `inverse` s
  * counts negative, which is also the gradient.  x, out: n token rows of heads * hd
  * values of `dt`, ldx / ldo values apart; table [n][half][2], 2 half <= hd.  out is
- * x (with ldo = ldx) or does not overlap it.  heads * hd is at most 2^30. */
+ * x (with ldo = ldx) or does not overlap it, nor the table.  heads * hd is at most 2^30. */
 int mh_rotary(int dt, const void *x, int64_t ldx, const float *table, void *out, int64_t ldo, int n, int heads, int hd, int half,
               int interleaved, int inverse, void *stream);
 /* mh_kv_store_paged of keys that are rotated on the way (the cache's 8 bits are
  * their only rounding; mh_kv_store_paged has the other arguments and what is
  * written), and in the same launch q [n][Hq * hd] (rows ldq values apart) rotated
- * into q_out (ldqo apart; q itself, or not overlapping q, k or v).  q NULL: none.
+ * into q_out (ldqo apart; q itself, or not overlapping q, k, v, table or slots).  q NULL: none.
  * Rows of q whose slot is -1 or outside the pool are left as they are in q_out.
  * Rows of q and q_out are multiples of 16 bytes apart, as are the pointers. */
 int mh_kv_store_rotary_paged(int dt, const void *k, const void *v, int64_t ldk, int64_t ldv, const float *table,
@@ -345,9 +345,9 @@ int mh_kv_store_rotary_paged(int dt, const void *k, const void *v, int64_t ldk, 
  * row's largest magnitude, at least 127 * 2^-126.  A row with NaN or infinities
  * gets the scale NaN (and q = 0): what is computed from it is NaN.  x [rows][cols]
  * of `dt`, rows ldx values apart, q ldq apart, of any alignment; q may not overlap
- * x. */
+ * x, nor scale either of them. */
 int mh_quantize_rows(int dt, const void *x, int64_t ldx, int8_t *q, int64_t ldq, float *scale, int rows, int cols, void *stream);
-/* out = q * scale of its row, rounded to `dt`. */
+/* out = q * scale of its row, rounded to `dt`; out overlaps neither. */
 int mh_dequantize_rows(int dt, const int8_t *q, int64_t ldq, const float *scale, void *out, int64_t ldo, int rows, int cols,
                        void *stream);
 /* out[m][n] = act(x_scale[m] w_scale[n] sum_k x[m][k] w[n][k] + bias[n]) + resid[m][n]:
@@ -357,7 +357,7 @@ int mh_dequantize_rows(int dt, const int8_t *q, int64_t ldq, const float *scale,
  * NULL; rows ldr apart) and out (ldo apart) are of `dt`; act is MH_ACT_*, GELU
  * x * sigmoid(1.702 x).  The sum is exact in int32 (K is at most 2^17 - 1), the rest
  * in fp32, rounded once.  out may be resid (with ldo = ldr), else it overlaps
- * neither it nor x or w. */
+ * neither it nor any other operand. */
 int mh_linear_i8(int dt, const int8_t *x, int64_t ldx, const float *x_scale, const int8_t *w, int64_t ldw, const float *w_scale,
                  const void *bias, const void *resid, int64_t ldr, void *out, int64_t ldo, int M, int N, int K, int act,
                  void *stream);

@@ -273,6 +273,8 @@ bool rows_meet(const RowSet &a, const RowSet &b) {
   }
   return true;
 }
+// n bytes from p, as one row
+RowSet whole(const void *p, int64_t n) { return {p, 1, n, n}; }
 void check_rotation(const char *op, const float *table, int hd, int half) {
   if (half < 1 || hd < 1 || half > hd / 2) throw Error(std::string(op) + ": the rotated part must be 2 values at least and fit the head");
   if (!table) throw Error(std::string(op) + ": null table");
@@ -782,6 +784,10 @@ int mh_rotary_table(const int32_t *positions, const double *freq, float *table, 
     if (n == 0) return 0;
     if (!positions || !freq || !table) throw Error("rotary_table: null argument");
     aligned16(table, "table");
+    if (int64_t(n) * half > int64_t(1) << 56) throw Error("rotary_table: table larger than any memory");
+    const RowSet o = whole(table, int64_t(n) * half * 8);
+    if (rows_meet(o, whole(positions, int64_t(n) * 4)) || rows_meet(o, whole(freq, int64_t(half) * 8)))
+      throw Error("rotary_table: table overlaps positions or freq");
     hip_check(rotary_table(positions, freq, table, n, half, magnitude, S_(stream)), "rotary_table");
   })
 }
@@ -798,6 +804,7 @@ int mh_rotary(int dt, const void *x, int64_t ldx, const float *table, void *out,
     check_whole_rows("rotary", "out", es, out, n, ldo, cols);
     if (!(x == out && (ldx == ldo || n == 1)) && rows_meet({x, n, ldx * es, cols * es}, {out, n, ldo * es, cols * es}))
       throw Error("rotary: out overlaps x without being it");
+    if (rows_meet({out, n, ldo * es, cols * es}, whole(table, int64_t(n) * half * 8))) throw Error("rotary: out overlaps table");
     Rotary p;
     p.x = x;
     p.out = out;
@@ -846,6 +853,8 @@ int mh_kv_store_rotary_paged(int dt, const void *k, const void *v, int64_t ldk, 
       if ((!(q == q_out && (ldq == ldqo || n == 1)) && rows_meet(o, {q, n, ldq * es, cols})) ||
           rows_meet(o, {k, n, ldk * es, int64_t(Hkv) * hd * es}) || rows_meet(o, {v, n, ldv * es, int64_t(Hkv) * hd * es}))
         throw Error("kv_store_rotary_paged: q_out overlaps q without being it, or k or v");
+      if (rows_meet(o, whole(table, int64_t(n) * half * 8)) || rows_meet(o, whole(slots, int64_t(n) * 4)))
+        throw Error("kv_store_rotary_paged: q_out overlaps table or slots");
       p.x = q;
       p.out = q_out;
       p.ldx = ldq;
@@ -869,6 +878,10 @@ int mh_quantize_rows(int dt, const void *x, int64_t ldx, int8_t *q, int64_t ldq,
     check_whole_rows("quantize_rows", "q", 1, q, rows, ldq, cols);
     if (!scale) throw Error("quantize_rows: null scale");
     if (rows_meet({x, rows, ldx * es, cols * es}, {q, rows, ldq, cols})) throw Error("quantize_rows: q overlaps x");
+    check_whole_rows("quantize_rows", "scale", 4, scale, 1, rows, rows);
+    const RowSet o = whole(scale, int64_t(rows) * 4);
+    if (rows_meet(o, {x, rows, ldx * es, cols * es}) || rows_meet(o, {q, rows, ldq, cols}))
+      throw Error("quantize_rows: scale overlaps x or q");
     QuantRows p;
     p.x = x;
     p.q = q;
@@ -891,6 +904,9 @@ int mh_dequantize_rows(int dt, const int8_t *q, int64_t ldq, const float *scale,
     check_whole_rows("dequantize_rows", "out", es, out, rows, ldo, cols);
     if (!scale) throw Error("dequantize_rows: null scale");
     if (rows_meet({out, rows, ldo * es, cols * es}, {q, rows, ldq, cols})) throw Error("dequantize_rows: out overlaps q");
+    check_whole_rows("dequantize_rows", "scale", 4, scale, 1, rows, rows);
+    if (rows_meet({out, rows, ldo * es, cols * es}, whole(scale, int64_t(rows) * 4)))
+      throw Error("dequantize_rows: out overlaps scale");
     QuantRows p;
     p.out = out;
     p.q = const_cast<int8_t *>(q);
@@ -917,6 +933,8 @@ int mh_linear_i8(int dt, const int8_t *x, int64_t ldx, const float *x_scale, con
     check_whole_rows("linear_i8", "w", 1, w, N, ldw, K);
     check_whole_rows("linear_i8", "out", es, out, M, ldo, N);
     if (!x_scale || !w_scale) throw Error("linear_i8: null scale");
+    check_whole_rows("linear_i8", "x_scale", 4, x_scale, 1, M, M);
+    check_whole_rows("linear_i8", "w_scale", 4, w_scale, 1, N, N);
     if (bias) check_whole_rows("linear_i8", "bias", es, bias, 1, N, N);
     const RowSet o{out, M, ldo * es, N * es};
     if (resid) {
@@ -925,6 +943,8 @@ int mh_linear_i8(int dt, const int8_t *x, int64_t ldx, const float *x_scale, con
         throw Error("linear_i8: out overlaps the residual without being it");
     }
     if (rows_meet(o, {x, M, ldx, K}) || rows_meet(o, {w, N, ldw, K})) throw Error("linear_i8: out overlaps x or w");
+    if (rows_meet(o, whole(x_scale, int64_t(M) * 4)) || rows_meet(o, whole(w_scale, int64_t(N) * 4)) || rows_meet(o, whole(bias, N * es)))
+      throw Error("linear_i8: out overlaps a scale or the bias");
     LinearI8 p;
     p.x = x;
     p.w = w;

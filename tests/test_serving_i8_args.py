@@ -87,7 +87,8 @@ def _table(**kw):
 
 @pytest.mark.parametrize("kw,match", [
     (dict(n=-1), "negative"), (dict(half=0), "no pairs"), (dict(positions=None), "null"), (dict(freq=None), "null"),
-    (dict(table=None), "null"), (dict(table=A + 8), "aligned")])
+    (dict(table=None), "null"), (dict(table=A + 8), "aligned"), (dict(freq=FAR), "overlaps"), (dict(positions=FAR), "overlaps"),
+    (dict(positions=A + 240, freq=FAR), "overlaps"), (dict(n=(1 << 31) - 1, half=(1 << 31) - 1), "larger")])
 def test_rotary_table_refusals(kw, match):
     with pytest.raises(_lib.HipError, match=match):
         _table(**kw)
@@ -105,7 +106,8 @@ def _rotary(**kw):
     (dict(half=-3), "rotated part"), (dict(half=0x7fffffff), "rotated part"), (dict(table=None), "null table"), (dict(table=A + 4), "aligned"),
     (dict(x=None), "null x"), (dict(out=None), "null out"), (dict(x=A + 1), "aligned to its type"), (dict(dt=F32, out=FAR + 2), "aligned to its type"),
     (dict(ldx=1023), "whole"), (dict(ldo=-5), "whole"), (dict(ldx=1 << 57), "far apart"), (dict(out=A + 16), "overlaps"), (dict(out=A, ldo=2048), "overlaps"),
-    (dict(out=A - 16), "overlaps"), (dict(ldx=2048, ldo=2048, out=A + 2046), "overlaps"), (dict(ldx=2048, ldo=2048, out=A + 2 * 2048 + 2046), "overlaps")])
+    (dict(out=A - 16), "overlaps"), (dict(ldx=2048, ldo=2048, out=A + 2046), "overlaps"), (dict(ldx=2048, ldo=2048, out=A + 2 * 2048 + 2046), "overlaps"),
+    (dict(table=FAR + 4096), "overlaps table"), (dict(table=FAR - 2032), "overlaps table")])
 def test_rotary_refusals(kw, match):
     with pytest.raises(_lib.HipError, match=match):
         _rotary(**kw)
@@ -125,7 +127,8 @@ def _store(**kw):
     (dict(table=A + 8), "aligned"), (dict(half=0), "rotated part"), (dict(half=65), "rotated part"), (dict(kc=None), "null cache"),
     (dict(Hq=0), "query head"), (dict(Hq=1 << 24), "query head"), (dict(q_out=None), "null q_out"), (dict(q=4 * FAR + 2), "aligned"),
     (dict(ldq=4095), "multiple of 16"), (dict(ldqo=2048), "whole"), (dict(q_out=4 * FAR, ldqo=8192), "overlaps"),
-    (dict(q_out=4 * FAR + 64), "overlaps"), (dict(k=8 * FAR), "overlaps"), (dict(v=8 * FAR + 4096), "overlaps"), (dict(ldk=1 << 58), "far apart")])
+    (dict(q_out=4 * FAR + 64), "overlaps"), (dict(k=8 * FAR), "overlaps"), (dict(v=8 * FAR + 4096), "overlaps"), (dict(ldk=1 << 58), "far apart"),
+    (dict(table=8 * FAR + 4096), "overlaps table"), (dict(slots=8 * FAR - 12), "overlaps table or slots")])
 def test_kv_store_rotary_paged_refusals(kw, match):
     with pytest.raises(_lib.HipError, match=match):
         _store(**kw)
@@ -140,7 +143,8 @@ def _quant(**kw):
 @pytest.mark.parametrize("kw,match", [
     (dict(dt=3), "dtype"), (dict(rows=-1), "bad row count"), (dict(cols=0), "empty rows"), (dict(x=None), "null x"), (dict(q=None), "null q"),
     (dict(scale=None), "null scale"), (dict(x=A + 1), "aligned to its type"), (dict(ldx=99), "whole"), (dict(ldq=99), "whole"),
-    (dict(q=A + 50), "overlaps"), (dict(ldq=1 << 60), "far apart")])
+    (dict(q=A + 50), "overlaps"), (dict(ldq=1 << 60), "far apart"), (dict(scale=FAR + 16), "scale overlaps"), (dict(scale=A + 796), "scale overlaps"),
+    (dict(scale=4 * FAR + 2), "aligned to its type")])
 def test_quantize_rows_refusals(kw, match):
     with pytest.raises(_lib.HipError, match=match):
         _quant(**kw)
@@ -155,7 +159,7 @@ def _dequant(**kw):
 @pytest.mark.parametrize("kw,match", [
     (dict(dt=3), "dtype"), (dict(rows=-1), "bad row count"), (dict(cols=0), "empty rows"), (dict(q=None), "null q"), (dict(out=None), "null out"),
     (dict(scale=None), "null scale"), (dict(out=FAR + 1), "aligned to its type"), (dict(ldo=99), "whole"), (dict(ldq=99), "whole"),
-    (dict(out=A + 50), "overlaps")])
+    (dict(out=A + 50), "overlaps"), (dict(scale=FAR + 796), "overlaps scale"), (dict(scale=FAR - 1), "aligned to its type")])
 def test_dequantize_rows_refusals(kw, match):
     with pytest.raises(_lib.HipError, match=match):
         _dequant(**kw)
@@ -174,7 +178,9 @@ def _linear(**kw):
     (dict(ldx=511), "whole"), (dict(ldw=100), "whole"), (dict(ldo=63), "whole"), (dict(out=4 * FAR + 1), "aligned to its type"),
     (dict(bias=A + 1), "aligned to its type"), (dict(resid=A + 1, ldr=64), "aligned to its type"), (dict(resid=A, ldr=63), "whole"),
     (dict(resid=4 * FAR, ldr=65), "overlaps the residual"), (dict(resid=4 * FAR + 2, ldr=64), "overlaps the residual"),
-    (dict(x=4 * FAR + 100), "overlaps x or w"), (dict(w=4 * FAR - 100), "overlaps x or w"), (dict(ldx=1 << 57), "far apart")])
+    (dict(x=4 * FAR + 100), "overlaps x or w"), (dict(w=4 * FAR - 100), "overlaps x or w"), (dict(ldx=1 << 57), "far apart"),
+    (dict(sx=4 * FAR + 8), "overlaps a scale"), (dict(sw=4 * FAR - 252), "overlaps a scale"), (dict(bias=4 * FAR + 1022), "or the bias"),
+    (dict(sx=A + 2), "aligned to its type"), (dict(sw=A + 1), "aligned to its type")])
 def test_linear_i8_refusals(kw, match):
     with pytest.raises(_lib.HipError, match=match):
         _linear(**kw)
