@@ -327,7 +327,7 @@ int mh_rotary(int dt, const void *x, int64_t ldx, const float *table, void *out,
               int interleaved, int inverse, void *stream);
 /* mh_kv_store_paged of keys that are rotated on the way (the cache's 8 bits are
  * their only rounding; mh_kv_store_paged has the other arguments and what is
- * written), and in the same launch q [n][Hq * hd] (rows ldq values apart) rotated
+ * written), and beside them q [n][Hq * hd] (rows ldq values apart) rotated
  * into q_out (ldqo apart; q itself, or not overlapping q, k, v, table or slots).  q NULL: none.
  * Rows of q whose slot is -1 or outside the pool are left as they are in q_out.
  * Rows of q and q_out are multiples of 16 bytes apart, as are the pointers. */

@@ -494,7 +494,7 @@ class HipBackend:
 
     def kv_store_rotary_paged(self, k, v, table, slots, k_cache, v_cache, k_scale, v_scale, q=None, q_out=None, interleaved=False):
         """``kv_store_paged`` of keys rotated by ``table`` [n, pairs, 2] on the way, and
-        ``q`` [n, Hq, hd] rotated into ``q_out`` (which may be ``q``) in the same launch
+        ``q`` [n, Hq, hd] rotated into ``q_out`` (which may be ``q``) beside them
         (mh_kv_store_rotary_paged).  Rows without a slot are left alone."""
         op, d, t = "kv_store_rotary_paged", k.get_device(), _torch()
         kc, vc, ks, vs, n_pages, Hkv, page, hd = _pool(op, d, k_cache, v_cache, k_scale, v_scale)
