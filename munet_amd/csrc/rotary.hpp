@@ -177,7 +177,7 @@ template <int DT> __device__ __forceinline__ void ldu4(const typename Store<DT>:
 // addresses allow it, else the largest power of two below that divides a head's parts.
 // 16500 tokens, 40 heads of 128 bf16 values, rotated parts of 128, 120, 100 and 42 by
 // halves: 69, 107, 115 and 185 us (one pair a thread wherever 16 bytes do not fit:
-// 180 and more).
+// 175 and more).
 inline int rotary_unit(int dt, const Rotary &p) {
   const int64_t es = int64_t(dt_size(dt)), e = 16 / es;
   const int most = rotary_most(dt, p.interleaved), tail = p.x == p.out ? 0 : p.hd - 2 * p.half;
