@@ -13,14 +13,27 @@ namespace {
 
 // (m cos a, m sin a) of a = position * frequency, in 64 bits: a document's
 // position is a million turns of the fastest pair, of which 32 bits would leave
-// four digits of the last one.  The angle is taken in turns, p + lo exactly, less
-// the whole ones and then the quarters; what is left, of at most an eighth, goes
+// four digits of the last one.  The angle is taken in turns, less the whole ones and
+// then the quarters.  A pair's turns a position are frequency / 2 pi to twice 64
+// bits, hi + lo (their rounding alone is 2^-25 of a turn at 2^31 positions), and
+// pos hi = p + its remainder exactly: no sum of these may be fused with a product, which
+// would hold the remainder already.  What is left, of at most an eighth, goes
 // through the Taylor series to x^17 and x^16 (the next terms are below 2^-58), and the
-// quarters say which is which.  A thread keeps its pair's frequency for all tokens.
-// 17000 tokens of 64 pairs: 5 to 6 us (1.7 TB/s written), 7.7 with a library sincos and a
+// quarters say which is which.  A thread keeps its pair's turns for all tokens.
+// 17000 tokens of 64 pairs: 5.8 us (1.5 TB/s written; 5.7 with the turns in 64 bits), 7.7 with a library sincos and a
 // division for each value.
-__device__ __forceinline__ float2 angle(double pos, double turns, double m) {
-  const double p = pos * turns, lo = fma(pos, turns, -p), t = (p - rint(p)) + lo;
+struct Turns {
+  double hi, lo;
+  __device__ __forceinline__ explicit Turns(double freq) {
+#pragma clang fp contract(off)
+    constexpr double kTurn = 0.15915494309189535, kRest = -9.839338337591243e-18;  // 1 / 2 pi = kTurn + kRest
+    hi = freq * kTurn;
+    lo = fma(freq, kTurn, -hi) + freq * kRest;
+  }
+};
+__device__ __forceinline__ float2 angle(double pos, Turns turns, double m) {
+#pragma clang fp contract(off)
+  const double p = pos * turns.hi, lo = fma(pos, turns.lo, fma(pos, turns.hi, -p)), t = (p - rint(p)) + lo;
   const double quarters = rint(4.0 * t), x = (t - 0.25 * quarters) * 6.283185307179586476925, y = x * x;
   double s = 1.0 / 355687428096000.0, c = 1.0 / 20922789888000.0;
   s = fma(s, y, -1.0 / 1307674368000.0);
@@ -49,7 +62,7 @@ __global__ void __launch_bounds__(256) rotary_table_kernel(const int32_t *__rest
   const int lr = threadIdx.x / cols, lc = threadIdx.x - lr * cols;
   if (lr >= rows) return;
   for (int j = lc; j < half; j += cols) {
-    const double turns = freq[j] * 0.159154943091895335768884;
+    const Turns turns(freq[j]);
     for (int64_t t = int64_t(blockIdx.x) * rows + lr; t < n; t += int64_t(gridDim.x) * rows) table[t * half + j] = angle(pos[t], turns, m);
   }
 }
