@@ -113,12 +113,12 @@ __device__ __forceinline__ void e4m3x4_dec(uint32_t w, float v[4]) {
   const f2 a = __builtin_amdgcn_cvt_pk_f32_fp8(int(w), false), b = __builtin_amdgcn_cvt_pk_f32_fp8(int(w), true);
   v[0] = a[0]; v[1] = a[1]; v[2] = b[0]; v[3] = b[1];
 }
+// (of ratios below 1: nothing becomes infinite, and NaN stays)
 __device__ __forceinline__ uint32_t rescale4(uint32_t w, float ratio) {
   float v[4];
   e4m3x4_dec(w, v);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] *= ratio;
-  return e4m3x4(v);
+  const int r = __builtin_amdgcn_cvt_pk_fp8_f32(v[0] * ratio, v[1] * ratio, 0, false);
+  return uint32_t(__builtin_amdgcn_cvt_pk_fp8_f32(v[2] * ratio, v[3] * ratio, r, true));
 }
 
 // eight consecutive values
@@ -263,31 +263,48 @@ struct PageScale {
     ratio = place > 0 && held > 0.f && held < now ? held * inv : 1.f;
   }
 };
-// The page's earlier tokens in a larger scale, by NT threads.
-template <int NT> __device__ __forceinline__ void rescale_keys(uint8_t *kd, int place, int hd, float ratio, int tid) {
-  for (int c = tid; c < place * hd / 16; c += NT) {
-    uint4 *p = reinterpret_cast<uint4 *>(kd) + c;
-    const uint4 w = *p;
-    *p = make_uint4(rescale4(w.x, ratio), rescale4(w.y, ratio), rescale4(w.z, ratio), rescale4(w.w, ratio));
+// The page's earlier tokens in a larger scale, by NT threads with U pieces of 16
+// bytes each in flight (places past the last piece read that one again, and store
+// nothing).
+template <int NT, int U> __device__ __forceinline__ void rescale_keys(uint8_t *kd, int place, int hd, float ratio, int tid) {
+  uint4 *p = reinterpret_cast<uint4 *>(kd);
+  const int all = place * hd / 16;
+  for (int c0 = tid; c0 < all; c0 += NT * U) {
+    uint4 w[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) w[u] = p[min(c0 + NT * u, all - 1)];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (c0 + NT * u < all)
+        p[c0 + NT * u] = make_uint4(rescale4(w[u].x, ratio), rescale4(w[u].y, ratio), rescale4(w[u].z, ratio), rescale4(w[u].w, ratio));
   }
 }
-template <int NT> __device__ __forceinline__ void rescale_values(uint8_t *vd, int place, int hd, int P, float ratio, int tid) {
+template <int NT, int U> __device__ __forceinline__ void rescale_values(uint8_t *vd, int place, int hd, int P, float ratio, int tid) {
   // (whole 16-byte pieces of a row: what lies behind the earlier tokens is kept, or
   // written afterwards)
-  const int pieces = (place + 15) / 16;
-  for (int c = tid; c < hd * pieces; c += NT) {
-    const int d = c / pieces, i = c - d * pieces;
-    uint4 *p = reinterpret_cast<uint4 *>(vd + int64_t(d) * P + 16 * i);
-    const uint4 w = *p;
-    const uint32_t o[4] = {w.x, w.y, w.z, w.w};
-    uint32_t r[4];
+  const int pieces = (place + 15) / 16, all = hd * pieces;
+  for (int c0 = tid; c0 < all; c0 += NT * U) {
+    uint4 *p[U], w[U];
+    int at[U];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int left = place - 16 * i - 4 * q;  // earlier tokens from this word on
-      const uint32_t m = left >= 4 ? 0xffffffffu : left <= 0 ? 0u : (1u << (8 * left)) - 1u;
-      r[q] = (rescale4(o[q], ratio) & m) | (o[q] & ~m);
+    for (int u = 0; u < U; ++u) {
+      const int c = min(c0 + NT * u, all - 1), d = c / pieces, i = c - d * pieces;
+      p[u] = reinterpret_cast<uint4 *>(vd + int64_t(d) * P + 16 * i);
+      w[u] = *p[u];
+      at[u] = 16 * i;
     }
-    *p = make_uint4(r[0], r[1], r[2], r[3]);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint32_t o[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
+      uint32_t r[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int left = place - at[u] - 4 * q;  // earlier tokens from this word on
+        const uint32_t m = left >= 4 ? 0xffffffffu : left <= 0 ? 0u : (1u << (8 * left)) - 1u;
+        r[q] = (rescale4(o[q], ratio) & m) | (o[q] & ~m);
+      }
+      if (c0 + NT * u < all) *p[u] = make_uint4(r[0], r[1], r[2], r[3]);
+    }
   }
 }
 
@@ -339,8 +356,12 @@ __global__ void __launch_bounds__(NT) kv_store_paged_kernel(StoreArgs a) {
   if constexpr (ONE) {
     // One token for the workgroup (a decode step).  Where it is a run of its own, the
     // first wave stores it without LDS or barriers, a key piece or a value piece to
-    // a lane; its row is loaded before its slot is known (64 tokens, 8 heads of 128:
-    // 4.3 us, through LDS 7.1; rotated, with 32 query heads 4.7, 12).
+    // a lane (64 tokens, 8 heads of 128: 4.2 us, through LDS 7.1; rotated, with 32 query
+    // heads 4.7, 12).  Its row, the slots and the scale are waited for one after
+    // another.  A page that moves to a larger scale keeps eight pieces a lane in flight
+    // (64 tokens whose pages all move, in pages of 64, 128 and 256: 7.2, 11.7 and 19 us; a piece
+    // at a time 11.9, 19.5 and 34.6).  All four waves at it took 6.3, 9.8 and 15.5, but they
+    // stay until the first one knows: 256 tokens whose pages stay as they are 8.4 us, so 7.5.
     const int vh = lane >> 5, c = lane & 31;
     const bool on = wave == 0 && c < h8;
     const KeyPiece<DT, ROT> piece(c, a.half);
@@ -366,9 +387,9 @@ __global__ void __launch_bounds__(NT) kv_store_paged_kernel(StoreArgs a) {
       const PageScale ps(big, held, place);
       uint8_t *kd = a.kc + page_base(page, a.Hkv, head, P, hd), *vd = a.vc + page_base(page, a.Hkv, head, P, hd);
       const float kratio = __shfl(ps.ratio, 0, 64), vratio = __shfl(ps.ratio, 32, 64);
-      if (kratio != 1.f) rescale_keys<64>(kd, place, hd, kratio, lane);
+      if (kratio != 1.f) rescale_keys<64, 8>(kd, place, hd, kratio, lane);
       if (vratio != 1.f) {
-        rescale_values<64>(vd, place, hd, P, vratio, lane);
+        rescale_values<64, 8>(vd, place, hd, P, vratio, lane);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the new place lies in a piece that was rewritten
       }
       if (on && vh) {
@@ -472,8 +493,8 @@ __global__ void __launch_bounds__(NT) kv_store_paged_kernel(StoreArgs a) {
       ratio[x] = ps.ratio;
     }
     // the page's earlier tokens in the larger scale
-    if (ratio[0] != 1.f) rescale_keys<NT>(kd, place, hd, ratio[0], tid);
-    if (ratio[1] != 1.f) rescale_values<NT>(vd, place, hd, P, ratio[1], tid);
+    if (ratio[0] != 1.f) rescale_keys<NT, 1>(kd, place, hd, ratio[0], tid);
+    if (ratio[1] != 1.f) rescale_values<NT, 1>(vd, place, hd, P, ratio[1], tid);
     __syncthreads();
 
     if (held_run) {
