@@ -329,6 +329,7 @@ int mh_rotary(int dt, const void *x, int64_t ldx, const float *table, void *out,
  * their only rounding; mh_kv_store_paged has the other arguments and what is
  * written), and beside them q [n][Hq * hd] (rows ldq values apart) rotated
  * into q_out (ldqo apart; q itself, or not overlapping q, k, v, table or slots).  q NULL: none.
+ * The caches and scales overlap neither each other nor any other operand.
  * Rows of q whose slot is -1 or outside the pool are left as they are in q_out.
  * Rows of q and q_out are multiples of 16 bytes apart, as are the pointers. */
 int mh_kv_store_rotary_paged(int dt, const void *k, const void *v, int64_t ldk, int64_t ldv, const float *table,

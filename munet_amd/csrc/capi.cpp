@@ -837,6 +837,11 @@ int mh_kv_store_rotary_paged(int dt, const void *k, const void *v, int64_t ldk, 
     check_rotation(op, table, hd, half);
     check_rows(op, "k", dt, k, ldk, int64_t(Hkv) * hd);
     check_rows(op, "v", dt, v, ldv, int64_t(Hkv) * hd);
+    const int64_t es = int64_t(dt_size(dt)), kcols = int64_t(Hkv) * hd * es, angles = int64_t(n) * half * 8;
+    const RowSet kr{k, n, ldk * es, kcols}, vr{v, n, ldv * es, kcols};
+    RowSet qr{nullptr, 0, 0, 0}, o = qr;
+    for (int64_t ld : {ldk, ldv})
+      if (ld > (int64_t(1) << 56) / n) throw Error("kv_store_rotary_paged: rows too far apart");
     Rotary p;
     p.table = table;
     p.n = n;
@@ -844,22 +849,30 @@ int mh_kv_store_rotary_paged(int dt, const void *k, const void *v, int64_t ldk, 
     p.half = half;
     p.interleaved = interleaved != 0;
     if (q) {
-      const int64_t es = int64_t(dt_size(dt)), cols = int64_t(Hq) * hd * es;
+      const int64_t cols = int64_t(Hq) * hd * es;
       check_rows(op, "q", dt, q, ldq, int64_t(Hq) * hd);
       check_rows(op, "q_out", dt, q_out, ldqo, int64_t(Hq) * hd);
-      for (int64_t ld : {ldk, ldv, ldq, ldqo})
+      for (int64_t ld : {ldq, ldqo})
         if (ld > (int64_t(1) << 56) / n) throw Error("kv_store_rotary_paged: rows too far apart");
-      const RowSet o{q_out, n, ldqo * es, cols};
-      if ((!(q == q_out && (ldq == ldqo || n == 1)) && rows_meet(o, {q, n, ldq * es, cols})) ||
-          rows_meet(o, {k, n, ldk * es, int64_t(Hkv) * hd * es}) || rows_meet(o, {v, n, ldv * es, int64_t(Hkv) * hd * es}))
+      qr = {q, n, ldq * es, cols};
+      o = {q_out, n, ldqo * es, cols};
+      if ((!(q == q_out && (ldq == ldqo || n == 1)) && rows_meet(o, qr)) || rows_meet(o, kr) || rows_meet(o, vr))
         throw Error("kv_store_rotary_paged: q_out overlaps q without being it, or k or v");
-      if (rows_meet(o, whole(table, int64_t(n) * half * 8)) || rows_meet(o, whole(slots, int64_t(n) * 4)))
+      if (rows_meet(o, whole(table, angles)) || rows_meet(o, whole(slots, int64_t(n) * 4)))
         throw Error("kv_store_rotary_paged: q_out overlaps table or slots");
       p.x = q;
       p.out = q_out;
       p.ldx = ldq;
       p.ldo = ldqo;
       p.heads = Hq;
+    }
+    const int64_t pool = int64_t(n_pages) * Hkv * page * hd, scales = int64_t(n_pages) * Hkv * 4;
+    const RowSet held[] = {whole(k_cache, pool), whole(v_cache, pool), whole(k_scale, scales), whole(v_scale, scales)};
+    for (const RowSet &h : held) {
+      for (const RowSet &x : {kr, vr, qr, o, whole(table, angles), whole(slots, int64_t(n) * 4)})
+        if (rows_meet(h, x)) throw Error("kv_store_rotary_paged: k, v, q, q_out, table or slots overlap a cache or a scale");
+      for (const RowSet *x = held; x < &h; ++x)
+        if (rows_meet(h, *x)) throw Error("kv_store_rotary_paged: caches and scales overlap each other");
     }
     hip_check(kv_store_paged(dt, k, v, long(ldk), long(ldv), slots, k_cache, v_cache, k_scale, v_scale, n, Hkv, hd, page, n_pages,
                              serving_error_flag(), S_(stream), &p),
