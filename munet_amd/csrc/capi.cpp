@@ -765,6 +765,7 @@ int mh_rotary_frequencies(double *freq, double *magnitude, int rot, double base,
     if (scaling == MH_ROTARY_TURNS && (!(original > 0) || !std::isfinite(original) || !(low >= 0) || !(high > low) || !std::isfinite(high)))
       throw Error("rotary_frequencies: needs original > 0 and 0 <= low < high");
     if (scaling == MH_ROTARY_BASE) base *= std::pow(factor, double(rot) / (rot - 2));
+    if (!(base > 0) || !std::isfinite(base)) throw Error("rotary_frequencies: the changed base is out of range");
     for (int j = 0; j < rot / 2; ++j) {
       double f = std::pow(base, -2.0 * j / rot);
       if (scaling == MH_ROTARY_LINEAR) f /= factor;
@@ -772,6 +773,7 @@ int mh_rotary_frequencies(double *freq, double *magnitude, int rot, double base,
         const double r = original * f / (2 * M_PI), g = std::min(1.0, std::max(0.0, (r - low) / (high - low)));
         f = g * f + (1 - g) * f / factor;
       }
+      if (!std::isfinite(f)) throw Error("rotary_frequencies: a frequency is out of range");
       freq[j] = f;
     }
     if (magnitude) *magnitude = scaling == MH_ROTARY_TURNS && factor > 1 ? 1 + 0.1 * std::log(factor) : 1.0;
