@@ -274,9 +274,10 @@ template <int NT, int U> __device__ __forceinline__ void rescale_keys(uint8_t *k
 #pragma unroll
     for (int u = 0; u < U; ++u) w[u] = p[min(c0 + NT * u, all - 1)];
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (c0 + NT * u < all)
-        p[c0 + NT * u] = make_uint4(rescale4(w[u].x, ratio), rescale4(w[u].y, ratio), rescale4(w[u].z, ratio), rescale4(w[u].w, ratio));
+    for (int u = 0; u < U; ++u) {
+      if (c0 + NT * u >= all) break;
+      p[c0 + NT * u] = make_uint4(rescale4(w[u].x, ratio), rescale4(w[u].y, ratio), rescale4(w[u].z, ratio), rescale4(w[u].w, ratio));
+    }
   }
 }
 template <int NT, int U> __device__ __forceinline__ void rescale_values(uint8_t *vd, int place, int hd, int P, float ratio, int tid) {
@@ -295,6 +296,7 @@ template <int NT, int U> __device__ __forceinline__ void rescale_values(uint8_t 
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
+      if (c0 + NT * u >= all) break;
       const uint32_t o[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
       uint32_t r[4];
 #pragma unroll
@@ -303,7 +305,7 @@ template <int NT, int U> __device__ __forceinline__ void rescale_values(uint8_t 
         const uint32_t m = left >= 4 ? 0xffffffffu : left <= 0 ? 0u : (1u << (8 * left)) - 1u;
         r[q] = (rescale4(o[q], ratio) & m) | (o[q] & ~m);
       }
-      if (c0 + NT * u < all) *p[u] = make_uint4(r[0], r[1], r[2], r[3]);
+      *p[u] = make_uint4(r[0], r[1], r[2], r[3]);
     }
   }
 }
@@ -359,7 +361,7 @@ __global__ void __launch_bounds__(NT) kv_store_paged_kernel(StoreArgs a) {
     // a lane (64 tokens, 8 heads of 128: 4.2 us, through LDS 7.1; rotated, with 32 query
     // heads 4.7, 12).  Its row, the slots and the scale are waited for one after
     // another.  A page that moves to a larger scale keeps eight pieces a lane in flight
-    // (64 tokens whose pages all move, in pages of 64, 128 and 256: 7.2, 11.7 and 19 us; a piece
+    // (64 tokens whose pages all move, in pages of 64, 128 and 256: 7.4, 11.5 and 19 us; a piece
     // at a time 11.9, 19.5 and 34.6).  All four waves at it took 6.3, 9.8 and 15.5, but they
     // stay until the first one knows: 256 tokens whose pages stay as they are 8.4 us, so 7.5.
     const int vh = lane >> 5, c = lane & 31;
