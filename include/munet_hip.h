@@ -308,8 +308,10 @@ int mh_attention_paged(int dt, const void *q, int64_t ldq, const void *k_cache, 
  *                     the `original` trained positions: from `high` turns on as it
  *                     is, up to `low` divided by factor, between in proportion
  *                     (g f + (1 - g) f / factor, g = (r - low) / (high - low)).
- * *magnitude (may be NULL) gets what tables are to be multiplied by: 1 + 0.1
- * ln(factor) for MH_ROTARY_TURNS with a factor above 1, else 1. */
+ * *magnitude (may be NULL) gets 1 + 0.1 ln(factor) for MH_ROTARY_TURNS with a factor
+ * above 1, else 1: what tables are to be multiplied by in models that were trained
+ * so.  Others that blend by turns take the frequencies and a table of magnitude 1.
+ * Frequencies that are no longer finite are refused. */
 #define MH_ROTARY_PLAIN 0
 #define MH_ROTARY_LINEAR 1
 #define MH_ROTARY_BASE 2
@@ -317,7 +319,8 @@ int mh_attention_paged(int dt, const void *q, int64_t ldq, const void *k_cache, 
 int mh_rotary_frequencies(double *freq, double *magnitude, int rot, double base, int scaling, double factor, double original,
                           double low, double high);
 /* table [n][half][2] = magnitude * (cos a, sin a), a = positions[t] * freq[j] (device
- * arrays; the angles in 64 bits, any int32 position).  table is 16-byte aligned and overlaps neither of them. */
+ * arrays; a exact to about 2^-50 behind its whole turns, at any int32 position).
+ * table is 16-byte aligned and overlaps neither of them. */
 int mh_rotary_table(const int32_t *positions, const double *freq, float *table, int n, int half, double magnitude, void *stream);
 /* out = x with its pairs (a, b) turned to (a c - b s, a s + b c); with `inverse` s
  * counts negative, which is also the gradient.  x, out: n token rows of heads * hd
@@ -353,7 +356,8 @@ int mh_dequantize_rows(int dt, const int8_t *q, int64_t ldq, const float *scale,
                        void *stream);
 /* out[m][n] = act(x_scale[m] w_scale[n] sum_k x[m][k] w[n][k] + bias[n]) + resid[m][n]:
  * mh_linear with both operands in int8, [M][K] rows ldx and [N][K] rows ldw apart, of
- * any alignment (multiples of 16 bytes are faster; of others whole 4-byte words that
+ * any alignment (K, spacings and addresses that are all multiples of 16 are up to
+ * twice as fast, K = 4090 in rows of 4096 is not; of others whole 4-byte words that
  * hold a value are read).  bias (may be NULL), resid (may be
  * NULL; rows ldr apart) and out (ldo apart) are of `dt`; act is MH_ACT_*, GELU
  * x * sigmoid(1.702 x).  The sum is exact in int32 (K is at most 2^17 - 1), the rest

@@ -237,7 +237,8 @@ ROTARY_SCALINGS = {None: 0, "linear": 1, "base": 2, "turns": 3}
 
 def rotary_frequencies(rot, base=10000.0, scaling=None, factor=1.0, original=0, low=1.0, high=32.0):
     """(frequencies, magnitude) for ``rotary_table`` (mh_rotary_frequencies): float64
-    [rot / 2] on the host; ``scaling`` None, "linear", "base" or "turns"."""
+    [rot / 2] on the host; ``scaling`` None, "linear", "base" or "turns" (whose magnitude
+    is for models that were trained with it)."""
     if scaling not in ROTARY_SCALINGS:
         raise ValueError(f"rotary_frequencies: scaling must be None, 'linear', 'base' or 'turns', not {scaling!r}")
     freq, m = (ctypes.c_double * max(1, rot // 2))(), ctypes.c_double()

@@ -2,7 +2,8 @@
 //
 // Both are bound by memory: a row is read once and held in registers while its
 // largest magnitude is found.  8192 rows of 8192 bf16 values: 40 us, 5.0 TB/s, which is
-// what a large copy reaches; back 30 us (read from the last-level cache).
+// what a large copy reaches; back 30 us (read from the last-level cache).  Rows past
+// 32768 values are read twice: 2048 of 40000 values 69 us, 3.6 TB/s of what is read once.
 #include <algorithm>
 
 #include "gemm_common.hpp"
